@@ -291,6 +291,92 @@ int glif_rate_dist_loss(const int32_t *count, int32_t count_rows, int32_t n_neur
                         float kappa, float rate_cost, int32_t shuffle, uint64_t seed, uint64_t offset,
                         float *loss_out, float *gz_neuron, void *ws, size_t ws_bytes, void *stream);
 
+/* ------------------------------------------------------ sequence operators --
+ * What reads a rollout out and is trained with it (the reference's Dense and softmax readouts, models.py:1138-1209,
+ * 1213-1392, are Keras layers): layer norm, dropout, a linear map with its epilogue, a short causal convolution and a
+ * selective state space scan, each with its backward, and single-tick forms of the last two.
+ *   - Activations are float32, bfloat16 or float16 (glif_dtype); parameters of the small operators (norm weights, taps,
+ *     biases) are float32 or of the activations' type (param_dtype).  Sums, statistics and states are float32.
+ *   - Sequences are time-major [T][B][D], channels contiguous; strides of ticks and batch entries are in elements.
+ *     Outputs are contiguous.  lengths [B] int32 (NULL: all T ticks; clamped to [0, T]): the ticks of a batch entry from
+ *     its length on are not read, give zeros, leave its state alone and take no part in any gradient.
+ *   - Sums run in a fixed order: the same call gives the same bits.
+ *   - Gradient outputs may be NULL where they are not wanted. */
+typedef enum { GLIF_F32 = 0, GLIF_BF16 = 1, GLIF_F16 = 2 } glif_dtype;
+typedef enum { GLIF_ACT_NONE = 0, GLIF_ACT_RELU = 1, GLIF_ACT_GELU = 2, GLIF_ACT_SILU = 3 } glif_activation;
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over rows of D elements (row stride x_stride); weight, bias [D] or
+ * NULL.  The backward takes the statistics from x; dweight and dbias are of param_dtype. */
+int glif_layer_norm_fwd(const void *x, int64_t x_stride, const void *weight, const void *bias, int32_t dtype,
+                        int32_t param_dtype, int64_t rows, int64_t D, float eps, void *y, void *stream);
+size_t glif_layer_norm_bwd_workspace(int64_t rows, int64_t D, int32_t want_params);
+int glif_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const void *weight,
+                        int32_t dtype, int32_t param_dtype, int64_t rows, int64_t D, float eps, void *dx, void *dweight,
+                        void *dbias, void *ws, size_t ws_bytes, void *stream);
+
+/* y[i] = (u >= p ? x[i] / (1 - p) : 0) + residual[i] (residual may be NULL), u the uniform of word offset + i of the
+ * Philox stream `seed` (see the input sampling below): a kept element is one glif_sample_bernoulli does not set at p.  The
+ * gradient is the same call on dy without a residual. */
+int glif_dropout(const void *x, const void *residual, int32_t dtype, int64_t n, double p, uint64_t seed, uint64_t offset,
+                 void *y, void *stream);
+
+/* y = act(x weight^T + bias) + residual: x [M][K], weight [N][K], bias [N] or NULL, residual [M][N] or NULL, row strides
+ * ld*; pre [M][N] (NULL: not kept) takes x weight^T + bias for the backward, rounded to dtype.
+ * Backward: dp = dy act'(pre) (act NONE: pre is not read); dx = dp weight, dweight = dp^T x, dbias = sum of dp's rows. */
+size_t glif_linear_fwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K);
+int glif_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const void *residual,
+                    int64_t ldr, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
+                    void *y, void *pre, void *ws, size_t ws_bytes, void *stream);
+size_t glif_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t activation);
+int glif_linear_bwd(const void *dy, int64_t lddy, const void *pre, const void *x, int64_t ldx, const void *weight,
+                    int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
+                    void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream);
+
+/* Causal convolution with W <= 8 taps per channel: y[t] = act(bias + sum_k weight[d][k] x[t - (W - 1) + k]), act the
+ * identity or silu.  state [B][W - 1][D] (NULL: zeros) holds the ticks before 0, last (may be NULL) the last W - 1 ones
+ * before each length.  The step moves `state` on in place. */
+int glif_short_conv_fwd(const void *x, int64_t x_stride_t, int64_t x_stride_b, const void *weight, const void *bias,
+                        const void *state, const int32_t *lengths, int32_t dtype, int32_t param_dtype, int32_t T, int32_t B,
+                        int32_t D, int32_t W, int32_t silu, void *y, void *last, void *stream);
+size_t glif_short_conv_bwd_workspace(int32_t T, int32_t B, int32_t D, int32_t W);
+int glif_short_conv_bwd(const void *dy, int64_t dy_stride_t, int64_t dy_stride_b, const void *dlast, const void *x,
+                        int64_t x_stride_t, int64_t x_stride_b, const void *weight, const void *bias, const void *state,
+                        const int32_t *lengths, int32_t dtype, int32_t param_dtype, int32_t T, int32_t B, int32_t D,
+                        int32_t W, int32_t silu, void *dx, void *dweight, void *dbias, void *dstate, void *ws,
+                        size_t ws_bytes, void *stream);
+int glif_short_conv_step(const void *x, int64_t x_stride_b, void *state, const void *weight, const void *bias, int32_t dtype,
+                         int32_t param_dtype, int32_t B, int32_t D, int32_t W, int32_t silu, void *y, void *stream);
+
+/* Selective state space, N <= 64 states per channel, B and C shared by the D / G channels of a group:
+ *   step = softplus ? log(1 + exp(delta + delta_bias)) : delta + delta_bias
+ *   h[t] = exp(step A) h[t - 1] + step B[t] u[t],   y[t] = (sum_n C[t][n] h[t][n] + D u[t]) (z ? z sigmoid(z) : 1) */
+typedef struct {
+    const void *u, *delta, *z;       /* [T][B][D]; z may be NULL */
+    const void *B, *C;               /* [T][B][G][N], the last two dimensions contiguous */
+    const float *A, *D, *delta_bias; /* [D][N], [D] or NULL, [D] or NULL */
+    const float *state;              /* [B][D][N] before the first tick, NULL: zeros */
+    const int32_t *lengths;
+    int64_t u_st, u_sb, delta_st, delta_sb, z_st, z_sb, B_st, B_sb, C_st, C_sb;
+    int32_t dtype, n_ticks, n_batch, n_channels, n_groups, n_state, softplus;
+} glif_scan;
+/* keep (NULL: evaluation only): glif_scan_keep_bytes() bytes of states on the way, which the backward reads.  last
+ * [B][D][N] float32 (may be NULL): the states after each length. */
+size_t glif_scan_keep_bytes(const glif_scan *s);
+size_t glif_scan_fwd_workspace(const glif_scan *s);
+int glif_scan_fwd(const glif_scan *s, void *y, float *last, void *keep, void *ws, size_t ws_bytes, void *stream);
+typedef struct {
+    const void *dy;          /* [T][B][D] */
+    int64_t dy_st, dy_sb;
+    const float *dlast;      /* [B][D][N] or NULL */
+    void *du, *ddelta, *dz;  /* contiguous, of dtype */
+    void *dB, *dC;
+    float *dA, *dD, *ddelta_bias, *dstate;
+} glif_scan_grad;
+size_t glif_scan_bwd_workspace(const glif_scan *s);
+int glif_scan_bwd(const glif_scan *s, const glif_scan_grad *g, const void *keep, void *ws, size_t ws_bytes, void *stream);
+/* One tick: u, delta, z [B][D], B and C [B][G][N] (s->n_ticks 1, tick strides unused); state [B][D][N] in place. */
+int glif_scan_step(const glif_scan *s, void *y, float *state, void *stream);
+
 /* ------------------------------------------------------------- optimizer ------
  * Replaces ExponentiatedAdam.update_step, dense branch (v1_model_utils/optimizers.py:
  * 354-376; alpha :273-283), followed by the variable's SignedConstraint (models.py:419-427, attached

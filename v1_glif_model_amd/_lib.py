@@ -40,6 +40,19 @@ class StateGrad(C.Structure):
     _fields_ = [("z_buf", vp), ("v", vp), ("asc", vp), ("psc_rise", vp), ("psc", vp)]
 
 
+class Scan(C.Structure):
+    """glif_scan."""
+    _fields_ = ([(n, vp) for n in ("u", "delta", "z", "B", "C", "A", "D", "delta_bias", "state", "lengths")]
+                + [(n, C.c_int64) for n in ("u_st", "u_sb", "delta_st", "delta_sb", "z_st", "z_sb", "B_st", "B_sb", "C_st", "C_sb")]
+                + [(n, C.c_int32) for n in ("dtype", "n_ticks", "n_batch", "n_channels", "n_groups", "n_state", "softplus")])
+
+
+class ScanGrad(C.Structure):
+    """glif_scan_grad."""
+    _fields_ = ([("dy", vp), ("dy_st", C.c_int64), ("dy_sb", C.c_int64)]
+                + [(n, vp) for n in ("dlast", "du", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias", "dstate")])
+
+
 SIGNATURES = {
     "glif_last_error": (C.c_char_p, []),
     "glif_version": (C.c_int, []),
@@ -81,6 +94,25 @@ SIGNATURES = {
                                 vp]),
     "glif_sample_bernoulli": (C.c_int, [vp, i64, C.c_uint64, C.c_uint64, vp, vp]),
     "glif_sample_poisson": (C.c_int, [C.c_float, C.c_float, i64, C.c_uint64, C.c_uint64, vp, vp]),
+    "glif_layer_norm_fwd": (C.c_int, [vp, i64, vp, vp, i32, i32, i64, i64, C.c_float, vp, vp]),
+    "glif_layer_norm_bwd_workspace": (sz, [i64, i64, i32]),
+    "glif_layer_norm_bwd": (C.c_int, [vp, i64, vp, i64, vp, i32, i32, i64, i64, C.c_float, vp, vp, vp, vp, sz, vp]),
+    "glif_dropout": (C.c_int, [vp, vp, i32, i64, C.c_double, C.c_uint64, C.c_uint64, vp, vp]),
+    "glif_linear_fwd_workspace": (sz, [i32, i64, i64, i64]),
+    "glif_linear_fwd": (C.c_int, [vp, i64, vp, i64, vp, vp, i64, i32, i32, i64, i64, i64, i32, vp, vp, vp, sz, vp]),
+    "glif_linear_bwd_workspace": (sz, [i32, i64, i64, i64, i32]),
+    "glif_linear_bwd": (C.c_int, [vp, i64, vp, vp, i64, vp, i64, i32, i32, i64, i64, i64, i32, vp, vp, vp, vp, sz, vp]),
+    "glif_short_conv_fwd": (C.c_int, [vp, i64, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
+    "glif_short_conv_bwd_workspace": (sz, [i32, i32, i32, i32]),
+    "glif_short_conv_bwd": (C.c_int, [vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp,
+                                      vp, vp, vp, sz, vp]),
+    "glif_short_conv_step": (C.c_int, [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
+    "glif_scan_keep_bytes": (sz, [C.POINTER(Scan)]),
+    "glif_scan_fwd_workspace": (sz, [C.POINTER(Scan)]),
+    "glif_scan_fwd": (C.c_int, [C.POINTER(Scan), vp, vp, vp, vp, sz, vp]),
+    "glif_scan_bwd_workspace": (sz, [C.POINTER(Scan)]),
+    "glif_scan_bwd": (C.c_int, [C.POINTER(Scan), C.POINTER(ScanGrad), vp, vp, sz, vp]),
+    "glif_scan_step": (C.c_int, [C.POINTER(Scan), vp, vp, vp]),
     "glif_prof_enable": (C.c_int, [C.c_uint32]),
     "glif_prof_stride": (C.c_int, [i32]),
     "glif_prof_collect": (C.c_int, [vp, vp, i32]),
