@@ -9,11 +9,16 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// C[m][n] = sum_k P(m, k) Q(n, k), P(m, k) = p[m * p_m + k * p_k], one of the two strides 1; likewise Q.
+// C[m][n] = sum_k P(m, k) Q(n, k): P(m, k) is p[m * p_ld + k], or p[k * p_ld + m] where its columns are contiguous;
+// likewise Q.
 struct GemmArgs {
     const void *p, *q;
-    int64_t p_m, p_k, q_n, q_k;
+    int64_t p_ld, q_ld;        // the stride that is not 1
     int64_t M, N, K;
+    int64_t k_part;            // k's of a split
+    int32_t tiles_m, tiles_n, splits;
+    float *part;               // [splits][M][part_ld], where splits > 1
+    int64_t part_ld;
     void *c, *pre;             // [M][N]
     const void *bias, *residual;
     int64_t ldr;
@@ -41,8 +46,6 @@ __device__ __forceinline__ float slope_of(float p, int act) {
         default: return 1.0f;
     }
 }
-
-constexpr int kTile = 64;
 
 // One matrix instruction's operands from a row-major LDS row of 32 k's: 16-bit types take 8 consecutive k's a lane.
 template <typename T>
@@ -72,52 +75,269 @@ struct Mma<f32> {
     }
 };
 
-// 64 x 64 of C by four waves of 32 x 32; k in steps of one matrix instruction.
+// ---- tiles in LDS -----------------------------------------------------------------------------------------------------
+// An operand's tile is ROWS rows (of m or n) of 128 bytes of k: 64 16-bit values or 32 float32.  The eight 16-byte chunks of
+// a row are permuted by the row, chunk c at c ^ (row ^ row / 8) mod 8: the lanes that read one chunk of 8 consecutive rows,
+// those that write a row's 8 chunks, and those that write one chunk of rows 8 or 4 apart all touch different banks.
+constexpr int kRowBytes = 128;
+
+__device__ __forceinline__ int lds_at(int row, int chunk) { return row * kRowBytes + (((chunk ^ row ^ (row >> 3)) & 7) << 4); }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Brings ROWS x 128 bytes of an operand from memory into LDS by way of registers, NT threads.  COL: k runs along the rows
+// of memory (m or n is contiguous), and the values are turned on their way: a thread takes 4 k's of 16 bytes of m.  Rows
+// past the operand's end repeat the last (their products are not written); k's past `k1` are 0.
+template <typename T, bool COL, int ROWS, int NT>
+struct Stage {
+    static constexpr int kV = 16 / static_cast<int>(sizeof(T));   // values of a chunk
+    static constexpr int kBK = 8 * kV;                            // k's of a tile
+    static constexpr int kN = ROWS * 8 / NT;                      // chunks a thread takes
+    static_assert(ROWS * 8 % NT == 0 && (!COL || kN % 4 == 0), "the tile does not divide among the threads");
+    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    vec r[kN];
+    const T *at[COL ? kN / 4 : kN];
+    int64_t ld;
+
+    // the place of unit i: COL (first row, first k), else (row, chunk)
+    static __device__ __forceinline__ void place(int i, int &row, int &k) {
+        const int u = threadIdx.x + i * NT;
+        if (!COL) {
+            row = u >> 3, k = u & 7;
+        } else if (sizeof(T) == 2) {   // 8 rows x 4 k's; neighbours take the two halves of a chunk
+            row = (u >> 1) % (ROWS / 8) * 8, k = (u >> 1) / (ROWS / 8) * 8 + (u & 1) * 4;
+        } else {                       // 4 rows x 4 k's
+            row = u % (ROWS / 4) * 4, k = u / (ROWS / 4) * 4;
+        }
+    }
+
+    __device__ __forceinline__ void init(const T *p, int64_t stride, int64_t row0, int64_t rows, int64_t k0) {
+        ld = stride;
+        int row, k;
+        if (!COL) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                place(i, row, k);
+                at[i] = p + min(row0 + row, rows - 1) * ld + k0 + k * kV;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN / 4; ++i) {
+                place(i, row, k);
+                at[i] = p + (k0 + k) * ld + row0 + row;
+            }
+        }
+    }
+
+    // k0: the tile's first k; left = k1 - k0, what there is of it
+    __device__ __forceinline__ void load(int64_t row0, int64_t rows, int64_t left) {
+        int row, k;
+        if (!COL) {
+            if (left >= kBK) {
+#pragma unroll
+                for (int i = 0; i < kN; ++i) r[i] = *reinterpret_cast<const vec *>(at[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    place(i, row, k);
+#pragma unroll
+                    for (int e = 0; e < kV; ++e) r[i][e] = k * kV + e < left ? at[i][e] : T(0.0f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kN; ++i) at[i] += kBK;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN / 4; ++i) {
+                place(i, row, k);
+                const int64_t have = rows - row0 - row;   // rows of the operand from this one on
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (k + j < left && have >= kV) {
+                        r[4 * i + j] = *reinterpret_cast<const vec *>(at[i] + j * ld);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kV; ++e) r[4 * i + j][e] = k + j < left && e < have ? at[i][j * ld + e] : T(0.0f);
+                    }
+                }
+                at[i] += kBK * ld;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(char *lds) const {
+        int row, k;
+        if (!COL) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                place(i, row, k);
+                *reinterpret_cast<u32x4 *>(lds + lds_at(row, k)) = __builtin_bit_cast(u32x4, r[i]);
+            }
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < kN / 4; ++i) {
+                place(i, row, k);
+                u32x4 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(u32x4, r[4 * i + j]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {   // row + e: its values of k .. k + 3
+                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                    const u32x2 v = {__builtin_amdgcn_perm(w[1][e / 2], w[0][e / 2], sel),
+                                     __builtin_amdgcn_perm(w[3][e / 2], w[2][e / 2], sel)};
+                    *reinterpret_cast<u32x2 *>(lds + lds_at(row + e, k >> 3) + (k & 4) * 2) = v;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN / 4; ++i) {
+                place(i, row, k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const vec v = {r[4 * i][e], r[4 * i + 1][e], r[4 * i + 2][e], r[4 * i + 3][e]};
+                    *reinterpret_cast<u32x4 *>(lds + lds_at(row + e, k >> 2)) = __builtin_bit_cast(u32x4, v);
+                }
+            }
+        }
+    }
+};
+
+// Four neighbouring results of row m: bias, activation, residual, and one rounding.
 template <typename T>
-__global__ void __launch_bounds__(kBlock) k_gemm(GemmArgs a) {
+__device__ __forceinline__ void finish(const GemmArgs &a, int64_t m, int64_t n, f32x4 v) {
+    const int have = static_cast<int>(min(static_cast<int64_t>(4), a.N - n));
+    typedef Vec<T, 4> vec;
+    if (a.bias)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < have) v[e] += load_param(a.bias, a.bias_dt, n + e);
+    T *pre = a.pre ? static_cast<T *>(a.pre) + m * a.N + n : nullptr, *c = static_cast<T *>(a.c) + m * a.N + n;
+    const T *res = a.residual ? static_cast<const T *>(a.residual) + m * a.ldr + n : nullptr;
+    if (have == 4) {
+        if (pre) *reinterpret_cast<vec *>(pre) = __builtin_convertvector(v, vec);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = act_of(v[e], a.act);
+        if (res) {
+            const vec q = *reinterpret_cast<const vec *>(res);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += to_f32(static_cast<T>(q[e]));
+        }
+        *reinterpret_cast<vec *>(c) = __builtin_convertvector(v, vec);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e >= have) continue;
+            if (pre) pre[e] = from_f32<T>(v[e]);
+            v[e] = act_of(v[e], a.act);
+            if (res) v[e] += to_f32(res[e]);
+            c[e] = from_f32<T>(v[e]);
+        }
+    }
+}
+
+// BM x BN of C by WM x WN waves, of k in [split's part).  Two tiles of each operand in LDS: while one is multiplied, the
+// next comes into registers, and from there into the other.
+template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL>
+__global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
     using M = Mma<T>;
-    constexpr int KS = 4 * M::kLane, LD = KS + 16 / static_cast<int>(sizeof(T));
-    __shared__ __attribute__((aligned(16))) T sp[kTile][LD], sq[kTile][LD];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16 * M::kLane;
-    const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile, n0 = static_cast<int64_t>(blockIdx.x) * kTile;
-    const int wm = wave / 2 * 32, wn = wave % 2 * 32;
-    f32x4 acc[2][2] = {};
-    const T *p = static_cast<const T *>(a.p), *q = static_cast<const T *>(a.q);
-    for (int64_t k0 = 0; k0 < a.K; k0 += KS) {
-        for (int i = threadIdx.x; i < kTile * KS; i += kBlock) {
-            int r = a.p_k == 1 ? i / KS : i % kTile, k = a.p_k == 1 ? i % KS : i / kTile;
-            sp[r][k] = m0 + r < a.M && k0 + k < a.K ? p[(m0 + r) * a.p_m + (k0 + k) * a.p_k] : T(0.0f);
-            r = a.q_k == 1 ? i / KS : i % kTile, k = a.q_k == 1 ? i % KS : i / kTile;
-            sq[r][k] = n0 + r < a.N && k0 + k < a.K ? q[(n0 + r) * a.q_n + (k0 + k) * a.q_k] : T(0.0f);
-        }
-        __syncthreads();
-        typename M::frag fp[2], fq[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fp[i] = *reinterpret_cast<const typename M::frag *>(&sp[wm + 16 * i + r16][kq]);
-            fq[i] = *reinterpret_cast<const typename M::frag *>(&sq[wn + 16 * i + r16][kq]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = M::run(fq[j], fp[i], acc[i][j]);   // rows of the result: n
+    constexpr int NT = WM * WN * kWave, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+    constexpr int BK = Stage<T, false, BM, NT>::kBK, kTile = (BM + BN) * kRowBytes;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16;
+    const int wm = wave / WN * TM, wn = wave % WN * TN;
+    // neighbouring tiles share an operand: the XCDs (block id mod 8) take consecutive runs of them, along the shorter side
+    int id = blockIdx.x;
+    const int tiles = gridDim.x;
+    if (tiles >= 8) {
+        const int x = id & 7, per = tiles >> 3, more = tiles & 7;
+        id = x * per + min(x, more) + (id >> 3);
+    }
+    const int split = id / (a.tiles_m * a.tiles_n), tile = id - split * a.tiles_m * a.tiles_n;
+    const int tm = a.tiles_m <= a.tiles_n ? tile % a.tiles_m : tile / a.tiles_n;
+    const int tn = a.tiles_m <= a.tiles_n ? tile / a.tiles_m : tile % a.tiles_n;
+    const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+    const int64_t k0 = split * a.k_part, k1 = min(a.K, k0 + a.k_part);
+    Stage<T, PCOL, BM, NT> sp;
+    Stage<T, QCOL, BN, NT> sq;
+    sp.init(static_cast<const T *>(a.p), a.p_ld, m0, a.M, k0);
+    sq.init(static_cast<const T *>(a.q), a.q_ld, n0, a.N, k0);
+    f32x4 acc[FM][FN] = {};
+    const int steps = static_cast<int>((k1 - k0 + BK - 1) / BK);
+    if (steps > 0) {
+        sp.load(m0, a.M, k1 - k0);
+        sq.load(n0, a.N, k1 - k0);
+        sp.store(lds);
+        sq.store(lds + BM * kRowBytes);
         __syncthreads();
     }
+    for (int s = 0; s < steps; ++s) {
+        const char *cur = lds + (s & 1) * kTile;
+        const bool more = s + 1 < steps;
+        if (more) {
+            const int64_t left = k1 - k0 - static_cast<int64_t>(s + 1) * BK;
+            sp.load(m0, a.M, left);
+            sq.load(n0, a.N, left);
+        }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int kk = 0; kk < 2; ++kk) {
+            typename M::frag fp[FM], fq[FN];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int i = 0; i < FM; ++i)
+                fp[i] = *reinterpret_cast<const typename M::frag *>(cur + lds_at(wm + 16 * i + r16, 4 * kk + kq));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t m = m0 + wm + 16 * i + r16, n = n0 + wn + 16 * j + lane / 16 * 4 + e;
-                if (m >= a.M || n >= a.N) continue;
-                float v = acc[i][j][e];
-                if (a.bias) v += load_param(a.bias, a.bias_dt, n);
-                if (a.pre) static_cast<T *>(a.pre)[m * a.N + n] = from_f32<T>(v);
-                v = act_of(v, a.act);
-                if (a.residual) v += to_f32(static_cast<const T *>(a.residual)[m * a.ldr + n]);
-                static_cast<T *>(a.c)[m * a.N + n] = from_f32<T>(v);
+            for (int j = 0; j < FN; ++j)
+                fq[j] = *reinterpret_cast<const typename M::frag *>(cur + BM * kRowBytes + lds_at(wn + 16 * j + r16, 4 * kk + kq));
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = M::run(fq[j], fp[i], acc[i][j]);   // rows of the result: n
+        }
+        if (more) {
+            char *next = lds + ((s + 1) & 1) * kTile;
+            sp.store(next);
+            sq.store(next + BM * kRowBytes);
+        }
+        __syncthreads();
+    }
+    // Each wave puts its results by way of a slab of its own in LDS: rows come out whole, and the epilogue stands once.  Quad
+    // q of row r lies at q ^ r mod the row's quads.
+    constexpr int kQuads = TN / 4, kSlab = 2 * kTile / (WM * WN), kRows = kSlab / (TN * 4) < TM ? kSlab / (TN * 4) : TM;
+    static_assert(kRows % 16 == 0 && TM % kRows == 0 && kWave % kQuads == 0, "slab");
+    f32x4 *slab = reinterpret_cast<f32x4 *>(lds + wave * kSlab);
+#pragma unroll
+    for (int h = 0; h < TM / kRows; ++h) {
+#pragma unroll
+        for (int i = 0; i < kRows / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int r = 16 * i + r16, q = 4 * j + kq;
+                slab[r * kQuads + (q ^ (r & (kQuads - 1)))] = acc[h * (kRows / 16) + i][j];
             }
+        const int q = lane % kQuads;
+        const int64_t n = n0 + wn + q * 4;
+        if (n < a.N)
+#pragma unroll 1
+            for (int r = lane / kQuads; r < kRows; r += kWave / kQuads) {
+                const int64_t m = m0 + wm + h * kRows + r;
+                if (m >= a.M) break;
+                const f32x4 v = slab[r * kQuads + (q ^ (r & (kQuads - 1)))];
+                if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part + (split * a.M + m) * a.part_ld + n) = v;
+                else finish<T>(a, m, n, v);
+            }
+    }
+}
+
+// The splits' sums, in order, and the epilogue.
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_gemm_join(GemmArgs a) {
+    const int64_t quads = a.part_ld / 4, n4 = a.M * quads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < n4; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+        const int64_t m = i / quads, n = (i - m * quads) * 4;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4 *>(a.part + (s * a.M + m) * a.part_ld + n);
+        finish<T>(a, m, n, v);
+    }
 }
 
 struct SlopeArgs {
@@ -153,12 +373,52 @@ __global__ void __launch_bounds__(kBlock) k_bias_join(const float *part, int par
     store_param(dbias, dt, n, s);
 }
 
-template <typename T>
-void run_gemm(const GemmArgs &a, hipStream_t s) {
-    if (a.M == 0 || a.N == 0) return;
-    hipLaunchKernelGGL(k_gemm<T>, dim3(static_cast<unsigned>(ceil_div(a.N, kTile)), static_cast<unsigned>(ceil_div(a.M, kTile))),
-                       dim3(kBlock), 0, s, a);
+// How a product is cut up.
+struct Plan {
+    int32_t splits;
+    int64_t k_part, part_ld;
+    size_t floats() const { return splits > 1 ? static_cast<size_t>(splits) * rows * part_ld : 0; }
+    int64_t rows;
+};
+
+constexpr int kBM = 256, kBN = 256;
+
+Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K) {
+    const int64_t bk = kRowBytes / static_cast<int64_t>(dtype_size(dtype)), steps = std::max<int64_t>((K + bk - 1) / bk, 1);
+    const int64_t tiles = ((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN);
+    int64_t splits = tiles ? std::max<int64_t>(1, std::min<int64_t>(256 / tiles, steps / 8)) : 1;
+    Plan p{};
+    p.k_part = (steps + splits - 1) / splits * bk;
+    p.splits = static_cast<int32_t>((steps * bk + p.k_part - 1) / p.k_part);
+    p.part_ld = (N + 3) / 4 * 4;
+    p.rows = M;
+    return p;
 }
+
+template <typename T, bool PCOL, bool QCOL>
+int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
+    if (a.M == 0 || a.N == 0) return GLIF_OK;
+    a.splits = p.splits, a.k_part = p.k_part, a.part_ld = p.part_ld, a.part = part;
+    a.tiles_m = ceil_div(a.M, kBM), a.tiles_n = ceil_div(a.N, kBN);
+    auto fn = k_gemm<T, kBM, kBN, 2, 4, PCOL, QCOL>;
+    constexpr int bytes = 2 * (kBM + kBN) * kRowBytes;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    GLIF_HIP(set);
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)), dim3(512), bytes, s, a);
+    if (a.splits > 1) {
+        const int64_t n4 = a.M * (a.part_ld / 4);
+        hipLaunchKernelGGL(k_gemm_join<T>, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))), dim3(kBlock),
+                           0, s, a);
+    }
+    return GLIF_OK;
+}
+
+template <typename T>
+int gemm_rr(const GemmArgs &a, const Plan &p, float *part, hipStream_t s) { return launch_gemm<T, false, false>(a, p, part, s); }
+template <typename T>
+int gemm_rc(const GemmArgs &a, const Plan &p, float *part, hipStream_t s) { return launch_gemm<T, false, true>(a, p, part, s); }
+template <typename T>
+int gemm_cc(const GemmArgs &a, const Plan &p, float *part, hipStream_t s) { return launch_gemm<T, true, true>(a, p, part, s); }
 
 template <typename T>
 void run_slope(const SlopeArgs &a, hipStream_t s) {
@@ -180,13 +440,16 @@ int check_linear(int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_
 
 struct Back {
     void *dp;
-    float *part;
+    float *part, *sums;   // of the products' splits (one after the other), of the bias's rows
     int32_t parts;
+    Plan dx, dw;
 };
 
-void carve(Carver &c, Back &b, int32_t dtype, int64_t M, int64_t N, int32_t act) {
+void carve(Carver &c, Back &b, int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act) {
     b.parts = row_parts(M);
-    b.part = c.take<float>(static_cast<size_t>(b.parts * N));
+    b.dx = plan_for(dtype, M, K, N), b.dw = plan_for(dtype, N, K, M);
+    b.sums = c.take<float>(static_cast<size_t>(b.parts * N));
+    b.part = c.take<float>(std::max(b.dx.floats(), b.dw.floats()));
     b.dp = act != GLIF_ACT_NONE ? c.take<char>(static_cast<size_t>(M * N) * dtype_size(dtype)) : nullptr;
 }
 
@@ -198,21 +461,26 @@ using namespace glif;
 extern "C" {
 
 size_t glif_linear_fwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K) {
-    (void)dtype, (void)M, (void)N, (void)K;
-    return 0;
+    if (check_linear(dtype, dtype, M, N, K, 0)) return 0;
+    Carver c(nullptr, 0);
+    if (const size_t n = plan_for(dtype, M, N, K).floats()) c.take<float>(n);
+    return c.off;
 }
 
 int glif_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const void *residual,
                     int64_t ldr, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
                     void *y, void *pre, void *ws, size_t ws_bytes, void *stream) {
-    (void)ws, (void)ws_bytes;
     if (int rc = check_linear(dtype, bias_dtype, M, N, K, activation)) return rc;
     if (M == 0 || N == 0) return GLIF_OK;
     if (!y || (K && (!x || !weight))) return fail(GLIF_EINVAL, "NULL argument");
     GemmArgs a{};
-    a.p = x, a.p_m = ldx, a.p_k = 1, a.q = weight, a.q_n = ldw, a.q_k = 1, a.M = M, a.N = N, a.K = K;
+    a.p = x, a.p_ld = ldx, a.q = weight, a.q_ld = ldw, a.M = M, a.N = N, a.K = K;
     a.c = y, a.pre = pre, a.bias = bias, a.residual = residual, a.ldr = ldr, a.bias_dt = bias_dtype, a.act = activation;
-    GLIF_BY_DTYPE(dtype, run_gemm, a, static_cast<hipStream_t>(stream));
+    const Plan p = plan_for(dtype, M, N, K);
+    Carver c(ws, ws_bytes);
+    float *part = c.take<float>(p.floats());
+    if (!c.ok() || (p.floats() && !ws)) return fail(GLIF_ENOMEM, "linear: workspace too small");
+    if (int rc = GLIF_BY_DTYPE(dtype, gemm_rr, a, p, part, static_cast<hipStream_t>(stream))) return rc;
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;
 }
@@ -221,7 +489,7 @@ size_t glif_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K,
     if (check_linear(dtype, dtype, M, N, K, activation)) return 0;
     Carver c(nullptr, 0);
     Back b{};
-    carve(c, b, dtype, M, N, activation);
+    carve(c, b, dtype, M, N, K, activation);
     return c.mark();
 }
 
@@ -235,27 +503,27 @@ int glif_linear_bwd(const void *dy, int64_t lddy, const void *pre, const void *x
     hipStream_t s = static_cast<hipStream_t>(stream);
     Back b{};
     Carver c(ws, ws_bytes);
-    carve(c, b, dtype, M, N, activation);
+    carve(c, b, dtype, M, N, K, activation);
     if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "linear: workspace too small");
     const void *dp = dy;
     int64_t lddp = lddy;
     if (activation != GLIF_ACT_NONE || dbias) {
-        SlopeArgs a{dy, pre, lddy, M, N, b.dp, dbias ? b.part : nullptr, activation, b.parts};
+        SlopeArgs a{dy, pre, lddy, M, N, b.dp, dbias ? b.sums : nullptr, activation, b.parts};
         GLIF_BY_DTYPE(dtype, run_slope, a, s);
         if (b.dp) dp = b.dp, lddp = N;
         if (dbias && N)
-            hipLaunchKernelGGL(k_bias_join, dim3(static_cast<unsigned>(ceil_div(N, kBlock))), dim3(kBlock), 0, s, b.part, b.parts,
+            hipLaunchKernelGGL(k_bias_join, dim3(static_cast<unsigned>(ceil_div(N, kBlock))), dim3(kBlock), 0, s, b.sums, b.parts,
                                N, dbias, bias_dtype);
     }
     if (dx) {
         GemmArgs a{};
-        a.p = dp, a.p_m = lddp, a.p_k = 1, a.q = weight, a.q_n = 1, a.q_k = ldw, a.M = M, a.N = K, a.K = N, a.c = dx;
-        GLIF_BY_DTYPE(dtype, run_gemm, a, s);
+        a.p = dp, a.p_ld = lddp, a.q = weight, a.q_ld = ldw, a.M = M, a.N = K, a.K = N, a.c = dx;
+        if (int rc = GLIF_BY_DTYPE(dtype, gemm_rc, a, b.dx, b.part, s)) return rc;
     }
     if (dweight) {
         GemmArgs a{};
-        a.p = dp, a.p_m = 1, a.p_k = lddp, a.q = x, a.q_n = 1, a.q_k = ldx, a.M = N, a.N = K, a.K = M, a.c = dweight;
-        GLIF_BY_DTYPE(dtype, run_gemm, a, s);
+        a.p = dp, a.p_ld = lddp, a.q = x, a.q_ld = ldx, a.M = N, a.N = K, a.K = M, a.c = dweight;
+        if (int rc = GLIF_BY_DTYPE(dtype, gemm_cc, a, b.dw, b.part, s)) return rc;
     }
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;
