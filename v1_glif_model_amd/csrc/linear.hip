@@ -52,13 +52,11 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
-    static constexpr int kLane = 8;
     typedef bf16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Mma<f16> {
-    static constexpr int kLane = 8;
     typedef f16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -66,7 +64,6 @@ struct Mma<f16> {
 // a sum is free, as long as both operands have it)
 template <>
 struct Mma<f32> {
-    static constexpr int kLane = 4;
     typedef f32 frag __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) {
 #pragma unroll
@@ -236,6 +233,49 @@ __device__ __forceinline__ void finish(const GemmArgs &a, int64_t m, int64_t n, 
     }
 }
 
+// A wave's TM x TN results by way of a slab of its own in LDS: rows come out whole, and the epilogue stands once.  Quad q of
+// row r lies at q ^ r mod the row's quads.
+template <typename T, int TM, int TN, int SLAB>
+__device__ __forceinline__ void put(const GemmArgs &a, f32x4 (&acc)[TM / 16][TN / 16], char *lds, int64_t m0, int64_t n0, int split) {
+    constexpr int kQuads = TN / 4, kRows = SLAB / (TN * 4) < TM ? SLAB / (TN * 4) : TM;
+    static_assert(kRows % 16 == 0 && TM % kRows == 0 && kWave % kQuads == 0, "slab");
+    const int lane = threadIdx.x % kWave, r16 = lane % 16, kq = lane / 16;
+    f32x4 *slab = reinterpret_cast<f32x4 *>(lds);
+#pragma unroll
+    for (int h = 0; h < TM / kRows; ++h) {
+#pragma unroll
+        for (int i = 0; i < kRows / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < TN / 16; ++j) {
+                const int r = 16 * i + r16, q = 4 * j + kq;
+                slab[r * kQuads + (q ^ (r & (kQuads - 1)))] = acc[h * (kRows / 16) + i][j];
+            }
+        const int q = lane % kQuads;
+        const int64_t n = n0 + q * 4;
+        if (n < a.N)
+#pragma unroll 1
+            for (int r = lane / kQuads; r < kRows; r += kWave / kQuads) {
+                const int64_t m = m0 + h * kRows + r;
+                if (m >= a.M) break;
+                const f32x4 v = slab[r * kQuads + (q ^ (r & (kQuads - 1)))];
+                if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part + (split * a.M + m) * a.part_ld + n) = v;
+                else finish<T>(a, m, n, v);
+            }
+    }
+}
+
+// The block's tile.  Neighbouring tiles share an operand: the XCDs (block id mod 8) take consecutive runs of them, along the
+// shorter side.
+__device__ __forceinline__ void my_tile(const GemmArgs &a, int &tm, int &tn, int &split) {
+    int id = blockIdx.x;
+    const int blocks = gridDim.x, x = id & 7, per = blocks >> 3, more = blocks & 7;
+    if (blocks >= 8) id = x * per + min(x, more) + (id >> 3);
+    split = id / (a.tiles_m * a.tiles_n);
+    const int tile = id - split * a.tiles_m * a.tiles_n;
+    tm = a.tiles_m <= a.tiles_n ? tile % a.tiles_m : tile / a.tiles_n;
+    tn = a.tiles_m <= a.tiles_n ? tile / a.tiles_m : tile % a.tiles_n;
+}
+
 // BM x BN of C by WM x WN waves, of k in [split's part).  Two tiles of each operand in LDS: while one is multiplied, the
 // next comes into registers, and from there into the other.
 template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL>
@@ -246,16 +286,8 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16;
     const int wm = wave / WN * TM, wn = wave % WN * TN;
-    // neighbouring tiles share an operand: the XCDs (block id mod 8) take consecutive runs of them, along the shorter side
-    int id = blockIdx.x;
-    const int tiles = gridDim.x;
-    if (tiles >= 8) {
-        const int x = id & 7, per = tiles >> 3, more = tiles & 7;
-        id = x * per + min(x, more) + (id >> 3);
-    }
-    const int split = id / (a.tiles_m * a.tiles_n), tile = id - split * a.tiles_m * a.tiles_n;
-    const int tm = a.tiles_m <= a.tiles_n ? tile % a.tiles_m : tile / a.tiles_n;
-    const int tn = a.tiles_m <= a.tiles_n ? tile / a.tiles_m : tile % a.tiles_n;
+    int tm, tn, split;
+    my_tile(a, tm, tn, split);
     const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
     const int64_t k0 = split * a.k_part, k1 = min(a.K, k0 + a.k_part);
     Stage<T, PCOL, BM, NT> sp;
@@ -300,32 +332,202 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
         }
         __syncthreads();
     }
-    // Each wave puts its results by way of a slab of its own in LDS: rows come out whole, and the epilogue stands once.  Quad
-    // q of row r lies at q ^ r mod the row's quads.
-    constexpr int kQuads = TN / 4, kSlab = 2 * kTile / (WM * WN), kRows = kSlab / (TN * 4) < TM ? kSlab / (TN * 4) : TM;
-    static_assert(kRows % 16 == 0 && TM % kRows == 0 && kWave % kQuads == 0, "slab");
-    f32x4 *slab = reinterpret_cast<f32x4 *>(lds + wave * kSlab);
-#pragma unroll
-    for (int h = 0; h < TM / kRows; ++h) {
-#pragma unroll
-        for (int i = 0; i < kRows / 16; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int r = 16 * i + r16, q = 4 * j + kq;
-                slab[r * kQuads + (q ^ (r & (kQuads - 1)))] = acc[h * (kRows / 16) + i][j];
-            }
-        const int q = lane % kQuads;
-        const int64_t n = n0 + wn + q * 4;
-        if (n < a.N)
-#pragma unroll 1
-            for (int r = lane / kQuads; r < kRows; r += kWave / kQuads) {
-                const int64_t m = m0 + wm + h * kRows + r;
-                if (m >= a.M) break;
-                const f32x4 v = slab[r * kQuads + (q ^ (r & (kQuads - 1)))];
-                if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part + (split * a.M + m) * a.part_ld + n) = v;
-                else finish<T>(a, m, n, v);
-            }
+    put<T, TM, TN, 2 * kTile / (WM * WN)>(a, acc, lds + wave * (2 * kTile / (WM * WN)), m0 + wm, n0 + wn, split);
+}
+
+#ifdef __HIP_DEVICE_COMPILE__   // the host's pass does not know the builtins
+// ---- operands straight into LDS ---------------------------------------------------------------------------------------
+// Memory to LDS without registers, 1 KB (64 x 16 bytes) of consecutive LDS a wave and instruction; the permutation of the
+// chunks is in the addresses that are read.  COL operands lie in LDS as they do in memory, rows of k, and are turned where
+// they are read: 16-bit types by the LDS transpose read (16 lanes take 4 k's of 16 m's), float32 by reading single values.
+// There the 16-m pieces of row k are permuted by those bits of k in which the rows of one read differ.
+// For 16-byte aligned rows only; K (of rows of k: M or N) counts in whole chunks, and a block's part of an operand in 32 bits.
+constexpr int kRawBuffer = 0x00020000;   // descriptor word 3: untyped 32-bit offsets
+template <typename T, bool COL, int ROWS, int WAVES>
+struct Direct {
+    static constexpr int kSize = static_cast<int>(sizeof(T)), kV = 16 / kSize, kBK = 8 * kV;
+    static constexpr int kN = ROWS * kRowBytes / 1024 / WAVES;    // instructions of a wave
+    static constexpr int kColBytes = ROWS * kSize, kPiece = 16 * kSize;
+    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+    __amdgpu_buffer_rsrc_t rsrc;   // from the first value of the block's rows and k's
+    uint32_t off[kN], at_k;        // of the lane's pieces in a tile, and of the next tile
+    uint32_t ld;                   // bytes
+
+    static __device__ __forceinline__ int col_key(int k) { return kSize == 2 ? (k & 3) | ((k >> 1) & 4) : (k >> 2) & 3; }
+
+    // what lands at lane's place of instruction i: COL (row k, byte of it), else (row, chunk)
+    static __device__ __forceinline__ void place(int wave, int lane, int i, int &row, int &at) {
+        const int byte = (wave * kN + i) * 1024 + lane * 16;
+        if (COL) {
+            row = byte / kColBytes, at = byte % kColBytes;
+            at = (at / kPiece ^ col_key(row)) * kPiece + at % kPiece;
+        } else {
+            row = byte / kRowBytes, at = ((byte / 16 ^ row ^ (row >> 3)) & 7);
+        }
     }
+
+    __device__ __forceinline__ void init(const void *p, int64_t stride, int64_t row0, int64_t rows, int64_t k0, int wave, int lane) {
+        ld = static_cast<uint32_t>(stride * kSize);
+        const char *base = static_cast<const char *>(p) + (COL ? k0 * stride + row0 : row0 * stride + k0) * kSize;
+        rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, -1, kRawBuffer);
+        at_k = 0;
+        const int have = static_cast<int>(min(rows - row0, static_cast<int64_t>(ROWS)));
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            int r, at;
+            place(wave, lane, i, r, at);
+            off[i] = COL ? r * ld + min(at, have * kSize - 16) : min(r, have - 1) * ld + at * 16;
+        }
+    }
+
+    // Before the load of a last tile with `left` k's: what would lie past them is read from the tile's first k's, and
+    // cleared by clear().
+    __device__ __forceinline__ void shorten(int left, int wave, int lane) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            int r, at;
+            place(wave, lane, i, r, at);
+            if (COL && r >= left) off[i] -= r * ld;
+            if (!COL && at * kV >= left) off[i] -= at * 16;
+        }
+    }
+
+    __device__ __forceinline__ void load(char *lds, int wave) {
+        typedef __attribute__((address_space(3))) void *lptr;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr)(lds + (wave * kN + i) * 1024), 16, off[i], at_k, 0, 0);
+        at_k += COL ? kBK * ld : kRowBytes;
+    }
+
+    static __device__ __forceinline__ void clear(char *lds, int left) {
+        for (int u = threadIdx.x; u < ROWS * 8; u += WAVES * kWave) {
+            const int row = COL ? u * 16 / kColBytes : u >> 3;
+            if (COL ? row >= left : (u & 7) * kV >= left)
+                *reinterpret_cast<u32x4 *>(lds + (COL ? u * 16 : lds_at(row, u & 7))) = u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+
+    // A wave's reads: fragment i, rows w + 16 i .. (w a multiple of 64), of matrix instruction kk of the tile.  What depends on
+    // the lane is one of a few offsets (the permutation is an exclusive or of a lane's part and of i's and kk's).
+    static constexpr int kAts = !COL ? 4 : kSize == 2 ? 8 : 4;
+    struct Reader {
+        int at[kAts];
+        __device__ __forceinline__ Reader(int w, int r16, int kq) {
+#pragma unroll
+            for (int c = 0; c < kAts; ++c) {
+                if (!COL) at[c] = (w + r16) * kRowBytes + ((kq ^ (r16 & 7) ^ (r16 >> 3) ^ (2 * c)) << 4);
+                else if (kSize == 2) at[c] = (8 * kq + (r16 >> 2)) * kColBytes + ((w / 16 + c) ^ col_key(8 * kq + (r16 >> 2))) * kPiece + (r16 & 3) * 8;
+                else at[c] = 4 * kq * kColBytes + ((w / 16 + c) ^ col_key(4 * kq)) * kPiece + r16 * 4;
+            }
+        }
+        __device__ __forceinline__ vec frag(const char *lds, int i, int kk) const {
+            if constexpr (!COL) {
+                return *reinterpret_cast<const vec *>(lds + at[(i ^ (2 * kk)) & 3] + i * 16 * kRowBytes);
+            } else if constexpr (kSize == 2) {
+                typedef short s4 __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) s4 *l4;
+                static_assert(ROWS <= 256, "eight fragments a wave");
+                const char *p = lds + at[i] + kk * 32 * kColBytes;
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(p));
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(p + 4 * kColBytes));
+                return __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            } else {
+                vec v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = *reinterpret_cast<const T *>(lds + at[i & 3] + (kk * 16 + e) * kColBytes + i / 4 * 4 * kPiece);
+                return v;
+            }
+        }
+    };
+};
+
+#endif
+
+// BM x BN of C by WM x WN waves, of k in the split's part.  Two tiles of each operand in LDS; the second half of a tile's
+// operands is in registers before the barrier at which the tile's LDS is given to the loads of the tile after next, and the
+// first half of the next tile's is read while that second half is multiplied.
+template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL>
+__global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
+#ifdef __HIP_DEVICE_COMPILE__
+    using M = Mma<T>;
+    constexpr int W = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+    using P = Direct<T, PCOL, BM, W>;
+    using Q = Direct<T, QCOL, BN, W>;
+    constexpr int BK = P::kBK, kQAt = BM * kRowBytes, kTile = (BM + BN) * kRowBytes;
+    __shared__ __attribute__((aligned(1024))) char lds0[kTile];
+    __shared__ __attribute__((aligned(1024))) char lds1[kTile];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
+    const int wm = wave / WN * TM, wn = wave % WN * TN;
+    int tm, tn, split;
+    my_tile(a, tm, tn, split);
+    const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+    const int64_t k0 = split * a.k_part, k1 = min(a.K, k0 + a.k_part);
+    const int steps = static_cast<int>((k1 - k0 + BK - 1) / BK);
+    const int tail = static_cast<int>(k1 - k0 - static_cast<int64_t>(steps - 1) * BK);   // k's of the last tile
+    P p;
+    Q q;
+    p.init(a.p, a.p_ld, m0, a.M, k0, wave, lane);
+    q.init(a.q, a.q_ld, n0, a.N, k0, wave, lane);
+    static_assert(TM % 64 == 0 && TN % 64 == 0, "a wave's rows");
+    const typename P::Reader rp(wm, r16, kq);
+    const typename Q::Reader rq(wn, r16, kq);
+    f32x4 acc[FM][FN] = {};
+    typename M::frag fp0[FM], fq0[FN], fp1[FM], fq1[FN];
+    auto fetch = [&](char *to, int s) {
+        if (s + 1 == steps && tail < BK) {
+            p.shorten(tail, wave, lane);
+            q.shorten(tail, wave, lane);
+        }
+        p.load(to, wave);
+        q.load(to + kQAt, wave);
+    };
+    // the tiles that are on their way have landed, and nobody reads the LDS that is loaded next any more
+    auto meet = [&](char *landed, bool last) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (last && tail < BK) {
+            P::clear(landed, tail);
+            Q::clear(landed + kQAt, tail);
+            __syncthreads();
+        }
+    };
+    auto half = [&](typename M::frag(&fp)[FM], typename M::frag(&fq)[FN], const char *from, int kk) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fp[i] = rp.frag(from, i, kk);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fq[j] = rq.frag(from + kQAt, j, kk);
+    };
+    auto mul = [&](typename M::frag(&fp)[FM], typename M::frag(&fq)[FN]) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = M::run(fq[j], fp[i], acc[i][j]);   // rows of the result: n
+    };
+    auto step = [&](char *cur, char *next, int s) {
+        half(fp1, fq1, cur, 1);
+        mul(fp0, fq0);
+        meet(next, s + 2 == steps);
+        if (s + 2 < steps) fetch(cur, s + 2);
+        half(fp0, fq0, next, 0);   // of no tile after the last, and then not used
+        mul(fp1, fq1);
+    };
+    fetch(lds0, 0);
+    meet(lds0, steps == 1);
+    if (steps > 1) fetch(lds1, 1);
+    half(fp0, fq0, lds0, 0);
+    for (int s = 0;; ) {
+        step(lds0, lds1, s);
+        if (++s == steps) break;
+        step(lds1, lds0, s);
+        if (++s == steps) break;
+    }
+    __syncthreads();
+    constexpr int kSlab = 2 * kTile / W;
+    char *slab = wave < W / 2 ? lds0 + wave * kSlab : lds1 + (wave - W / 2) * kSlab;
+    put<T, TM, TN, kSlab>(a, acc, slab, m0 + wm, n0 + wn, split);
+#endif
 }
 
 // The splits' sums, in order, and the epilogue.
@@ -381,6 +583,10 @@ struct Plan {
     int64_t rows;
 };
 
+#ifndef GWM
+#define GWM 2
+#define GWN 4
+#endif
 constexpr int kBM = 256, kBN = 256;
 
 Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K) {
@@ -395,16 +601,29 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K) {
     return p;
 }
 
+// Whether an operand's rows can go to LDS directly: 16-byte pieces that lie on 16-byte addresses, 32-bit offsets in a tile.
+template <typename T>
+bool aligned(const void *p, int64_t ld, int64_t along, int64_t rows) {
+    const int64_t v = 16 / static_cast<int64_t>(sizeof(T));
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % v == 0 && along % v == 0 && (ld * rows + along) * static_cast<int64_t>(sizeof(T)) < (int64_t(1) << 32);
+}
+
 template <typename T, bool PCOL, bool QCOL>
 int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return GLIF_OK;
     a.splits = p.splits, a.k_part = p.k_part, a.part_ld = p.part_ld, a.part = part;
     a.tiles_m = ceil_div(a.M, kBM), a.tiles_n = ceil_div(a.N, kBN);
-    auto fn = k_gemm<T, kBM, kBN, 2, 4, PCOL, QCOL>;
-    constexpr int bytes = 2 * (kBM + kBN) * kRowBytes;
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    GLIF_HIP(set);
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)), dim3(512), bytes, s, a);
+    const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits));
+    if (a.K > 0 && aligned<T>(a.p, a.p_ld, PCOL ? a.M : a.K, PCOL ? a.k_part : kBM) &&
+        aligned<T>(a.q, a.q_ld, QCOL ? a.N : a.K, QCOL ? a.k_part : kBN)) {
+        hipLaunchKernelGGL((k_gemm_direct<T, kBM, kBN, GWM, GWN, PCOL, QCOL>), grid, dim3(GWM * GWN * 64), 0, s, a);
+    } else {
+        auto fn = k_gemm<T, kBM, kBN, 2, 4, PCOL, QCOL>;
+        constexpr int bytes = 2 * (kBM + kBN) * kRowBytes;
+        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        GLIF_HIP(set);
+        hipLaunchKernelGGL(fn, grid, dim3(512), bytes, s, a);
+    }
     if (a.splits > 1) {
         const int64_t n4 = a.M * (a.part_ld / 4);
         hipLaunchKernelGGL(k_gemm_join<T>, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))), dim3(kBlock),
