@@ -200,46 +200,60 @@ struct Stage {
     }
 };
 
-// Four neighbouring results of row m: bias, activation, residual, and one rounding.
+// Four neighbouring results: bias, activation, residual, and one rounding.  The parts that come from memory are read ahead.
 template <typename T>
-__device__ __forceinline__ void finish(const GemmArgs &a, int64_t m, int64_t n, f32x4 v) {
-    const int have = static_cast<int>(min(static_cast<int64_t>(4), a.N - n));
+struct Finish {
     typedef Vec<T, 4> vec;
-    if (a.bias)
+    f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+    int64_t n;
+    int have;
+    __device__ __forceinline__ Finish(const GemmArgs &a, int64_t col) : n(col), have(static_cast<int>(min(static_cast<int64_t>(4), a.N - col))) {
+        if (a.bias)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < have) bias[e] = load_param(a.bias, a.bias_dt, n + e);
+    }
+    __device__ __forceinline__ vec residual(const GemmArgs &a, int64_t m) const {
+        vec q = {};
+        if (!a.residual) return q;
+        const T *p = static_cast<const T *>(a.residual) + m * a.ldr + n;
+        if (have == 4) return *reinterpret_cast<const vec *>(p);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (e < have) v[e] += load_param(a.bias, a.bias_dt, n + e);
-    T *pre = a.pre ? static_cast<T *>(a.pre) + m * a.N + n : nullptr, *c = static_cast<T *>(a.c) + m * a.N + n;
-    const T *res = a.residual ? static_cast<const T *>(a.residual) + m * a.ldr + n : nullptr;
-    if (have == 4) {
-        if (pre) *reinterpret_cast<vec *>(pre) = __builtin_convertvector(v, vec);
+            if (e < have) q[e] = p[e];
+        return q;
+    }
+    static __device__ __forceinline__ void write(T *p, f32x4 v, int have) {
+        if (have == 4) {
+            *reinterpret_cast<vec *>(p) = __builtin_convertvector(v, vec);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = act_of(v[e], a.act);
-        if (res) {
-            const vec q = *reinterpret_cast<const vec *>(res);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += to_f32(static_cast<T>(q[e]));
-        }
-        *reinterpret_cast<vec *>(c) = __builtin_convertvector(v, vec);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (e >= have) continue;
-            if (pre) pre[e] = from_f32<T>(v[e]);
-            v[e] = act_of(v[e], a.act);
-            if (res) v[e] += to_f32(res[e]);
-            c[e] = from_f32<T>(v[e]);
+            for (int e = 0; e < 4; ++e)
+                if (e < have) p[e] = from_f32<T>(v[e]);
         }
     }
-}
+    __device__ __forceinline__ void operator()(const GemmArgs &a, int64_t m, f32x4 v, vec res) const {
+        v += bias;
+        if (a.pre) write(static_cast<T *>(a.pre) + m * a.N + n, v, have);
+        if (a.act != GLIF_ACT_NONE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = act_of(v[e], a.act);
+        }
+        if (a.residual) v += __builtin_convertvector(res, f32x4);
+        write(static_cast<T *>(a.c) + m * a.N + n, v, have);
+    }
+};
 
 // A wave's TM x TN results by way of a slab of its own in LDS: rows come out whole, and the epilogue stands once.  Quad q of
 // row r lies at q ^ r mod the row's quads.
 template <typename T, int TM, int TN, int SLAB>
 __device__ __forceinline__ void put(const GemmArgs &a, f32x4 (&acc)[TM / 16][TN / 16], char *lds, int64_t m0, int64_t n0, int split) {
     constexpr int kQuads = TN / 4, kRows = SLAB / (TN * 4) < TM ? SLAB / (TN * 4) : TM;
-    static_assert(kRows % 16 == 0 && TM % kRows == 0 && kWave % kQuads == 0, "slab");
-    const int lane = threadIdx.x % kWave, r16 = lane % 16, kq = lane / 16;
+    constexpr int kStep = kWave / kQuads, kAhead = 4;
+    static_assert(kRows % 16 == 0 && TM % kRows == 0 && kWave % kQuads == 0 && kRows % (kStep * kAhead) == 0, "slab");
+    const int lane = threadIdx.x % kWave, r16 = lane % 16, kq = lane / 16, q = lane % kQuads;
+    const int64_t n = n0 + q * 4;
+    const Finish<T> finish(a, n);
     f32x4 *slab = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
     for (int h = 0; h < TM / kRows; ++h) {
@@ -250,17 +264,27 @@ __device__ __forceinline__ void put(const GemmArgs &a, f32x4 (&acc)[TM / 16][TN 
                 const int r = 16 * i + r16, q = 4 * j + kq;
                 slab[r * kQuads + (q ^ (r & (kQuads - 1)))] = acc[h * (kRows / 16) + i][j];
             }
-        const int q = lane % kQuads;
-        const int64_t n = n0 + q * 4;
-        if (n < a.N)
+        if (n >= a.N) continue;
+        const int left = static_cast<int>(min(a.M - m0 - h * kRows, static_cast<int64_t>(kRows)));
 #pragma unroll 1
-            for (int r = lane / kQuads; r < kRows; r += kWave / kQuads) {
-                const int64_t m = m0 + h * kRows + r;
-                if (m >= a.M) break;
-                const f32x4 v = slab[r * kQuads + (q ^ (r & (kQuads - 1)))];
-                if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part + (split * a.M + m) * a.part_ld + n) = v;
-                else finish<T>(a, m, n, v);
+        for (int r = lane / kQuads; r < kRows; r += kStep * kAhead) {
+            f32x4 v[kAhead];
+            typename Finish<T>::vec res[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int at = r + u * kStep;
+                v[u] = slab[at * kQuads + (q ^ (at & (kQuads - 1)))];
+                if (a.residual && a.splits == 1 && at < left) res[u] = finish.residual(a, m0 + h * kRows + at);
             }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int at = r + u * kStep;
+                const int64_t m = m0 + h * kRows + at;
+                if (at >= left) continue;
+                if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part + (split * a.M + m) * a.part_ld + n) = v[u];
+                else finish(a, m, v[u], res[u]);
+            }
+        }
     }
 }
 
@@ -536,9 +560,11 @@ __global__ void __launch_bounds__(kBlock) k_gemm_join(GemmArgs a) {
     const int64_t quads = a.part_ld / 4, n4 = a.M * quads;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < n4; i += static_cast<int64_t>(gridDim.x) * kBlock) {
         const int64_t m = i / quads, n = (i - m * quads) * 4;
+        const Finish<T> finish(a, n);
+        const typename Finish<T>::vec res = finish.residual(a, m);
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4 *>(a.part + (s * a.M + m) * a.part_ld + n);
-        finish<T>(a, m, n, v);
+        finish(a, m, v, res);
     }
 }
 
