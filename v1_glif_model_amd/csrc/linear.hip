@@ -52,11 +52,13 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
+    static constexpr int kEach = 1;   // matrix instructions of a fragment
     typedef bf16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Mma<f16> {
+    static constexpr int kEach = 1;
     typedef f16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -64,6 +66,7 @@ struct Mma<f16> {
 // a sum is free, as long as both operands have it)
 template <>
 struct Mma<f32> {
+    static constexpr int kEach = 4;
     typedef f32 frag __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) {
 #pragma unroll
@@ -73,12 +76,15 @@ struct Mma<f32> {
 };
 
 // ---- tiles in LDS -----------------------------------------------------------------------------------------------------
-// An operand's tile is ROWS rows (of m or n) of 128 bytes of k: 64 16-bit values or 32 float32.  The eight 16-byte chunks of
-// a row are permuted by the row, chunk c at c ^ (row ^ row / 8) mod 8: the lanes that read one chunk of 8 consecutive rows,
-// those that write a row's 8 chunks, and those that write one chunk of rows 8 or 4 apart all touch different banks.
+// An operand's tile is ROWS rows (of m or n) of 128 bytes of k: 64 16-bit values or 32 float32.  LDS gives 256 bytes a clock:
+// 16 lanes of 16-byte reads, and those are not neighbours but of two fragments' quarters (measured: permuted by the row mod
+// 8, half of the clocks of the reads went to bank conflicts).  So the eight 16-byte chunks of a row are permuted by row / 2
+// mod 8, which tells all even and all odd rows of a fragment apart for any chunk.
 constexpr int kRowBytes = 128;
 
-__device__ __forceinline__ int lds_at(int row, int chunk) { return row * kRowBytes + (((chunk ^ row ^ (row >> 3)) & 7) << 4); }
+__device__ __forceinline__ int lds_at(int row, int chunk) { return row * kRowBytes + (((chunk ^ (row >> 1)) & 7) << 4); }
+// The same for tiles that are written by rows 8 or 4 apart: those are told apart by bits 4 and 5 of the row.
+__device__ __forceinline__ int lds_at_turned(int row, int chunk) { return lds_at(row, chunk ^ ((row >> 4) & 3)); }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -169,7 +175,7 @@ struct Stage {
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 place(i, row, k);
-                *reinterpret_cast<u32x4 *>(lds + lds_at(row, k)) = __builtin_bit_cast(u32x4, r[i]);
+                *reinterpret_cast<u32x4 *>(lds + lds_at_turned(row, k)) = __builtin_bit_cast(u32x4, r[i]);
             }
         } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -183,7 +189,7 @@ struct Stage {
                     const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
                     const u32x2 v = {__builtin_amdgcn_perm(w[1][e / 2], w[0][e / 2], sel),
                                      __builtin_amdgcn_perm(w[3][e / 2], w[2][e / 2], sel)};
-                    *reinterpret_cast<u32x2 *>(lds + lds_at(row + e, k >> 3) + (k & 4) * 2) = v;
+                    *reinterpret_cast<u32x2 *>(lds + lds_at_turned(row + e, k >> 3) + (k & 4) * 2) = v;
                 }
             }
         } else {
@@ -193,7 +199,7 @@ struct Stage {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const vec v = {r[4 * i][e], r[4 * i + 1][e], r[4 * i + 2][e], r[4 * i + 3][e]};
-                    *reinterpret_cast<u32x4 *>(lds + lds_at(row + e, k >> 2)) = __builtin_bit_cast(u32x4, v);
+                    *reinterpret_cast<u32x4 *>(lds + lds_at_turned(row + e, k >> 2)) = __builtin_bit_cast(u32x4, v);
                 }
             }
         }
@@ -340,10 +346,10 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
             typename M::frag fp[FM], fq[FN];
 #pragma unroll
             for (int i = 0; i < FM; ++i)
-                fp[i] = *reinterpret_cast<const typename M::frag *>(cur + lds_at(wm + 16 * i + r16, 4 * kk + kq));
+                fp[i] = *reinterpret_cast<const typename M::frag *>(cur + lds_at_turned(wm + 16 * i + r16, 4 * kk + kq));
 #pragma unroll
             for (int j = 0; j < FN; ++j)
-                fq[j] = *reinterpret_cast<const typename M::frag *>(cur + BM * kRowBytes + lds_at(wn + 16 * j + r16, 4 * kk + kq));
+                fq[j] = *reinterpret_cast<const typename M::frag *>(cur + BM * kRowBytes + lds_at_turned(wn + 16 * j + r16, 4 * kk + kq));
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -386,7 +392,7 @@ struct Direct {
             row = byte / kColBytes, at = byte % kColBytes;
             at = (at / kPiece ^ col_key(row)) * kPiece + at % kPiece;
         } else {
-            row = byte / kRowBytes, at = ((byte / 16 ^ row ^ (row >> 3)) & 7);
+            row = byte / kRowBytes, at = (byte / 16 ^ (row >> 1)) & 7;
         }
     }
 
@@ -416,6 +422,9 @@ struct Direct {
         }
     }
 
+    // Every further load is of an empty range.
+    __device__ __forceinline__ void stop() { rsrc = __builtin_amdgcn_make_buffer_rsrc(nullptr, 0, 0, kRawBuffer); }
+
     __device__ __forceinline__ void load(char *lds, int wave) {
         typedef __attribute__((address_space(3))) void *lptr;
 #pragma unroll
@@ -434,20 +443,21 @@ struct Direct {
 
     // A wave's reads: fragment i, rows w + 16 i .. (w a multiple of 64), of matrix instruction kk of the tile.  What depends on
     // the lane is one of a few offsets (the permutation is an exclusive or of a lane's part and of i's and kk's).
-    static constexpr int kAts = !COL ? 4 : kSize == 2 ? 8 : 4;
+    static constexpr int kReads = !COL ? 1 : kSize == 2 ? 2 : 4;   // LDS reads of a fragment
+    static constexpr int kAts = !COL ? 2 : kSize == 2 ? 8 : 4;
     struct Reader {
         int at[kAts];
         __device__ __forceinline__ Reader(int w, int r16, int kq) {
 #pragma unroll
             for (int c = 0; c < kAts; ++c) {
-                if (!COL) at[c] = (w + r16) * kRowBytes + ((kq ^ (r16 & 7) ^ (r16 >> 3) ^ (2 * c)) << 4);
+                if (!COL) at[c] = lds_at(w + r16, 4 * c + kq);
                 else if (kSize == 2) at[c] = (8 * kq + (r16 >> 2)) * kColBytes + ((w / 16 + c) ^ col_key(8 * kq + (r16 >> 2))) * kPiece + (r16 & 3) * 8;
                 else at[c] = 4 * kq * kColBytes + ((w / 16 + c) ^ col_key(4 * kq)) * kPiece + r16 * 4;
             }
         }
         __device__ __forceinline__ vec frag(const char *lds, int i, int kk) const {
             if constexpr (!COL) {
-                return *reinterpret_cast<const vec *>(lds + at[(i ^ (2 * kk)) & 3] + i * 16 * kRowBytes);
+                return *reinterpret_cast<const vec *>(lds + at[kk] + i * 16 * kRowBytes);
             } else if constexpr (kSize == 2) {
                 typedef short s4 __attribute__((ext_vector_type(4)));
                 typedef __attribute__((address_space(3))) s4 *l4;
@@ -499,11 +509,13 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
     const typename Q::Reader rq(wn, r16, kq);
     f32x4 acc[FM][FN] = {};
     typename M::frag fp0[FM], fq0[FN], fp1[FM], fq1[FN];
-    auto fetch = [&](char *to, int s) {
+    auto shorten = [&](int s) {   // before the load of tile s
         if (s + 1 == steps && tail < BK) {
             p.shorten(tail, wave, lane);
             q.shorten(tail, wave, lane);
         }
+    };
+    auto fetch = [&](char *to) {
         p.load(to, wave);
         q.load(to + kQAt, wave);
     };
@@ -529,24 +541,41 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = M::run(fq[j], fp[i], acc[i][j]);   // rows of the result: n
     };
+    // A wave issues in order and the loads wait for their turn at the address unit, so they are spread among the matrix
+    // instructions; for that they are always there, past the last tile with an empty range (nothing is read).
     auto step = [&](char *cur, char *next, int s) {
+        shorten(s + 2);
         half(fp1, fq1, cur, 1);
         mul(fp0, fq0);
+        if (s + 2 >= steps) p.stop(), q.stop();
         meet(next, s + 2 == steps);
-        if (s + 2 < steps) fetch(cur, s + 2);
+        fetch(cur);
         half(fp0, fq0, next, 0);   // of no tile after the last, and then not used
         mul(fp1, fq1);
+#ifndef NOSG
+        constexpr int kLoads = P::kN + Q::kN, kMul = FM * FN * M::kEach, kReads = FM * P::kReads + FN * Q::kReads;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kLoads - 1) / kLoads, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, kMul / kLoads, 0);
+            __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+        }
+#endif
     };
-    fetch(lds0, 0);
+    shorten(0);
+    fetch(lds0);
     meet(lds0, steps == 1);
-    if (steps > 1) fetch(lds1, 1);
+    shorten(1);
+    if (steps == 1) p.stop(), q.stop();
+    fetch(lds1);
     half(fp0, fq0, lds0, 0);
-    for (int s = 0;; ) {
+    for (int s = 0;;) {
         step(lds0, lds1, s);
         if (++s == steps) break;
         step(lds1, lds0, s);
         if (++s == steps) break;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the empty loads still write to LDS
     __syncthreads();
     constexpr int kSlab = 2 * kTile / W;
     char *slab = wave < W / 2 ? lds0 + wave * kSlab : lds1 + (wave - W / 2) * kSlab;
