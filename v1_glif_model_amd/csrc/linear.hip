@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
     using M = Mma<T>;
     constexpr int NT = WM * WN * kWave, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
     constexpr int BK = Stage<T, false, BM, NT>::kBK, kTile = (BM + BN) * kRowBytes;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ __attribute__((aligned(16))) char lds[2 * kTile];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16;
     const int wm = wave / WN * TM, wn = wave % WN * TN;
     int tm, tn, split;
@@ -552,7 +552,6 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
         fetch(cur);
         half(fp0, fq0, next, 0);   // of no tile after the last, and then not used
         mul(fp1, fq1);
-#ifndef NOSG
         constexpr int kLoads = P::kN + Q::kN, kMul = FM * FN * M::kEach, kReads = FM * P::kReads + FN * Q::kReads;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -560,7 +559,6 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
             __builtin_amdgcn_sched_group_barrier(0x008, kMul / kLoads, 0);
             __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
         }
-#endif
     };
     shorten(0);
     fetch(lds0);
@@ -581,6 +579,74 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
     char *slab = wave < W / 2 ? lds0 + wave * kSlab : lds1 + (wave - W / 2) * kSlab;
     put<T, TM, TN, kSlab>(a, acc, slab, m0 + wm, n0 + wn, split);
 #endif
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------
+// Products of which one side has at most 16 MT rows (single ticks; a readout of few classes): the other side's 16 rows of a
+// block stream from memory straight into operands, each of the block's four waves over a part of the block's k's, and the
+// few rows come from the caches.  NFEW: the few are q's rows (n), else p's (m).
+template <typename T, int MT, bool NFEW>
+__global__ void __launch_bounds__(kBlock) k_few(GemmArgs a) {
+    using M = Mma<T>;
+    constexpr int kV = 16 / static_cast<int>(sizeof(T)), KS = 4 * kV, U = MT == 4 ? 2 : 4, kWaves = kBlock / kWave;
+    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    __shared__ f32x4 sums[kWaves][MT][kWave];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16;
+    const int64_t many = NFEW ? a.M : a.N, few = NFEW ? a.N : a.M;
+    const int groups = NFEW ? a.tiles_m : a.tiles_n, split = blockIdx.x / groups;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x - split * groups) * 16;
+    // the wave's k's, in whole matrix instructions
+    const int64_t b0 = split * a.k_part, b1 = min(a.K, b0 + a.k_part), part = (b1 - b0 + kWaves * KS - 1) / (kWaves * KS) * KS;
+    const int64_t k0 = min(b0 + wave * part, b1), k1 = min(k0 + part, b1);
+    const T *pm = static_cast<const T *>(NFEW ? a.p : a.q) + min(row0 + r16, many - 1) * (NFEW ? a.p_ld : a.q_ld) + kq * kV;
+    const T *pf[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+        pf[i] = static_cast<const T *>(NFEW ? a.q : a.p) + min(static_cast<int64_t>(16 * i + r16), few - 1) * (NFEW ? a.q_ld : a.p_ld) + kq * kV;
+    f32x4 acc[MT] = {};
+    auto mul = [&](typename M::frag f, typename M::frag w, f32x4 c) { return NFEW ? M::run(f, w, c) : M::run(w, f, c); };   // rows: n
+    int64_t k = k0;
+    for (; k + U * KS <= k1; k += U * KS) {
+        vec w[U], f[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = *reinterpret_cast<const vec *>(pm + k + u * KS);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) f[u][i] = *reinterpret_cast<const vec *>(pf[i] + k + u * KS);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = mul(f[u][i], w[u], acc[i]);
+    }
+    for (; k < k1; k += KS) {
+        const int64_t left = k1 - k - kq * kV;
+        auto load = [&](const T *p) {
+            if (left >= kV) return *reinterpret_cast<const vec *>(p + k);
+            vec v;
+#pragma unroll
+            for (int e = 0; e < kV; ++e) v[e] = e < left ? p[k + e] : T(0.0f);
+            return v;
+        };
+        const vec w = load(pm);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i] = mul(load(pf[i]), w, acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4 v = sums[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += sums[w][wave][lane];
+    const int64_t m = NFEW ? row0 + r16 : 16 * wave + r16, n = (NFEW ? 16 * wave : row0) + kq * 4;
+    if (m >= a.M || n >= a.N) return;
+    if (a.splits > 1) {
+        *reinterpret_cast<f32x4 *>(a.part + (split * a.M + m) * a.part_ld + n) = v;
+    } else {
+        const Finish<T> finish(a, n);
+        finish(a, m, v, finish.residual(a, m));
+    }
 }
 
 // The splits' sums, in order, and the epilogue.
@@ -630,29 +696,52 @@ __global__ void __launch_bounds__(kBlock) k_bias_join(const float *part, int par
     store_param(dbias, dt, n, s);
 }
 
-// How a product is cut up.
+// How a product is cut up: the tile, and the parts of k whose sums are added afterwards.
+enum Kind { kFew16, kFew32, kFew64, kTile128, kTile256 };
 struct Plan {
+    Kind kind;
     int32_t splits;
-    int64_t k_part, part_ld;
+    int64_t k_part, part_ld, rows;
     size_t floats() const { return splits > 1 ? static_cast<size_t>(splits) * rows * part_ld : 0; }
-    int64_t rows;
 };
 
-#ifndef GWM
-#define GWM 2
-#define GWN 4
-#endif
-constexpr int kBM = 256, kBN = 256;
-
-Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K) {
-    const int64_t bk = kRowBytes / static_cast<int64_t>(dtype_size(dtype)), steps = std::max<int64_t>((K + bk - 1) / bk, 1);
-    const int64_t tiles = ((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN);
-    int64_t splits = tiles ? std::max<int64_t>(1, std::min<int64_t>(256 / tiles, steps / 8)) : 1;
+// rr: both operands have k along their rows.
+//
+// At most 64 rows on one side: k is split until the chip has about eight waves a SIMD to keep the stream of the other side
+// going, but no part under 512 k's.
+//
+// Otherwise the cheapest of both tiles and some splits, by what a step (128 bytes of k) of a tile costs a compute unit and
+// what goes on around the steps, in us: 16-bit 256 x 256 1.7 + 5, 128 x 128 0.6 + 2; float32, whose products run at 1/16,
+// 7.5 + 5 and 2.0 + 2; a split costs its sums' way to memory and back and the launch that adds them.  A float32 sum runs over
+// at most 4096 k's, so that long ones do not lose their last digits.
+Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
     Plan p{};
-    p.k_part = (steps + splits - 1) / splits * bk;
+    p.rows = M, p.part_ld = (N + 3) / 4 * 4, p.splits = 1, p.kind = kTile128;
+    const int64_t size = static_cast<int64_t>(dtype_size(dtype)), bk = kRowBytes / size, steps = std::max<int64_t>((K + bk - 1) / bk, 1);
+    p.k_part = steps * bk;
+    if (M <= 0 || N <= 0) return p;
+    const int64_t few = std::min(M, N), many = std::max(M, N);
+    int64_t splits = 1;
+    if (rr && few <= 64) {
+        p.kind = few <= 16 ? kFew16 : few <= 32 ? kFew32 : kFew64;
+        splits = std::max<int64_t>(1, std::min<int64_t>(2048 / ((many + 15) / 16), K / 512));
+        p.k_part = (steps + splits - 1) / splits * bk;
+    } else {
+        double best = 1e30;
+        for (const int tile : {128, 256}) {
+            const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+            const double step = size == 2 ? (tile == 256 ? 1.7 : 0.6) : (tile == 256 ? 7.5 : 2.0), around = tile == 256 ? 5.0 : 2.0;
+            for (int64_t c = 1; c <= std::min<int64_t>(64, steps); ++c) {
+                const int64_t each = (steps + c - 1) / c, n = (steps + each - 1) / each;
+                if (size == 4 && each * bk > 4096 && c < std::min<int64_t>(64, steps)) continue;
+                if (c > 1 && each < 4 && !(size == 4 && K > 4096)) break;
+                const double cost = static_cast<double>((tiles * n + 255) / 256) * (static_cast<double>(each) * step + around) +
+                                    (n > 1 ? 5.0 + static_cast<double>(n * M * N) * 8e-6 / 4.0 : 0.0);
+                if (cost < best) best = cost, p.kind = tile == 256 ? kTile256 : kTile128, p.k_part = each * bk;
+            }
+        }
+    }
     p.splits = static_cast<int32_t>((steps * bk + p.k_part - 1) / p.k_part);
-    p.part_ld = (N + 3) / 4 * 4;
-    p.rows = M;
     return p;
 }
 
@@ -663,22 +752,43 @@ bool aligned(const void *p, int64_t ld, int64_t along, int64_t rows) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % v == 0 && along % v == 0 && (ld * rows + along) * static_cast<int64_t>(sizeof(T)) < (int64_t(1) << 32);
 }
 
+template <typename T, int TILE, int WM, int WN, bool PCOL, bool QCOL>
+bool launch_tile(GemmArgs &a, hipStream_t s) {
+    a.tiles_m = ceil_div(a.M, TILE), a.tiles_n = ceil_div(a.N, TILE);
+    const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits));
+    if (!(a.K > 0 && aligned<T>(a.p, a.p_ld, PCOL ? a.M : a.K, PCOL ? a.k_part : TILE) &&
+          aligned<T>(a.q, a.q_ld, QCOL ? a.N : a.K, QCOL ? a.k_part : TILE)))
+        return false;
+    hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL>), grid, dim3(WM * WN * kWave), 0, s, a);
+    return true;
+}
+
+template <typename T, int MT>
+void launch_few(GemmArgs &a, hipStream_t s) {
+    const bool nfew = a.N < a.M;
+    a.tiles_m = ceil_div(a.M, 16), a.tiles_n = ceil_div(a.N, 16);
+    const dim3 grid(static_cast<unsigned>((nfew ? a.tiles_m : a.tiles_n) * a.splits));
+    if (nfew) hipLaunchKernelGGL((k_few<T, MT, true>), grid, dim3(kBlock), 0, s, a);
+    else hipLaunchKernelGGL((k_few<T, MT, false>), grid, dim3(kBlock), 0, s, a);
+}
+
 template <typename T, bool PCOL, bool QCOL>
 int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return GLIF_OK;
     a.splits = p.splits, a.k_part = p.k_part, a.part_ld = p.part_ld, a.part = part;
-    a.tiles_m = ceil_div(a.M, kBM), a.tiles_n = ceil_div(a.N, kBN);
-    const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits));
-    if (a.K > 0 && aligned<T>(a.p, a.p_ld, PCOL ? a.M : a.K, PCOL ? a.k_part : kBM) &&
-        aligned<T>(a.q, a.q_ld, QCOL ? a.N : a.K, QCOL ? a.k_part : kBN)) {
-        hipLaunchKernelGGL((k_gemm_direct<T, kBM, kBN, GWM, GWN, PCOL, QCOL>), grid, dim3(GWM * GWN * 64), 0, s, a);
-    } else {
-        auto fn = k_gemm<T, kBM, kBN, 2, 4, PCOL, QCOL>;
-        constexpr int bytes = 2 * (kBM + kBN) * kRowBytes;
-        static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        GLIF_HIP(set);
-        hipLaunchKernelGGL(fn, grid, dim3(512), bytes, s, a);
+    bool done = false;
+    if constexpr (!PCOL && !QCOL) {
+        done = true;
+        if (p.kind == kFew16) launch_few<T, 1>(a, s);
+        else if (p.kind == kFew32) launch_few<T, 2>(a, s);
+        else if (p.kind == kFew64) launch_few<T, 4>(a, s);
+        else done = false;
     }
+    if (!done && p.kind == kTile256) done = launch_tile<T, 256, 2, 4, PCOL, QCOL>(a, s);
+    if (!done) done = launch_tile<T, 128, 2, 2, PCOL, QCOL>(a, s);
+    if (!done)
+        hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2, PCOL, QCOL>), dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)),
+                           dim3(kBlock), 0, s, a);
     if (a.splits > 1) {
         const int64_t n4 = a.M * (a.part_ld / 4);
         hipLaunchKernelGGL(k_gemm_join<T>, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))), dim3(kBlock),
@@ -721,7 +831,7 @@ struct Back {
 
 void carve(Carver &c, Back &b, int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act) {
     b.parts = row_parts(M);
-    b.dx = plan_for(dtype, M, K, N), b.dw = plan_for(dtype, N, K, M);
+    b.dx = plan_for(dtype, M, K, N, false), b.dw = plan_for(dtype, N, K, M, false);
     b.sums = c.take<float>(static_cast<size_t>(b.parts * N));
     b.part = c.take<float>(std::max(b.dx.floats(), b.dw.floats()));
     b.dp = act != GLIF_ACT_NONE ? c.take<char>(static_cast<size_t>(M * N) * dtype_size(dtype)) : nullptr;
@@ -737,7 +847,7 @@ extern "C" {
 size_t glif_linear_fwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K) {
     if (check_linear(dtype, dtype, M, N, K, 0)) return 0;
     Carver c(nullptr, 0);
-    if (const size_t n = plan_for(dtype, M, N, K).floats()) c.take<float>(n);
+    if (const size_t n = plan_for(dtype, M, N, K, true).floats()) c.take<float>(n);
     return c.off;
 }
 
@@ -750,7 +860,7 @@ int glif_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw,
     GemmArgs a{};
     a.p = x, a.p_ld = ldx, a.q = weight, a.q_ld = ldw, a.M = M, a.N = N, a.K = K;
     a.c = y, a.pre = pre, a.bias = bias, a.residual = residual, a.ldr = ldr, a.bias_dt = bias_dtype, a.act = activation;
-    const Plan p = plan_for(dtype, M, N, K);
+    const Plan p = plan_for(dtype, M, N, K, true);
     Carver c(ws, ws_bytes);
     float *part = c.take<float>(p.floats());
     if (!c.ok() || (p.floats() && !ws)) return fail(GLIF_ENOMEM, "linear: workspace too small");
