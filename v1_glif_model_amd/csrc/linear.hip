@@ -383,7 +383,7 @@ struct Direct {
     uint32_t off[kN], at_k;        // of the lane's pieces in a tile, and of the next tile
     uint32_t ld;                   // bytes
 
-    static __device__ __forceinline__ int col_key(int k) { return kSize == 2 ? (k & 3) | ((k >> 1) & 4) : (k >> 2) & 3; }
+    static __device__ __forceinline__ int col_key(int k) { return (kSize == 2 ? (k & 3) | ((k >> 1) & 4) : (k >> 2) & 3) & (ROWS / 16 - 1); }
 
     // what lands at lane's place of instruction i: COL (row k, byte of it), else (row, chunk)
     static __device__ __forceinline__ void place(int wave, int lane, int i, int &row, int &at) {
@@ -441,7 +441,7 @@ struct Direct {
         }
     }
 
-    // A wave's reads: fragment i, rows w + 16 i .. (w a multiple of 64), of matrix instruction kk of the tile.  What depends on
+    // A wave's reads: fragment i, rows w + 16 i .., of matrix instruction kk of the tile.  What depends on
     // the lane is one of a few offsets (the permutation is an exclusive or of a lane's part and of i's and kk's).
     static constexpr int kReads = !COL ? 1 : kSize == 2 ? 2 : 4;   // LDS reads of a fragment
     static constexpr int kAts = !COL ? 2 : kSize == 2 ? 8 : 4;
@@ -504,7 +504,6 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
     Q q;
     p.init(a.p, a.p_ld, m0, a.M, k0, wave, lane);
     q.init(a.q, a.q_ld, n0, a.N, k0, wave, lane);
-    static_assert(TM % 64 == 0 && TN % 64 == 0, "a wave's rows");
     const typename P::Reader rp(wm, r16, kq);
     const typename Q::Reader rq(wn, r16, kq);
     f32x4 acc[FM][FN] = {};
@@ -649,17 +648,25 @@ __global__ void __launch_bounds__(kBlock) k_few(GemmArgs a) {
     }
 }
 
-// The splits' sums, in order, and the epilogue.
-template <typename T>
+// The splits' sums and the epilogue: four results by G lanes, which take the splits in turn (their sums are joined by a fixed
+// tree).
+template <typename T, int G>
 __global__ void __launch_bounds__(kBlock) k_gemm_join(GemmArgs a) {
-    const int64_t quads = a.part_ld / 4, n4 = a.M * quads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < n4; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t quads = a.part_ld / 4, n4 = a.M * quads, step = static_cast<int64_t>(gridDim.x) * (kBlock / G);
+    const int g = threadIdx.x % G;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kBlock / G) + threadIdx.x / G; i < n4; i += step) {
         const int64_t m = i / quads, n = (i - m * quads) * 4;
         const Finish<T> finish(a, n);
         const typename Finish<T>::vec res = finish.residual(a, m);
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4 *>(a.part + (s * a.M + m) * a.part_ld + n);
-        finish(a, m, v, res);
+        const float *p = a.part + (g * a.M + m) * a.part_ld + n;
+#pragma unroll 4
+        for (int s = g; s < a.splits; s += G, p += G * a.M * a.part_ld) v += *reinterpret_cast<const f32x4 *>(p);
+#pragma unroll
+        for (int x = 1; x < G; x <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], x, kWave);
+        if (g == 0) finish(a, m, v, res);
     }
 }
 
@@ -697,7 +704,7 @@ __global__ void __launch_bounds__(kBlock) k_bias_join(const float *part, int par
 }
 
 // How a product is cut up: the tile, and the parts of k whose sums are added afterwards.
-enum Kind { kFew16, kFew32, kFew64, kTile128, kTile256 };
+enum Kind { kFew16, kFew32, kFew64, kTile64, kTile128, kTile256 };
 struct Plan {
     Kind kind;
     int32_t splits;
@@ -710,10 +717,11 @@ struct Plan {
 // At most 64 rows on one side: k is split until the chip has about eight waves a SIMD to keep the stream of the other side
 // going, but no part under 512 k's.
 //
-// Otherwise the cheapest of both tiles and some splits, by what a step (128 bytes of k) of a tile costs a compute unit and
-// what goes on around the steps, in us: 16-bit 256 x 256 1.7 + 5, 128 x 128 0.6 + 2; float32, whose products run at 1/16,
-// 7.5 + 5 and 2.0 + 2; a split costs its sums' way to memory and back and the launch that adds them.  A float32 sum runs over
-// at most 4096 k's, so that long ones do not lose their last digits.
+// Otherwise the cheapest of the tiles and some splits, by what a step (128 bytes of k) of a tile costs a compute unit and
+// what goes on around the steps, in us (measured over full chips): 16-bit 256 x 256 1.9 + 5, 128 x 128 0.67 + 2, 64 x 64
+// 0.25 + 1; float32, whose products run at 1/16, 128 x 128 2.1 + 2, 64 x 64 0.55 + 1 (larger tiles save traffic that is not
+// its bound); a split costs its sums' way to memory and back and the launch that adds them.  A float32 sum runs over at most
+// 4096 k's, so that long ones do not lose their last digits.
 Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
     Plan p{};
     p.rows = M, p.part_ld = (N + 3) / 4 * 4, p.splits = 1, p.kind = kTile128;
@@ -728,16 +736,18 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
         p.k_part = (steps + splits - 1) / splits * bk;
     } else {
         double best = 1e30;
-        for (const int tile : {128, 256}) {
+        for (const int tile : {64, 128, 256}) {
+            if (size == 4 && tile == 256) continue;
             const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
-            const double step = size == 2 ? (tile == 256 ? 1.7 : 0.6) : (tile == 256 ? 7.5 : 2.0), around = tile == 256 ? 5.0 : 2.0;
+            const double step = size == 2 ? (tile == 256 ? 1.9 : tile == 128 ? 0.67 : 0.25) : (tile == 128 ? 2.1 : 0.55);
+            const double around = tile == 256 ? 5.0 : tile == 128 ? 2.0 : 1.0;
             for (int64_t c = 1; c <= std::min<int64_t>(64, steps); ++c) {
                 const int64_t each = (steps + c - 1) / c, n = (steps + each - 1) / each;
                 if (size == 4 && each * bk > 4096 && c < std::min<int64_t>(64, steps)) continue;
                 if (c > 1 && each < 4 && !(size == 4 && K > 4096)) break;
                 const double cost = static_cast<double>((tiles * n + 255) / 256) * (static_cast<double>(each) * step + around) +
                                     (n > 1 ? 5.0 + static_cast<double>(n * M * N) * 8e-6 / 4.0 : 0.0);
-                if (cost < best) best = cost, p.kind = tile == 256 ? kTile256 : kTile128, p.k_part = each * bk;
+                if (cost < best) best = cost, p.kind = tile == 256 ? kTile256 : tile == 128 ? kTile128 : kTile64, p.k_part = each * bk;
             }
         }
     }
@@ -763,6 +773,12 @@ bool launch_tile(GemmArgs &a, hipStream_t s) {
     return true;
 }
 
+template <typename T, int TILE, int WM, int WN, bool PCOL, bool QCOL>
+void launch_staged(GemmArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((k_gemm<T, TILE, TILE, WM, WN, PCOL, QCOL>), dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)),
+                       dim3(WM * WN * kWave), 0, s, a);
+}
+
 template <typename T, int MT>
 void launch_few(GemmArgs &a, hipStream_t s) {
     const bool nfew = a.N < a.M;
@@ -784,15 +800,23 @@ int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
         else if (p.kind == kFew64) launch_few<T, 4>(a, s);
         else done = false;
     }
-    if (!done && p.kind == kTile256) done = launch_tile<T, 256, 2, 4, PCOL, QCOL>(a, s);
-    if (!done) done = launch_tile<T, 128, 2, 2, PCOL, QCOL>(a, s);
-    if (!done)
-        hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2, PCOL, QCOL>), dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)),
-                           dim3(kBlock), 0, s, a);
+    if constexpr (sizeof(T) == 2)
+        if (!done && p.kind == kTile256) done = launch_tile<T, 256, 2, 4, PCOL, QCOL>(a, s);
+    if (!done && p.kind == kTile64) {
+        done = launch_tile<T, 64, 2, 2, PCOL, QCOL>(a, s);
+        if (!done) launch_staged<T, 64, 2, 1, PCOL, QCOL>(a, s);
+    } else if (!done) {
+        done = launch_tile<T, 128, 2, 2, PCOL, QCOL>(a, s);
+        if (!done) launch_staged<T, 128, 2, 2, PCOL, QCOL>(a, s);
+    }
     if (a.splits > 1) {
+        // where the results alone do not fill the chip, lanes over the splits: 5 x 66000 x 512 in 64 parts 14 us -> 4
         const int64_t n4 = a.M * (a.part_ld / 4);
-        hipLaunchKernelGGL(k_gemm_join<T>, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))), dim3(kBlock),
-                           0, s, a);
+        if (n4 < 32768 && a.splits >= 16)
+            hipLaunchKernelGGL((k_gemm_join<T, 16>), dim3(static_cast<unsigned>(ceil_div(n4, kBlock / 16))), dim3(kBlock), 0, s, a);
+        else
+            hipLaunchKernelGGL((k_gemm_join<T, 1>), dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))),
+                               dim3(kBlock), 0, s, a);
     }
     return GLIF_OK;
 }
