@@ -15,6 +15,9 @@ struct GemmArgs {
     const void *p, *q;
     int64_t p_ld, q_ld;        // the stride that is not 1
     int64_t M, N, K;
+    // what can be read of an operand whose rows run along k (k_cols >= K) and of one of columns (p_rows >= M, q_rows >= N):
+    // more than there is where it is padded (with zeros)
+    int64_t k_cols, p_rows, q_rows;
     int64_t k_part;            // k's of a split
     int32_t tiles_m, tiles_n, splits;
     float *part;               // [splits][M][part_ld], where splits > 1
@@ -83,125 +86,48 @@ struct Mma<f32> {
 constexpr int kRowBytes = 128;
 
 __device__ __forceinline__ int lds_at(int row, int chunk) { return row * kRowBytes + (((chunk ^ (row >> 1)) & 7) << 4); }
-// The same for tiles that are written by rows 8 or 4 apart: those are told apart by bits 4 and 5 of the row.
-__device__ __forceinline__ int lds_at_turned(int row, int chunk) { return lds_at(row, chunk ^ ((row >> 4) & 3)); }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// Brings ROWS x 128 bytes of an operand from memory into LDS by way of registers, NT threads.  COL: k runs along the rows
-// of memory (m or n is contiguous), and the values are turned on their way: a thread takes 4 k's of 16 bytes of m.  Rows
-// past the operand's end repeat the last (their products are not written); k's past `k1` are 0.
-template <typename T, bool COL, int ROWS, int NT>
+// Brings ROWS x 128 bytes of an operand whose rows run along k from memory into LDS by way of registers, NT threads.  Rows
+// past the operand's end repeat the last (their products are not written); k's past the part's end are 0.
+template <typename T, int ROWS, int NT>
 struct Stage {
     static constexpr int kV = 16 / static_cast<int>(sizeof(T));   // values of a chunk
     static constexpr int kBK = 8 * kV;                            // k's of a tile
     static constexpr int kN = ROWS * 8 / NT;                      // chunks a thread takes
-    static_assert(ROWS * 8 % NT == 0 && (!COL || kN % 4 == 0), "the tile does not divide among the threads");
+    static_assert(ROWS * 8 % NT == 0, "the tile does not divide among the threads");
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
     vec r[kN];
-    const T *at[COL ? kN / 4 : kN];
-    int64_t ld;
+    const T *at[kN];
 
-    // the place of unit i: COL (first row, first k), else (row, chunk)
-    static __device__ __forceinline__ void place(int i, int &row, int &k) {
-        const int u = threadIdx.x + i * NT;
-        if (!COL) {
-            row = u >> 3, k = u & 7;
-        } else if (sizeof(T) == 2) {   // 8 rows x 4 k's; neighbours take the two halves of a chunk
-            row = (u >> 1) % (ROWS / 8) * 8, k = (u >> 1) / (ROWS / 8) * 8 + (u & 1) * 4;
-        } else {                       // 4 rows x 4 k's
-            row = u % (ROWS / 4) * 4, k = u / (ROWS / 4) * 4;
+    __device__ __forceinline__ void init(const T *p, int64_t ld, int64_t row0, int64_t rows, int64_t k0) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int u = threadIdx.x + i * NT;
+            at[i] = p + min(row0 + (u >> 3), rows - 1) * ld + k0 + (u & 7) * kV;
         }
     }
-
-    __device__ __forceinline__ void init(const T *p, int64_t stride, int64_t row0, int64_t rows, int64_t k0) {
-        ld = stride;
-        int row, k;
-        if (!COL) {
+    // left: the k's from the tile's first one on
+    __device__ __forceinline__ void load(int64_t left) {
+        if (left >= kBK) {
 #pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                place(i, row, k);
-                at[i] = p + min(row0 + row, rows - 1) * ld + k0 + k * kV;
-            }
+            for (int i = 0; i < kN; ++i) r[i] = *reinterpret_cast<const vec *>(at[i]);
         } else {
+            const int have = static_cast<int>(left) - (threadIdx.x & 7) * kV;
 #pragma unroll
-            for (int i = 0; i < kN / 4; ++i) {
-                place(i, row, k);
-                at[i] = p + (k0 + k) * ld + row0 + row;
-            }
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int e = 0; e < kV; ++e) r[i][e] = e < have ? at[i][e] : T(0.0f);
         }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) at[i] += kBK;
     }
-
-    // k0: the tile's first k; left = k1 - k0, what there is of it
-    __device__ __forceinline__ void load(int64_t row0, int64_t rows, int64_t left) {
-        int row, k;
-        if (!COL) {
-            if (left >= kBK) {
-#pragma unroll
-                for (int i = 0; i < kN; ++i) r[i] = *reinterpret_cast<const vec *>(at[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    place(i, row, k);
-#pragma unroll
-                    for (int e = 0; e < kV; ++e) r[i][e] = k * kV + e < left ? at[i][e] : T(0.0f);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kN; ++i) at[i] += kBK;
-        } else {
-#pragma unroll
-            for (int i = 0; i < kN / 4; ++i) {
-                place(i, row, k);
-                const int64_t have = rows - row0 - row;   // rows of the operand from this one on
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (k + j < left && have >= kV) {
-                        r[4 * i + j] = *reinterpret_cast<const vec *>(at[i] + j * ld);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < kV; ++e) r[4 * i + j][e] = k + j < left && e < have ? at[i][j * ld + e] : T(0.0f);
-                    }
-                }
-                at[i] += kBK * ld;
-            }
-        }
-    }
-
     __device__ __forceinline__ void store(char *lds) const {
-        int row, k;
-        if (!COL) {
 #pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                place(i, row, k);
-                *reinterpret_cast<u32x4 *>(lds + lds_at_turned(row, k)) = __builtin_bit_cast(u32x4, r[i]);
-            }
-        } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < kN / 4; ++i) {
-                place(i, row, k);
-                u32x4 w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(u32x4, r[4 * i + j]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {   // row + e: its values of k .. k + 3
-                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                    const u32x2 v = {__builtin_amdgcn_perm(w[1][e / 2], w[0][e / 2], sel),
-                                     __builtin_amdgcn_perm(w[3][e / 2], w[2][e / 2], sel)};
-                    *reinterpret_cast<u32x2 *>(lds + lds_at_turned(row + e, k >> 3) + (k & 4) * 2) = v;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kN / 4; ++i) {
-                place(i, row, k);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const vec v = {r[4 * i][e], r[4 * i + 1][e], r[4 * i + 2][e], r[4 * i + 3][e]};
-                    *reinterpret_cast<u32x4 *>(lds + lds_at_turned(row + e, k >> 2)) = __builtin_bit_cast(u32x4, v);
-                }
-            }
+        for (int i = 0; i < kN; ++i) {
+            const int u = threadIdx.x + i * NT;
+            *reinterpret_cast<u32x4 *>(lds + lds_at(u >> 3, u & 7)) = __builtin_bit_cast(u32x4, r[i]);
         }
     }
 };
@@ -306,13 +232,13 @@ __device__ __forceinline__ void my_tile(const GemmArgs &a, int &tm, int &tn, int
     tn = a.tiles_m <= a.tiles_n ? tile / a.tiles_m : tile % a.tiles_n;
 }
 
-// BM x BN of C by WM x WN waves, of k in [split's part).  Two tiles of each operand in LDS: while one is multiplied, the
-// next comes into registers, and from there into the other.
-template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL>
+// BM x BN of C by WM x WN waves, of k in the split's part, for operands of 16-bit rows of k that start anywhere.  Two tiles of
+// each operand in LDS: while one is multiplied, the next comes into registers, and from there into the other.
+template <typename T, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
     using M = Mma<T>;
     constexpr int NT = WM * WN * kWave, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-    constexpr int BK = Stage<T, false, BM, NT>::kBK, kTile = (BM + BN) * kRowBytes;
+    constexpr int BK = Stage<T, BM, NT>::kBK, kTile = (BM + BN) * kRowBytes;
     __shared__ __attribute__((aligned(16))) char lds[2 * kTile];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16;
     const int wm = wave / WN * TM, wn = wave % WN * TN;
@@ -320,15 +246,15 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
     my_tile(a, tm, tn, split);
     const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
     const int64_t k0 = split * a.k_part, k1 = min(a.K, k0 + a.k_part);
-    Stage<T, PCOL, BM, NT> sp;
-    Stage<T, QCOL, BN, NT> sq;
+    Stage<T, BM, NT> sp;
+    Stage<T, BN, NT> sq;
     sp.init(static_cast<const T *>(a.p), a.p_ld, m0, a.M, k0);
     sq.init(static_cast<const T *>(a.q), a.q_ld, n0, a.N, k0);
     f32x4 acc[FM][FN] = {};
     const int steps = static_cast<int>((k1 - k0 + BK - 1) / BK);
     if (steps > 0) {
-        sp.load(m0, a.M, k1 - k0);
-        sq.load(n0, a.N, k1 - k0);
+        sp.load(k1 - k0);
+        sq.load(k1 - k0);
         sp.store(lds);
         sq.store(lds + BM * kRowBytes);
         __syncthreads();
@@ -338,18 +264,18 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
         const bool more = s + 1 < steps;
         if (more) {
             const int64_t left = k1 - k0 - static_cast<int64_t>(s + 1) * BK;
-            sp.load(m0, a.M, left);
-            sq.load(n0, a.N, left);
+            sp.load(left);
+            sq.load(left);
         }
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             typename M::frag fp[FM], fq[FN];
 #pragma unroll
             for (int i = 0; i < FM; ++i)
-                fp[i] = *reinterpret_cast<const typename M::frag *>(cur + lds_at_turned(wm + 16 * i + r16, 4 * kk + kq));
+                fp[i] = *reinterpret_cast<const typename M::frag *>(cur + lds_at(wm + 16 * i + r16, 4 * kk + kq));
 #pragma unroll
             for (int j = 0; j < FN; ++j)
-                fq[j] = *reinterpret_cast<const typename M::frag *>(cur + BM * kRowBytes + lds_at_turned(wn + 16 * j + r16, 4 * kk + kq));
+                fq[j] = *reinterpret_cast<const typename M::frag *>(cur + BM * kRowBytes + lds_at(wn + 16 * j + r16, 4 * kk + kq));
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -367,46 +293,47 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
 
 #ifdef __HIP_DEVICE_COMPILE__   // the host's pass does not know the builtins
 // ---- operands straight into LDS ---------------------------------------------------------------------------------------
-// Memory to LDS without registers, 1 KB (64 x 16 bytes) of consecutive LDS a wave and instruction; the permutation of the
-// chunks is in the addresses that are read.  COL operands lie in LDS as they do in memory, rows of k, and are turned where
-// they are read: 16-bit types by the LDS transpose read (16 lanes take 4 k's of 16 m's), float32 by reading single values.
-// There the 16-m pieces of row k are permuted by those bits of k in which the rows of one read differ.
-// For 16-byte aligned rows only; K (of rows of k: M or N) counts in whole chunks, and a block's part of an operand in 32 bits.
+// Memory to LDS without registers, 64 x PB bytes of consecutive LDS a wave and instruction; the permutation of the chunks is
+// in the addresses that are read.  COL operands lie in LDS as they do in memory, rows of k, and are turned where they are
+// read: 16-bit types by the LDS transpose read (16 lanes take 4 k's of 16 m's), float32 by reading single values.  There the
+// 16-m pieces of row k are permuted by those bits of k in which the rows of one read differ.
+// PB 16 is for rows on 16-byte addresses and of whole chunks, PB 4 for rows on 4-byte ones; a tile of an operand lies within
+// 32 bits.
 constexpr int kRawBuffer = 0x00020000;   // descriptor word 3: untyped 32-bit offsets
-template <typename T, bool COL, int ROWS, int WAVES>
+template <typename T, bool COL, int ROWS, int WAVES, int PB>
 struct Direct {
-    static constexpr int kSize = static_cast<int>(sizeof(T)), kV = 16 / kSize, kBK = 8 * kV;
-    static constexpr int kN = ROWS * kRowBytes / 1024 / WAVES;    // instructions of a wave
+    static constexpr int kSize = static_cast<int>(sizeof(T)), kBK = kRowBytes / kSize;
+    static constexpr int kLoad = kWave * PB, kN = ROWS * kRowBytes / kLoad / WAVES;    // bytes of an instruction, those of a wave
     static constexpr int kColBytes = ROWS * kSize, kPiece = 16 * kSize;
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
-    __amdgpu_buffer_rsrc_t rsrc;   // from the first value of the block's rows and k's
-    uint32_t off[kN], at_k;        // of the lane's pieces in a tile, and of the next tile
+    const char *base;              // the next tile's first value, uniform
+    uint32_t off[kN];              // of the lane's pieces in a tile
     uint32_t ld;                   // bytes
+    int range;                     // of the addresses a load may touch: all, or none
 
     static __device__ __forceinline__ int col_key(int k) { return (kSize == 2 ? (k & 3) | ((k >> 1) & 4) : (k >> 2) & 3) & (ROWS / 16 - 1); }
 
-    // what lands at lane's place of instruction i: COL (row k, byte of it), else (row, chunk)
+    // what lands at lane's place of instruction i: COL (row k, byte of it), else (row, byte of its k's)
     static __device__ __forceinline__ void place(int wave, int lane, int i, int &row, int &at) {
-        const int byte = (wave * kN + i) * 1024 + lane * 16;
+        const int byte = (wave * kN + i) * kLoad + lane * PB;
         if (COL) {
             row = byte / kColBytes, at = byte % kColBytes;
             at = (at / kPiece ^ col_key(row)) * kPiece + at % kPiece;
         } else {
-            row = byte / kRowBytes, at = (byte / 16 ^ (row >> 1)) & 7;
+            row = byte / kRowBytes, at = ((byte / 16 ^ (row >> 1)) & 7) * 16 + byte % 16;
         }
     }
 
     __device__ __forceinline__ void init(const void *p, int64_t stride, int64_t row0, int64_t rows, int64_t k0, int wave, int lane) {
         ld = static_cast<uint32_t>(stride * kSize);
-        const char *base = static_cast<const char *>(p) + (COL ? k0 * stride + row0 : row0 * stride + k0) * kSize;
-        rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, -1, kRawBuffer);
-        at_k = 0;
+        base = static_cast<const char *>(p) + (COL ? k0 * stride + row0 : row0 * stride + k0) * kSize;
+        range = -1;
         const int have = static_cast<int>(min(rows - row0, static_cast<int64_t>(ROWS)));
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             int r, at;
             place(wave, lane, i, r, at);
-            off[i] = COL ? r * ld + min(at, have * kSize - 16) : min(r, have - 1) * ld + at * 16;
+            off[i] = COL ? r * ld + min(at, have * kSize - PB) : min(r, have - 1) * ld + at;
         }
     }
 
@@ -418,26 +345,27 @@ struct Direct {
             int r, at;
             place(wave, lane, i, r, at);
             if (COL && r >= left) off[i] -= r * ld;
-            if (!COL && at * kV >= left) off[i] -= at * 16;
+            if (!COL && at >= left * kSize) off[i] -= at;
         }
     }
 
     // Every further load is of an empty range.
-    __device__ __forceinline__ void stop() { rsrc = __builtin_amdgcn_make_buffer_rsrc(nullptr, 0, 0, kRawBuffer); }
+    __device__ __forceinline__ void stop() { range = 0; }
 
     __device__ __forceinline__ void load(char *lds, int wave) {
         typedef __attribute__((address_space(3))) void *lptr;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, range, kRawBuffer);
 #pragma unroll
         for (int i = 0; i < kN; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr)(lds + (wave * kN + i) * 1024), 16, off[i], at_k, 0, 0);
-        at_k += COL ? kBK * ld : kRowBytes;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr)(lds + (wave * kN + i) * kLoad), PB, off[i], 0, 0, 0);
+        base += COL ? static_cast<int64_t>(kBK) * ld : kRowBytes;
     }
 
     static __device__ __forceinline__ void clear(char *lds, int left) {
-        for (int u = threadIdx.x; u < ROWS * 8; u += WAVES * kWave) {
-            const int row = COL ? u * 16 / kColBytes : u >> 3;
-            if (COL ? row >= left : (u & 7) * kV >= left)
-                *reinterpret_cast<u32x4 *>(lds + (COL ? u * 16 : lds_at(row, u & 7))) = u32x4{0u, 0u, 0u, 0u};
+        for (int u = threadIdx.x; u < ROWS * kRowBytes / 4; u += WAVES * kWave) {
+            const int row = COL ? u * 4 / kColBytes : u / 32, at = u * 4 % kRowBytes;
+            if (COL ? row >= left : at >= left * kSize)
+                *reinterpret_cast<uint32_t *>(lds + (COL ? u * 4 : lds_at(row, at / 16) + at % 16)) = 0u;
         }
     }
 
@@ -482,13 +410,13 @@ struct Direct {
 // BM x BN of C by WM x WN waves, of k in the split's part.  Two tiles of each operand in LDS; the second half of a tile's
 // operands is in registers before the barrier at which the tile's LDS is given to the loads of the tile after next, and the
 // first half of the next tile's is read while that second half is multiplied.
-template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL>
+template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL, int PB>
 __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
 #ifdef __HIP_DEVICE_COMPILE__
     using M = Mma<T>;
     constexpr int W = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-    using P = Direct<T, PCOL, BM, W>;
-    using Q = Direct<T, QCOL, BN, W>;
+    using P = Direct<T, PCOL, BM, W, PB>;
+    using Q = Direct<T, QCOL, BN, W, PB>;
     constexpr int BK = P::kBK, kQAt = BM * kRowBytes, kTile = (BM + BN) * kRowBytes;
     __shared__ __attribute__((aligned(1024))) char lds0[kTile];
     __shared__ __attribute__((aligned(1024))) char lds1[kTile];
@@ -502,8 +430,8 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
     const int tail = static_cast<int>(k1 - k0 - static_cast<int64_t>(steps - 1) * BK);   // k's of the last tile
     P p;
     Q q;
-    p.init(a.p, a.p_ld, m0, a.M, k0, wave, lane);
-    q.init(a.q, a.q_ld, n0, a.N, k0, wave, lane);
+    p.init(a.p, a.p_ld, m0, a.p_rows, k0, wave, lane);
+    q.init(a.q, a.q_ld, n0, a.q_rows, k0, wave, lane);
     const typename P::Reader rp(wm, r16, kq);
     const typename Q::Reader rq(wn, r16, kq);
     f32x4 acc[FM][FN] = {};
@@ -587,7 +515,7 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
 template <typename T, int MT, bool NFEW>
 __global__ void __launch_bounds__(kBlock) k_few(GemmArgs a) {
     using M = Mma<T>;
-    constexpr int kV = 16 / static_cast<int>(sizeof(T)), KS = 4 * kV, U = MT == 4 ? 2 : 4, kWaves = kBlock / kWave;
+    constexpr int kV = 16 / static_cast<int>(sizeof(T)), KS = 4 * kV, U = 4, kWaves = kBlock / kWave;
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
     __shared__ f32x4 sums[kWaves][MT][kWave];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16;
@@ -673,26 +601,48 @@ __global__ void __launch_bounds__(kBlock) k_gemm_join(GemmArgs a) {
 struct SlopeArgs {
     const void *dy, *pre;
     int64_t lddy, M, N;
-    void *dp;            // [M][N] or NULL
+    void *dp;            // [M][lddp] or NULL
+    int64_t lddp;
     float *part;         // [parts][N] or NULL
     int32_t act, parts;
 };
 
-// dp = dy act'(pre), rounded to the activations' type for the products, and the column sums of the unrounded values over a
-// chunk of rows.
+// dp = dy act'(pre), rounded to the activations' type for the products (zeros past N), and the column sums of the unrounded
+// values over a chunk of rows.
 template <typename T>
 __global__ void __launch_bounds__(kBlock) k_slope(SlopeArgs a) {
     const int64_t n = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-    if (n >= a.N) return;
+    if (n >= (a.dp ? a.lddp : a.N)) return;
     const int64_t r0 = a.M * blockIdx.y / a.parts, r1 = a.M * (blockIdx.y + 1) / a.parts;
     float s = 0.0f;
     for (int64_t m = r0; m < r1; ++m) {
-        float g = to_f32(static_cast<const T *>(a.dy)[m * a.lddy + n]);
-        if (a.act != GLIF_ACT_NONE) g *= slope_of(to_f32(static_cast<const T *>(a.pre)[m * a.N + n]), a.act);
-        if (a.dp) static_cast<T *>(a.dp)[m * a.N + n] = from_f32<T>(g);
+        float g = 0.0f;
+        if (n < a.N) {
+            g = to_f32(static_cast<const T *>(a.dy)[m * a.lddy + n]);
+            if (a.act != GLIF_ACT_NONE) g *= slope_of(to_f32(static_cast<const T *>(a.pre)[m * a.N + n]), a.act);
+        }
+        if (a.dp) static_cast<T *>(a.dp)[m * a.lddp + n] = from_f32<T>(g);
         s += g;
     }
-    if (a.part) a.part[static_cast<int64_t>(blockIdx.y) * a.N + n] = s;
+    if (a.part && n < a.N) a.part[static_cast<int64_t>(blockIdx.y) * a.N + n] = s;
+}
+
+// 16-bit rows onto 16-byte addresses: out [rows][ldo], ldo a multiple of 8, zeros past cols.
+__global__ void __launch_bounds__(kBlock) k_repack(const uint16_t *in, int64_t ld, int64_t rows, int64_t cols, uint16_t *out, int64_t ldo) {
+    typedef Vec<uint16_t, 8> vec;
+    const int64_t per = ldo / 8, n = rows * per;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+        const int64_t r = i / per, c = (i - r * per) * 8;
+        const uint16_t *p = in + r * ld + c;
+        vec v;
+        if (c + 8 <= cols) {
+            v = *reinterpret_cast<const vec *>(p);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[e] : 0;
+        }
+        *reinterpret_cast<vec *>(out + i * 8) = v;
+    }
 }
 
 __global__ void __launch_bounds__(kBlock) k_bias_join(const float *part, int parts, int64_t N, void *dbias, int32_t dt) {
@@ -704,7 +654,7 @@ __global__ void __launch_bounds__(kBlock) k_bias_join(const float *part, int par
 }
 
 // How a product is cut up: the tile, and the parts of k whose sums are added afterwards.
-enum Kind { kFew16, kFew32, kFew64, kTile64, kTile128, kTile256 };
+enum Kind { kFew16, kFew32, kTile64, kTile128, kTile256 };
 struct Plan {
     Kind kind;
     int32_t splits;
@@ -714,14 +664,14 @@ struct Plan {
 
 // rr: both operands have k along their rows.
 //
-// At most 64 rows on one side: k is split until the chip has about eight waves a SIMD to keep the stream of the other side
-// going, but no part under 512 k's.
+// At most 32 rows on one side: k is split until the chip has about eight waves a SIMD to keep the stream of the other side
+// going, but no part under 512 k's.  (40 rows by this kernel: 16000 x 4096 x 40 59 us, by 64 x 64 tiles 30.)
 //
-// Otherwise the cheapest of the tiles and some splits, by what a step (128 bytes of k) of a tile costs a compute unit and
-// what goes on around the steps, in us (measured over full chips): 16-bit 256 x 256 1.9 + 5, 128 x 128 0.67 + 2, 64 x 64
-// 0.25 + 1; float32, whose products run at 1/16, 128 x 128 2.1 + 2, 64 x 64 0.55 + 1 (larger tiles save traffic that is not
-// its bound); a split costs its sums' way to memory and back and the launch that adds them.  A float32 sum runs over at most
-// 4096 k's, so that long ones do not lose their last digits.
+// Otherwise the cheapest of the tiles and some splits.  A step (128 bytes of k) of a block that is alone on its compute unit
+// takes, in us, 16-bit 256 x 256 1.7, 128 x 128 1.0, 64 x 64 0.5, and float32, whose products run at 1/16, 128 x 128 3.0, 64
+// x 64 1.1; a step of all of the 1, 2 or 5 blocks that a compute unit holds 1.9, 1.35, 1.2, and 4.3, 2.9 (measured over
+// sweeps of tiles and splits at 15 shapes).  Around the steps go 10, 5 and 3; a split costs its sums' way to memory and back
+// and the launch that adds them.  A float32 sum runs over at most 4096 k's, so that long ones do not lose their last digits.
 Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
     Plan p{};
     p.rows = M, p.part_ld = (N + 3) / 4 * 4, p.splits = 1, p.kind = kTile128;
@@ -730,8 +680,8 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
     if (M <= 0 || N <= 0) return p;
     const int64_t few = std::min(M, N), many = std::max(M, N);
     int64_t splits = 1;
-    if (rr && few <= 64) {
-        p.kind = few <= 16 ? kFew16 : few <= 32 ? kFew32 : kFew64;
+    if (rr && few <= 32) {
+        p.kind = few <= 16 ? kFew16 : kFew32;
         splits = std::max<int64_t>(1, std::min<int64_t>(2048 / ((many + 15) / 16), K / 512));
         p.k_part = (steps + splits - 1) / splits * bk;
     } else {
@@ -739,14 +689,18 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
         for (const int tile : {64, 128, 256}) {
             if (size == 4 && tile == 256) continue;
             const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
-            const double step = size == 2 ? (tile == 256 ? 1.9 : tile == 128 ? 0.67 : 0.25) : (tile == 128 ? 2.1 : 0.55);
-            const double around = tile == 256 ? 5.0 : tile == 128 ? 2.0 : 1.0;
+            const int64_t cap = tile == 256 ? 1 : tile == 128 ? 2 : 5;
+            const double alone = size == 2 ? (tile == 256 ? 1.7 : tile == 128 ? 1.0 : 0.5) : (tile == 128 ? 3.0 : 1.1);
+            const double full = size == 2 ? (tile == 256 ? 1.9 : tile == 128 ? 1.35 : 1.2) : (tile == 128 ? 4.3 : 2.9);
+            const double around = tile == 256 ? 10.0 : tile == 128 ? 5.0 : 3.0;
             for (int64_t c = 1; c <= std::min<int64_t>(64, steps); ++c) {
                 const int64_t each = (steps + c - 1) / c, n = (steps + each - 1) / each;
                 if (size == 4 && each * bk > 4096 && c < std::min<int64_t>(64, steps)) continue;
                 if (c > 1 && each < 4 && !(size == 4 && K > 4096)) break;
-                const double cost = static_cast<double>((tiles * n + 255) / 256) * (static_cast<double>(each) * step + around) +
-                                    (n > 1 ? 5.0 + static_cast<double>(n * M * N) * 8e-6 / 4.0 : 0.0);
+                const int64_t unit = (tiles * n + 255) / 256, together = std::min(cap, unit);   // blocks of a compute unit
+                const double step = cap == 1 ? full : alone + (full - alone) * static_cast<double>(together - 1) / static_cast<double>(cap - 1);
+                const double cost = static_cast<double>(unit) / static_cast<double>(together) * (static_cast<double>(each) * step + around) +
+                                    (n > 1 ? 4.0 + static_cast<double>(n * M * N) * 8e-6 / 6.0 : 0.0);
                 if (cost < best) best = cost, p.kind = tile == 256 ? kTile256 : tile == 128 ? kTile128 : kTile64, p.k_part = each * bk;
             }
         }
@@ -755,28 +709,26 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
     return p;
 }
 
-// Whether an operand's rows can go to LDS directly: 16-byte pieces that lie on 16-byte addresses, 32-bit offsets in a tile.
-template <typename T>
-bool aligned(const void *p, int64_t ld, int64_t along, int64_t rows) {
-    const int64_t v = 16 / static_cast<int64_t>(sizeof(T));
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % v == 0 && along % v == 0 && (ld * rows + along) * static_cast<int64_t>(sizeof(T)) < (int64_t(1) << 32);
+// Whether an operand's rows lie in 16-byte pieces.
+bool on_16(const void *p, int64_t ld, int64_t along, size_t size) {
+    const int64_t v = 16 / static_cast<int64_t>(size);
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % v == 0 && along % v == 0;
 }
 
+// float32 rows may start on any float32; 16-bit rows of k that do not lie on 16 bytes come by way of registers (16-bit
+// operands of columns have been put on 16 bytes).
 template <typename T, int TILE, int WM, int WN, bool PCOL, bool QCOL>
-bool launch_tile(GemmArgs &a, hipStream_t s) {
+void launch_tile(GemmArgs &a, hipStream_t s) {
     a.tiles_m = ceil_div(a.M, TILE), a.tiles_n = ceil_div(a.N, TILE);
-    const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits));
-    if (!(a.K > 0 && aligned<T>(a.p, a.p_ld, PCOL ? a.M : a.K, PCOL ? a.k_part : TILE) &&
-          aligned<T>(a.q, a.q_ld, QCOL ? a.N : a.K, QCOL ? a.k_part : TILE)))
-        return false;
-    hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL>), grid, dim3(WM * WN * kWave), 0, s, a);
-    return true;
-}
-
-template <typename T, int TILE, int WM, int WN, bool PCOL, bool QCOL>
-void launch_staged(GemmArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((k_gemm<T, TILE, TILE, WM, WN, PCOL, QCOL>), dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)),
-                       dim3(WM * WN * kWave), 0, s, a);
+    const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)), block(WM * WN * kWave);
+    if (on_16(a.p, a.p_ld, PCOL ? a.p_rows : a.k_cols, sizeof(T)) && on_16(a.q, a.q_ld, QCOL ? a.q_rows : a.k_cols, sizeof(T))) {
+        hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL, 16>), grid, block, 0, s, a);
+    } else if constexpr (sizeof(T) == 4) {
+        hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL, 4>), grid, block, 0, s, a);
+    } else if constexpr (!PCOL && !QCOL) {
+        if constexpr (TILE == 64) hipLaunchKernelGGL((k_gemm<T, 64, 64, 2, 1>), grid, dim3(2 * kWave), 0, s, a);
+        else hipLaunchKernelGGL((k_gemm<T, TILE, TILE, WM, WN>), grid, block, 0, s, a);
+    }
 }
 
 template <typename T, int MT>
@@ -792,24 +744,21 @@ template <typename T, bool PCOL, bool QCOL>
 int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return GLIF_OK;
     a.splits = p.splits, a.k_part = p.k_part, a.part_ld = p.part_ld, a.part = part;
-    bool done = false;
-    if constexpr (!PCOL && !QCOL) {
-        done = true;
-        if (p.kind == kFew16) launch_few<T, 1>(a, s);
-        else if (p.kind == kFew32) launch_few<T, 2>(a, s);
-        else if (p.kind == kFew64) launch_few<T, 4>(a, s);
-        else done = false;
+    // a tile's rows of k within 32-bit offsets
+    const int64_t ld = std::max(PCOL ? 0 : a.p_ld, QCOL ? 0 : a.q_ld) * static_cast<int64_t>(sizeof(T));
+    const int64_t most = ((int64_t(1) << 32) - 1) / std::max<int64_t>(ld, 1);
+    if (a.K == 0) {
+        a.splits = 0;   // the epilogue of empty sums (the tile kernels load a first tile whatever there is)
+    } else if (p.kind == kFew16 || p.kind == kFew32) {
+        if constexpr (!PCOL && !QCOL) p.kind == kFew16 ? launch_few<T, 1>(a, s) : launch_few<T, 2>(a, s);
+    } else if (sizeof(T) == 2 && p.kind == kTile256 && most >= 256) {
+        if constexpr (sizeof(T) == 2) launch_tile<T, 256, 2, 4, PCOL, QCOL>(a, s);
+    } else if (p.kind != kTile64 && most >= 128) {
+        launch_tile<T, 128, 2, 2, PCOL, QCOL>(a, s);
+    } else {
+        launch_tile<T, 64, 2, 2, PCOL, QCOL>(a, s);
     }
-    if constexpr (sizeof(T) == 2)
-        if (!done && p.kind == kTile256) done = launch_tile<T, 256, 2, 4, PCOL, QCOL>(a, s);
-    if (!done && p.kind == kTile64) {
-        done = launch_tile<T, 64, 2, 2, PCOL, QCOL>(a, s);
-        if (!done) launch_staged<T, 64, 2, 1, PCOL, QCOL>(a, s);
-    } else if (!done) {
-        done = launch_tile<T, 128, 2, 2, PCOL, QCOL>(a, s);
-        if (!done) launch_staged<T, 128, 2, 2, PCOL, QCOL>(a, s);
-    }
-    if (a.splits > 1) {
+    if (a.splits != 1) {
         // where the results alone do not fill the chip, lanes over the splits: 5 x 66000 x 512 in 64 parts 14 us -> 4
         const int64_t n4 = a.M * (a.part_ld / 4);
         if (n4 < 32768 && a.splits >= 16)
@@ -831,34 +780,57 @@ int gemm_cc(const GemmArgs &a, const Plan &p, float *part, hipStream_t s) { retu
 template <typename T>
 void run_slope(const SlopeArgs &a, hipStream_t s) {
     if (a.N == 0) return;
-    hipLaunchKernelGGL(k_slope<T>, dim3(static_cast<unsigned>(ceil_div(a.N, kBlock)), static_cast<unsigned>(a.parts)),
+    hipLaunchKernelGGL(k_slope<T>, dim3(static_cast<unsigned>(ceil_div(a.dp ? a.lddp : a.N, kBlock)), static_cast<unsigned>(a.parts)),
                        dim3(kBlock), 0, s, a);
 }
 
 int row_parts(int64_t M) { return static_cast<int>(std::min<int64_t>(std::max<int64_t>(M / 16, 1), 256)); }
 
+// Rows whose tiles would pass 32-bit offsets.
+int check_strides(int64_t a, int64_t b, int64_t c) {
+    if (std::max({a, b, c}) >= (1 << 24)) return fail(GLIF_EINVAL, "linear: row strides must be below 2^24");
+    return GLIF_OK;
+}
+
 int check_linear(int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t act) {
     if (!known_dtype(dtype) || (bias_dtype != GLIF_F32 && bias_dtype != dtype))
         return fail(GLIF_EINVAL, "linear: the bias is float32 or of x's type");
-    if (M < 0 || N < 0 || K < 0 || M > (1 << 21) || N > (1 << 21) || K > (1 << 24))
-        return fail(GLIF_EINVAL, "linear: M and N in [0, 2^21], K in [0, 2^24]");
+    if (M < 0 || N < 0 || K < 0 || M > (1 << 21) || N > (1 << 21) || K >= (1 << 24))
+        return fail(GLIF_EINVAL, "linear: M and N in [0, 2^21], K in [0, 2^24)");
     if (act < GLIF_ACT_NONE || act > GLIF_ACT_SILU) return fail(GLIF_EINVAL, "linear: unknown activation");
     return GLIF_OK;
 }
 
 struct Back {
-    void *dp;
+    void *dp, *w, *x;     // dp, and the operands put on 16 bytes
     float *part, *sums;   // of the products' splits (one after the other), of the bias's rows
     int32_t parts;
+    int64_t np, kp;       // N and K in whole 16 bytes, for 16-bit types
     Plan dx, dw;
 };
 
-void carve(Carver &c, Back &b, int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act) {
+// repack: some operand of a 16-bit type does not lie on 16 bytes
+void carve(Carver &c, Back &b, int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act, bool repack) {
+    const bool half = dtype != GLIF_F32;
+    const size_t size = dtype_size(dtype);
     b.parts = row_parts(M);
+    b.np = half ? (N + 7) / 8 * 8 : N, b.kp = half ? (K + 7) / 8 * 8 : K;
     b.dx = plan_for(dtype, M, K, N, false), b.dw = plan_for(dtype, N, K, M, false);
     b.sums = c.take<float>(static_cast<size_t>(b.parts * N));
     b.part = c.take<float>(std::max(b.dx.floats(), b.dw.floats()));
-    b.dp = act != GLIF_ACT_NONE ? c.take<char>(static_cast<size_t>(M * N) * dtype_size(dtype)) : nullptr;
+    repack = repack && half;
+    if (act != GLIF_ACT_NONE || repack) b.dp = c.take<char>(static_cast<size_t>(M * b.np) * size);
+    if (repack) {
+        b.w = c.take<char>(static_cast<size_t>(N * b.kp) * size);
+        b.x = c.take<char>(static_cast<size_t>(M * b.kp) * size);
+    }
+}
+
+void run_repack(const void *in, int64_t ld, int64_t rows, int64_t cols, void *out, int64_t ldo, hipStream_t s) {
+    const int64_t n = rows * (ldo / 8);
+    if (n == 0) return;
+    hipLaunchKernelGGL(k_repack, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n, kBlock), 16384))), dim3(kBlock), 0, s,
+                       static_cast<const uint16_t *>(in), ld, rows, cols, static_cast<uint16_t *>(out), ldo);
 }
 
 }  // namespace
@@ -879,10 +851,11 @@ int glif_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw,
                     int64_t ldr, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
                     void *y, void *pre, void *ws, size_t ws_bytes, void *stream) {
     if (int rc = check_linear(dtype, bias_dtype, M, N, K, activation)) return rc;
+    if (int rc = check_strides(ldx, ldw, 0)) return rc;
     if (M == 0 || N == 0) return GLIF_OK;
     if (!y || (K && (!x || !weight))) return fail(GLIF_EINVAL, "NULL argument");
     GemmArgs a{};
-    a.p = x, a.p_ld = ldx, a.q = weight, a.q_ld = ldw, a.M = M, a.N = N, a.K = K;
+    a.p = x, a.p_ld = ldx, a.q = weight, a.q_ld = ldw, a.M = a.p_rows = M, a.N = a.q_rows = N, a.K = a.k_cols = K;
     a.c = y, a.pre = pre, a.bias = bias, a.residual = residual, a.ldr = ldr, a.bias_dt = bias_dtype, a.act = activation;
     const Plan p = plan_for(dtype, M, N, K, true);
     Carver c(ws, ws_bytes);
@@ -893,11 +866,11 @@ int glif_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw,
     return GLIF_OK;
 }
 
-size_t glif_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t activation) {
+size_t glif_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t activation, int32_t unaligned) {
     if (check_linear(dtype, dtype, M, N, K, activation)) return 0;
     Carver c(nullptr, 0);
     Back b{};
-    carve(c, b, dtype, M, N, K, activation);
+    carve(c, b, dtype, M, N, K, activation, unaligned != 0);
     return c.mark();
 }
 
@@ -905,32 +878,43 @@ int glif_linear_bwd(const void *dy, int64_t lddy, const void *pre, const void *x
                     int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
                     void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream) {
     if (int rc = check_linear(dtype, bias_dtype, M, N, K, activation)) return rc;
+    if (int rc = check_strides(lddy, ldx, ldw)) return rc;
     const bool some = M && N;
     if (some && (!dy || (activation != GLIF_ACT_NONE && !pre) || (dx && K && !weight) || (dweight && K && !x)))
         return fail(GLIF_EINVAL, "NULL argument");
     hipStream_t s = static_cast<hipStream_t>(stream);
+    const size_t size = dtype_size(dtype);
+    const bool half = size == 2;
+    const bool move_dy = half && (dx || dweight) && !on_16(dy, lddy, N, size);
+    const bool move_w = half && dx && !on_16(weight, ldw, K, size), move_x = half && dweight && !on_16(x, ldx, K, size);
     Back b{};
     Carver c(ws, ws_bytes);
-    carve(c, b, dtype, M, N, K, activation);
+    carve(c, b, dtype, M, N, K, activation, move_dy || move_w || move_x);
     if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "linear: workspace too small");
     const void *dp = dy;
-    int64_t lddp = lddy;
-    if (activation != GLIF_ACT_NONE || dbias) {
-        SlopeArgs a{dy, pre, lddy, M, N, b.dp, dbias ? b.sums : nullptr, activation, b.parts};
+    int64_t lddp = lddy, n_cols = N, k_cols = K;
+    const bool own_dp = activation != GLIF_ACT_NONE || move_dy;
+    if (own_dp || dbias) {
+        SlopeArgs a{dy, pre, lddy, M, N, own_dp ? b.dp : nullptr, b.np, dbias ? b.sums : nullptr, activation, b.parts};
         GLIF_BY_DTYPE(dtype, run_slope, a, s);
-        if (b.dp) dp = b.dp, lddp = N;
+        if (own_dp) dp = b.dp, lddp = n_cols = b.np;
         if (dbias && N)
             hipLaunchKernelGGL(k_bias_join, dim3(static_cast<unsigned>(ceil_div(N, kBlock))), dim3(kBlock), 0, s, b.sums, b.parts,
                                N, dbias, bias_dtype);
     }
     if (dx) {
         GemmArgs a{};
-        a.p = dp, a.p_ld = lddp, a.q = weight, a.q_ld = ldw, a.M = M, a.N = K, a.K = N, a.c = dx;
+        if (move_w) run_repack(weight, ldw, N, K, b.w, b.kp, s), weight = b.w, ldw = k_cols = b.kp;
+        a.p = dp, a.p_ld = lddp, a.q = weight, a.q_ld = ldw, a.M = a.p_rows = M, a.N = K, a.q_rows = k_cols, a.K = N, a.k_cols = n_cols;
+        a.c = dx;
         if (int rc = GLIF_BY_DTYPE(dtype, gemm_rc, a, b.dx, b.part, s)) return rc;
     }
     if (dweight) {
         GemmArgs a{};
-        a.p = dp, a.p_ld = lddp, a.q = x, a.q_ld = ldx, a.M = N, a.N = K, a.K = M, a.c = dweight;
+        k_cols = K;
+        if (move_x) run_repack(x, ldx, M, K, b.x, b.kp, s), x = b.x, ldx = k_cols = b.kp;
+        a.p = dp, a.p_ld = lddp, a.q = x, a.q_ld = ldx, a.M = N, a.p_rows = n_cols, a.N = K, a.q_rows = k_cols, a.K = a.k_cols = M;
+        a.c = dweight;
         if (int rc = GLIF_BY_DTYPE(dtype, gemm_cc, a, b.dw, b.part, s)) return rc;
     }
     GLIF_HIP(hipGetLastError());

@@ -82,7 +82,7 @@ def _rows(t, D):
             r = t.view(n, D)
         except RuntimeError:
             r = t.contiguous().view(n, D)
-    if D > 1 and r.stride(1) != 1:
+    if (D > 1 and r.stride(1) != 1) or (n > 1 and r.stride(0) >= 1 << 24):
         r = r.contiguous()
     return r, r.stride(0) if n > 1 else D
 
@@ -261,7 +261,8 @@ class _Linear(torch.autograd.Function):
         db = torch.empty(N, dtype=ctx.bdt, device=dev) if wb else None
         if wx or ww or wb:
             L = lib()
-            ws = _workspace(L.glif_linear_bwd_workspace(dt, M, N, K, ctx.act), dev)
+            odd = any(v % (16 // x.element_size()) for v in (ldx, ldw, ldg, N, K)) or any(t.data_ptr() % 16 for t in (xr, wr, gr))
+            ws = _workspace(L.glif_linear_bwd_workspace(dt, M, N, K, ctx.act, int(odd)), dev)
             with _on(dev):
                 check(L.glif_linear_bwd(ptr(gr), ldg, ptr(pre), ptr(xr), ldx, ptr(wr), ldw, dt, DTYPES[ctx.bdt], M, N, K,
                                         ctx.act, ptr(dx), ptr(dw), ptr(db), ptr(ws), _size(ws), stream_ptr(dev)))
