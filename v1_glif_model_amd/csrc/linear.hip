@@ -55,13 +55,11 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
-    static constexpr int kEach = 1;   // matrix instructions of a fragment
     typedef bf16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Mma<f16> {
-    static constexpr int kEach = 1;
     typedef f16 frag __attribute__((ext_vector_type(8)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -69,7 +67,6 @@ struct Mma<f16> {
 // a sum is free, as long as both operands have it)
 template <>
 struct Mma<f32> {
-    static constexpr int kEach = 4;
     typedef f32 frag __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) {
 #pragma unroll
@@ -479,7 +476,7 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
         fetch(cur);
         half(fp0, fq0, next, 0);   // of no tile after the last, and then not used
         mul(fp1, fq1);
-        constexpr int kLoads = P::kN + Q::kN, kMul = FM * FN * M::kEach, kReads = FM * P::kReads + FN * Q::kReads;
+        constexpr int kLoads = P::kN + Q::kN, kMul = FM * FN * (sizeof(T) == 4 ? 4 : 1), kReads = FM * P::kReads + FN * Q::kReads;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kLoads - 1) / kLoads, 0);
