@@ -309,7 +309,7 @@ typedef enum { GLIF_ACT_NONE = 0, GLIF_ACT_RELU = 1, GLIF_ACT_GELU = 2, GLIF_ACT
  * NULL.  The backward takes the statistics from x; dweight and dbias are of param_dtype. */
 int glif_layer_norm_fwd(const void *x, int64_t x_stride, const void *weight, const void *bias, int32_t dtype,
                         int32_t param_dtype, int64_t rows, int64_t D, float eps, void *y, void *stream);
-size_t glif_layer_norm_bwd_workspace(int64_t rows, int64_t D, int32_t want_params);
+size_t glif_layer_norm_bwd_workspace(int64_t rows, int64_t D, int32_t dtype, int32_t want_params);
 int glif_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const void *weight,
                         int32_t dtype, int32_t param_dtype, int64_t rows, int64_t D, float eps, void *dx, void *dweight,
                         void *dbias, void *ws, size_t ws_bytes, void *stream);

@@ -95,7 +95,7 @@ SIGNATURES = {
     "glif_sample_bernoulli": (C.c_int, [vp, i64, C.c_uint64, C.c_uint64, vp, vp]),
     "glif_sample_poisson": (C.c_int, [C.c_float, C.c_float, i64, C.c_uint64, C.c_uint64, vp, vp]),
     "glif_layer_norm_fwd": (C.c_int, [vp, i64, vp, vp, i32, i32, i64, i64, C.c_float, vp, vp]),
-    "glif_layer_norm_bwd_workspace": (sz, [i64, i64, i32]),
+    "glif_layer_norm_bwd_workspace": (sz, [i64, i64, i32, i32]),
     "glif_layer_norm_bwd": (C.c_int, [vp, i64, vp, i64, vp, i32, i32, i64, i64, C.c_float, vp, vp, vp, vp, sz, vp]),
     "glif_dropout": (C.c_int, [vp, vp, i32, i64, C.c_double, C.c_uint64, C.c_uint64, vp, vp]),
     "glif_linear_fwd_workspace": (sz, [i32, i64, i64, i64]),

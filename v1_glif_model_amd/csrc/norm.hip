@@ -4,143 +4,555 @@
 //   dx = rstd (dyw - mean(dyw) - xh mean(dyw xh)),  dyw = dy w;   dw = sum_rows dy xh,  db = sum_rows dy
 // The backward takes the statistics from x itself, so the forward leaves nothing behind.  All sums are float32 in a
 // fixed order; y and dx are rounded once.
+//
+// Bound by memory: x in and y out, or x and dy in and dx out.  A row is read once, in 16-byte pieces, into the registers of
+// the L threads that share it (8 of a wave up to a block of 1024), and its mean, variance and results are taken from there.
+// In the backward the same threads keep the columns' sums over the rows they go through, as long as those fit beside the
+// row.  Wider rows are gone through twice: once for their statistics, once, by columns, for dx and the columns' sums, in
+// turns over parts of the rows that the last-level cache still holds.
 #include "seq.h"
-
 namespace glif {
 
 namespace {
-
-constexpr int kParts = 256;   // row chunks of the parameter gradients, at most
 
 struct NormArgs {
     const void *x, *dy, *weight, *bias;
     void *y, *dx, *dweight, *dbias;
     int64_t rows, D, x_stride, dy_stride;
+    int64_t row0;      // first row of this launch
     int32_t pdt;
     float eps;
-    float2 *stat;      // [rows] mean, rstd (backward)
-    float *part;       // [2][parts][D]
-    int32_t parts;
+    float4 *stat;      // [rows] mean, rstd, mean(dyw), mean(dyw xh) (backward of wide rows)
+    float *part;       // [parts][2][D] sums of dw and db
+    int32_t parts, part0;
 };
 
-__device__ inline float block_sum(float v, float *red) {
-    v = wave_sum(v);
-    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float s = 0.0f;
-    for (int i = 0; i < static_cast<int>(blockDim.x) / kWave; ++i) s += red[i];
-    __syncthreads();
-    return s;
-}
-
-template <typename T>
-__device__ inline float2 row_stats(const T *x, int64_t D, float eps, float *red) {
-    float s = 0.0f;
-    for (int64_t i = threadIdx.x; i < D; i += blockDim.x) s += to_f32(x[i]);
-    const float mean = block_sum(s, red) / static_cast<float>(D);
-    float q = 0.0f;
-    for (int64_t i = threadIdx.x; i < D; i += blockDim.x) {
-        const float d = to_f32(x[i]) - mean;
-        q = fmaf(d, d, q);
+// ---- the threads of a row -----------------------------------------------------------------------------------------------
+// L threads: a part of a wave, or the whole block.  Sum over them, in all of them.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float *red) {
+    if constexpr (L <= kWave) {
+#pragma unroll
+        for (int m = 1; m < L; m <<= 1) v += __shfl_xor(v, m, kWave);
+        return v;
+    } else {
+        constexpr int kW = L / kWave;
+        v = wave_sum(v);
+        __syncthreads();   // the last sum's readers are done
+        if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
+        __syncthreads();
+        float s = red[threadIdx.x % kW];
+#pragma unroll
+        for (int m = 1; m < kW; m <<= 1) s += __shfl_xor(s, m, kWave);
+        return s;
     }
-    return make_float2(mean, 1.0f / sqrtf(block_sum(q, red) / static_cast<float>(D) + eps));
+}
+// two at once
+template <int L>
+__device__ __forceinline__ float2 row_sum2(float a, float b, float *red) {
+    if constexpr (L <= kWave) {
+        return make_float2(row_sum<L>(a, red), row_sum<L>(b, red));
+    } else {
+        constexpr int kW = L / kWave;
+        a = wave_sum(a), b = wave_sum(b);
+        __syncthreads();
+        if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = a, red[kW + threadIdx.x / kWave] = b;
+        __syncthreads();
+        float s = red[threadIdx.x % kW], t = red[kW + threadIdx.x % kW];
+#pragma unroll
+        for (int m = 1; m < kW; m <<= 1) s += __shfl_xor(s, m, kWave), t += __shfl_xor(t, m, kWave);
+        return make_float2(s, t);
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBlock) k_norm_fwd(NormArgs a) {
-    __shared__ float red[kBlock / kWave];
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
-        T *y = static_cast<T *>(a.y) + r * a.D;
-        const float2 st = row_stats(x, a.D, a.eps, red);
-        for (int64_t i = threadIdx.x; i < a.D; i += blockDim.x) {
-            const float w = a.weight ? load_param(a.weight, a.pdt, i) : 1.0f;
-            const float b = a.bias ? load_param(a.bias, a.pdt, i) : 0.0f;
-            y[i] = from_f32<T>(fmaf((to_f32(x[i]) - st.x) * st.y, w, b));
+// A row in the registers of L threads, R pieces of V elements each; piece i of thread t starts at (i L + t) V.
+template <typename T, int L, int R>
+struct Row {
+    static constexpr int V = kVecBytes16<T>;
+    typedef Vec<T, V> vec;
+    vec r[R];
+    static __device__ __forceinline__ int at(int i) { return (i * L + static_cast<int>(threadIdx.x) % L) * V; }
+    __device__ __forceinline__ void load(int i, const T *p, int D) {
+        const int c = at(i);
+        r[i] = vec{};
+        if (c + V <= D) {
+            r[i] = *reinterpret_cast<const vec *>(p + c);
+        } else if (c < D) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (c + e < D) r[i][e] = p[c + e];
         }
     }
+    __device__ __forceinline__ void load(const T *p, int D) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) load(i, p, D);
+    }
+    __device__ __forceinline__ float get(int i, int e) const { return to_f32(static_cast<T>(r[i][e])); }
+    // Between the passes over a long row: its float32 values are made again rather than kept in twice the registers.
+    __device__ __forceinline__ void again() {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        if constexpr (R > 2 && sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                u32x4 q = __builtin_bit_cast(u32x4, r[i]);
+                asm volatile("" : "+v"(q));
+                r[i] = __builtin_bit_cast(vec, q);
+            }
+        }
+    }
+    static __device__ __forceinline__ void put(T *p, int c, int D, const float (&v)[V]) {
+        if (c + V <= D) {
+            vec o;
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = from_f32<T>(v[e]);
+            *reinterpret_cast<vec *>(p + c) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (c + e < D) p[c + e] = from_f32<T>(v[e]);
+        }
+    }
+    __device__ __forceinline__ float2 stats(int D, float eps, float *red) {
+        float s = 0.0f;   // pieces past the row are zeros
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += get(i, e);
+        const float mean = row_sum<L>(s, red) / static_cast<float>(D);
+        again();
+        float q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = get(i, e) - mean;
+                q = at(i) + e < D ? fmaf(d, d, q) : q;
+            }
+        return make_float2(mean, 1.0f / sqrtf(row_sum<L>(q, red) / static_cast<float>(D) + eps));
+    }
+};
+
+// V parameters from column c on; `other` past the row and where there are none.
+template <int V>
+__device__ __forceinline__ void params(float (&v)[V], const void *p, int32_t dt, int c, int D, float other) {
+    if (!p) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = other;
+    } else if (dt == GLIF_F32 && c + V <= D) {
+        const Vec<float, 4> *q = reinterpret_cast<const Vec<float, 4> *>(static_cast<const float *>(p) + c);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = q[e / 4][e % 4];
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = c + e < D ? load_param(p, dt, c + e) : other;
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBlock) k_norm_dx(NormArgs a) {
-    __shared__ float red[kBlock / kWave];
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T *x = static_cast<const T *>(a.x) + r * a.x_stride, *dy = static_cast<const T *>(a.dy) + r * a.dy_stride;
-        const float2 st = row_stats(x, a.D, a.eps, red);
+// ---- rows in registers ----------------------------------------------------------------------------------------------------
+template <typename T, int L, int R>
+__global__ void __launch_bounds__(L > kBlock ? L : kBlock, L > kBlock ? 8 : 1) k_norm_fwd(NormArgs a) {
+    constexpr int V = Row<T, L, R>::V, kRows = L > kBlock ? 1 : kBlock / L;
+    __shared__ float red[32];
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / L;
+    if (r >= a.rows) return;
+    const int D = static_cast<int>(a.D);
+    Row<T, L, R> x;
+    x.load(static_cast<const T *>(a.x) + r * a.x_stride, D);
+    const float2 st = x.stats(D, a.eps, red);
+    x.again();
+    T *y = static_cast<T *>(a.y) + r * a.D;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int c = x.at(i);
+        if (c >= D) continue;
+        float w[V], b[V], o[V];
+        params<V>(w, a.weight, a.pdt, c, D, 1.0f);
+        params<V>(b, a.bias, a.pdt, c, D, 0.0f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = fmaf((x.get(i, e) - st.x) * st.y, w[e], b[e]);
+        x.put(y, c, D, o);
+    }
+}
+
+// dx, and the columns' sums over the block's rows.
+template <typename T, int L, int R>
+__global__ void __launch_bounds__(kBlock) k_norm_bwd(NormArgs a) {
+    constexpr int V = Row<T, L, R>::V, kRows = kBlock / L;
+    __shared__ float red[2 * kBlock / kWave];
+    float dw[R][V] = {}, db[R][V] = {};
+    const int D = static_cast<int>(a.D);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / L;
+    constexpr bool kNext = R <= 2;   // the next row is on its way while this one is worked on
+    Row<T, L, R> next_x, next_dy;
+    if (kNext && first < a.rows) {
+        next_x.load(static_cast<const T *>(a.x) + first * a.x_stride, D);
+        next_dy.load(static_cast<const T *>(a.dy) + first * a.dy_stride, D);
+    }
+    for (int64_t r = first; r < a.rows; r += step) {
+        // the weights are read again for every row: kept, they would take the registers that other waves live in
+        const void *weight = a.weight;
+        asm volatile("" : "+s"(weight));
+        Row<T, L, R> x, dy;
+        if constexpr (kNext) {
+            x = next_x, dy = next_dy;
+            if (r + step < a.rows) {
+                next_x.load(static_cast<const T *>(a.x) + (r + step) * a.x_stride, D);
+                next_dy.load(static_cast<const T *>(a.dy) + (r + step) * a.dy_stride, D);
+            }
+        } else {
+            x.load(static_cast<const T *>(a.x) + r * a.x_stride, D);
+            dy.load(static_cast<const T *>(a.dy) + r * a.dy_stride, D);
+        }
+        const float2 st = x.stats(D, a.eps, red);
+        x.again();
         float s1 = 0.0f, s2 = 0.0f;
-        for (int64_t i = threadIdx.x; i < a.D; i += blockDim.x) {
-            const float g = to_f32(dy[i]) * (a.weight ? load_param(a.weight, a.pdt, i) : 1.0f);
-            s1 += g;
-            s2 = fmaf(g, (to_f32(x[i]) - st.x) * st.y, s2);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = x.at(i);
+            if (c >= D) continue;
+            float w[V];
+                params<V>(w, weight, a.pdt, c, D, 1.0f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float g = dy.get(i, e), xh = (x.get(i, e) - st.x) * st.y;   // past the row g is 0
+                s1 = fmaf(g, w[e], s1);
+                s2 = fmaf(g * w[e], xh, s2);
+                dw[i][e] = fmaf(g, xh, dw[i][e]), db[i][e] += g;
+            }
         }
-        s1 = block_sum(s1, red) / static_cast<float>(a.D);
-        s2 = block_sum(s2, red) / static_cast<float>(a.D);
-        if (threadIdx.x == 0) a.stat[r] = st;
+        const float2 s = row_sum2<L>(s1, s2, red);
+        const float m1 = s.x / static_cast<float>(D), m2 = s.y / static_cast<float>(D);
         if (!a.dx) continue;
         T *dx = static_cast<T *>(a.dx) + r * a.D;
-        for (int64_t i = threadIdx.x; i < a.D; i += blockDim.x) {
-            const float g = to_f32(dy[i]) * (a.weight ? load_param(a.weight, a.pdt, i) : 1.0f);
-            dx[i] = from_f32<T>(st.y * (g - s1 - (to_f32(x[i]) - st.x) * st.y * s2));
+        asm volatile("" : "+s"(weight));
+        x.again(), dy.again();
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = x.at(i);
+            if (c >= D) continue;
+            float w[V], o[V];
+                params<V>(w, weight, a.pdt, c, D, 1.0f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = st.y * (dy.get(i, e) * w[e] - m1 - (x.get(i, e) - st.x) * st.y * m2);
+            x.put(dx, c, D, o);
+        }
+    }
+    if (!a.part) return;
+    float *part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.D;
+    if constexpr (L >= kBlock) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int c = Row<T, L, R>::at(i) + e;
+                if (c < D) part[c] = dw[i][e], part[a.D + c] = db[i][e];
+            }
+    } else {
+        // the block's rows side by side: their threads' sums one piece after the other through LDS
+        constexpr int kCols = L * V;
+        __shared__ float sum[2][kBlock / L][kCols];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                sum[0][threadIdx.x / L][(threadIdx.x % L) * V + e] = dw[i][e];
+                sum[1][threadIdx.x / L][(threadIdx.x % L) * V + e] = db[i][e];
+            }
+            __syncthreads();
+            for (int q = threadIdx.x; q < 2 * kCols; q += kBlock) {
+                const int k = q / kCols, c = q % kCols;
+                float v = 0.0f;
+#pragma unroll
+                for (int row = 0; row < kBlock / L; ++row) v += sum[k][row][c];
+                if (i * kCols + c < a.D) part[k * a.D + i * kCols + c] = v;
+            }
         }
     }
 }
 
-// A thread per column over one chunk of rows.
+// ---- wide rows --------------------------------------------------------------------------------------------------------------
+// A block's threads go through a row in pieces and through it again for the results; a compute unit holds several such
+// rows, and the second time comes from cache.  (Rows of 66,000 in registers leave one block a compute unit: 207 us for 2500
+// of them in bfloat16, and their backward spills.)
+constexpr int kWide = 512;
+
+// Count, mean and sum of squared differences from it, of the elements seen.  A thread takes its sums from its own first
+// element on, so that a mean far from zero costs no digits.
+struct Moments {
+    float n, mean, m2;
+};
+__device__ __forceinline__ Moments both(Moments a, Moments b) {
+    const float n = a.n + b.n, d = b.mean - a.mean, share = n > 0.0f ? b.n / n : 0.0f;
+    return {n, fmaf(d, share, a.mean), a.m2 + b.m2 + d * d * a.n * share};
+}
+template <int L>
+__device__ __forceinline__ Moments all_moments(Moments v, Moments *red) {
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) v = both(v, {__shfl_xor(v.n, m, kWave), __shfl_xor(v.mean, m, kWave), __shfl_xor(v.m2, m, kWave)});
+    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = red[0];
+    for (int w = 1; w < L / kWave; ++w) v = both(v, red[w]);   // in order, the same in all threads
+    return v;
+}
+
+// f(column, count, values...) for every piece of this thread
+template <typename T, typename F>
+__device__ __forceinline__ void pieces(const T *p, int D, F f) {
+    constexpr int V = kVecBytes16<T>;
+    typedef Vec<T, V> vec;
+    const int whole = D / V;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < whole; i += kWide) f(i * V, V, *reinterpret_cast<const vec *>(p + i * V));
+    if (D % V && static_cast<int>(threadIdx.x) == whole % kWide) {
+        vec v = {};
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (whole * V + e < D) v[e] = p[whole * V + e];
+        f(whole * V, D - whole * V, v);
+    }
+}
+template <typename T, typename F>
+__device__ __forceinline__ void pieces2(const T *p, const T *q, int D, F f) {
+    constexpr int V = kVecBytes16<T>;
+    typedef Vec<T, V> vec;
+    const int whole = D / V;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < whole; i += kWide)
+        f(i * V, V, *reinterpret_cast<const vec *>(p + i * V), *reinterpret_cast<const vec *>(q + i * V));
+    if (D % V && static_cast<int>(threadIdx.x) == whole % kWide) {
+        vec v = {}, w = {};
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (whole * V + e < D) v[e] = p[whole * V + e], w[e] = q[whole * V + e];
+        f(whole * V, D - whole * V, v, w);
+    }
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kBlock) k_norm_dparam(NormArgs a) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-    if (i >= a.D) return;
-    const int64_t r0 = a.rows * blockIdx.y / a.parts, r1 = a.rows * (blockIdx.y + 1) / a.parts;
-    float dw = 0.0f, db = 0.0f;
-    for (int64_t r = r0; r < r1; ++r) {
-        const float2 st = a.stat[r];
-        const float g = to_f32(static_cast<const T *>(a.dy)[r * a.dy_stride + i]);
-        dw = fmaf(g, (to_f32(static_cast<const T *>(a.x)[r * a.x_stride + i]) - st.x) * st.y, dw);
-        db += g;
-    }
-    a.part[static_cast<int64_t>(blockIdx.y) * a.D + i] = dw;
-    a.part[static_cast<int64_t>(a.parts + blockIdx.y) * a.D + i] = db;
+__global__ void __launch_bounds__(kWide) k_norm_fwd_wide(NormArgs a) {
+    constexpr int V = kVecBytes16<T>;
+    typedef Vec<T, V> vec;
+    __shared__ Moments red[kWide / kWave];
+    const int64_t r = blockIdx.x;
+    const int D = static_cast<int>(a.D), first = threadIdx.x * V;
+    const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
+    const float k = first < D ? to_f32(x[first]) : 0.0f;
+    float s = 0.0f, q = 0.0f, n = 0.0f;
+    pieces(x, D, [&](int, int have, vec v) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = e < have ? to_f32(static_cast<T>(v[e])) - k : 0.0f;
+            s += d;
+            q = fmaf(d, d, q);
+        }
+        n += static_cast<float>(have);
+    });
+    const float d = n > 0.0f ? s / n : 0.0f;
+    const Moments m = all_moments<kWide>({n, k + d, q - s * d}, red);
+    const float rstd = 1.0f / sqrtf(m.m2 / static_cast<float>(D) + a.eps);
+    T *y = static_cast<T *>(a.y) + r * a.D;
+    pieces(x, D, [&](int c, int have, vec v) {
+        float w[V], b[V], o[V];
+        params<V>(w, a.weight, a.pdt, c, D, 1.0f);
+        params<V>(b, a.bias, a.pdt, c, D, 0.0f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = fmaf((to_f32(static_cast<T>(v[e])) - m.mean) * rstd, w[e], b[e]);
+        Row<T, 1, 1>::put(y, c, D, o);
+    });
 }
 
+// Per row mean, rstd, mean(dyw), mean(dyw xh).
+template <typename T>
+__global__ void __launch_bounds__(kWide) k_norm_stats(NormArgs a) {
+    constexpr int V = kVecBytes16<T>;
+    typedef Vec<T, V> vec;
+    __shared__ Moments red[kWide / kWave];
+    __shared__ float red2[2 * kWide / kWave];
+    const int64_t r = a.row0 + blockIdx.x;
+    const int D = static_cast<int>(a.D), first = threadIdx.x * V;
+    const T *x = static_cast<const T *>(a.x) + r * a.x_stride, *dy = static_cast<const T *>(a.dy) + r * a.dy_stride;
+    const float k = first < D ? to_f32(x[first]) : 0.0f;
+    float s = 0.0f, q = 0.0f, n = 0.0f, g1 = 0.0f, g2 = 0.0f;
+    pieces2(x, dy, D, [&](int c, int have, vec v, vec g) {
+        float w[V];
+        params<V>(w, a.weight, a.pdt, c, D, 1.0f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = e < have ? to_f32(static_cast<T>(v[e])) - k : 0.0f, gw = to_f32(static_cast<T>(g[e])) * w[e];
+            s += d;
+            q = fmaf(d, d, q);
+            g1 += gw;
+            g2 = fmaf(gw, d, g2);
+        }
+        n += static_cast<float>(have);
+    });
+    const float d = n > 0.0f ? s / n : 0.0f;
+    const Moments m = all_moments<kWide>({n, k + d, q - s * d}, red);
+    const float rstd = 1.0f / sqrtf(m.m2 / static_cast<float>(D) + a.eps);
+    const float2 g = row_sum2<kWide>(g1, rstd * fmaf(k - m.mean, g1, g2), red2);
+    if (threadIdx.x == 0) a.stat[r] = make_float4(m.mean, rstd, g.x / static_cast<float>(D), g.y / static_cast<float>(D));
+}
+
+// dx and the columns' sums: a thread per 16 bytes of columns over one of the launch's parts of its rows.
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_norm_columns(NormArgs a, int32_t parts) {
+    constexpr int V = kVecBytes16<T>;
+    typedef Vec<T, V> vec;
+    const int D = static_cast<int>(a.D);
+    const int64_t c64 = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * V;
+    if (c64 >= D) return;
+    const int c = static_cast<int>(c64);
+    const int64_t n = a.rows - a.row0, r0 = a.row0 + n * blockIdx.y / parts, r1 = a.row0 + n * (blockIdx.y + 1) / parts;
+    float dw[V] = {}, db[V] = {}, w[V];
+    params<V>(w, a.weight, a.pdt, c, D, 1.0f);
+    const T *x = static_cast<const T *>(a.x) + c, *dy = static_cast<const T *>(a.dy) + c;
+    T *dx = static_cast<T *>(a.dx);
+    auto add = [&](vec xv, vec gv, int64_t r) {
+        const float4 st = a.stat[r];
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float g = to_f32(static_cast<T>(gv[e])), xh = (to_f32(static_cast<T>(xv[e])) - st.x) * st.y;
+            dw[e] = fmaf(g, xh, dw[e]);
+            db[e] += g;
+            o[e] = st.y * (g * w[e] - st.z - xh * st.w);
+        }
+        if (dx) Row<T, 1, 1>::put(dx + r * a.D, c, D, o);
+    };
+    if (c + V <= D) {
+#pragma unroll 4
+        for (int64_t r = r0; r < r1; ++r)
+            add(*reinterpret_cast<const vec *>(x + r * a.x_stride), *reinterpret_cast<const vec *>(dy + r * a.dy_stride), r);
+    } else {
+        for (int64_t r = r0; r < r1; ++r) {
+            vec xv = {}, gv = {};
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (c + e < D) xv[e] = x[r * a.x_stride + e], gv[e] = dy[r * a.dy_stride + e];
+            add(xv, gv, r);
+        }
+    }
+    if (!a.part) return;
+    float *part = a.part + static_cast<int64_t>(a.part0 + blockIdx.y) * 2 * a.D + c;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (c + e < D) part[e] = dw[e], part[a.D + e] = db[e];
+}
+
+// The parts' sums: 32 columns by 8 threads each, which take the parts in turn.
 __global__ void __launch_bounds__(kBlock) k_norm_join(NormArgs a) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-    if (i >= a.D) return;
+    __shared__ float sum[2][8][32];
+    const int col = threadIdx.x % 32, lot = threadIdx.x / 32;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + col;
     float dw = 0.0f, db = 0.0f;
-    for (int p = 0; p < a.parts; ++p) {
-        dw += a.part[static_cast<int64_t>(p) * a.D + i];
-        db += a.part[static_cast<int64_t>(a.parts + p) * a.D + i];
+    if (c < a.D) {
+#pragma unroll 4
+        for (int p = lot; p < a.parts; p += 8) {
+            dw += a.part[static_cast<int64_t>(p) * 2 * a.D + c];
+            db += a.part[(static_cast<int64_t>(p) * 2 + 1) * a.D + c];
+        }
     }
-    if (a.dweight) store_param(a.dweight, a.pdt, i, dw);
-    if (a.dbias) store_param(a.dbias, a.pdt, i, db);
+    sum[0][lot][col] = dw, sum[1][lot][col] = db;
+    __syncthreads();
+    if (lot > 1 || c >= a.D) return;
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += sum[lot][i][col];
+    if (lot == 0 && a.dweight) store_param(a.dweight, a.pdt, c, v);
+    if (lot == 1 && a.dbias) store_param(a.dbias, a.pdt, c, v);
 }
 
-int parts_for(int64_t rows) { return static_cast<int>(std::min<int64_t>(std::max<int64_t>(rows / 16, 1), kParts)); }
+// ---- launches ---------------------------------------------------------------------------------------------------------------
+constexpr int64_t kFused = 16384;   // bytes of the widest row whose columns' sums are kept beside it
 
-void carve(Carver &c, NormArgs &a, bool param) {
-    a.parts = parts_for(a.rows);
-    a.stat = c.take<float2>(static_cast<size_t>(a.rows));
-    if (param) a.part = c.take<float>(static_cast<size_t>(2 * a.parts * a.D));
+// Blocks of a fused backward, and parts of its sums: at least four rows for every thread group, as each part costs its way
+// to memory and back (16000 x 1024 bfloat16 in 256, 512, 1024 and 2048 parts 50, 37, 40 and 53 us).
+int fused_blocks(int64_t rows, int64_t D, int64_t size) {
+    const int64_t bytes = D * size, per = bytes <= 4096 ? kBlock / std::max<int64_t>(8, std::min<int64_t>(64, (bytes + 15) / 16)) : 1;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + 4 * per - 1) / (4 * per), 512)));
 }
 
-dim3 row_grid(int64_t rows) { return dim3(static_cast<unsigned>(std::min<int64_t>(rows, 1 << 20))); }
+// A wide backward's rounds of rows (both passes over 96 MB of x and dy), and parts of a round.
+int64_t round_rows(int64_t rows, int64_t D, int64_t size) {
+    return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t(48) << 20) / (D * size)));
+}
+int round_parts(int64_t n, int64_t D, int64_t size) {
+    const int64_t cols = (D * size / 16 + kBlock) / kBlock;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, 1024 / cols)));
+}
 
+void carve(Carver &c, NormArgs &a, int64_t size, bool param) {
+    if (a.D * size <= kFused) {
+        a.parts = fused_blocks(a.rows, a.D, size);
+    } else {
+        const int64_t n = round_rows(a.rows, a.D, size);
+        a.parts = static_cast<int32_t>((a.rows + n - 1) / n) * round_parts(n, a.D, size);
+        a.stat = c.take<float4>(static_cast<size_t>(a.rows));
+    }
+    if (param) a.part = c.take<float>(static_cast<size_t>(a.parts) * 2 * a.D);
+}
+
+template <typename T, int L, int R>
+void fwd(const NormArgs &a, hipStream_t s) {
+    constexpr int kRows = L > kBlock ? 1 : kBlock / L;
+    hipLaunchKernelGGL((k_norm_fwd<T, L, R>), dim3(static_cast<unsigned>((a.rows + kRows - 1) / kRows)), dim3(L > kBlock ? L : kBlock),
+                       0, s, a);
+}
+
+// The threads of a row: as few as hold it in one piece each, up to a wave with four, a block with four, 1024 with four.
 template <typename T>
 void run_fwd(const NormArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL(k_norm_fwd<T>, row_grid(a.rows), dim3(kBlock), 0, s, a);
+    const int64_t p = (a.D + kVecBytes16<T> - 1) / kVecBytes16<T>;   // pieces
+    if (p <= 8) fwd<T, 8, 1>(a, s);
+    else if (p <= 16) fwd<T, 16, 1>(a, s);
+    else if (p <= 32) fwd<T, 32, 1>(a, s);
+    else if (p <= 64) fwd<T, 64, 1>(a, s);
+    else if (p <= 128) fwd<T, 64, 2>(a, s);
+    else if (p <= 256) fwd<T, 64, 4>(a, s);
+    else if (p <= 512) fwd<T, 256, 2>(a, s);
+    else if (p <= 1024) fwd<T, 256, 4>(a, s);
+    else if (p <= 4096) fwd<T, 1024, 4>(a, s);
+    else hipLaunchKernelGGL(k_norm_fwd_wide<T>, dim3(static_cast<unsigned>(a.rows)), dim3(kWide), 0, s, a);
+}
+
+template <typename T, int L, int R>
+void bwd(const NormArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((k_norm_bwd<T, L, R>), dim3(static_cast<unsigned>(a.parts)), dim3(kBlock), 0, s, a);
 }
 
 template <typename T>
-void run_bwd(const NormArgs &a, hipStream_t s) {
-    const unsigned cols = static_cast<unsigned>(ceil_div(a.D, kBlock));
-    if (a.rows) hipLaunchKernelGGL(k_norm_dx<T>, row_grid(a.rows), dim3(kBlock), 0, s, a);
-    if (!a.dweight && !a.dbias) return;
-    hipLaunchKernelGGL(k_norm_dparam<T>, dim3(cols, static_cast<unsigned>(a.parts)), dim3(kBlock), 0, s, a);
-    hipLaunchKernelGGL(k_norm_join, dim3(cols), dim3(kBlock), 0, s, a);
+void run_bwd(const NormArgs &all, hipStream_t s) {
+    NormArgs a = all;
+    const int64_t p = (a.D + kVecBytes16<T> - 1) / kVecBytes16<T>, size = sizeof(T);
+    if (a.D * size <= kFused) {
+        if (p <= 8) bwd<T, 8, 1>(a, s);
+        else if (p <= 16) bwd<T, 16, 1>(a, s);
+        else if (p <= 32) bwd<T, 32, 1>(a, s);
+        else if (p <= 64) bwd<T, 64, 1>(a, s);
+        else if (p <= 128) bwd<T, 64, 2>(a, s);
+        else if (p <= 256) bwd<T, 64, 4>(a, s);
+        else if (p <= 512) bwd<T, 256, 2>(a, s);
+        else bwd<T, 256, 4>(a, s);
+    } else {
+        const int64_t n = round_rows(all.rows, a.D, size), cols = (p + kBlock - 1) / kBlock;
+        const int parts = round_parts(n, a.D, size);
+        for (int64_t r = 0; r < all.rows; r += n, a.part0 += parts) {
+            a.row0 = r, a.rows = std::min(all.rows, r + n);
+            hipLaunchKernelGGL(k_norm_stats<T>, dim3(static_cast<unsigned>(a.rows - r)), dim3(kWide), 0, s, a);
+            hipLaunchKernelGGL(k_norm_columns<T>, dim3(static_cast<unsigned>(cols), static_cast<unsigned>(parts)), dim3(kBlock), 0, s, a,
+                               parts);
+        }
+    }
+    if (a.part)
+        hipLaunchKernelGGL(k_norm_join, dim3(static_cast<unsigned>((a.D + 31) / 32)), dim3(kBlock), 0, s, all);
 }
 
 int check_norm(int64_t rows, int64_t D, int32_t dtype, int32_t pdt, float eps) {
-    if (rows < 0 || D < 1 || D >= (int64_t(1) << 31) || rows >= (int64_t(1) << 40))
-        return fail(GLIF_EINVAL, "layer norm: rows must be >= 0 and 1 <= D < 2^31");
+    if (rows < 0 || D < 1 || D >= (int64_t(1) << 31) || rows >= (int64_t(1) << 31))
+        return fail(GLIF_EINVAL, "layer norm: rows in [0, 2^31) and D in [1, 2^31)");
     if (!known_dtype(dtype) || (pdt != GLIF_F32 && pdt != dtype))
         return fail(GLIF_EINVAL, "layer norm: parameters are float32 or of x's type");
     if (!(eps >= 0.0f)) return fail(GLIF_EINVAL, "layer norm: eps must be >= 0");
@@ -167,12 +579,12 @@ int glif_layer_norm_fwd(const void *x, int64_t x_stride, const void *weight, con
     return GLIF_OK;
 }
 
-size_t glif_layer_norm_bwd_workspace(int64_t rows, int64_t D, int32_t want_params) {
-    if (rows < 0 || D < 1) return 0;
+size_t glif_layer_norm_bwd_workspace(int64_t rows, int64_t D, int32_t dtype, int32_t want_params) {
+    if (check_norm(rows, D, dtype, dtype, 0.0f)) return 0;
     NormArgs a{};
     a.rows = rows, a.D = D;
     Carver c(nullptr, 0);
-    carve(c, a, want_params != 0);
+    carve(c, a, static_cast<int64_t>(dtype_size(dtype)), want_params != 0);
     return c.mark();
 }
 
@@ -186,8 +598,8 @@ int glif_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_
     a.x = x, a.dy = dy, a.weight = weight, a.dx = dx, a.dweight = dweight, a.dbias = dbias;
     a.rows = rows, a.D = D, a.x_stride = x_stride, a.dy_stride = dy_stride, a.pdt = param_dtype, a.eps = eps;
     Carver c(ws, ws_bytes);
-    carve(c, a, dweight || dbias);
-    if (!c.ok() || !ws) return fail(GLIF_ENOMEM, "layer norm: workspace too small");
+    carve(c, a, static_cast<int64_t>(dtype_size(dtype)), dweight || dbias);
+    if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "layer norm: workspace too small");
     GLIF_BY_DTYPE(dtype, run_bwd, a, static_cast<hipStream_t>(stream));
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;

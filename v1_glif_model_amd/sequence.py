@@ -166,7 +166,7 @@ class _LayerNorm(torch.autograd.Function):
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if wx else None
         dw = torch.empty(D, dtype=ctx.pdt, device=x.device) if ww else None
         db = torch.empty(D, dtype=ctx.pdt, device=x.device) if wb else None
-        ws = _workspace(lib().glif_layer_norm_bwd_workspace(xr.shape[0], D, int(ww or wb)), x.device)
+        ws = _workspace(lib().glif_layer_norm_bwd_workspace(xr.shape[0], D, DTYPES[x.dtype], int(ww or wb)), x.device)
         w = _dense(weight)
         with _on(x.device):
             check(lib().glif_layer_norm_bwd(ptr(gr), gs, ptr(xr), xs, ptr(w), DTYPES[x.dtype], DTYPES[ctx.pdt], xr.shape[0], D,
