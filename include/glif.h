@@ -340,7 +340,7 @@ int glif_linear_bwd(const void *dy, int64_t lddy, const void *pre, const void *x
 int glif_short_conv_fwd(const void *x, int64_t x_stride_t, int64_t x_stride_b, const void *weight, const void *bias,
                         const void *state, const int32_t *lengths, int32_t dtype, int32_t param_dtype, int32_t T, int32_t B,
                         int32_t D, int32_t W, int32_t silu, void *y, void *last, void *stream);
-size_t glif_short_conv_bwd_workspace(int32_t T, int32_t B, int32_t D, int32_t W);
+size_t glif_short_conv_bwd_workspace(int32_t dtype, int32_t T, int32_t B, int32_t D, int32_t W);
 int glif_short_conv_bwd(const void *dy, int64_t dy_stride_t, int64_t dy_stride_b, const void *dlast, const void *x,
                         int64_t x_stride_t, int64_t x_stride_b, const void *weight, const void *bias, const void *state,
                         const int32_t *lengths, int32_t dtype, int32_t param_dtype, int32_t T, int32_t B, int32_t D,

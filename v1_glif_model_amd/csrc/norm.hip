@@ -19,12 +19,11 @@ struct NormArgs {
     const void *x, *dy, *weight, *bias;
     void *y, *dx, *dweight, *dbias;
     int64_t rows, D, x_stride, dy_stride;
-    int64_t row0;      // first row of this launch
     int32_t pdt;
     float eps;
     float4 *stat;      // [rows] mean, rstd, mean(dyw), mean(dyw xh) (backward of wide rows)
     float *part;       // [parts][2][D] sums of dw and db
-    int32_t parts, part0;
+    int32_t parts;
 };
 
 // ---- the threads of a row -----------------------------------------------------------------------------------------------
@@ -366,12 +365,11 @@ __global__ void __launch_bounds__(kWide) k_norm_fwd_wide(NormArgs a) {
 
 // Per row mean, rstd, mean(dyw), mean(dyw xh).
 template <typename T>
-__global__ void __launch_bounds__(kWide) k_norm_stats(NormArgs a) {
+__device__ __forceinline__ void wide_stats(const NormArgs &a, int64_t r) {
     constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
     __shared__ Moments red[kWide / kWave];
     __shared__ float red2[2 * kWide / kWave];
-    const int64_t r = a.row0 + blockIdx.x;
     const int D = static_cast<int>(a.D), first = threadIdx.x * V;
     const T *x = static_cast<const T *>(a.x) + r * a.x_stride, *dy = static_cast<const T *>(a.dy) + r * a.dy_stride;
     const float k = first < D ? to_f32(x[first]) : 0.0f;
@@ -396,16 +394,15 @@ __global__ void __launch_bounds__(kWide) k_norm_stats(NormArgs a) {
     if (threadIdx.x == 0) a.stat[r] = make_float4(m.mean, rstd, g.x / static_cast<float>(D), g.y / static_cast<float>(D));
 }
 
-// dx and the columns' sums: a thread per 16 bytes of columns over one of the launch's parts of its rows.
+// dx of rows r0 .. r1 - 1 and the columns' sums over them, to a part: a thread per 16 bytes of columns.
 template <typename T>
-__global__ void __launch_bounds__(kBlock) k_norm_columns(NormArgs a, int32_t parts) {
+__device__ __forceinline__ void wide_columns(const NormArgs &a, int block, int64_t r0, int64_t r1, int to) {
     constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
     const int D = static_cast<int>(a.D);
-    const int64_t c64 = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * V;
+    const int64_t c64 = (static_cast<int64_t>(block) * kWide + threadIdx.x) * V;
     if (c64 >= D) return;
     const int c = static_cast<int>(c64);
-    const int64_t n = a.rows - a.row0, r0 = a.row0 + n * blockIdx.y / parts, r1 = a.row0 + n * (blockIdx.y + 1) / parts;
     float dw[V] = {}, db[V] = {}, w[V];
     params<V>(w, a.weight, a.pdt, c, D, 1.0f);
     const T *x = static_cast<const T *>(a.x) + c, *dy = static_cast<const T *>(a.dy) + c;
@@ -436,10 +433,28 @@ __global__ void __launch_bounds__(kBlock) k_norm_columns(NormArgs a, int32_t par
         }
     }
     if (!a.part) return;
-    float *part = a.part + static_cast<int64_t>(a.part0 + blockIdx.y) * 2 * a.D + c;
+    float *part = a.part + static_cast<int64_t>(to) * 2 * a.D + c;
 #pragma unroll
     for (int e = 0; e < V; ++e)
         if (c + e < D) part[e] = dw[e], part[a.D + e] = db[e];
+}
+
+// One launch of a wide backward: the columns of the rows [col0, col1), whose statistics the launch before took, and the
+// statistics of the next rows [row0, row1) beside them.
+struct Round {
+    int64_t col0, col1, row0, row1;
+    int32_t cols, parts, part0;   // column blocks, parts, the first part
+};
+template <typename T>
+__global__ void __launch_bounds__(kWide) k_norm_round(NormArgs a, Round k) {
+    const int64_t rows = k.row1 - k.row0;
+    if (blockIdx.x < rows) {
+        wide_stats<T>(a, k.row0 + blockIdx.x);
+    } else {
+        const int b = static_cast<int>(blockIdx.x - rows), part = b / k.cols;
+        const int64_t n = k.col1 - k.col0;
+        wide_columns<T>(a, b % k.cols, k.col0 + n * part / k.parts, k.col0 + n * (part + 1) / k.parts, k.part0 + part);
+    }
 }
 
 // The parts' sums: 32 columns by 8 threads each, which take the parts in turn.
@@ -475,13 +490,14 @@ int fused_blocks(int64_t rows, int64_t D, int64_t size) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + 4 * per - 1) / (4 * per), 512)));
 }
 
-// A wide backward's rounds of rows (both passes over 96 MB of x and dy), and parts of a round.
+// A wide backward's rounds of rows: 96 MB of x and dy (64 and 144 are slower by 10 and 3 percent at 2500 x 66000), and parts of
+// a round: a block a compute unit.
 int64_t round_rows(int64_t rows, int64_t D, int64_t size) {
     return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t(48) << 20) / (D * size)));
 }
 int round_parts(int64_t n, int64_t D, int64_t size) {
-    const int64_t cols = (D * size / 16 + kBlock) / kBlock;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, 1024 / cols)));
+    const int64_t cols = ((D * size + 15) / 16 + kWide - 1) / kWide;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, 272 / cols)));
 }
 
 void carve(Carver &c, NormArgs &a, int64_t size, bool param) {
@@ -524,8 +540,7 @@ void bwd(const NormArgs &a, hipStream_t s) {
 }
 
 template <typename T>
-void run_bwd(const NormArgs &all, hipStream_t s) {
-    NormArgs a = all;
+void run_bwd(const NormArgs &a, hipStream_t s) {
     const int64_t p = (a.D + kVecBytes16<T> - 1) / kVecBytes16<T>, size = sizeof(T);
     if (a.D * size <= kFused) {
         if (p <= 8) bwd<T, 8, 1>(a, s);
@@ -537,17 +552,19 @@ void run_bwd(const NormArgs &all, hipStream_t s) {
         else if (p <= 512) bwd<T, 256, 2>(a, s);
         else bwd<T, 256, 4>(a, s);
     } else {
-        const int64_t n = round_rows(all.rows, a.D, size), cols = (p + kBlock - 1) / kBlock;
-        const int parts = round_parts(n, a.D, size);
-        for (int64_t r = 0; r < all.rows; r += n, a.part0 += parts) {
-            a.row0 = r, a.rows = std::min(all.rows, r + n);
-            hipLaunchKernelGGL(k_norm_stats<T>, dim3(static_cast<unsigned>(a.rows - r)), dim3(kWide), 0, s, a);
-            hipLaunchKernelGGL(k_norm_columns<T>, dim3(static_cast<unsigned>(cols), static_cast<unsigned>(parts)), dim3(kBlock), 0, s, a,
-                               parts);
+        const int64_t n = round_rows(a.rows, a.D, size);
+        Round k{};
+        k.cols = static_cast<int32_t>((p + kWide - 1) / kWide), k.parts = round_parts(n, a.D, size), k.part0 = -k.parts;
+        while (k.col1 < a.rows) {
+            k.col0 = k.col1, k.col1 = k.row1;
+            k.row0 = k.row1, k.row1 = std::min(a.rows, k.row0 + n);
+            const int64_t blocks = k.row1 - k.row0 + (k.col1 > k.col0 ? static_cast<int64_t>(k.cols) * k.parts : 0);
+            hipLaunchKernelGGL(k_norm_round<T>, dim3(static_cast<unsigned>(blocks)), dim3(kWide), 0, s, a, k);
+            k.part0 += k.parts;
         }
     }
     if (a.part)
-        hipLaunchKernelGGL(k_norm_join, dim3(static_cast<unsigned>((a.D + 31) / 32)), dim3(kBlock), 0, s, all);
+        hipLaunchKernelGGL(k_norm_join, dim3(static_cast<unsigned>((a.D + 31) / 32)), dim3(kBlock), 0, s, a);
 }
 
 int check_norm(int64_t rows, int64_t D, int32_t dtype, int32_t pdt, float eps) {

@@ -32,6 +32,22 @@ __device__ inline uint32_t philox_word(uint64_t seed, uint64_t i) {
     return w == 0 ? c0 : (w == 1 ? c1 : (w == 2 ? c2 : c3));
 }
 
+// The four words of a block (elements 4 blk .. 4 blk + 3).
+__device__ inline void philox_block(uint64_t seed, uint64_t blk, uint32_t (&c)[4]) {
+    c[0] = static_cast<uint32_t>(blk), c[1] = static_cast<uint32_t>(blk >> 32), c[2] = 0u, c[3] = 0u;
+    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t p0 = static_cast<uint64_t>(kPhM0) * c[0], p1 = static_cast<uint64_t>(kPhM1) * c[2];
+        c[0] = static_cast<uint32_t>(p1 >> 32) ^ c[1] ^ k0;
+        c[2] = static_cast<uint32_t>(p0 >> 32) ^ c[3] ^ k1;
+        c[1] = static_cast<uint32_t>(p1);
+        c[3] = static_cast<uint32_t>(p0);
+        k0 += kPhW0;
+        k1 += kPhW1;
+    }
+}
+
 // fp32 in [0, 1): the word's top 24 bits times 2^-24 (exact)
 __device__ inline float philox_uniform(uint64_t seed, uint64_t i) {
     return static_cast<float>(philox_word(seed, i) >> 8) * 5.9604644775390625e-08f;

@@ -317,7 +317,7 @@ class _ShortConv(torch.autograd.Function):
         dw = torch.empty((D, W), dtype=ctx.pdt, device=dev) if ww else None
         db = torch.empty(D, dtype=ctx.pdt, device=dev) if wb else None
         ds = torch.empty((B, W - 1, D), dtype=x.dtype, device=dev) if ws_ else None
-        ws = _workspace(lib().glif_short_conv_bwd_workspace(T, B, D, W) if ww or wb else 0, dev)
+        ws = _workspace(lib().glif_short_conv_bwd_workspace(DTYPES[x.dtype], T, B, D, W) if ww or wb else 0, dev)
         with _on(dev):
             check(lib().glif_short_conv_bwd(ptr(dy), dy.stride(0), dy.stride(1), ptr(dlast), ptr(xs), xs.stride(0), xs.stride(1),
                                             ptr(w), ptr(b), ptr(st), ptr(lengths), DTYPES[x.dtype], DTYPES[ctx.pdt], T, B, D, W,
