@@ -4,14 +4,11 @@
 // inputs before `len`.  Ticks from `len` on are not read, their y is 0 and they take no part in any gradient:
 //   dp[t] = dy[t] act'(pre[t]),   dx[t] = sum_k w[k] dp[t + (W - 1) - k] (+ the state's gradient where x[t] is in it)
 //   dw[k] = sum_{t, b} dp[t] x[t - (W - 1) + k],   db = sum_{t, b} dp[t]
-// Sequences are [T][B][D], channels next to each other.  A thread owns the channels of 16 bytes and walks a segment of ticks,
+// Sequences are [T][B][D], channels next to each other.  A thread owns a few neighbouring channels and walks a segment of ticks,
 // four at a time with the next four on their way, its taps and its window of inputs in registers; a block is C such threads
 // side by side by 256 / C segments, whose sums of dw and db it adds up.  Bound by memory: x in and y out, x and dy in and dx
 // out.  The last W - 1 ticks' inputs of the segment before are read again, from cache.
 #include "seq.h"
-#ifndef SEG0
-#define SEG0 64
-#endif
 
 namespace glif {
 namespace {
@@ -35,9 +32,8 @@ __device__ __forceinline__ int length_of(const int32_t *lengths, int b, int T) {
 }
 
 // The channels of a thread: V from c on, `have` of which exist.
-template <typename T>
+template <typename T, int V>
 struct Chan {
-    static constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
     int c, have, seg;
     __device__ __forceinline__ Chan(const ConvArgs &a) {
@@ -92,17 +88,16 @@ struct Chan {
 };
 
 // x at tick t, which may lie in the state
-template <typename T, int W>
-__device__ __forceinline__ Vec<T, kVecBytes16<T>> x_at(const ConvArgs &a, const Chan<T> &me, int t, int b) {
+template <typename T, int V, int W>
+__device__ __forceinline__ Vec<T, V> x_at(const ConvArgs &a, const Chan<T, V> &me, int t, int b) {
     if (t >= 0) return me.load(static_cast<const T *>(a.x) + t * a.x_st + b * a.x_sb);
     if (a.state) return me.load(static_cast<const T *>(a.state) + (static_cast<int64_t>(b) * (W - 1) + (W - 1 + t)) * a.D);
     return {};
 }
 
 // W - 1 ticks before the segment, then kAhead of it at a time
-template <typename T, int W>
+template <typename T, int V, int W>
 struct Window {
-    static constexpr int V = kVecBytes16<T>;
     float x[W - 1 + kAhead][V];
     __device__ __forceinline__ void set(int i, Vec<T, V> v) {
 #pragma unroll
@@ -116,11 +111,10 @@ struct Window {
     }
 };
 
-template <typename T, int W>
+template <typename T, int V, int W>
 __global__ void __launch_bounds__(kBlock) k_conv_fwd(ConvArgs a) {
-    constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
-    const Chan<T> me(a);
+    const Chan<T, V> me(a);
     if (me.have <= 0 || me.seg >= a.segs) return;
     const int b = blockIdx.z, t0 = me.seg * a.seg, t1 = min(t0 + a.seg, a.T), len = length_of(a.lengths, b, a.T), end = min(t1, len);
     float w[W][V], bias[V];
@@ -128,7 +122,7 @@ __global__ void __launch_bounds__(kBlock) k_conv_fwd(ConvArgs a) {
     const T *x = static_cast<const T *>(a.x) + b * a.x_sb;
     T *y = static_cast<T *>(a.y) + static_cast<int64_t>(b) * a.D;
     const int64_t y_st = static_cast<int64_t>(a.B) * a.D;
-    Window<T, W> win;
+    Window<T, V, W> win;
     vec next[kAhead];
     auto fetch = [&](int t) {
 #pragma unroll
@@ -136,7 +130,7 @@ __global__ void __launch_bounds__(kBlock) k_conv_fwd(ConvArgs a) {
     };
     if (t0 < end) {
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) win.set(k, x_at<T, W>(a, me, t0 - (W - 1) + k, b));
+        for (int k = 0; k < W - 1; ++k) win.set(k, x_at<T, V, W>(a, me, t0 - (W - 1) + k, b));
         fetch(t0);
     }
     for (int t = t0; t < end; t += kAhead) {
@@ -162,7 +156,7 @@ __global__ void __launch_bounds__(kBlock) k_conv_fwd(ConvArgs a) {
     for (int t = max(t0, end); t < t1; ++t) me.store(y + t * y_st, zero);
     if (a.last && me.seg == 0)
         for (int j = 0; j < W - 1; ++j) {
-            const vec v = x_at<T, W>(a, me, len - (W - 1) + j, b);
+            const vec v = x_at<T, V, W>(a, me, len - (W - 1) + j, b);
             float f[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) f[e] = to_f32(static_cast<T>(v[e]));
@@ -170,12 +164,11 @@ __global__ void __launch_bounds__(kBlock) k_conv_fwd(ConvArgs a) {
         }
 }
 
-template <typename T, int W>
+template <typename T, int V, int W>
 __global__ void __launch_bounds__(kBlock) k_conv_bwd(ConvArgs a) {
-    constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
     __shared__ float sum[kBlock * V];
-    const Chan<T> me(a);
+    const Chan<T, V> me(a);
     const bool on = me.have > 0 && me.seg < a.segs;
     const int b = blockIdx.z, t0 = me.seg * a.seg, t1 = min(t0 + a.seg, a.T), len = length_of(a.lengths, b, a.T);
     float dw[W][V] = {}, db[V] = {};
@@ -186,7 +179,7 @@ __global__ void __launch_bounds__(kBlock) k_conv_bwd(ConvArgs a) {
         T *dx = a.dx ? static_cast<T *>(a.dx) + static_cast<int64_t>(b) * a.D : nullptr;
         const int64_t dx_st = static_cast<int64_t>(a.B) * a.D;
         const int end = min(t1 + W - 1, len), first = me.seg == 0 ? -(W - 1) : t0;   // the first tick whose gradient this segment writes
-        Window<T, W> win;
+        Window<T, V, W> win;
         float dp[W - 1 + kAhead][V] = {};   // dp[W - 1 + i] of tick t + i
         vec next_x[kAhead], next_g[kAhead];
         auto fetch = [&](int t) {
@@ -197,7 +190,7 @@ __global__ void __launch_bounds__(kBlock) k_conv_bwd(ConvArgs a) {
             }
         };
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) win.set(k, t0 < len ? x_at<T, W>(a, me, t0 - (W - 1) + k, b) : vec{});
+        for (int k = 0; k < W - 1; ++k) win.set(k, t0 < len ? x_at<T, V, W>(a, me, t0 - (W - 1) + k, b) : vec{});
         fetch(t0);
         for (int t = t0; t < t1 + W - 1; t += kAhead) {
 #pragma unroll
@@ -296,11 +289,10 @@ __global__ void __launch_bounds__(kBlock) k_conv_join(ConvArgs a) {
 }
 
 // One tick: y from the state and x, and the state moved on by x.
-template <typename T, int W>
+template <typename T, int V, int W>
 __global__ void __launch_bounds__(kBlock) k_conv_step(ConvArgs a) {
-    constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
-    const Chan<T> me(a);
+    const Chan<T, V> me(a);
     const int b = blockIdx.z * (kBlock / a.C) + threadIdx.x / a.C;
     if (me.have <= 0 || b >= a.B) return;
     T *st = static_cast<T *>(a.last) + static_cast<int64_t>(b) * (W - 1) * a.D;
@@ -329,14 +321,15 @@ __global__ void __launch_bounds__(kBlock) k_conv_step(ConvArgs a) {
 
 enum Pass { kFwd, kBwd, kStep };
 
-// Threads side by side: as many as there are 16 bytes of channels, up to a wave.  Segments of 64 ticks, or of 32 or 16 where
-// that gives fewer than 4096 waves.
-void shape(ConvArgs &a, int32_t dtype) {
-    const int v = 16 / static_cast<int>(dtype_size(dtype)), across = ceil_div(a.D, v);
+// Threads side by side: as many as there are pieces of v channels, up to a wave (forward 16 bytes; backward 4 channels: with
+// the 8 of a 16-bit type its windows and sums take the registers of half the waves, 500 x 32 x 2048 x 4 104 us for 57).
+// Segments of 64 ticks, or of 32 or 16 where that gives fewer than 2048 waves.
+void shape(ConvArgs &a, int v) {
+    const int across = ceil_div(a.D, v);
     a.C = 1;
     while (a.C < across && a.C < kWave) a.C *= 2;
-    a.seg = SEG0;
-    while (a.seg > 16 && static_cast<int64_t>(ceil_div(across, a.C)) * a.C * a.B * ceil_div(a.T, a.seg) < 4096 * kWave) a.seg /= 2;
+    a.seg = 64;
+    while (a.seg > 16 && static_cast<int64_t>(ceil_div(across, a.C)) * a.C * a.B * ceil_div(a.T, a.seg) < 2048 * kWave) a.seg /= 2;
     a.segs = std::max(1, ceil_div(a.T, a.seg));
     a.parts = a.B * ceil_div(a.segs, kBlock / a.C);
 }
@@ -348,11 +341,12 @@ void join(const ConvArgs &a, hipStream_t s) {
 
 template <typename T, int W>
 void launch(const ConvArgs &a, Pass pass, hipStream_t s) {
-    const unsigned cols = static_cast<unsigned>(ceil_div(ceil_div(a.D, kVecBytes16<T>), a.C)), deep = kBlock / a.C;
+    constexpr int V = kVecBytes16<T>, VB = 4;
+    const unsigned cols = static_cast<unsigned>(ceil_div(ceil_div(a.D, pass == kBwd ? VB : V), a.C)), deep = kBlock / a.C;
     const dim3 grid(cols, (a.segs + deep - 1) / deep, static_cast<unsigned>(a.B));
-    if (pass == kStep) hipLaunchKernelGGL((k_conv_step<T, W>), dim3(cols, 1, (a.B + deep - 1) / deep), dim3(kBlock), 0, s, a);
-    else if (pass == kFwd) hipLaunchKernelGGL((k_conv_fwd<T, W>), grid, dim3(kBlock), 0, s, a);
-    else hipLaunchKernelGGL((k_conv_bwd<T, W>), grid, dim3(kBlock), 0, s, a);
+    if (pass == kStep) hipLaunchKernelGGL((k_conv_step<T, V, W>), dim3(cols, 1, (a.B + deep - 1) / deep), dim3(kBlock), 0, s, a);
+    else if (pass == kFwd) hipLaunchKernelGGL((k_conv_fwd<T, V, W>), grid, dim3(kBlock), 0, s, a);
+    else hipLaunchKernelGGL((k_conv_bwd<T, VB, W>), grid, dim3(kBlock), 0, s, a);
 }
 
 template <typename T>
@@ -393,7 +387,7 @@ int glif_short_conv_fwd(const void *x, int64_t x_stride_t, int64_t x_stride_b, c
     ConvArgs a{};
     a.x = x, a.weight = weight, a.bias = bias, a.state = state, a.lengths = lengths, a.y = y, a.last = W > 1 ? last : nullptr;
     a.x_st = x_stride_t, a.x_sb = x_stride_b, a.T = T, a.B = B, a.D = D, a.W = W, a.pdt = param_dtype, a.silu = silu;
-    shape(a, dtype);
+    shape(a, 16 / static_cast<int>(dtype_size(dtype)));
     GLIF_BY_DTYPE(dtype, by_taps, a, W, kFwd, static_cast<hipStream_t>(stream));
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;
@@ -403,7 +397,7 @@ size_t glif_short_conv_bwd_workspace(int32_t dtype, int32_t T, int32_t B, int32_
     if (check_conv(dtype, dtype, T, B, D, W)) return 0;
     ConvArgs a{};
     a.T = T, a.B = B, a.D = D;
-    shape(a, dtype);
+    shape(a, 4);
     return static_cast<size_t>(a.parts) * (W + 1) * D * sizeof(float) + 256;
 }
 
@@ -419,7 +413,7 @@ int glif_short_conv_bwd(const void *dy, int64_t dy_stride_t, int64_t dy_stride_b
     a.dx = dx, a.dweight = dweight, a.dbias = dbias, a.dstate = W > 1 ? dstate : nullptr;
     a.x_st = x_stride_t, a.x_sb = x_stride_b, a.dy_st = dy_stride_t, a.dy_sb = dy_stride_b;
     a.T = T, a.B = B, a.D = D, a.W = W, a.pdt = param_dtype, a.silu = silu;
-    shape(a, dtype);
+    shape(a, 4);
     if (dweight || dbias) {
         Carver c(ws, ws_bytes);
         a.part = c.take<float>(static_cast<size_t>(a.parts) * (W + 1) * D);
@@ -440,7 +434,7 @@ int glif_short_conv_step(const void *x, int64_t x_stride_b, void *state, const v
     ConvArgs a{};
     a.x = x, a.weight = weight, a.bias = bias, a.last = state, a.y = y;
     a.x_sb = x_stride_b, a.T = 1, a.B = B, a.D = D, a.W = W, a.pdt = param_dtype, a.silu = silu;
-    shape(a, dtype);
+    shape(a, 16 / static_cast<int>(dtype_size(dtype)));
     GLIF_BY_DTYPE(dtype, by_taps, a, W, kStep, static_cast<hipStream_t>(stream));
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;
