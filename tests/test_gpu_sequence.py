@@ -630,6 +630,16 @@ def test_refusals():
             print("not refused:", k)
 
 
+def test_no_second_gradient():
+    """The backwards are not recorded: a graph of them is refused."""
+    from v1_glif_model_amd import sequence as seq
+    x = rnd(295, 4, 8).requires_grad_(True)
+    for y in (seq.layer_norm(x), seq.dropout(x, 0.5, 1), seq.linear(x, rnd(296, 3, 8), activation="gelu"),
+              seq.short_conv(x[:, None], rnd(297, 8, 2))[0]):
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_c_entries_refuse():
     """The C entries check for themselves: status codes and a message, nothing launched."""
     import ctypes as C

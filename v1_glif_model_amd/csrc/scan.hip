@@ -570,31 +570,47 @@ __global__ void __launch_bounds__(kBlock) k_scan_step(ScanArgs a) {
     const glif_scan &s = a.s;
     const Lane<SPL> me(a);
     if (!me.on) return;
-    const int N = s.n_state;
-    const int64_t chan = static_cast<int64_t>(me.b) * s.n_channels + me.d, map = static_cast<int64_t>(me.g) * N;
-    const T *B = static_cast<const T *>(s.B) + me.b * s.B_sb + map, *C = static_cast<const T *>(s.C) + me.b * s.C_sb + map;
-    float A[kQ], h[kQ], slope, y[1] = {0.0f};
-    load_q(A, s.A, static_cast<int64_t>(me.d) * N, me.n0, N);
-    load_q(h, a.last, chan * N, me.n0, N);
+    const int N = s.n_state, n0 = me.n0;
+    const int64_t chan = static_cast<int64_t>(me.b) * s.n_channels + me.d, map = static_cast<int64_t>(me.g) * N + n0;
+    const T *Bp = static_cast<const T *>(s.B) + me.b * s.B_sb + map, *Cp = static_cast<const T *>(s.C) + me.b * s.C_sb + map;
+    float *hp = a.last + chan * N + n0;
+    const float *Ap = s.A + static_cast<int64_t>(me.d) * N + n0;
+    typedef Vec<float, kQ> fvec;
+    typedef Vec<T, kQ> tvec;
+    fvec A = {}, h = {};
+    tvec B = {}, C = {};
+    const bool whole = n0 + kQ <= N;
+    if (whole) {
+        A = *reinterpret_cast<const fvec *>(Ap), h = *reinterpret_cast<const fvec *>(hp);
+        B = *reinterpret_cast<const tvec *>(Bp), C = *reinterpret_cast<const tvec *>(Cp);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kQ; ++j)
+            if (n0 + j < N) A[j] = Ap[j], h[j] = hp[j], B[j] = Bp[j], C[j] = Cp[j];
+    }
     const float u = to_f32(static_cast<const T *>(s.u)[me.b * s.u_sb + me.d]);
     const float raw = to_f32(static_cast<const T *>(s.delta)[me.b * s.delta_sb + me.d]) + (s.delta_bias ? s.delta_bias[me.d] : 0.0f);
+    const float q = s.z ? to_f32(static_cast<const T *>(s.z)[me.b * s.z_sb + me.d]) : 0.0f, skip = s.D ? s.D[me.d] : 0.0f;
+    float slope, y = 0.0f;
     const float step = step_of(raw, s.softplus, true, slope), su = step * u;
 #pragma unroll
     for (int j = 0; j < kQ; ++j) {
-        const bool real = me.n0 + j < N;
-        h[j] = fmaf(__builtin_amdgcn_exp2f(step * (A[j] * kLog2e)), h[j], su * (real ? to_f32(B[me.n0 + j]) : 0.0f));
-        y[0] = fmaf(real ? to_f32(C[me.n0 + j]) : 0.0f, h[j], y[0]);
-        if (real) a.last[chan * N + me.n0 + j] = h[j];
+        h[j] = fmaf(__builtin_amdgcn_exp2f(step * (A[j] * kLog2e)), h[j], su * to_f32(static_cast<T>(B[j])));
+        y = fmaf(to_f32(static_cast<T>(C[j])), h[j], y);
+    }
+    if (whole) {
+        *reinterpret_cast<fvec *>(hp) = h;
+    } else {
+#pragma unroll
+        for (int j = 0; j < kQ; ++j)
+            if (n0 + j < N) hp[j] = h[j];
     }
 #pragma unroll
-    for (int m = 1; m < SPL; m <<= 1) y[0] += __shfl_xor(y[0], m, kWave);
+    for (int m = 1; m < SPL; m <<= 1) y += __shfl_xor(y, m, kWave);
     if (me.s != 0) return;
-    float v = fmaf(s.D ? s.D[me.d] : 0.0f, u, y[0]);
-    if (s.z) {
-        const float q = to_f32(static_cast<const T *>(s.z)[me.b * s.z_sb + me.d]);
-        v *= q * sigmoid_f(q);
-    }
-    static_cast<T *>(a.y)[chan] = from_f32<T>(v);
+    y = fmaf(skip, u, y);
+    if (s.z) y *= q * sigmoid_f(q);
+    static_cast<T *>(a.y)[chan] = from_f32<T>(y);
 }
 
 int lanes_for(int32_t N) {
@@ -603,9 +619,6 @@ int lanes_for(int32_t N) {
     return l;
 }
 
-#ifndef SEGW
-#define SEGW 4096
-#endif
 // Blocks and segments.  Time is split where the channels give fewer than 2 waves a SIMD, into segments of at least 64 ticks
 // until there are about 4.
 void shape(ScanArgs &a) {
@@ -613,7 +626,7 @@ void shape(ScanArgs &a) {
     a.np = spl * kQ;
     a.blocks = ceil_div(a.s.n_channels / a.s.n_groups, chan * kWaves);
     const int64_t waves = static_cast<int64_t>(a.blocks) * a.s.n_groups * kWaves * std::max(a.s.n_batch, 1);
-    int64_t segs = waves >= 2048 ? 1 : std::max<int64_t>(1, std::min<int64_t>(SEGW / waves, a.s.n_ticks / 64));
+    int64_t segs = waves >= 2048 ? 1 : std::max<int64_t>(1, std::min<int64_t>(4096 / waves, a.s.n_ticks / 64));
     a.seg = std::max(ceil_div(ceil_div(a.s.n_ticks, segs), chunk) * chunk, chunk);
     a.segs = std::max(1, ceil_div(a.s.n_ticks, a.seg));
 }

@@ -21,10 +21,9 @@ import math
 from ctypes import byref
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_ptr
+from ._lib import check, lib
 
 __all__ = ["layer_norm", "dropout", "linear", "short_conv", "short_conv_step", "state_space_scan", "state_space_step"]
 
@@ -35,15 +34,16 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 # ------------------------------------------------------------------ the arguments ----
 def _need(t, name, shape=None, dtype=None, device=None):
     """ValueError unless ``t`` is a device tensor of the wanted shape (None: any size), type and device."""
-    if not torch.is_tensor(t) or not t.is_cuda:
-        if torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        if isinstance(t, torch.Tensor):
             _lib.require_gpu()
         raise ValueError(f"{name} must be a tensor on the GPU")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other arguments are on {device}")
-    if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+    if dtype is not None and t.dtype is not dtype and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
         raise ValueError(f"{name} must be of type {dtype}, got {t.dtype}")
-    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != h for w, h in zip(shape, t.shape))):
+    if shape is not None and t.shape != shape and (
+            t.dim() != len(shape) or any(w is not None and w != h for w, h in zip(shape, t.shape))):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
@@ -111,13 +111,35 @@ def _size(ws):
     return 0 if ws is None else ws.numel()
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """The calls below launch on the current device: make it the tensors'."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _p(t):
+    """A tensor's address for a C argument (None: NULL)."""
+    return None if t is None else t.data_ptr()
+
+
+def _stream(device):
+    return _lib._raw_stream(device.index)
+
+
+def _first_only(name):
+    """The gradients are computed outside autograd: a graph of them would be wrong without a word."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} is differentiable once: create_graph is not supported")
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _refuse_grad(name, *tensors):
@@ -149,15 +171,15 @@ class _LayerNorm(torch.autograd.Function):
         w, b = _dense(weight), _dense(bias)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         with _on(x.device):
-            check(lib().glif_layer_norm_fwd(ptr(xr), xs, ptr(w), ptr(b), DTYPES[x.dtype], DTYPES[pdt], xr.shape[0], D, eps,
-                                            ptr(y), stream_ptr(x.device)))
+            check(lib().glif_layer_norm_fwd(_p(xr), xs, _p(w), _p(b), DTYPES[x.dtype], DTYPES[pdt], xr.shape[0], D, eps,
+                                            _p(y), _stream(x.device)))
         ctx.save_for_backward(x, weight)
         ctx.eps, ctx.pdt = eps, pdt
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_only("layer_norm")
         x, weight = ctx.saved_tensors
         D = x.shape[-1]
         xr, xs = _rows(x, D)
@@ -169,8 +191,8 @@ class _LayerNorm(torch.autograd.Function):
         ws = _workspace(lib().glif_layer_norm_bwd_workspace(xr.shape[0], D, DTYPES[x.dtype], int(ww or wb)), x.device)
         w = _dense(weight)
         with _on(x.device):
-            check(lib().glif_layer_norm_bwd(ptr(gr), gs, ptr(xr), xs, ptr(w), DTYPES[x.dtype], DTYPES[ctx.pdt], xr.shape[0], D,
-                                            ctx.eps, ptr(dx), ptr(dw), ptr(db), ptr(ws), _size(ws), stream_ptr(x.device)))
+            check(lib().glif_layer_norm_bwd(_p(gr), gs, _p(xr), xs, _p(w), DTYPES[x.dtype], DTYPES[ctx.pdt], xr.shape[0], D,
+                                            ctx.eps, _p(dx), _p(dw), _p(db), _p(ws), _size(ws), _stream(x.device)))
         return dx, dw, db, None, None
 
 
@@ -192,7 +214,7 @@ def _dropout(x, residual, p, seed, offset):
     x, residual = _dense(x), _dense(residual)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     with _on(x.device):
-        check(lib().glif_dropout(ptr(x), ptr(residual), DTYPES[x.dtype], x.numel(), p, seed, offset, ptr(y), stream_ptr(x.device)))
+        check(lib().glif_dropout(_p(x), _p(residual), DTYPES[x.dtype], x.numel(), p, seed, offset, _p(y), _stream(x.device)))
     return y
 
 
@@ -203,8 +225,8 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, residual, p, seed, offset)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_only("dropout")
         dx = _dropout(dy, None, *ctx.draw) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
@@ -240,15 +262,15 @@ class _Linear(torch.autograd.Function):
         L = lib()
         ws = _workspace(L.glif_linear_fwd_workspace(dt, M, N, K), x.device)
         with _on(x.device):
-            check(L.glif_linear_fwd(ptr(xr), ldx, ptr(wr), ldw, ptr(b), ptr(rr), ldr, dt, DTYPES[bdt], M, N, K, act, ptr(y),
-                                    ptr(pre), ptr(ws), _size(ws), stream_ptr(x.device)))
+            check(L.glif_linear_fwd(_p(xr), ldx, _p(wr), ldw, _p(b), _p(rr), ldr, dt, DTYPES[bdt], M, N, K, act, _p(y),
+                                    _p(pre), _p(ws), _size(ws), _stream(x.device)))
         ctx.save_for_backward(x, weight, pre)
         ctx.act, ctx.bdt, ctx.M = act, bdt, M
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_only("linear")
         x, weight, pre = ctx.saved_tensors
         N, K = weight.shape
         M, dt, dev = ctx.M, DTYPES[x.dtype], x.device
@@ -264,8 +286,8 @@ class _Linear(torch.autograd.Function):
             odd = any(v % (16 // x.element_size()) for v in (ldx, ldw, ldg, N, K)) or any(t.data_ptr() % 16 for t in (xr, wr, gr))
             ws = _workspace(L.glif_linear_bwd_workspace(dt, M, N, K, ctx.act, int(odd)), dev)
             with _on(dev):
-                check(L.glif_linear_bwd(ptr(gr), ldg, ptr(pre), ptr(xr), ldx, ptr(wr), ldw, dt, DTYPES[ctx.bdt], M, N, K,
-                                        ctx.act, ptr(dx), ptr(dw), ptr(db), ptr(ws), _size(ws), stream_ptr(dev)))
+                check(L.glif_linear_bwd(_p(gr), ldg, _p(pre), _p(xr), ldx, _p(wr), ldw, dt, DTYPES[ctx.bdt], M, N, K,
+                                        ctx.act, _p(dx), _p(dw), _p(db), _p(ws), _size(ws), _stream(dev)))
         return dx, dw, db, dy if wr_ else None, None, None
 
 
@@ -298,16 +320,16 @@ class _ShortConv(torch.autograd.Function):
         y = torch.empty((T, B, D), dtype=x.dtype, device=x.device)
         last = torch.empty((B, W - 1, D), dtype=x.dtype, device=x.device)
         with _on(x.device):
-            check(lib().glif_short_conv_fwd(ptr(xs), xs.stride(0), xs.stride(1), ptr(w), ptr(b), ptr(st), ptr(lengths),
-                                            DTYPES[x.dtype], DTYPES[pdt], T, B, D, W, silu, ptr(y), ptr(last),
-                                            stream_ptr(x.device)))
+            check(lib().glif_short_conv_fwd(_p(xs), xs.stride(0), xs.stride(1), _p(w), _p(b), _p(st), _p(lengths),
+                                            DTYPES[x.dtype], DTYPES[pdt], T, B, D, W, silu, _p(y), _p(last),
+                                            _stream(x.device)))
         ctx.save_for_backward(x, weight, bias, state, lengths)
         ctx.silu, ctx.pdt = silu, pdt
         return y, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dlast):
+        _first_only("short_conv")
         x, weight, bias, state, lengths = ctx.saved_tensors
         (T, B, D), W, dev = x.shape, weight.shape[1], x.device
         wx, ww, wb, ws_ = ctx.needs_input_grad[:4]
@@ -319,9 +341,9 @@ class _ShortConv(torch.autograd.Function):
         ds = torch.empty((B, W - 1, D), dtype=x.dtype, device=dev) if ws_ else None
         ws = _workspace(lib().glif_short_conv_bwd_workspace(DTYPES[x.dtype], T, B, D, W) if ww or wb else 0, dev)
         with _on(dev):
-            check(lib().glif_short_conv_bwd(ptr(dy), dy.stride(0), dy.stride(1), ptr(dlast), ptr(xs), xs.stride(0), xs.stride(1),
-                                            ptr(w), ptr(b), ptr(st), ptr(lengths), DTYPES[x.dtype], DTYPES[ctx.pdt], T, B, D, W,
-                                            ctx.silu, ptr(dx), ptr(dw), ptr(db), ptr(ds), ptr(ws), _size(ws), stream_ptr(dev)))
+            check(lib().glif_short_conv_bwd(_p(dy), dy.stride(0), dy.stride(1), _p(dlast), _p(xs), xs.stride(0), xs.stride(1),
+                                            _p(w), _p(b), _p(st), _p(lengths), DTYPES[x.dtype], DTYPES[ctx.pdt], T, B, D, W,
+                                            ctx.silu, _p(dx), _p(dw), _p(db), _p(ds), _p(ws), _size(ws), _stream(dev)))
         return dx, dw, db, ds, None, None, None
 
 
@@ -368,8 +390,8 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     w, b = _dense(weight), _dense(bias)
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
     with _on(x.device):
-        check(lib().glif_short_conv_step(ptr(x), x.stride(0), ptr(state), ptr(w), ptr(b), DTYPES[x.dtype], DTYPES[pdt], B, D, W,
-                                         silu, ptr(y), stream_ptr(x.device)))
+        check(lib().glif_short_conv_step(_p(x), x.stride(0), _p(state), _p(w), _p(b), DTYPES[x.dtype], DTYPES[pdt], B, D, W,
+                                         silu, _p(y), _stream(x.device)))
     torch.autograd.graph.increment_version(state)
     return y
 
@@ -377,24 +399,13 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
 # ------------------------------------------------------------------------ state space ----
 def _scan_struct(u, delta, A, B_, C_, D, z, bias, state, lengths, softplus, ticks):
     """glif_scan of contiguous-enough tensors (held by the caller)."""
-    s = _lib.Scan()
-    s.u, s.delta, s.z, s.B, s.C = (t.data_ptr() if t is not None else None for t in (u, delta, z, B_, C_))
-    s.A = A.data_ptr()
-    s.D, s.delta_bias, s.state, s.lengths = (t.data_ptr() if t is not None else None for t in (D, bias, state, lengths))
     if ticks:
-        s.u_st, s.u_sb, s.delta_st, s.delta_sb = u.stride(0), u.stride(1), delta.stride(0), delta.stride(1)
-        s.B_st, s.B_sb, s.C_st, s.C_sb = B_.stride(0), B_.stride(1), C_.stride(0), C_.stride(1)
-        if z is not None:
-            s.z_st, s.z_sb = z.stride(0), z.stride(1)
-        s.n_ticks = u.shape[0]
+        strides = [t.stride()[:2] if t is not None else (0, 0) for t in (u, delta, z, B_, C_)]
     else:
-        s.u_sb, s.delta_sb, s.B_sb, s.C_sb = u.stride(0), delta.stride(0), B_.stride(0), C_.stride(0)
-        if z is not None:
-            s.z_sb = z.stride(0)
-        s.n_ticks = 1
-    s.dtype, s.n_batch, s.n_channels, s.n_groups = DTYPES[u.dtype], u.shape[-2], u.shape[-1], B_.shape[-2]
-    s.n_state, s.softplus = A.shape[1], softplus
-    return s
+        strides = [(0, t.stride(0)) if t is not None else (0, 0) for t in (u, delta, z, B_, C_)]
+    return _lib.Scan(_p(u), _p(delta), _p(z), _p(B_), _p(C_), _p(A), _p(D), _p(bias), _p(state), _p(lengths),
+                     *(n for pair in strides for n in pair), DTYPES[u.dtype], u.shape[0] if ticks else 1, u.shape[-2], u.shape[-1],
+                     B_.shape[-2], A.shape[1], softplus)
 
 
 class _Scan(torch.autograd.Function):
@@ -410,14 +421,14 @@ class _Scan(torch.autograd.Function):
         keep = _workspace(L.glif_scan_keep_bytes(byref(s)), dev) if any(ctx.needs_input_grad) else None
         ws = _workspace(L.glif_scan_fwd_workspace(byref(s)), dev)
         with _on(dev):
-            check(L.glif_scan_fwd(byref(s), ptr(y), ptr(last), ptr(keep), ptr(ws), _size(ws), stream_ptr(dev)))
+            check(L.glif_scan_fwd(byref(s), _p(y), _p(last), _p(keep), _p(ws), _size(ws), _stream(dev)))
         ctx.save_for_backward(u, delta, A, B_, C_, D, z, bias, state, lengths, keep)
         ctx.softplus = softplus
         return y, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dlast):
+        _first_only("state_space_scan")
         u, delta, A, B_, C_, D, z, bias, state, lengths, keep = ctx.saved_tensors
         (T, B, Dc), dev = u.shape, u.device
         held = [_seq(u), _seq(delta), _dense(A), _seq(B_), _seq(C_), _dense(D), _seq(z), _dense(bias), _dense(state), lengths]
@@ -434,7 +445,7 @@ class _Scan(torch.autograd.Function):
         L = lib()
         ws = _workspace(L.glif_scan_bwd_workspace(byref(s)), dev)
         with _on(dev):
-            check(L.glif_scan_bwd(byref(s), byref(g), ptr(keep), ptr(ws), _size(ws), stream_ptr(dev)))
+            check(L.glif_scan_bwd(byref(s), byref(g), _p(keep), _p(ws), _size(ws), _stream(dev)))
         return (*outs, None, None)
 
 
@@ -493,7 +504,7 @@ def state_space_step(u, state, delta, A, B, C, D=None, z=None, delta_bias=None, 
     s = _scan_struct(*held, int(bool(delta_softplus)), False)
     y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
     with _on(u.device):
-        check(lib().glif_scan_step(byref(s), ptr(y), ptr(state), stream_ptr(u.device)))
+        check(lib().glif_scan_step(byref(s), _p(y), _p(state), _stream(u.device)))
     torch.autograd.graph.increment_version(state)
     return y
 
