@@ -58,6 +58,33 @@ def test_layer_norm(shape, dtype):
     norm_case(x, rnd(3, shape[-1], shift=1.0, scale=0.3), rnd(4, shape[-1]), dy)
 
 
+@pytest.mark.parametrize("rows,D,dtype", [(1200, 66001, torch.bfloat16), (1200, 30001, torch.float32), (1100, 50000, torch.float16),
+                                          (700, 80000, torch.bfloat16)])
+def test_layer_norm_over_more_than_the_caches_hold(rows, D, dtype):
+    """Long rows and results larger than the caches, in several rounds of the backward: every row's ends and middle, and all
+    columns' sums, against 64 bits taken on the device."""
+    from v1_glif_model_amd import sequence as seq
+    x, dy = (torch.randn(rows, D, generator=torch.Generator(DEV).manual_seed(k), device=DEV).to(dtype) for k in (1, 2))
+    w, b = rnd(3, D, shift=1.0, scale=0.3).requires_grad_(True), rnd(4, D).requires_grad_(True)
+    xs = x.requires_grad_(True)
+    y = seq.layer_norm(xs, w, b)
+    dx, dw, db = grads(y, dy, xs, w, b)
+    with torch.no_grad():
+        x6, g6, w6 = x.double(), dy.double(), w.double()
+        mean = x6.mean(-1, keepdim=True)
+        rstd = 1.0 / torch.sqrt(((x6 - mean) ** 2).mean(-1, keepdim=True) + 1e-5)
+        xh = (x6 - mean) * rstd
+        far = (x6.abs() + x6.abs().mean(-1, keepdim=True)) * rstd
+        gw, ga = g6 * w6, g6.abs() * w6.abs()
+        dx6 = rstd * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
+        terms = rstd * (ga + ga.mean(-1, keepdim=True) * (1 + far) + far * (ga * far).mean(-1, keepdim=True))
+        for part in (slice(0, 70), slice(D // 2, D // 2 + 70), slice(D - 70, D)):
+            near(y[:, part], (xh * w6 + b.double())[:, part].cpu(), (far * w6.abs() + b.abs())[:, part].cpu(), "y")
+            near(dx[:, part], dx6[:, part].cpu(), terms[:, part].cpu(), "dx")
+        near(dw, (g6 * xh).sum(0).cpu(), (g6.abs() * far).sum(0).cpu(), "dw")
+        near(db, g6.sum(0).cpu(), g6.abs().sum(0).cpu(), "db")
+
+
 @pytest.mark.parametrize("given", [(False, False), (True, False), (False, True)])
 def test_layer_norm_without_parameters(given):
     for dtype, shape in ((torch.bfloat16, (37, 300)), (F32, (21, 66001))):

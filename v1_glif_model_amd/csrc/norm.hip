@@ -24,6 +24,7 @@ struct NormArgs {
     float4 *stat;      // [rows] mean, rstd, mean(dyw), mean(dyw xh) (backward of wide rows)
     float *part;       // [parts][2][D] sums of dw and db
     int32_t parts;
+    int32_t past;      // results go past the caches: they are larger than these
 };
 
 // ---- the threads of a row -----------------------------------------------------------------------------------------------
@@ -64,47 +65,54 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float *red) {
     }
 }
 
+// 16 bytes of a row from column c on, zeros past its end.  Whole words throughout: a piece put together from its elements
+// would live in a register for each of them.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ u32x4 piece(const T *p, int c, int D) {
+    constexpr int V = kVecBytes16<T>;
+    u32x4 q = {};
+    if (c + V <= D) {
+        q = __builtin_bit_cast(u32x4, *reinterpret_cast<const Vec<T, V> *>(p + c));
+    } else if (c < D) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (c + e >= D) continue;
+            if constexpr (sizeof(T) == 4) q[e] = __builtin_bit_cast(uint32_t, p[c + e]);
+            else q[e / 2] |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, p[c + e])) << (e % 2 * 16);
+        }
+    }
+    return q;
+}
+
 // A row in the registers of L threads, R pieces of V elements each; piece i of thread t starts at (i L + t) V.
 template <typename T, int L, int R>
 struct Row {
-    static constexpr int V = kVecBytes16<T>;
+    static constexpr int V = kVecBytes16<T>, kR = R;
     typedef Vec<T, V> vec;
-    vec r[R];
+    u32x4 r[R];
     static __device__ __forceinline__ int at(int i) { return (i * L + static_cast<int>(threadIdx.x) % L) * V; }
-    __device__ __forceinline__ void load(int i, const T *p, int D) {
-        const int c = at(i);
-        r[i] = vec{};
-        if (c + V <= D) {
-            r[i] = *reinterpret_cast<const vec *>(p + c);
-        } else if (c < D) {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (c + e < D) r[i][e] = p[c + e];
-        }
-    }
+    __device__ __forceinline__ void load(int i, const T *p, int D) { r[i] = piece<T>(p, at(i), D); }
     __device__ __forceinline__ void load(const T *p, int D) {
 #pragma unroll
         for (int i = 0; i < R; ++i) load(i, p, D);
     }
-    __device__ __forceinline__ float get(int i, int e) const { return to_f32(static_cast<T>(r[i][e])); }
+    __device__ __forceinline__ float get(int i, int e) const { return to_f32(static_cast<T>(__builtin_bit_cast(vec, r[i])[e])); }
     // Between the passes over a long row: its float32 values are made again rather than kept in twice the registers.
     __device__ __forceinline__ void again() {
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
         if constexpr (R > 2 && sizeof(T) == 2) {
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                u32x4 q = __builtin_bit_cast(u32x4, r[i]);
-                asm volatile("" : "+v"(q));
-                r[i] = __builtin_bit_cast(vec, q);
-            }
+            for (int i = 0; i < R; ++i) asm volatile("" : "+v"(r[i]));
         }
     }
+    template <bool PAST = false>
     static __device__ __forceinline__ void put(T *p, int c, int D, const float (&v)[V]) {
         if (c + V <= D) {
             vec o;
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = from_f32<T>(v[e]);
-            *reinterpret_cast<vec *>(p + c) = o;
+            if constexpr (PAST) __builtin_nontemporal_store(o, reinterpret_cast<vec *>(p + c));
+            else *reinterpret_cast<vec *>(p + c) = o;
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e)
@@ -144,6 +152,24 @@ __device__ __forceinline__ void params(float (&v)[V], const void *p, int32_t dt,
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = c + e < D ? load_param(p, dt, c + e) : other;
+    }
+}
+
+// V sums to the columns from c on of a part (more: added to what it holds), in pieces of 16 bytes.
+template <int V>
+__device__ __forceinline__ void flush(float *part, int c, int D, const float (&v)[V], bool more) {
+    typedef Vec<float, 4> f4;
+    if (c + V <= D) {
+#pragma unroll
+        for (int h = 0; h < V; h += 4) {
+            f4 o = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+            if (more) o += *reinterpret_cast<const f4 *>(part + c + h);
+            *reinterpret_cast<f4 *>(part + c + h) = o;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (c + e < D) part[c + e] = more ? part[c + e] + v[e] : v[e];
     }
 }
 
@@ -242,11 +268,7 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormArgs a) {
     if constexpr (L >= kBlock) {
 #pragma unroll
         for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int c = Row<T, L, R>::at(i) + e;
-                if (c < D) part[c] = dw[i][e], part[a.D + c] = db[i][e];
-            }
+            flush(part, Row<T, L, R>::at(i), D, dw[i], false), flush(part + a.D, Row<T, L, R>::at(i), D, db[i], false);
     } else {
         // the block's rows side by side: their threads' sums one piece after the other through LDS
         constexpr int kCols = L * V;
@@ -273,9 +295,8 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormArgs a) {
 
 // ---- wide rows --------------------------------------------------------------------------------------------------------------
 // A block's threads go through a row in pieces and through it again for the results; a compute unit holds several such
-// rows, and the second time comes from cache.  (Rows of 66,000 in registers leave one block a compute unit: 207 us for 2500
-// of them in bfloat16, and their backward spills.)
-constexpr int kWide = 512;
+// rows, and the second time comes from cache.
+constexpr int kWide = 512, kLong = 1024, kLongR = 9, kLongFrom = 6144;
 
 // Count, mean and sum of squared differences from it, of the elements seen.  A thread takes its sums from its own first
 // element on, so that a mean far from zero costs no digits.
@@ -318,7 +339,7 @@ __device__ __forceinline__ void pieces2(const T *p, const T *q, int D, F f) {
     constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
     const int whole = D / V;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = threadIdx.x; i < whole; i += kWide)
         f(i * V, V, *reinterpret_cast<const vec *>(p + i * V), *reinterpret_cast<const vec *>(q + i * V));
     if (D % V && static_cast<int>(threadIdx.x) == whole % kWide) {
@@ -330,7 +351,7 @@ __device__ __forceinline__ void pieces2(const T *p, const T *q, int D, F f) {
     }
 }
 
-template <typename T>
+template <typename T, bool PAST>
 __global__ void __launch_bounds__(kWide) k_norm_fwd_wide(NormArgs a) {
     constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
@@ -359,8 +380,57 @@ __global__ void __launch_bounds__(kWide) k_norm_fwd_wide(NormArgs a) {
         params<V>(b, a.bias, a.pdt, c, D, 0.0f);
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = fmaf((to_f32(static_cast<T>(v[e])) - m.mean) * rstd, w[e], b[e]);
-        Row<T, 1, 1>::put(y, c, D, o);
+        Row<T, 1, 1>::template put<PAST>(y, c, D, o);
     });
+}
+
+// Rows of more than kLongFrom pieces in the registers of one block, which has a compute unit to itself (2500 x 66000 bfloat16
+// 163 us, 4.0 TB/s; gone through twice 197.  2500 x 40000 96 and 87: there several rows a unit come from the L2 again).
+template <typename T>
+__global__ void __launch_bounds__(kLong, 4) k_norm_fwd_long(NormArgs a) {
+    typedef Row<T, kLong, kLongR> row;
+    constexpr int V = row::V;
+    __shared__ float red[kLong / kWave];
+    const int D = static_cast<int>(a.D);
+    const int64_t r = blockIdx.x;
+    row x;
+    x.load(static_cast<const T *>(a.x) + r * a.x_stride, D);
+    float s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kLongR; ++i) {   // the barriers: values are made from the row again rather than kept beside it
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += x.get(i, e);
+        asm volatile("" : "+v"(x.r[i]), "+v"(s));
+    }
+    const float mean = row_sum<kLong>(s, red) / static_cast<float>(D);
+#pragma unroll
+    for (int i = 0; i < kLongR; ++i) {
+        const int left = D - row::at(i);
+        if (left >= V) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) q = fmaf(x.get(i, e) - mean, x.get(i, e) - mean, q);
+        } else if (left > 0) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) q = e < left ? fmaf(x.get(i, e) - mean, x.get(i, e) - mean, q) : q;
+        }
+        asm volatile("" : "+v"(x.r[i]), "+v"(q));
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<kLong>(q, red) / static_cast<float>(D) + a.eps);
+    T *y = static_cast<T *>(a.y) + r * a.D;
+#pragma unroll
+    for (int i = 0; i < kLongR; ++i) {
+        const int c = row::at(i);
+        asm volatile("" : "+v"(x.r[i]));
+        if (c < D) {
+            float w[V], b[V], o[V];
+            params<V>(w, a.weight, a.pdt, c, D, 1.0f);
+            params<V>(b, a.bias, a.pdt, c, D, 0.0f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = fmaf((x.get(i, e) - mean) * rstd, w[e], b[e]);
+            row::template put<true>(y, c, D, o);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // Per row mean, rstd, mean(dyw), mean(dyw xh).
@@ -394,9 +464,9 @@ __device__ __forceinline__ void wide_stats(const NormArgs &a, int64_t r) {
     if (threadIdx.x == 0) a.stat[r] = make_float4(m.mean, rstd, g.x / static_cast<float>(D), g.y / static_cast<float>(D));
 }
 
-// dx of rows r0 .. r1 - 1 and the columns' sums over them, to a part: a thread per 16 bytes of columns.
-template <typename T>
-__device__ __forceinline__ void wide_columns(const NormArgs &a, int block, int64_t r0, int64_t r1, int to) {
+// dx of rows r0 .. r1 - 1 and the columns' sums over them, to a part (more: added to what it holds): a thread per 16 bytes of columns.
+template <typename T, bool PAST>
+__device__ __forceinline__ void wide_columns(const NormArgs &a, int block, int64_t r0, int64_t r1, int to, bool more) {
     constexpr int V = kVecBytes16<T>;
     typedef Vec<T, V> vec;
     const int D = static_cast<int>(a.D);
@@ -417,10 +487,10 @@ __device__ __forceinline__ void wide_columns(const NormArgs &a, int block, int64
             db[e] += g;
             o[e] = st.y * (g * w[e] - st.z - xh * st.w);
         }
-        if (dx) Row<T, 1, 1>::put(dx + r * a.D, c, D, o);
+        if (dx) Row<T, 1, 1>::template put<PAST>(dx + r * a.D, c, D, o);
     };
     if (c + V <= D) {
-#pragma unroll 4
+#pragma unroll 2
         for (int64_t r = r0; r < r1; ++r)
             add(*reinterpret_cast<const vec *>(x + r * a.x_stride), *reinterpret_cast<const vec *>(dy + r * a.dy_stride), r);
     } else {
@@ -433,27 +503,25 @@ __device__ __forceinline__ void wide_columns(const NormArgs &a, int block, int64
         }
     }
     if (!a.part) return;
-    float *part = a.part + static_cast<int64_t>(to) * 2 * a.D + c;
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-        if (c + e < D) part[e] = dw[e], part[a.D + e] = db[e];
+    float *part = a.part + static_cast<int64_t>(to) * 2 * a.D;
+    flush(part, c, D, dw, more), flush(part + a.D, c, D, db, more);
 }
 
-// One launch of a wide backward: the columns of the rows [col0, col1), whose statistics the launch before took, and the
+// One launch of a wide backward, at three blocks a compute unit: the columns of the rows [col0, col1), whose statistics the launch before took, and the
 // statistics of the next rows [row0, row1) beside them.
 struct Round {
     int64_t col0, col1, row0, row1;
-    int32_t cols, parts, part0;   // column blocks, parts, the first part
+    int32_t cols, parts;   // column blocks and parts
 };
-template <typename T>
-__global__ void __launch_bounds__(kWide) k_norm_round(NormArgs a, Round k) {
+template <typename T, bool PAST>
+__global__ void __launch_bounds__(kWide, 6) k_norm_round(NormArgs a, Round k) {
     const int64_t rows = k.row1 - k.row0;
     if (blockIdx.x < rows) {
         wide_stats<T>(a, k.row0 + blockIdx.x);
     } else {
         const int b = static_cast<int>(blockIdx.x - rows), part = b / k.cols;
         const int64_t n = k.col1 - k.col0;
-        wide_columns<T>(a, b % k.cols, k.col0 + n * part / k.parts, k.col0 + n * (part + 1) / k.parts, k.part0 + part);
+        wide_columns<T, PAST>(a, b % k.cols, k.col0 + n * part / k.parts, k.col0 + n * (part + 1) / k.parts, part, k.col0 > 0);
     }
 }
 
@@ -490,22 +558,28 @@ int fused_blocks(int64_t rows, int64_t D, int64_t size) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + 4 * per - 1) / (4 * per), 512)));
 }
 
-// A wide backward's rounds of rows: 96 MB of x and dy (64 and 144 are slower by 10 and 3 percent at 2500 x 66000), and parts of
-// a round: a block a compute unit.
+// A wide backward's rounds of rows: 128 MB of x and dy (2500 x 66000 bfloat16 378 us; 96 and 160 MB 398 and 394), and parts of
+// a round: two blocks a compute unit (272, 408, 544 and 816 blocks 455, 404, 398 and 398 us in rounds of 96 MB), whose sums go
+// on from round to round.
 int64_t round_rows(int64_t rows, int64_t D, int64_t size) {
-    return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t(48) << 20) / (D * size)));
+    return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t(64) << 20) / (D * size)));
 }
 int round_parts(int64_t n, int64_t D, int64_t size) {
     const int64_t cols = ((D * size + 15) / 16 + kWide - 1) / kWide;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, 272 / cols)));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, 544 / cols)));
 }
+
+// Results that the caches would not hold for their reader go past them and leave the rows there for their second reading
+// (two layers after each other on 1000 x 66000 bfloat16 156 us, 167 without; on 500 x 66000 70 and 69).
+constexpr int64_t kPast = int64_t(96) << 20;
+bool past_caches(const NormArgs &a, int32_t dtype) { return a.rows * a.D * static_cast<int64_t>(dtype_size(dtype)) > kPast; }
 
 void carve(Carver &c, NormArgs &a, int64_t size, bool param) {
     if (a.D * size <= kFused) {
         a.parts = fused_blocks(a.rows, a.D, size);
     } else {
         const int64_t n = round_rows(a.rows, a.D, size);
-        a.parts = static_cast<int32_t>((a.rows + n - 1) / n) * round_parts(n, a.D, size);
+        a.parts = round_parts(n, a.D, size);
         a.stat = c.take<float4>(static_cast<size_t>(a.rows));
     }
     if (param) a.part = c.take<float>(static_cast<size_t>(a.parts) * 2 * a.D);
@@ -531,7 +605,10 @@ void run_fwd(const NormArgs &a, hipStream_t s) {
     else if (p <= 512) fwd<T, 256, 2>(a, s);
     else if (p <= 1024) fwd<T, 256, 4>(a, s);
     else if (p <= 4096) fwd<T, 1024, 4>(a, s);
-    else hipLaunchKernelGGL(k_norm_fwd_wide<T>, dim3(static_cast<unsigned>(a.rows)), dim3(kWide), 0, s, a);
+    else if (p > kLongFrom && p <= kLong * kLongR && a.past)
+        hipLaunchKernelGGL(k_norm_fwd_long<T>, dim3(static_cast<unsigned>(a.rows)), dim3(kLong), 0, s, a);
+    else if (a.past) hipLaunchKernelGGL((k_norm_fwd_wide<T, true>), dim3(static_cast<unsigned>(a.rows)), dim3(kWide), 0, s, a);
+    else hipLaunchKernelGGL((k_norm_fwd_wide<T, false>), dim3(static_cast<unsigned>(a.rows)), dim3(kWide), 0, s, a);
 }
 
 template <typename T, int L, int R>
@@ -554,13 +631,13 @@ void run_bwd(const NormArgs &a, hipStream_t s) {
     } else {
         const int64_t n = round_rows(a.rows, a.D, size);
         Round k{};
-        k.cols = static_cast<int32_t>((p + kWide - 1) / kWide), k.parts = round_parts(n, a.D, size), k.part0 = -k.parts;
+        k.cols = static_cast<int32_t>((p + kWide - 1) / kWide), k.parts = round_parts(n, a.D, size);
         while (k.col1 < a.rows) {
             k.col0 = k.col1, k.col1 = k.row1;
             k.row0 = k.row1, k.row1 = std::min(a.rows, k.row0 + n);
             const int64_t blocks = k.row1 - k.row0 + (k.col1 > k.col0 ? static_cast<int64_t>(k.cols) * k.parts : 0);
-            hipLaunchKernelGGL(k_norm_round<T>, dim3(static_cast<unsigned>(blocks)), dim3(kWide), 0, s, a, k);
-            k.part0 += k.parts;
+            if (a.past) hipLaunchKernelGGL((k_norm_round<T, true>), dim3(static_cast<unsigned>(blocks)), dim3(kWide), 0, s, a, k);
+            else hipLaunchKernelGGL((k_norm_round<T, false>), dim3(static_cast<unsigned>(blocks)), dim3(kWide), 0, s, a, k);
         }
     }
     if (a.part)
@@ -591,6 +668,7 @@ int glif_layer_norm_fwd(const void *x, int64_t x_stride, const void *weight, con
     NormArgs a{};
     a.x = x, a.weight = weight, a.bias = bias, a.y = y;
     a.rows = rows, a.D = D, a.x_stride = x_stride, a.pdt = param_dtype, a.eps = eps;
+    a.past = past_caches(a, dtype);
     GLIF_BY_DTYPE(dtype, run_fwd, a, static_cast<hipStream_t>(stream));
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;
@@ -614,6 +692,7 @@ int glif_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_
     NormArgs a{};
     a.x = x, a.dy = dy, a.weight = weight, a.dx = dx, a.dweight = dweight, a.dbias = dbias;
     a.rows = rows, a.D = D, a.x_stride = x_stride, a.dy_stride = dy_stride, a.pdt = param_dtype, a.eps = eps;
+    a.past = past_caches(a, dtype);
     Carver c(ws, ws_bytes);
     carve(c, a, static_cast<int64_t>(dtype_size(dtype)), dweight || dbias);
     if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "layer norm: workspace too small");
