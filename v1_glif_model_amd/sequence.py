@@ -55,15 +55,19 @@ def _activations(t, name):
     return t
 
 
-def _params(x, shape, **given):
-    """The small parameters that are given, contiguous and of one type: float32 or x's."""
-    kinds = {t.dtype for t in given.values() if t is not None}
-    if len(kinds) > 1:
-        raise ValueError(f"{' and '.join(given)} must be of one type")
-    for name, t in given.items():
-        if t is not None:
-            _need(t, name, shape[name], (torch.float32, x.dtype), x.device)
-    return kinds.pop() if kinds else torch.float32
+def _params(x, weight, wshape, bias, bshape):
+    """The type of the small parameters that are given: float32 or x's, the same for both."""
+    w = weight if weight is not None else bias
+    if w is None:
+        return torch.float32
+    kind = w.dtype if isinstance(w, torch.Tensor) else None
+    if weight is not None:
+        _need(weight, "weight", wshape, (torch.float32, x.dtype), x.device)
+    if bias is not None:
+        _need(bias, "bias", bshape, (torch.float32, x.dtype), x.device)
+        if bias.dtype is not kind:
+            raise ValueError("weight and bias must be of one type")
+    return kind
 
 
 def _dense(t):
@@ -71,20 +75,22 @@ def _dense(t):
 
 
 def _rows(t, D):
-    """t [..., D] as rows of D contiguous elements at one stride (copied only if it is not laid out so)."""
-    n = t.numel() // D if D else 0
+    """t [..., D] as rows of D contiguous elements at one stride, which is returned with it (copied only if it is not laid
+    out so)."""
+    if t.is_contiguous():
+        return t, D
     if t.dim() == 2:
         r = t
-    elif t.is_contiguous():
-        r = t.view(n, D)
     else:
+        n = t.numel() // D if D else 0
         try:
             r = t.view(n, D)
         except RuntimeError:
-            r = t.contiguous().view(n, D)
-    if (D > 1 and r.stride(1) != 1) or (n > 1 and r.stride(0) >= 1 << 24):
-        r = r.contiguous()
-    return r, r.stride(0) if n > 1 else D
+            return t.contiguous(), D
+    n, step = r.shape[0], r.stride(0)
+    if (D > 1 and r.stride(1) != 1) or (n > 1 and step >= 1 << 24):
+        return r.contiguous(), D
+    return r, step if n > 1 else D
 
 
 def _seq(t):
@@ -168,11 +174,11 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, pdt):
         D = x.shape[-1]
         xr, xs = _rows(x, D)
-        w, b = _dense(weight), _dense(bias)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        with _on(x.device):
-            check(lib().glif_layer_norm_fwd(_p(xr), xs, _p(w), _p(b), DTYPES[x.dtype], DTYPES[pdt], xr.shape[0], D, eps,
-                                            _p(y), _stream(x.device)))
+        w, b, dev = _dense(weight), _dense(bias), x.device
+        y = x.new_empty(x.shape)
+        with _on(dev):
+            check(lib().glif_layer_norm_fwd(_p(xr), xs, _p(w), _p(b), DTYPES[x.dtype], DTYPES[pdt], x.numel() // D, D, eps,
+                                            _p(y), _stream(dev)))
         ctx.save_for_backward(x, weight)
         ctx.eps, ctx.pdt = eps, pdt
         return y
@@ -181,18 +187,19 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         _first_only("layer_norm")
         x, weight = ctx.saved_tensors
-        D = x.shape[-1]
+        D, dev, dt, L = x.shape[-1], x.device, DTYPES[x.dtype], lib()
         xr, xs = _rows(x, D)
         gr, gs = _rows(dy, D)
         wx, ww, wb = ctx.needs_input_grad[:3]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if wx else None
-        dw = torch.empty(D, dtype=ctx.pdt, device=x.device) if ww else None
-        db = torch.empty(D, dtype=ctx.pdt, device=x.device) if wb else None
-        ws = _workspace(lib().glif_layer_norm_bwd_workspace(xr.shape[0], D, DTYPES[x.dtype], int(ww or wb)), x.device)
-        w = _dense(weight)
-        with _on(x.device):
-            check(lib().glif_layer_norm_bwd(_p(gr), gs, _p(xr), xs, _p(w), DTYPES[x.dtype], DTYPES[ctx.pdt], xr.shape[0], D,
-                                            ctx.eps, _p(dx), _p(dw), _p(db), _p(ws), _size(ws), _stream(x.device)))
+        dx = x.new_empty(x.shape) if wx else None
+        dw = torch.empty(D, dtype=ctx.pdt, device=dev) if ww else None
+        db = torch.empty(D, dtype=ctx.pdt, device=dev) if wb else None
+        rows = x.numel() // D
+        n = L.glif_layer_norm_bwd_workspace(rows, D, dt, ww or wb)
+        ws, w = _workspace(n, dev), _dense(weight)
+        with _on(dev):
+            check(L.glif_layer_norm_bwd(_p(gr), gs, _p(xr), xs, _p(w), dt, DTYPES[ctx.pdt], rows, D, ctx.eps, _p(dx), _p(dw),
+                                        _p(db), _p(ws), n, _stream(dev)))
         return dx, dw, db, None, None
 
 
@@ -205,14 +212,14 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5) -> to
     if not eps >= 0.0:
         raise ValueError(f"eps must be >= 0, got {eps}")
     D = x.shape[-1]
-    pdt = _params(x, dict(weight=(D,), bias=(D,)), weight=weight, bias=bias)
+    pdt = _params(x, weight, (D,), bias, (D,))
     return _apply(_LayerNorm, _wants_grad(x, weight, bias), x, weight, bias, float(eps), pdt)
 
 
 # --------------------------------------------------------------------------- dropout ----
 def _dropout(x, residual, p, seed, offset):
     x, residual = _dense(x), _dense(residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     with _on(x.device):
         check(lib().glif_dropout(_p(x), _p(residual), DTYPES[x.dtype], x.numel(), p, seed, offset, _p(y), _stream(x.device)))
     return y
@@ -256,14 +263,14 @@ class _Linear(torch.autograd.Function):
         wr, ldw = _rows(weight, K) if K else (weight, 0)
         rr, ldr = _rows(residual, N) if residual is not None else (None, 0)
         b = _dense(bias)
-        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-        back = any(ctx.needs_input_grad[:3])
-        pre = torch.empty((M, N), dtype=x.dtype, device=x.device) if back and act else None
-        L = lib()
-        ws = _workspace(L.glif_linear_fwd_workspace(dt, M, N, K), x.device)
-        with _on(x.device):
+        y = x.new_empty((*x.shape[:-1], N))
+        pre = x.new_empty((M, N)) if act and any(ctx.needs_input_grad[:3]) else None
+        L, dev = lib(), x.device
+        n = L.glif_linear_fwd_workspace(dt, M, N, K)
+        ws = _workspace(n, dev)
+        with _on(dev):
             check(L.glif_linear_fwd(_p(xr), ldx, _p(wr), ldw, _p(b), _p(rr), ldr, dt, DTYPES[bdt], M, N, K, act, _p(y),
-                                    _p(pre), _p(ws), _size(ws), _stream(x.device)))
+                                    _p(pre), _p(ws), n, _stream(dev)))
         ctx.save_for_backward(x, weight, pre)
         ctx.act, ctx.bdt, ctx.M = act, bdt, M
         return y
@@ -278,16 +285,18 @@ class _Linear(torch.autograd.Function):
         wr, ldw = _rows(weight, K) if K else (weight, 0)
         gr, ldg = _rows(dy, N) if N else (dy, 0)
         wx, ww, wb, wr_ = ctx.needs_input_grad[:4]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if wx else None
-        dw = torch.empty((N, K), dtype=x.dtype, device=dev) if ww else None
+        dx = x.new_empty(x.shape) if wx else None
+        dw = x.new_empty((N, K)) if ww else None
         db = torch.empty(N, dtype=ctx.bdt, device=dev) if wb else None
         if wx or ww or wb:
-            L = lib()
-            odd = any(v % (16 // x.element_size()) for v in (ldx, ldw, ldg, N, K)) or any(t.data_ptr() % 16 for t in (xr, wr, gr))
-            ws = _workspace(L.glif_linear_bwd_workspace(dt, M, N, K, ctx.act, int(odd)), dev)
+            L, V = lib(), 16 // x.element_size()
+            px, pw, pg = xr.data_ptr(), wr.data_ptr(), gr.data_ptr()
+            odd = (ldx % V or ldw % V or ldg % V or N % V or K % V or (px | pw | pg) % 16) != 0
+            n = L.glif_linear_bwd_workspace(dt, M, N, K, ctx.act, odd)
+            ws = _workspace(n, dev)
             with _on(dev):
-                check(L.glif_linear_bwd(_p(gr), ldg, _p(pre), _p(xr), ldx, _p(wr), ldw, dt, DTYPES[ctx.bdt], M, N, K,
-                                        ctx.act, _p(dx), _p(dw), _p(db), _p(ws), _size(ws), _stream(dev)))
+                check(L.glif_linear_bwd(pg, ldg, _p(pre), px, ldx, pw, ldw, dt, DTYPES[ctx.bdt], M, N, K, ctx.act, _p(dx),
+                                        _p(dw), _p(db), _p(ws), n, _stream(dev)))
         return dx, dw, db, dy if wr_ else None, None, None
 
 
@@ -303,7 +312,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias=None, activation=None, re
         raise ValueError("x must have at least one axis")
     _need(weight, "weight", (None, x.shape[-1]), x.dtype, x.device)
     N = weight.shape[0]
-    bdt = _params(x, dict(bias=(N,)), bias=bias)
+    bdt = _params(x, None, None, bias, (N,))
     if residual is not None:
         _need(residual, "residual", (*x.shape[:-1], N), x.dtype, x.device)
     return _apply(_Linear, _wants_grad(x, weight, bias, residual), x, weight, bias, residual, ACTIVATIONS[activation], bdt)
@@ -317,8 +326,7 @@ class _ShortConv(torch.autograd.Function):
         W = weight.shape[1]
         ctx.set_materialize_grads(False)
         xs, w, b, st = _seq(x), _dense(weight), _dense(bias), _dense(state)
-        y = torch.empty((T, B, D), dtype=x.dtype, device=x.device)
-        last = torch.empty((B, W - 1, D), dtype=x.dtype, device=x.device)
+        y, last = x.new_empty((T, B, D)), x.new_empty((B, W - 1, D))
         with _on(x.device):
             check(lib().glif_short_conv_fwd(_p(xs), xs.stride(0), xs.stride(1), _p(w), _p(b), _p(st), _p(lengths),
                                             DTYPES[x.dtype], DTYPES[pdt], T, B, D, W, silu, _p(y), _p(last),
@@ -335,15 +343,16 @@ class _ShortConv(torch.autograd.Function):
         wx, ww, wb, ws_ = ctx.needs_input_grad[:4]
         dy = _seq(dy) if dy is not None else torch.zeros((T, B, D), dtype=x.dtype, device=dev)
         dlast, xs, w, b, st = _dense(dlast), _seq(x), _dense(weight), _dense(bias), _dense(state)
-        dx = torch.empty((T, B, D), dtype=x.dtype, device=dev) if wx else None
+        dx = x.new_empty((T, B, D)) if wx else None
         dw = torch.empty((D, W), dtype=ctx.pdt, device=dev) if ww else None
         db = torch.empty(D, dtype=ctx.pdt, device=dev) if wb else None
-        ds = torch.empty((B, W - 1, D), dtype=x.dtype, device=dev) if ws_ else None
-        ws = _workspace(lib().glif_short_conv_bwd_workspace(DTYPES[x.dtype], T, B, D, W) if ww or wb else 0, dev)
+        ds = x.new_empty((B, W - 1, D)) if ws_ else None
+        n = lib().glif_short_conv_bwd_workspace(DTYPES[x.dtype], T, B, D, W) if ww or wb else 0
+        ws = _workspace(n, dev)
         with _on(dev):
             check(lib().glif_short_conv_bwd(_p(dy), dy.stride(0), dy.stride(1), _p(dlast), _p(xs), xs.stride(0), xs.stride(1),
                                             _p(w), _p(b), _p(st), _p(lengths), DTYPES[x.dtype], DTYPES[ctx.pdt], T, B, D, W,
-                                            ctx.silu, _p(dx), _p(dw), _p(db), _p(ds), _p(ws), _size(ws), _stream(dev)))
+                                            ctx.silu, _p(dx), _p(dw), _p(db), _p(ds), _p(ws), n, _stream(dev)))
         return dx, dw, db, ds, None, None, None
 
 
@@ -357,7 +366,7 @@ def _conv_args(x, weight, bias, activation):
     W = weight.shape[1]
     if not 1 <= W <= 8:
         raise ValueError(f"weight must have 1 to 8 taps, got {W}")
-    return int(activation == "silu"), W, _params(x, dict(weight=(D, W), bias=(D,)), weight=weight, bias=bias)
+    return int(activation == "silu"), W, _params(x, weight, (D, W), bias, (D,))
 
 
 def short_conv(x: torch.Tensor, weight: torch.Tensor, bias=None, activation=None, initial_state=None, lengths=None):
