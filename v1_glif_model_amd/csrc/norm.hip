@@ -569,10 +569,8 @@ int round_parts(int64_t n, int64_t D, int64_t size) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, 544 / cols)));
 }
 
-// Results that the caches would not hold for their reader go past them and leave the rows there for their second reading
-// (two layers after each other on 1000 x 66000 bfloat16 156 us, 167 without; on 500 x 66000 70 and 69).
-constexpr int64_t kPast = int64_t(96) << 20;
-bool past_caches(const NormArgs &a, int32_t dtype) { return a.rows * a.D * static_cast<int64_t>(dtype_size(dtype)) > kPast; }
+// (two layers after each other on 1000 x 66000 bfloat16 156 us, 167 without; on 500 x 66000 70 and 69)
+bool past_caches(const NormArgs &a, int32_t dtype) { return a.rows * a.D * static_cast<int64_t>(dtype_size(dtype)) > kPastCaches; }
 
 void carve(Carver &c, NormArgs &a, int64_t size, bool param) {
     if (a.D * size <= kFused) {

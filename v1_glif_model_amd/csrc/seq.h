@@ -19,6 +19,10 @@ struct VecOf {
 template <typename T, int V>
 using Vec = typename VecOf<T, V>::type;
 
+// Results of more bytes than this go past the caches: these would not hold them for their reader anyway, and keep what the
+// kernel itself reads again.
+constexpr int64_t kPastCaches = int64_t(96) << 20;
+
 template <typename T>
 constexpr int kVecBytes16 = 16 / static_cast<int>(sizeof(T));   // elements in a 16-byte access
 
