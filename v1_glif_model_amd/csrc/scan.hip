@@ -14,6 +14,10 @@
 // Few channels do not fill the chip: time is then split into segments.  A first pass takes each segment's end state from
 // zero and its sum of steps (its decay is exp(A sum)), a join runs over the segments, a second pass goes from the right
 // states; the backward does the same from the other side.
+//
+// Bound by instruction issue: per state and tick an exponential (a quarter of the rate of the rest) and four products and
+// sums forward, some 24 operations backward; what a channel needs per tick adds about a third (vector units busy 85 to 98
+// percent of the time).  Memory would allow 27 us for 16.4M channels' ticks forward and 55 backward.
 #include "seq.h"
 
 namespace glif {
@@ -220,7 +224,8 @@ __device__ __forceinline__ float step_of(float raw, bool softplus, bool live, fl
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
-// ENDS: the first pass over segments, which leaves the segment's end state from zero and its sum of steps.
+// ENDS: the first pass over segments, which leaves the segment's end state from zero and its sum of steps.  500 x 32 x 1024 x 16
+// bfloat16 108 us; one recording, 8000 x 1 x 2048 x 16, which segments make possible, 66 for the ends and 95.
 template <typename T, int SPL, bool ENDS>
 __global__ void __launch_bounds__(kBlock) k_scan_fwd(ScanArgs a) {
     constexpr int kCh = chunk_of(SPL), kNp = SPL * kQ, kE = kCh / SPL;
@@ -348,7 +353,7 @@ __global__ void __launch_bounds__(kBlock) k_scan_join(ScanArgs a) {
 // ---- backward ---------------------------------------------------------------------------------------------------------------
 // ENDS: the first pass over segments, which leaves what a segment hands to the one before it, and its sum of steps.  Else a
 // chunk's states are run again from the kept one, and then the chunk backwards; its decays are taken again, too (kept in
-// registers they leave one wave a SIMD: 500 x 32 x 1024 x 16 training 522 us, taken again 402).
+// registers they leave one wave a SIMD: 500 x 32 x 1024 x 16 training 522 us, taken again 402, of which 284 are this kernel).
 template <typename T, int SPL, bool ENDS>
 __global__ void __launch_bounds__(kBlock) k_scan_bwd(ScanArgs a) {
     constexpr int kCh = chunk_of(SPL), kNp = SPL * kQ, kE = kCh / SPL;
@@ -565,6 +570,7 @@ __global__ void __launch_bounds__(kBlock) k_scan_join_param(ScanArgs a) {
 }
 
 // ---- one tick ---------------------------------------------------------------------------------------------------------------
+// A lane's four states in 16 bytes.  Bound by the launch, then by the state's way in and out: 32 x 2048 x 16 4.4 us, 8.4 MB.
 template <typename T, int SPL>
 __global__ void __launch_bounds__(kBlock) k_scan_step(ScanArgs a) {
     const glif_scan &s = a.s;
