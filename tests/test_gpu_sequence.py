@@ -257,6 +257,23 @@ def test_linear_empty_and_not_finite():
     assert torch.equal(y[other], clean[other]) and not y[7].isfinite().any() and bool(y[60].isnan().all())
 
 
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("rows", [3, 70])
+def test_linear_nan_stays(rows, act):
+    """A row that holds NaN answers NaN through every activation, and its gradients are NaN; the other rows' are not."""
+    from v1_glif_model_amd import sequence as seq
+    x, w, b = rnd(66, rows, 40), rnd(63, 12, 40), rnd(64, 12)
+    x[1, 7] = float("nan")
+    xs = x.requires_grad_(True)
+    y = seq.linear(xs, w, b, activation=act)
+    other = [r for r in range(rows) if r != 1]
+    assert bool(y[1].isnan().all()) and not y[other].isnan().any()
+    (dx,) = grads(y, torch.ones_like(y), xs)
+    assert not dx[other].isnan().any()
+    if act in ("gelu", "silu"):
+        assert bool(dx[1].isnan().all())
+
+
 # ----------------------------------------------------------------- short convolution ----
 def conv_case(x, w, b, act, state, lengths, dy, dlast, poison=False):
     """poison: what the op must not look at is NaN in its inputs, 0 in the reference's."""
@@ -557,6 +574,65 @@ def test_same_bits_every_time():
     first = once()
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(first, once()))
+
+
+# ------------------------------------------------------------ more than 2^31 elements ----
+def big(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator(DEV).manual_seed(seed), device=DEV, dtype=torch.bfloat16)
+
+
+def test_layer_norm_and_dropout_past_32_bits():
+    from v1_glif_model_amd import sequence as seq
+    x = big(1, 33_000, 66_000)
+    n = 70 * 66_000
+    end = x[-70:].clone()
+    y = seq.dropout(x, 0.3, 5, 7)
+    assert torch.equal(y[-70:], seq.dropout(end, 0.3, 5, 7 + x.numel() - n)) and torch.equal(y[:1], seq.dropout(x[:1], 0.3, 5, 7))
+    xs, dy = x.requires_grad_(True), y
+    w = torch.ones(66_000, device=DEV, requires_grad=True)
+    out = seq.layer_norm(xs, w)
+    dx, dw = grads(out, dy, xs, w)
+    x6, g6 = f64(end, False), f64(dy[-70:], False)
+    mean = x6.mean(-1, keepdim=True)
+    rstd = 1.0 / torch.sqrt(((x6 - mean) ** 2).mean(-1, keepdim=True) + 1e-5)
+    xh = (x6 - mean) * rstd
+    far = (x6.abs() + x6.abs().mean(-1, keepdim=True)) * rstd
+    near(out[-70:], xh, far, "y")
+    near(dx[-70:], rstd * (g6 - g6.mean(-1, keepdim=True) - xh * (g6 * xh).mean(-1, keepdim=True)),
+         rstd * (g6.abs() + g6.abs().mean(-1, keepdim=True) * (1 + far) + far * (g6.abs() * far).mean(-1, keepdim=True)), "dx")
+    assert bool(dw.isfinite().all())
+
+
+def test_sequences_past_32_bits():
+    """The last channels of the last entry: a channel's convolution is the same arithmetic wherever it lies; its state space
+    is cut into segments of time here and not there, by float32 roundings of the carried state (1e-5 of the largest)."""
+    from v1_glif_model_amd import sequence as seq
+    T, B, D, N = 16_400, 64, 2048, 4
+    x = big(2, T, B, D)
+    w = rnd(91, D, 4)
+    y, last = seq.short_conv(x, w, activation="silu")
+    part = x[:, -1:, -64:].contiguous()
+    yp, lp = seq.short_conv(part, w[-64:].contiguous(), activation="silu")
+    assert torch.equal(y[:, -1:, -64:], yp) and torch.equal(last[-1:, :, -64:], lp)
+    del y
+    maps, A = big(3, T, B, 1, N), -torch.exp(rnd(92, D, N))
+    y, last = seq.state_space_scan(x, x, A, maps, maps)
+    yp, lp = seq.state_space_scan(part, part, A[-64:].contiguous(), maps[:, -1:], maps[:, -1:])
+    a, b = y[:, -1:, -64:].double(), yp.double()
+    assert float(((a - b).abs() - 2.0 ** -7 * b.abs()).max()) <= 1e-5 * float(b.abs().max())
+    assert float((last[-1:, -64:] - lp).abs().max()) <= 1e-5 * float(lp.abs().max())
+
+
+def test_linear_past_32_bits():
+    from v1_glif_model_amd import sequence as seq
+    x, w = big(4, 33_000, 32).requires_grad_(True), big(5, 66_000, 32)
+    y = seq.linear(x, w)
+    x6, w6 = f64(x[-70:], False), f64(w, False)
+    near(y[-70:], x6 @ w6.t(), x6.abs() @ w6.abs().t(), "y")
+    (dx,) = grads(y, y, x)
+    g6 = f64(y[-70:], False)
+    near(dx[-70:], g6 @ w6, g6.abs() @ w6.abs(), "dx")
+
 
 
 def test_streams_and_capture():

@@ -35,7 +35,7 @@ struct GemmArgs {
 
 __device__ __forceinline__ float act_of(float p, int act) {
     switch (act) {
-        case GLIF_ACT_RELU: return fmaxf(p, 0.0f);
+        case GLIF_ACT_RELU: return p < 0.0f ? 0.0f : p;   // NaN stays
         case GLIF_ACT_GELU: return 0.5f * p * (1.0f + erff(p * 0.70710678118654752f));
         case GLIF_ACT_SILU: return p * sigmoid_f(p);
         default: return p;
@@ -44,7 +44,7 @@ __device__ __forceinline__ float act_of(float p, int act) {
 
 __device__ __forceinline__ float slope_of(float p, int act) {
     switch (act) {
-        case GLIF_ACT_RELU: return p > 0.0f ? 1.0f : 0.0f;
+        case GLIF_ACT_RELU: return p <= 0.0f ? 0.0f : 1.0f;
         case GLIF_ACT_GELU:
             return fmaf(p * 0.39894228040143268f, expf(-0.5f * p * p), 0.5f * (1.0f + erff(p * 0.70710678118654752f)));
         case GLIF_ACT_SILU: {
