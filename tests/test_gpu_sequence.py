@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import seq_ref as ref
-from tests.seq_ref import f64, near
+from tests.seq_ref import UNIT, f64, near
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -255,6 +255,34 @@ def test_linear_empty_and_not_finite():
     y = seq.linear(x, w, b)
     other = [r for r in range(70) if r not in (7, 60)]
     assert torch.equal(y[other], clean[other]) and not y[7].isfinite().any() and bool(y[60].isnan().all())
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(512, 66_000, 640, torch.bfloat16), (66_001, 250, 640, torch.float16), (300, 50_007, 520, F32),
+                                         (33_003, 500, 641, torch.bfloat16)])
+def test_linear_of_a_few_tiles_more_than_whole_rounds(M, N, K, dtype):
+    """Products of whole rounds of tiles and a rest: every row's and column's ends and middle, with all of the epilogue."""
+    from v1_glif_model_amd import sequence as seq
+    x, w = rnd(67, M, K, dtype=dtype).requires_grad_(True), rnd(68, N, K, dtype=dtype, scale=K ** -0.5).requires_grad_(True)
+    b, res, dy = rnd(69, N).requires_grad_(True), rnd(70, M, N, dtype=dtype), rnd(71, M, N, dtype=dtype)
+    y = seq.linear(x, w, b, activation="silu", residual=res)
+    dx, dw, db = grads(y, dy, x, w, b)
+    with torch.no_grad():
+        x6, w6, b6, g6, r6 = (t.double() for t in (x, w, b, dy, res))
+        pre = x6 @ w6.t() + b6
+        q = torch.sigmoid(pre)
+        mass = x6.abs() @ w6.abs().t() + b6.abs()
+        kept = UNIT[dtype] * pre.abs() if dtype is not F32 else 0.0       # the kept argument's rounding
+        dp, ga = g6 * q * (1 + pre * (1 - q)), g6.abs() * (q * (1 + pre.abs() * (1 - q)))
+        ga_more = g6.abs() * (0.5 * kept + 2e-5 * mass) + UNIT[dtype] * dp.abs()   # |silu''| <= 1/2; dp is rounded for the products
+        spots = lambda n: torch.cat([torch.arange(0, 40), torch.arange(n // 2, n // 2 + 40), torch.arange(n - 700, n)] if n > 800
+                                    else [torch.arange(n)]).to(DEV)
+        i, j, k = spots(M)[:, None], spots(N)[None], spots(K)
+        near(y.detach()[i, j], (pre * q + r6)[i, j].cpu(), (1.1 * mass + r6.abs())[i, j].cpu(), "y")
+        i = i[:, 0]
+        near(dx[i], (dp[i] @ w6).cpu(), (ga[i] @ w6.abs()).cpu(), "dx", (ga_more[i] @ w6.abs()).cpu())
+        j = j[0]
+        near(dw[j], (dp[:, j].t() @ x6).cpu(), (ga[:, j].t() @ x6.abs()).cpu(), "dw", (ga_more[:, j].t() @ x6.abs()).cpu())
+        near(db, dp.sum(0).cpu(), ga.sum(0).cpu(), "db", (g6.abs() * (0.5 * kept + 2e-5 * mass)).sum(0).cpu())
 
 
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])

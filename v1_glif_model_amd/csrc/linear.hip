@@ -5,7 +5,7 @@
 //
 // Large products are bound by the matrix cores and what feeds them from LDS (8192^3 bfloat16 837 us, 1314 TFLOP/s of 2500);
 // short ones and ones of few tiles by the fill and drain of their blocks and by the way of their operands from memory (2500 x
-// 66000 x 512 bfloat16 forward 230 us, dx 271, dW 226); single ticks by the stream of the weights.
+// 66000 x 512 bfloat16 forward 228 us, dx 263, dW 177); single ticks by the stream of the weights.
 #include "seq.h"
 
 namespace glif {
@@ -26,7 +26,8 @@ struct GemmArgs {
     int32_t tiles_m, tiles_n, splits;
     float *part;               // [splits][M][part_ld], where splits > 1
     int64_t part_ld;
-    void *c, *pre;             // [M][N]
+    void *c, *pre;             // rows of ldc
+    int64_t ldc;
     const void *bias, *residual;
     int64_t ldr;
     int32_t bias_dt, act;
@@ -175,13 +176,13 @@ struct Finish {
     }
     __device__ __forceinline__ void operator()(const GemmArgs &a, int64_t m, f32x4 v, vec res) const {
         v += bias;
-        if (a.pre) write(static_cast<T *>(a.pre) + m * a.N + n, v, have, a.past);
+        if (a.pre) write(static_cast<T *>(a.pre) + m * a.ldc + n, v, have, a.past);
         if (a.act != GLIF_ACT_NONE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = act_of(v[e], a.act);
         }
         if (a.residual) v += __builtin_convertvector(res, f32x4);
-        write(static_cast<T *>(a.c) + m * a.N + n, v, have, a.past);
+        write(static_cast<T *>(a.c) + m * a.ldc + n, v, have, a.past);
     }
 };
 
@@ -712,13 +713,19 @@ __global__ void __launch_bounds__(kBlock) k_bias_join(const float *part, int par
     store_param(dbias, dt, n, s);
 }
 
-// How a product is cut up: the tile, and the parts of k whose sums are added afterwards.
+// How a product, or one of two pieces of it, is cut up: the tile, and the parts of k whose sums are added afterwards.
 enum Kind { kFew16, kFew32, kTile64, kTile128, kTile256 };
-struct Plan {
+struct Piece {
     Kind kind;
     int32_t splits;
     int64_t k_part, part_ld, rows;
     size_t floats() const { return splits > 1 ? static_cast<size_t>(splits) * rows * part_ld : 0; }
+};
+struct Plan {
+    Piece one, two;     // two: of the rows (cut_m) or columns from `cut` on, where that is not 0
+    int64_t cut;
+    bool cut_m;
+    size_t floats() const { return std::max(one.floats(), cut ? two.floats() : 0); }
 };
 
 // rr: both operands have k along their rows.
@@ -731,8 +738,9 @@ struct Plan {
 // x 64 1.1; a step of all of the 1, 2 or 5 blocks that a compute unit holds 1.9, 1.35, 1.2, and 4.3, 2.9 (measured over
 // sweeps of tiles and splits at 15 shapes).  Around the steps go 10, 5 and 3; a split costs its sums' way to memory and back
 // and the launch that adds them.  A float32 sum runs over at most 4096 k's, so that long ones do not lose their last digits.
-Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
-    Plan p{};
+Piece piece_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr, double &best) {
+    Piece p{};
+    best = 0.0;
     p.rows = M, p.part_ld = (N + 3) / 4 * 4, p.splits = 1, p.kind = kTile128;
     const int64_t size = static_cast<int64_t>(dtype_size(dtype)), bk = kRowBytes / size, steps = std::max<int64_t>((K + bk - 1) / bk, 1);
     p.k_part = steps * bk;
@@ -743,8 +751,9 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
         p.kind = few <= 16 ? kFew16 : kFew32;
         splits = std::max<int64_t>(1, std::min<int64_t>(2048 / ((many + 15) / 16), K / 512));
         p.k_part = (steps + splits - 1) / splits * bk;
+        best = 10.0 + static_cast<double>(many * K * size) / 4e6;   // the stream at 4 TB/s
     } else {
-        double best = 1e30;
+        best = 1e30;
         for (const int tile : {64, 128, 256}) {
             if (size == 4 && tile == 256) continue;
             const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
@@ -765,6 +774,29 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
         }
     }
     p.splits = static_cast<int32_t>((steps * bk + p.k_part - 1) / p.k_part);
+    return p;
+}
+
+// Tiles that are a few more than whole rounds of the chip's blocks cost one round more.  Where it is cheaper, and by more than
+// a launch, the whole rounds are one piece, and the rest, as short tiles or with k in parts, is another (2500 x 66000 x 512
+// bfloat16, dW of 516 tiles of 256 x 256, 226 us in one, 177 in two).
+Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
+    Plan p{};
+    double best;
+    p.one = piece_for(dtype, M, N, K, rr, best);
+    p.cut_m = M > N;
+    const int64_t across = std::min(M, N), along = std::max(M, N);
+    if (across <= 32) return p;
+    for (const int tile : {128, 256}) {
+        if (dtype_size(dtype) == 4 && tile == 256) continue;
+        const int64_t slots = tile == 256 ? 256 : 512, wide = (across + tile - 1) / tile;
+        const int64_t cut = wide * ((along + tile - 1) / tile) / slots * slots / wide * tile;
+        if (cut == 0 || cut >= along) continue;
+        double first, rest;
+        const Piece one = p.cut_m ? piece_for(dtype, cut, N, K, rr, first) : piece_for(dtype, M, cut, K, rr, first);
+        const Piece two = p.cut_m ? piece_for(dtype, M - cut, N, K, rr, rest) : piece_for(dtype, M, N - cut, K, rr, rest);
+        if (first + rest + 4.0 < best) best = first + rest + 4.0, p.one = one, p.two = two, p.cut = cut;
+    }
     return p;
 }
 
@@ -800,10 +832,7 @@ void launch_few(GemmArgs &a, hipStream_t s) {
 }
 
 template <typename T, bool PCOL, bool QCOL>
-int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
-    if (a.M == 0 || a.N == 0) return GLIF_OK;
-    // (8192^3 bfloat16 1009 us -> 846; 2500 x 512 x 66000, 330 MB of results, 292 -> 271; 2500 x 512 x 12007, 60 MB, 57 and 63)
-    a.past = a.M * a.N * static_cast<int64_t>(sizeof(T)) > kPastCaches;
+void launch_piece(GemmArgs a, const Piece &p, float *part, hipStream_t s) {
     a.splits = p.splits, a.k_part = p.k_part, a.part_ld = p.part_ld, a.part = part;
     // a tile's rows of k within 32-bit offsets
     const int64_t ld = std::max(PCOL ? 0 : a.p_ld, QCOL ? 0 : a.q_ld) * static_cast<int64_t>(sizeof(T));
@@ -828,6 +857,33 @@ int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
             hipLaunchKernelGGL((k_gemm_join<T, 1>), dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))),
                                dim3(kBlock), 0, s, a);
     }
+}
+
+template <typename T, bool PCOL, bool QCOL>
+int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
+    if (a.M == 0 || a.N == 0) return GLIF_OK;
+    // (8192^3 bfloat16 1009 us -> 846; 2500 x 512 x 66000, 330 MB of results, 292 -> 271; 2500 x 512 x 12007, 60 MB, 57 and 63)
+    a.past = a.M * a.N * static_cast<int64_t>(sizeof(T)) > kPastCaches;
+    a.ldc = a.N;
+    if (p.cut == 0) {
+        launch_piece<T, PCOL, QCOL>(a, p.one, part, s);
+        return GLIF_OK;
+    }
+    GemmArgs b = a;
+    auto on = [](auto &at, int64_t by) { at = at ? const_cast<char *>(static_cast<const char *>(at)) + by : nullptr; };
+    const int64_t size = sizeof(T);
+    if (p.cut_m) {
+        a.M = p.cut, b.M -= p.cut, b.p_rows -= p.cut;
+        on(b.p, p.cut * size * (PCOL ? 1 : b.p_ld));
+        on(b.c, p.cut * size * b.ldc), on(b.pre, p.cut * size * b.ldc), on(b.residual, p.cut * size * b.ldr);
+    } else {
+        a.N = p.cut, b.N -= p.cut, b.q_rows -= p.cut;
+        on(b.q, p.cut * size * (QCOL ? 1 : b.q_ld));
+        on(b.c, p.cut * size), on(b.pre, p.cut * size), on(b.residual, p.cut * size);
+        on(b.bias, p.cut * static_cast<int64_t>(dtype_size(b.bias_dt)));
+    }
+    launch_piece<T, PCOL, QCOL>(a, p.one, part, s);
+    launch_piece<T, PCOL, QCOL>(b, p.two, part, s);
     return GLIF_OK;
 }
 
