@@ -321,16 +321,17 @@ int glif_dropout(const void *x, const void *residual, int32_t dtype, int64_t n, 
                  void *y, void *stream);
 
 /* y = act(x weight^T + bias) + residual: x [M][K], weight [N][K], bias [N] or NULL, residual [M][N] or NULL, row strides
- * ld*; pre [M][N] (NULL: not kept) takes x weight^T + bias for the backward, rounded to dtype.
- * Backward: dp = dy act'(pre) (act NONE: pre is not read); dx = dp weight, dweight = dp^T x, dbias = sum of dp's rows.
+ * ld*; pre [M][N] (NULL: not kept) takes x weight^T + bias for the backward, in float32.
+ * Backward: dp = dy act'(pre) (act NONE: pre is not read); dx = dp weight, dweight = dp^T x, dbias = sum of dp's rows.  The
+ * two products take dp rounded to dtype, dbias is summed from its float32 values.
  * Its workspace takes copies of 16-bit operands whose rows do not all lie on 16-byte addresses in whole pieces (unaligned != 0:
  * dy, x or weight has a pointer, stride or width that is no multiple of 16 bytes).  Row strides are below 2^24. */
 size_t glif_linear_fwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K);
 int glif_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const void *residual,
                     int64_t ldr, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
-                    void *y, void *pre, void *ws, size_t ws_bytes, void *stream);
+                    void *y, float *pre, void *ws, size_t ws_bytes, void *stream);
 size_t glif_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t activation, int32_t unaligned);
-int glif_linear_bwd(const void *dy, int64_t lddy, const void *pre, const void *x, int64_t ldx, const void *weight,
+int glif_linear_bwd(const void *dy, int64_t lddy, const float *pre, const void *x, int64_t ldx, const void *weight,
                     int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
                     void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream);
 

@@ -1,0 +1,70 @@
+"""Faults that the sequence operators and the readout once had, each by the smallest call that shows it, against the
+definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from tests.seq_ref import UNIT, f64, near
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def rnd(seed, *shape, dtype=F32, scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale + shift).to(dtype).to(DEV)
+
+
+def slope(p, act):
+    """act'(p), also where exp(-p) passes 64 bits."""
+    if act == "gelu":
+        return 0.5 * torch.erfc(-p / math.sqrt(2.0)) + p * torch.exp(-0.5 * p * p) / math.sqrt(2.0 * math.pi)
+    q = torch.sigmoid(p)
+    return q * (1.0 + p * (1.0 - q))
+
+
+# ---------------------------------------------------------------------------- linear ----
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_keeps_the_activations_argument_in_full(dtype, act):
+    """The bias's gradient of a few rows, whose terms are products of dy and the slope alone: off by the float32 sums'
+    rounding (1e-5 of dp's terms, of which the slope turns by at most 0.8 per unit), with nothing for an argument in 16 bits
+    (which would be 2^-9 and 2^-12 of up to 0.35 dy)."""
+    from v1_glif_model_amd import sequence as seq
+    M, N, K = 3, 200, 4
+    x, w = rnd(1, M, K, dtype=dtype), rnd(2, N, K, dtype=dtype, scale=0.7)
+    b, dy = rnd(3, N).requires_grad_(True), rnd(4, M, N, dtype=dtype)
+    (db,) = torch.autograd.grad(seq.linear(x, w, b, activation=act), b, dy)
+    x6, w6, b6, g6 = (f64(t, False) for t in (x, w, b, dy))
+    pre = x6 @ w6.t() + b6
+    dp = g6 * slope(pre, act)
+    terms = dp.abs() + 0.8 * g6.abs() * (x6.abs() @ w6.abs().t() + b6.abs())
+    near(db, dp.sum(0), terms.sum(0), "db")
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_linear_float16_arguments_beyond_float16(act):
+    """An argument of -7e4, whose activation is 0 and whose slope is 0, and one of 7e4, whose slope is 1, among ordinary ones."""
+    from v1_glif_model_amd import sequence as seq
+    M, N, K = 40, 24, 16
+    x, w = rnd(5, M, K, dtype=F16), rnd(6, N, K, dtype=F16, scale=0.25)
+    x[7], w[5], x[20] = 0.0, 0.0, 0.0
+    x[7, 3], w[5, 3], x[20, 3] = -256.0, 274.0, 256.0
+    b, dy = rnd(7, N), rnd(8, M, N, dtype=F16)
+    xs, ws, bs = (t.requires_grad_(True) for t in (x, w, b))
+    y = seq.linear(xs, ws, bs, activation=act)
+    assert float(y.detach()[7, 5]) == 0.0
+    got = torch.autograd.grad(y, (xs, ws, bs), dy)
+    x6, w6, b6, g6 = (f64(t, False) for t in (x, w, b, dy))
+    pre = x6 @ w6.t() + b6
+    assert float(pre[7, 5]) < -65520 and float(pre[20, 5]) > 65520
+    dp = g6 * slope(pre, act)
+    # float32 sums; |slope'| <= 0.8 and 0 far out, where the terms are large; dp is rounded once for the products
+    turn = torch.where(pre.abs() > 1e4, 0.0, 0.8)
+    terms = dp.abs() + turn * g6.abs() * (x6.abs() @ w6.abs().t() + b6.abs())
+    one = UNIT[F16] * dp.abs()
+    near(got[0], dp @ w6, terms @ w6.abs(), "dx", more=one @ w6.abs())
+    near(got[1], dp.t() @ x6, terms.t() @ x6.abs(), "dw", more=one.t() @ x6.abs())
+    near(got[2], dp.sum(0), terms.sum(0), "db")

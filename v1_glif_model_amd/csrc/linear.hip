@@ -26,7 +26,8 @@ struct GemmArgs {
     int32_t tiles_m, tiles_n, splits;
     float *part;               // [splits][M][part_ld], where splits > 1
     int64_t part_ld;
-    void *c, *pre;             // rows of ldc
+    void *c;                   // rows of ldc
+    float *pre;                // likewise, or NULL
     int64_t ldc;
     const void *bias, *residual;
     int64_t ldr;
@@ -158,25 +159,27 @@ struct Finish {
             if (e < have) q[e] = p[e];
         return q;
     }
-    static __device__ __forceinline__ void write(T *p, f32x4 v, int have, int32_t past) {
+    template <typename O>
+    static __device__ __forceinline__ void write(O *p, f32x4 v, int have, int32_t past) {
+        typedef Vec<O, 4> out;
         if (have == 4) {
-            const vec o = __builtin_convertvector(v, vec);
+            const out o = __builtin_convertvector(v, out);
             if (past) {   // kept apart from the other store, or they become one again
                 asm volatile("" ::: "memory");
-                __builtin_nontemporal_store(o, reinterpret_cast<vec *>(p));
+                __builtin_nontemporal_store(o, reinterpret_cast<out *>(p));
                 asm volatile("" ::: "memory");
             } else {
-                *reinterpret_cast<vec *>(p) = o;
+                *reinterpret_cast<out *>(p) = o;
             }
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (e < have) p[e] = from_f32<T>(v[e]);
+                if (e < have) p[e] = from_f32<O>(v[e]);
         }
     }
     __device__ __forceinline__ void operator()(const GemmArgs &a, int64_t m, f32x4 v, vec res) const {
         v += bias;
-        if (a.pre) write(static_cast<T *>(a.pre) + m * a.ldc + n, v, have, a.past);
+        if (a.pre) write(a.pre + m * a.ldc + n, v, have, a.past);
         if (a.act != GLIF_ACT_NONE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = act_of(v[e], a.act);
@@ -612,7 +615,8 @@ __global__ void __launch_bounds__(kBlock) k_gemm_join(GemmArgs a) {
 
 constexpr int kSlopeCols = 32, kSlopeLots = kBlock / kSlopeCols;
 struct SlopeArgs {
-    const void *dy, *pre;
+    const void *dy;
+    const float *pre;    // [M][N]
     int64_t lddy, M, N;
     void *dp;            // [M][lddp] or NULL
     int64_t lddp;
@@ -620,8 +624,9 @@ struct SlopeArgs {
     int32_t act, parts;
 };
 
-// dp = dy act'(pre), rounded to the activations' type for the products (zeros past N), and the column sums of the unrounded
-// values over a chunk of rows: 32 pieces of 16 bytes by 8 rows a block (2500 x 512 bfloat16 with gelu, and the sums' join
+// dp = dy act'(pre), rounded to the activations' type for the products (zeros past N: the matrix instructions take both
+// operands in one type, and a second product for what the rounding leaves would double their time), and the column sums of the
+// unrounded values over a chunk of rows: 32 pieces of 16 bytes by 8 rows a block (2500 x 512 bfloat16 with gelu, and the sums' join
 // below: a column a thread 18 and 39 us, so 11 and 4).
 template <typename T>
 __global__ void __launch_bounds__(kBlock) k_slope(SlopeArgs a) {
@@ -631,18 +636,20 @@ __global__ void __launch_bounds__(kBlock) k_slope(SlopeArgs a) {
     const int col = threadIdx.x % kSlopeCols, lot = threadIdx.x / kSlopeCols;
     const int64_t n = (static_cast<int64_t>(blockIdx.x) * kSlopeCols + col) * V, cols = a.dp ? a.lddp : a.N;
     const int64_t r0 = a.M * blockIdx.y / a.parts, r1 = a.M * (blockIdx.y + 1) / a.parts;
-    const T *dy = static_cast<const T *>(a.dy) + n, *pre = static_cast<const T *>(a.pre) + n;
+    const T *dy = static_cast<const T *>(a.dy) + n;
+    const float *pre = a.pre + n;
     T *dp = static_cast<T *>(a.dp) + n;
     float s[V] = {};
     if (n + V <= a.N) {
 #pragma unroll 2
         for (int64_t m = r0 + lot; m < r1; m += kSlopeLots) {
             const vec g = *reinterpret_cast<const vec *>(dy + m * a.lddy);
-            vec p = {}, o;
-            if (a.act != GLIF_ACT_NONE) p = *reinterpret_cast<const vec *>(pre + m * a.N);
+            Vec<float, V> p = {};
+            vec o;
+            if (a.act != GLIF_ACT_NONE) p = *reinterpret_cast<const Vec<float, V> *>(pre + m * a.N);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float v = to_f32(static_cast<T>(g[e])) * slope_of(to_f32(static_cast<T>(p[e])), a.act);
+                const float v = to_f32(static_cast<T>(g[e])) * slope_of(p[e], a.act);
                 o[e] = from_f32<T>(v);
                 s[e] += v;
             }
@@ -655,7 +662,7 @@ __global__ void __launch_bounds__(kBlock) k_slope(SlopeArgs a) {
                 float v = 0.0f;
                 if (n + e < a.N) {
                     v = to_f32(dy[m * a.lddy + e]);
-                    if (a.act != GLIF_ACT_NONE) v *= slope_of(to_f32(pre[m * a.N + e]), a.act);
+                    if (a.act != GLIF_ACT_NONE) v *= slope_of(pre[m * a.N + e], a.act);
                 }
                 if (a.dp && n + e < cols) dp[m * a.lddp + e] = from_f32<T>(v);
                 s[e] += v;
@@ -875,11 +882,13 @@ int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
     if (p.cut_m) {
         a.M = p.cut, b.M -= p.cut, b.p_rows -= p.cut;
         on(b.p, p.cut * size * (PCOL ? 1 : b.p_ld));
-        on(b.c, p.cut * size * b.ldc), on(b.pre, p.cut * size * b.ldc), on(b.residual, p.cut * size * b.ldr);
+        on(b.c, p.cut * size * b.ldc), on(b.residual, p.cut * size * b.ldr);
+        if (b.pre) b.pre += p.cut * b.ldc;
     } else {
         a.N = p.cut, b.N -= p.cut, b.q_rows -= p.cut;
         on(b.q, p.cut * size * (QCOL ? 1 : b.q_ld));
-        on(b.c, p.cut * size), on(b.pre, p.cut * size), on(b.residual, p.cut * size);
+        on(b.c, p.cut * size), on(b.residual, p.cut * size);
+        if (b.pre) b.pre += p.cut;
         on(b.bias, p.cut * static_cast<int64_t>(dtype_size(b.bias_dt)));
     }
     launch_piece<T, PCOL, QCOL>(a, p.one, part, s);
@@ -967,7 +976,7 @@ size_t glif_linear_fwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K)
 
 int glif_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const void *residual,
                     int64_t ldr, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
-                    void *y, void *pre, void *ws, size_t ws_bytes, void *stream) {
+                    void *y, float *pre, void *ws, size_t ws_bytes, void *stream) {
     if (int rc = check_linear(dtype, bias_dtype, M, N, K, activation)) return rc;
     if (int rc = check_strides(ldx, ldw, 0)) return rc;
     if (M == 0 || N == 0) return GLIF_OK;
@@ -992,7 +1001,7 @@ size_t glif_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K,
     return c.mark();
 }
 
-int glif_linear_bwd(const void *dy, int64_t lddy, const void *pre, const void *x, int64_t ldx, const void *weight,
+int glif_linear_bwd(const void *dy, int64_t lddy, const float *pre, const void *x, int64_t ldx, const void *weight,
                     int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
                     void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream) {
     if (int rc = check_linear(dtype, bias_dtype, M, N, K, activation)) return rc;

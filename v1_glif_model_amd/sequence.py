@@ -264,7 +264,7 @@ class _Linear(torch.autograd.Function):
         rr, ldr = _rows(residual, N) if residual is not None else (None, 0)
         b = _dense(bias)
         y = x.new_empty((*x.shape[:-1], N))
-        pre = x.new_empty((M, N)) if act and any(ctx.needs_input_grad[:3]) else None
+        pre = torch.empty((M, N), dtype=torch.float32, device=x.device) if act and any(ctx.needs_input_grad[:3]) else None
         L, dev = lib(), x.device
         n = L.glif_linear_fwd_workspace(dt, M, N, K)
         ws = _workspace(n, dev)
@@ -304,7 +304,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias=None, activation=None, re
     """``act(x @ weight.T + bias) + residual``: x [..., K], weight [N, K] of x's type, bias [N] float32 or of x's type,
     residual [..., N]; ``activation``: None, "relu", "gelu" (the error function's) or "silu".
 
-    For the gradient of an activation its argument is kept, rounded to x's type."""
+    For the gradient of an activation its argument is kept in float32.  The gradient behind the activation is rounded to x's
+    type for the products that give the gradients of x and weight (the matrix cores take no wider operands beside 16-bit
+    ones); the bias's is summed from its float32 values."""
     _activations(x, "x")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {[a for a in ACTIVATIONS]}, got {activation!r}")
