@@ -25,6 +25,25 @@ def slope(p, act):
     return q * (1.0 + p * (1.0 - q))
 
 
+def litter(*sizes):
+    """Leaves NaN in the memory that torch hands out next for these sizes (bytes)."""
+    bad = [torch.full((n // 4,), float("nan"), device=DEV) for n in sizes for _ in range(4)]
+    del bad
+
+
+# ------------------------------------------------------------------------ layer norm ----
+@pytest.mark.parametrize("D,dtype", [(64, F32), (8193, BF16), (66_000, BF16), (5000, F32), (66_000, F32)])
+def test_layer_norm_of_no_rows(D, dtype):
+    """The parameters' gradients are sums of nothing, at every width."""
+    from v1_glif_model_amd import sequence as seq
+    x = torch.empty(0, D, dtype=dtype, device=DEV, requires_grad=True)
+    w, b = (torch.ones(D, device=DEV, requires_grad=True) for _ in range(2))
+    y = seq.layer_norm(x, w, b)
+    litter(4 * D, 8 * D, 8 * D + 256)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert y.shape == dx.shape == (0, D) and not dw.any() and not db.any()
+
+
 # ---------------------------------------------------------------------------- linear ----
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("dtype", [BF16, F16])

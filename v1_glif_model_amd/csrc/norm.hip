@@ -618,7 +618,8 @@ void bwd(const NormArgs &a, hipStream_t s) {
 template <typename T>
 void run_bwd(const NormArgs &a, hipStream_t s) {
     const int64_t p = (a.D + kVecBytes16<T> - 1) / kVecBytes16<T>, size = sizeof(T);
-    if (a.D * size <= kFused) {
+    if (a.parts == 0) {   // no rows: the join gives the empty sums
+    } else if (a.D * size <= kFused) {
         if (p <= 8) bwd<T, 8, 1>(a, s);
         else if (p <= 16) bwd<T, 16, 1>(a, s);
         else if (p <= 32) bwd<T, 32, 1>(a, s);
@@ -695,6 +696,7 @@ int glif_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_
     Carver c(ws, ws_bytes);
     carve(c, a, static_cast<int64_t>(dtype_size(dtype)), dweight || dbias);
     if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "layer norm: workspace too small");
+    if (rows == 0) a.parts = 0;
     GLIF_BY_DTYPE(dtype, run_bwd, a, static_cast<hipStream_t>(stream));
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;
