@@ -87,3 +87,39 @@ def test_linear_float16_arguments_beyond_float16(act):
     near(got[0], dp @ w6, terms @ w6.abs(), "dx", more=one @ w6.abs())
     near(got[1], dp.t() @ x6, terms.t() @ x6.abs(), "dw", more=one.t() @ x6.abs())
     near(got[2], dp.sum(0), terms.sum(0), "db")
+
+
+# ----------------------------------------------------------------------- state space ----
+def scan_leaves(seed, T, B, D, G, N):
+    k = iter(range(seed, seed + 9))
+    t = [rnd(next(k), T, B, D), rnd(next(k), T, B, D), -torch.exp(rnd(next(k), D, N)), rnd(next(k), T, B, G, N), rnd(next(k), T, B, G, N),
+         rnd(next(k), D), rnd(next(k), T, B, D), rnd(next(k), D), rnd(next(k), B, D, N)]
+    return [v.requires_grad_(True) for v in t]
+
+
+@pytest.mark.parametrize("T", [0, 4, 200])
+def test_scan_of_an_empty_batch(T):
+    """The shared parameters' gradients are sums of nothing; the others are empty, as they are."""
+    from v1_glif_model_amd import sequence as seq
+    leaf = scan_leaves(20, T, 0, 6, 2, 16)
+    u, delta, A, B, C, D, z, bias, state = leaf
+    y, last = seq.state_space_scan(u, delta, A, B, C, D, z, bias, initial_state=state)
+    assert y.shape == (T, 0, 6) and last.shape == (0, 6, 16)
+    litter(6 * 16 * 4, 6 * 4)
+    got = torch.autograd.grad((y, last), leaf, (torch.empty_like(y), torch.empty_like(last)))
+    for g, v in zip(got, leaf):
+        assert g.shape == v.shape and not g.any()
+
+
+def test_other_operators_of_an_empty_batch():
+    from v1_glif_model_amd import sequence as seq
+    x, w, b = (rnd(30, *s).requires_grad_(True) for s in ((7, 0, 12), (12, 4), (12,)))
+    st = torch.empty(0, 3, 12, device=DEV, requires_grad=True)
+    litter(12 * 4 * 4, 12 * 4)
+    y, last = seq.short_conv(x, w, b, "silu", st)
+    got = torch.autograd.grad((y, last), (x, w, b, st), (torch.empty_like(y), torch.empty_like(last)))
+    assert all(g.shape == v.shape and not g.any() for g, v in zip(got, (x, w, b, st)))
+    lw, lb = rnd(31, 5, 12).requires_grad_(True), rnd(32, 5).requires_grad_(True)
+    y = seq.linear(x, lw, lb, activation="gelu")
+    got = torch.autograd.grad(y, (x, lw, lb), torch.empty_like(y))
+    assert y.shape == (7, 0, 5) and all(g.shape == v.shape and not g.any() for g, v in zip(got, (x, lw, lb)))

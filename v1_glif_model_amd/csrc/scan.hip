@@ -780,7 +780,7 @@ int glif_scan_bwd(const glif_scan *s, const glif_scan_grad *g, const void *keep,
     shape(a);
     Carver c(ws, ws_bytes);
     carve(c, a);
-    if (!ws || !c.ok()) return fail(GLIF_ENOMEM, "state space: workspace too small");
+    if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "state space: workspace too small");
     if (!g->dB && !g->dC) a.part_bc = nullptr;
     GLIF_BY_DTYPE(s->dtype, run_bwd, a, static_cast<hipStream_t>(stream));
     GLIF_HIP(hipGetLastError());
