@@ -123,3 +123,32 @@ def test_other_operators_of_an_empty_batch():
     y = seq.linear(x, lw, lb, activation="gelu")
     got = torch.autograd.grad(y, (x, lw, lb), torch.empty_like(y))
     assert y.shape == (7, 0, 5) and all(g.shape == v.shape and not g.any() for g, v in zip(got, (x, lw, lb)))
+
+
+# ------------------------------------------------------------- forward-mode derivatives ----
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(grad):
+    """Every operator on an input with a tangent, and the readout: none may answer as if it had none."""
+    from torch.autograd import forward_ad
+
+    from v1_glif_model_amd import sequence as seq
+    from v1_glif_model_amd.readout import SequenceReadout
+    x, w, cw = rnd(40, 6, 2, 8), rnd(41, 5, 8), rnd(42, 8, 4)
+    A, maps = -torch.exp(rnd(43, 8, 4)), rnd(44, 6, 2, 1, 4)
+    mem, h = rnd(45, 2, 3, 8), rnd(46, 2, 8, 4)
+    mem0, h0 = mem.clone(), h.clone()
+    m = SequenceReadout(8, 3, width=16, channels=8, states=4, rank=2, dtype=F32).eval()
+    calls = [lambda v: seq.layer_norm(v), lambda v: seq.dropout(v, 0.5, 1), lambda v: seq.dropout(x, 0.5, 1, residual=v),
+             lambda v: seq.linear(v, w), lambda v: seq.linear(x, v[0, 0, :, None].expand(8, 8).contiguous()),
+             lambda v: seq.short_conv(v, cw), lambda v: seq.short_conv(x, cw, initial_state=v[:2, :, :3].reshape(2, 3, 8)),
+             lambda v: seq.state_space_scan(v, x, A, maps, maps), lambda v: seq.state_space_scan(x, x, A, maps, maps, z=v),
+             lambda v: seq.short_conv_step(v[0], mem, cw), lambda v: seq.state_space_step(x[0], h, v[0], A, maps[0], maps[0]),
+             lambda v: m(v)]
+    for k, call in enumerate(calls):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+                print("not refused:", k)
+    assert torch.equal(mem, mem0) and torch.equal(h, h0)
+    with torch.no_grad(), forward_ad.dual_level():      # a level alone changes nothing
+        assert torch.equal(seq.layer_norm(x), seq.layer_norm(x.clone().requires_grad_(True)).detach())

@@ -12,7 +12,7 @@ these are the operators of a trained readout over whole training windows and, ti
 Activations are float32, bfloat16 or float16 tensors on the GPU; statistics, sums and states are float32 and every output
 is rounded once.  Sequences are time-major ``[T, B, D]`` like the rollouts.  ``lengths`` (int32 ``[B]``, on the device)
 gives every batch entry's own number of ticks: those behind it are not read, give zeros and take no part in gradients.
-All operators but the steps are differentiable once.  Each runs in libglif on the current stream; there is no CPU path.
+All operators but the steps are differentiable once, backwards; forward-mode derivatives are refused.  Each runs in libglif on the current stream; there is no CPU path.
 """
 from __future__ import annotations
 
@@ -21,6 +21,7 @@ import math
 from ctypes import byref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -140,15 +141,23 @@ def _first_only(name):
         raise RuntimeError(f"{name} is differentiable once: create_graph is not supported")
 
 
+def _has_tangent(*tensors):
+    """Whether a tensor carries a forward-mode derivative, which does not make it require a gradient."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _wants_grad(*tensors):
+    """Whether autograd has to see the call: for a gradient, or to refuse a forward-mode derivative."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    return _has_tangent(*tensors)
 
 
 def _refuse_grad(name, *tensors):
+    if _has_tangent(*tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
     if _wants_grad(*tensors):
         raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), or use the form for whole sequences")
 
