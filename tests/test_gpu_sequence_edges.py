@@ -111,6 +111,29 @@ def test_scan_of_an_empty_batch(T):
         assert g.shape == v.shape and not g.any()
 
 
+@pytest.mark.parametrize("D,N", [(70, 16), (3, 4), (5, 64)])
+def test_scan_steps_that_the_bias_makes(D, N):
+    """Plain steps of 0.25, as delta 20.25 less a bias of 20: with a delta of 0, as where a block has no more channels, the
+    decays would be infinite.  B's and C's gradients are sums over the channels that there are."""
+    from tests import seq_ref as ref
+    from v1_glif_model_amd import sequence as seq
+    T, B = 19, 2
+    u, dy = rnd(50, T, B, D), rnd(51, T, B, D)
+    A, Bm, Cm = -torch.linspace(1.0, 8.0, D * N, device=DEV).view(D, N), rnd(52, T, B, 1, N), rnd(53, T, B, 1, N)
+    delta, bias = torch.full((T, B, D), 20.25, device=DEV), torch.full((D,), -20.0, device=DEV)
+    leaf = [t.requires_grad_(True) for t in (u, delta, A, Bm, Cm, bias)]
+    y, _ = seq.state_space_scan(*leaf[:5], delta_bias=bias, delta_softplus=False)
+    got = torch.autograd.grad(y, leaf, dy)
+    own = [f64(t) for t in leaf]
+    y6, _ = ref.scan(*own[:5], bias=own[5], softplus=False)
+    want = torch.autograd.grad(y6, own, f64(dy, False))
+    ab = [(t if i in (1, 2, 5) else t.abs()).detach().requires_grad_(True) for i, t in enumerate(own)]
+    ya, _ = ref.scan(*ab[:5], bias=ab[5], softplus=False, sums=True)
+    near(y, y6, ya.detach(), "y")
+    for g, e, s, name in zip(got, want, torch.autograd.grad(ya, ab, f64(dy, False).abs()), ("u", "delta", "A", "B", "C", "bias")):
+        near(g, e, s.abs(), "d" + name)
+
+
 def test_other_operators_of_an_empty_batch():
     from v1_glif_model_amd import sequence as seq
     x, w, b = (rnd(30, *s).requires_grad_(True) for s in ((7, 0, 12), (12, 4), (12,)))

@@ -367,7 +367,8 @@ __global__ void __launch_bounds__(kBlock) k_scan_bwd(ScanArgs a) {
     const int64_t row = (static_cast<int64_t>(blockIdx.z) * s.n_batch) * s.n_channels + chan;
     const int64_t map_b = me.b * s.B_sb + static_cast<int64_t>(me.g) * N, map_c = me.b * s.C_sb + static_cast<int64_t>(me.g) * N;
     float A[kQ], gh[kQ] = {}, dA[kQ] = {}, steps = 0.0f, dskip = 0.0f, dbias = 0.0f;
-    load_q(A, s.A, static_cast<int64_t>(me.d) * N, me.n0, N);
+    // a lane without a channel adds its zeros to the channels' sums: its decay is 1, as another channel's might be infinite
+    load_q(A, s.A, static_cast<int64_t>(me.d) * N, me.n0, me.on ? N : 0);
 #pragma unroll
     for (int j = 0; j < kQ; ++j) A[j] *= kLog2e;
     if (!ENDS && me.on) {
