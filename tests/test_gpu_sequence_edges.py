@@ -134,6 +134,56 @@ def test_scan_steps_that_the_bias_makes(D, N):
         near(g, e, s.abs(), "d" + name)
 
 
+def test_scan_of_growing_states_that_are_zero():
+    """Rates above 0, steps of 2, inputs in the last ticks and dy in the first: states and adjoints are 0 over most of 600
+    ticks, over which they would grow by e^1200, and finite.  Time is cut into segments here."""
+    from tests import seq_ref as ref
+    from v1_glif_model_amd import sequence as seq
+    T, B, D, N = 600, 1, 3, 16
+    u, dy = rnd(60, T, B, D), rnd(61, T, B, D)
+    u[:-5], dy[5:] = 0.0, 0.0
+    A, Bm, Cm = torch.ones(D, N, device=DEV), rnd(62, T, B, 1, N), rnd(63, T, B, 1, N)
+    leaf = [t.requires_grad_(True) for t in (u, torch.full((T, B, D), 2.0, device=DEV), A, Bm, Cm)]
+    y, last = seq.state_space_scan(*leaf, delta_softplus=False)
+    got = torch.autograd.grad(y, leaf, dy)
+    own = [f64(t) for t in leaf]
+    y6, last6 = ref.scan(*own, softplus=False)
+    want = torch.autograd.grad(y6, own, f64(dy, False))
+    ab = [t.detach().abs().requires_grad_(True) for t in own]
+    ya, la = ref.scan(*ab, softplus=False, sums=True)
+    near(y, y6, ya.detach(), "y")
+    near(last, last6, la.detach(), "last")
+    assert bool(last.isfinite().all()) and float(last.detach().abs().max()) > 1
+    for g, e, s, name in zip(got, want, torch.autograd.grad(ya, ab, f64(dy, False).abs()), ("u", "delta", "A", "B", "C")):
+        assert bool(e.isfinite().all())
+        near(g, e, s.abs(), "d" + name)
+
+
+def test_scan_of_growth_past_float32_over_a_segment():
+    """A state of 1e-30 that grows by e^96 over the first of two segments of time and by e^6 over the second, and adjoints of
+    1e-30 the other way: everything stays within float32, the growth does not."""
+    from tests import seq_ref as ref
+    from v1_glif_model_amd import sequence as seq
+    T, B, D, N = 128, 1, 5, 4
+    delta = torch.full((T, B, D), 1.5, device=DEV)
+    delta[64:] = 0.1
+    t = [rnd(70, T, B, D, scale=1e-30), delta, torch.ones(D, N, device=DEV), rnd(71, T, B, 1, N), rnd(72, T, B, 1, N)]
+    state, dy = rnd(73, B, D, N, scale=1e-30), rnd(74, T, B, D, scale=1e-30)
+    leaf = [v.requires_grad_(True) for v in (*t, state)]
+    y, last = seq.state_space_scan(*leaf[:5], delta_softplus=False, initial_state=state)
+    got = torch.autograd.grad(y, leaf, dy)
+    own = [f64(v) for v in leaf]
+    y6, last6 = ref.scan(*own[:5], softplus=False, state=own[5])
+    want = torch.autograd.grad(y6, own, f64(dy, False))
+    ab = [v.detach().abs().requires_grad_(True) for v in own]
+    ya, la = ref.scan(*ab[:5], softplus=False, state=ab[5], sums=True)
+    # a growth of e^96 carries the float32 rounding of its exponent, 2^-24 of 96 a step of the sum: 64 x 96 x 2^-24 = 4e-4
+    near(y, y6, 40 * ya.detach(), "y")
+    near(last, last6, 40 * la.detach(), "last")
+    for g, e, s, name in zip(got, want, torch.autograd.grad(ya, ab, f64(dy, False).abs()), ("u", "delta", "A", "B", "C", "state")):
+        near(g, e, 40 * s.abs(), "d" + name)
+
+
 def test_other_operators_of_an_empty_batch():
     from v1_glif_model_amd import sequence as seq
     x, w, b = (rnd(30, *s).requires_grad_(True) for s in ((7, 0, 12), (12, 4), (12,)))

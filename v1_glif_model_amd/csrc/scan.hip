@@ -344,7 +344,9 @@ __global__ void __launch_bounds__(kBlock) k_scan_join(ScanArgs a) {
                 if (k0 + u >= a.segs) continue;
                 const int k = BACK ? a.segs - 1 - k0 - u : k0 + u;
                 a.seg_state[k * n + i] = h;
-                h = fmaf(__builtin_amdgcn_exp2f(A * steps[u]), h, end[u]);
+                // In two halves: growth past float32 over a segment may still meet a state small enough, and 0 stays 0.
+                const float half = __builtin_amdgcn_exp2f(0.5f * A * steps[u]);
+                h = h == 0.0f ? end[u] : fmaf(half, half * h, end[u]);
             }
         }
     }
