@@ -184,6 +184,26 @@ def test_scan_of_growth_past_float32_over_a_segment():
         near(g, e, 40 * s.abs(), "d" + name)
 
 
+@pytest.mark.parametrize("T", [16, 21, 700])
+def test_scan_of_rates_of_minus_infinity(T):
+    """States that keep nothing (exp(log_rate) past float32) hold the last live tick's input, at every length: the ticks behind
+    one, and those that fill a chunk of ticks up, leave the state alone."""
+    from v1_glif_model_amd import sequence as seq
+    B, D, N = 4, 6, 5
+    lens = torch.tensor([T, 1, T // 2, T - 1], dtype=torch.int32, device=DEV)
+    u, delta, Bm, Cm = rnd(80, T, B, D), rnd(81, T, B, D), rnd(82, T, B, 1, N), rnd(83, T, B, 1, N)
+    A = -torch.exp(rnd(84, D, N))
+    A[:, 1], A[2] = -math.inf, -math.inf
+    for ln in (None, lens):
+        end = (ln if ln is not None else torch.full((B,), T, device=DEV)).long() - 1
+        y, last = seq.state_space_scan(u, delta, A, Bm, Cm, lengths=ln)
+        i = torch.arange(B, device=DEV)
+        want = (torch.nn.functional.softplus(delta.double()) * u.double())[end, i][..., None] * Bm.double()[end, i]
+        dead = A == -math.inf
+        assert bool(y.isfinite().all()) and bool(last.isfinite().all())
+        near(last[:, dead], want[:, dead].cpu(), want[:, dead].abs().cpu(), "last")
+
+
 def test_other_operators_of_an_empty_batch():
     from v1_glif_model_amd import sequence as seq
     x, w, b = (rnd(30, *s).requires_grad_(True) for s in ((7, 0, 12), (12, 4), (12,)))

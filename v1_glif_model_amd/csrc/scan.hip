@@ -18,6 +18,9 @@
 // Bound by instruction issue: per state and tick an exponential (a quarter of the rate of the rest) and four products and
 // sums forward, some 24 operations backward; what a channel needs per tick adds about a third (vector units busy 85 to 98
 // percent of the time).  Memory would allow 27 us for 16.4M channels' ticks forward and 55 backward.
+#include <cfloat>
+#include <cmath>
+
 #include "seq.h"
 
 namespace glif {
@@ -167,6 +170,13 @@ __device__ __forceinline__ int scan_length(const glif_scan &s, int b) {
     return s.lengths ? min(max(s.lengths[b], 0), s.n_ticks) : s.n_ticks;
 }
 
+// A for powers of 2.  A rate of -infinity (a decay of 0 over any step) is the largest there is: times the step of a tick behind
+// a length, 0, it is a decay of 1.
+__device__ __forceinline__ float rate_of(float A) {
+    const float v = A * kLog2e;
+    return v == -INFINITY ? -FLT_MAX : v;
+}
+
 __device__ __forceinline__ void load_q(float (&v)[kQ], const float *p, int64_t at, int n0, int N) {
 #pragma unroll
     for (int j = 0; j < kQ; ++j) v[j] = n0 + j < N ? p[at + n0 + j] : 0.0f;
@@ -239,7 +249,7 @@ __global__ void __launch_bounds__(kBlock) k_scan_fwd(ScanArgs a) {
     float A[kQ], h[kQ] = {}, steps = 0.0f;
     load_q(A, s.A, static_cast<int64_t>(me.d) * N, me.n0, N);
 #pragma unroll
-    for (int j = 0; j < kQ; ++j) A[j] *= kLog2e;
+    for (int j = 0; j < kQ; ++j) A[j] = rate_of(A[j]);
     if (!ENDS) {
         if (a.segs > 1) load_4(h, a.seg_state + row * kNp + me.n0);
         else if (s.state) load_q(h, s.state, chan * N, me.n0, N);
@@ -326,7 +336,7 @@ __global__ void __launch_bounds__(kBlock) k_scan_join(ScanArgs a) {
         const int64_t chan = i / a.np;
         const int st = static_cast<int>(i - chan * a.np), d = static_cast<int>(chan % s.n_channels);
         const bool real = st < s.n_state;
-        const float A = real ? s.A[static_cast<int64_t>(d) * s.n_state + st] * kLog2e : 0.0f;
+        const float A = real ? rate_of(s.A[static_cast<int64_t>(d) * s.n_state + st]) : 0.0f;
         const float *from = BACK ? a.g.dlast : s.state;
         float h = from && real ? from[chan * s.n_state + st] : 0.0f;
         constexpr int kAhead = 8;
@@ -372,7 +382,7 @@ __global__ void __launch_bounds__(kBlock) k_scan_bwd(ScanArgs a) {
     // a lane without a channel adds its zeros to the channels' sums: its decay is 1, as another channel's might be infinite
     load_q(A, s.A, static_cast<int64_t>(me.d) * N, me.n0, me.on ? N : 0);
 #pragma unroll
-    for (int j = 0; j < kQ; ++j) A[j] *= kLog2e;
+    for (int j = 0; j < kQ; ++j) A[j] = rate_of(A[j]);
     if (!ENDS && me.on) {
         if (a.segs > 1) load_4(gh, a.seg_state + row * kNp + me.n0);
         else if (gr.dlast) load_q(gh, gr.dlast, chan * N, me.n0, N);
