@@ -44,6 +44,27 @@ def test_layer_norm_of_no_rows(D, dtype):
     assert y.shape == dx.shape == (0, D) and not dw.any() and not db.any()
 
 
+@pytest.mark.parametrize("D", [40_000, 66_001])
+@pytest.mark.parametrize("value", [0.1, 0.7, 1.2345, -3.3])
+def test_layer_norm_of_one_active_neuron(D, value):
+    """Wide float32 rows of zeros with one value, first among a thread's own or not: the spread is all that value's."""
+    from v1_glif_model_amd import sequence as seq
+    x, dy, w = torch.zeros(4, D, device=DEV), rnd(10, 4, D), rnd(11, D, shift=1.0, scale=0.3)
+    for r, c in enumerate((0, 4, 1777, D - 1)):
+        x[r, c] = value
+    xs = x.requires_grad_(True)
+    y = seq.layer_norm(xs, w)
+    (dx,) = torch.autograd.grad(y, xs, dy)
+    x6, g6, w6 = (f64(t, False) for t in (x, dy, w))
+    mean = x6.mean(-1, keepdim=True)
+    rstd = 1.0 / torch.sqrt(((x6 - mean) ** 2).mean(-1, keepdim=True) + 1e-5)
+    xh, far = (x6 - mean) * rstd, (x6.abs() + x6.abs().mean(-1, keepdim=True)) * rstd
+    near(y, xh * w6, far * w6.abs(), "y")
+    gw, ga = g6 * w6, g6.abs() * w6.abs()
+    near(dx, rstd * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True)),
+         rstd * (ga + ga.mean(-1, keepdim=True) * (1 + far) + far * (ga * far).mean(-1, keepdim=True)), "dx")
+
+
 # ---------------------------------------------------------------------------- linear ----
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("dtype", [BF16, F16])

@@ -299,10 +299,25 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormArgs a) {
 // rows, and the second time comes from cache.
 constexpr int kWide = 512, kLong = 1024, kLongR = 9, kLongFrom = 6144;
 
-// Count, mean and sum of squared differences from it, of the elements seen.  A thread takes its sums from its own first
-// element on, so that a mean far from zero costs no digits.
+// Count, mean and sum of squared differences from it, of the elements seen.  A thread takes them from its own first element
+// on, so that a mean far from zero costs no digits, and piece by piece about each piece's own mean, so that a first element far
+// from the others costs none either (one sum of squares about it lost 4e-4 of the variance where it was the row's only one).
 struct Moments {
     float n, mean, m2;
+    template <int V>
+    __device__ __forceinline__ void add(const float (&d)[V], int have) {   // d: 0 from `have` on
+        float s = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += d[e];
+        const float h = static_cast<float>(have), its = s / h;
+#pragma unroll
+        for (int e = 0; e < V; ++e) q = e < have ? fmaf(d[e] - its, d[e] - its, q) : q;
+        const float before = n, far = its - mean;
+        n += h;
+        const float share = h * __builtin_amdgcn_rcpf(n);
+        m2 = fmaf(far * far, before * share, m2 + q);
+        mean = fmaf(far, share, mean);
+    }
 };
 __device__ __forceinline__ Moments both(Moments a, Moments b) {
     const float n = a.n + b.n, d = b.mean - a.mean, share = n > 0.0f ? b.n / n : 0.0f;
@@ -361,18 +376,14 @@ __global__ void __launch_bounds__(kWide) k_norm_fwd_wide(NormArgs a) {
     const int D = static_cast<int>(a.D), first = threadIdx.x * V;
     const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
     const float k = first < D ? to_f32(x[first]) : 0.0f;
-    float s = 0.0f, q = 0.0f, n = 0.0f;
+    Moments own{};
     pieces(x, D, [&](int, int have, vec v) {
+        float d[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float d = e < have ? to_f32(static_cast<T>(v[e])) - k : 0.0f;
-            s += d;
-            q = fmaf(d, d, q);
-        }
-        n += static_cast<float>(have);
+        for (int e = 0; e < V; ++e) d[e] = e < have ? to_f32(static_cast<T>(v[e])) - k : 0.0f;
+        own.add<V>(d, have);
     });
-    const float d = n > 0.0f ? s / n : 0.0f;
-    const Moments m = all_moments<kWide>({n, k + d, q - s * d}, red);
+    const Moments m = all_moments<kWide>({own.n, k + own.mean, own.m2}, red);
     const float rstd = 1.0f / sqrtf(m.m2 / static_cast<float>(D) + a.eps);
     T *y = static_cast<T *>(a.y) + r * a.D;
     pieces(x, D, [&](int c, int have, vec v) {
@@ -444,22 +455,21 @@ __device__ __forceinline__ void wide_stats(const NormArgs &a, int64_t r) {
     const int D = static_cast<int>(a.D), first = threadIdx.x * V;
     const T *x = static_cast<const T *>(a.x) + r * a.x_stride, *dy = static_cast<const T *>(a.dy) + r * a.dy_stride;
     const float k = first < D ? to_f32(x[first]) : 0.0f;
-    float s = 0.0f, q = 0.0f, n = 0.0f, g1 = 0.0f, g2 = 0.0f;
+    Moments own{};
+    float g1 = 0.0f, g2 = 0.0f;
     pieces2(x, dy, D, [&](int c, int have, vec v, vec g) {
-        float w[V];
+        float w[V], d[V];
         params<V>(w, a.weight, a.pdt, c, D, 1.0f);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float d = e < have ? to_f32(static_cast<T>(v[e])) - k : 0.0f, gw = to_f32(static_cast<T>(g[e])) * w[e];
-            s += d;
-            q = fmaf(d, d, q);
+            d[e] = e < have ? to_f32(static_cast<T>(v[e])) - k : 0.0f;
+            const float gw = to_f32(static_cast<T>(g[e])) * w[e];
             g1 += gw;
-            g2 = fmaf(gw, d, g2);
+            g2 = fmaf(gw, d[e], g2);
         }
-        n += static_cast<float>(have);
+        own.add<V>(d, have);
     });
-    const float d = n > 0.0f ? s / n : 0.0f;
-    const Moments m = all_moments<kWide>({n, k + d, q - s * d}, red);
+    const Moments m = all_moments<kWide>({own.n, k + own.mean, own.m2}, red);
     const float rstd = 1.0f / sqrtf(m.m2 / static_cast<float>(D) + a.eps);
     const float2 g = row_sum2<kWide>(g1, rstd * fmaf(k - m.mean, g1, g2), red2);
     if (threadIdx.x == 0) a.stat[r] = make_float4(m.mean, rstd, g.x / static_cast<float>(D), g.y / static_cast<float>(D));
