@@ -65,6 +65,37 @@ def test_layer_norm_of_one_active_neuron(D, value):
          rstd * (ga + ga.mean(-1, keepdim=True) * (1 + far) + far * (ga * far).mean(-1, keepdim=True)), "dx")
 
 
+@pytest.mark.parametrize("D", [2 ** 30])
+def test_layer_norm_of_the_longest_rows(D):
+    """Millions of terms a thread, as exact as a hundred."""
+    from v1_glif_model_amd import sequence as seq
+    step = 2 ** 28
+    x, dy = torch.empty(1, D, dtype=F16, device=DEV), torch.empty(1, D, dtype=F16, device=DEV)
+    g = torch.Generator(DEV).manual_seed(12)
+    for at in range(0, D, step):
+        n = min(step, D - at)
+        x[0, at:at + n].copy_(torch.randn(n, generator=g, device=DEV))
+        dy[0, at:at + n].copy_(torch.rand(n, generator=g, device=DEV) + x[0, at:at + n])
+    xs = x.requires_grad_(True)
+    y = seq.layer_norm(xs)
+    (dx,) = torch.autograd.grad(y, xs, dy)
+    cut = [slice(at, min(at + step, D)) for at in range(0, D, step)]
+    with torch.no_grad():
+        mean = sum(x[0, c].double().sum() for c in cut) / D
+        rstd = 1.0 / torch.sqrt(sum(((x[0, c].double() - mean) ** 2).sum() for c in cut) / D + 1e-5)
+        size = sum(x[0, c].double().abs().sum() for c in cut) / D
+        sums = [0.0] * 4
+        for c in cut:
+            xh, far, gw = (x[0, c].double() - mean) * rstd, (x[0, c].double().abs() + size) * rstd, dy[0, c].double()
+            sums = [a + float(b) / D for a, b in zip(sums, (gw.sum(), (gw * xh).sum(), gw.abs().sum(), (gw.abs() * far).sum()))]
+        for c in (slice(0, 70), slice(D // 2, D // 2 + 70), slice(D - 70, D)):
+            x6, gw = x[0, c].double().cpu(), dy[0, c].double().cpu()
+            m, r = mean.cpu(), rstd.cpu()
+            xh, far = (x6 - m) * r, (x6.abs() + size.cpu()) * r
+            near(y[0, c], xh, far, "y")
+            near(dx[0, c], r * (gw - sums[0] - xh * sums[1]), r * (gw.abs() + sums[2] * (1 + far) + far * sums[3]), "dx")
+
+
 # ---------------------------------------------------------------------------- linear ----
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("dtype", [BF16, F16])

@@ -66,8 +66,8 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float *red) {
     }
 }
 
-// 16 bytes of a row from column c on, zeros past its end.  Whole words throughout: a piece put together from its elements
-// would live in a register for each of them.
+// 16 bytes of a row from column c on, zeros past its end.  Whole words throughout: a piece put together from its elements would
+// live in a register for each of them.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
 __device__ __forceinline__ u32x4 piece(const T *p, int c, int D) {
@@ -315,7 +315,7 @@ struct Moments {
         const float before = n, far = its - mean;
         n += h;
         const float share = h * __builtin_amdgcn_rcpf(n);
-        m2 = fmaf(far * far, before * share, m2 + q);
+        m2 += fmaf(far * far, before * share, q);
         mean = fmaf(far, share, mean);
     }
 };
@@ -458,15 +458,16 @@ __device__ __forceinline__ void wide_stats(const NormArgs &a, int64_t r) {
     Moments own{};
     float g1 = 0.0f, g2 = 0.0f;
     pieces2(x, dy, D, [&](int c, int have, vec v, vec g) {
-        float w[V], d[V];
+        float w[V], d[V], p1 = 0.0f, p2 = 0.0f;   // a piece's sums first: single terms would be lost beside a long row's
         params<V>(w, a.weight, a.pdt, c, D, 1.0f);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             d[e] = e < have ? to_f32(static_cast<T>(v[e])) - k : 0.0f;
             const float gw = to_f32(static_cast<T>(g[e])) * w[e];
-            g1 += gw;
-            g2 = fmaf(gw, d[e], g2);
+            p1 += gw;
+            p2 = fmaf(gw, d[e], p2);
         }
+        g1 += p1, g2 += p2;
         own.add<V>(d, have);
     });
     const Moments m = all_moments<kWide>({own.n, k + own.mean, own.m2}, red);
