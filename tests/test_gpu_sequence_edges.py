@@ -65,9 +65,9 @@ def test_layer_norm_of_one_active_neuron(D, value):
          rstd * (ga + ga.mean(-1, keepdim=True) * (1 + far) + far * (ga * far).mean(-1, keepdim=True)), "dx")
 
 
-@pytest.mark.parametrize("D", [2 ** 30])
+@pytest.mark.parametrize("D", [2 ** 30, 2 ** 31 - 1])
 def test_layer_norm_of_the_longest_rows(D):
-    """Millions of terms a thread, as exact as a hundred."""
+    """Millions of terms a thread, as exact as a hundred; and 2^31 - 1 columns, whose last piece ends where 31 bits do."""
     from v1_glif_model_amd import sequence as seq
     step = 2 ** 28
     x, dy = torch.empty(1, D, dtype=F16, device=DEV), torch.empty(1, D, dtype=F16, device=DEV)

@@ -67,13 +67,14 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float *red) {
 }
 
 // 16 bytes of a row from column c on, zeros past its end.  Whole words throughout: a piece put together from its elements would
-// live in a register for each of them.
+// live in a register for each of them.  (Here and below a whole piece is one with c <= D - V: c + V passes 31 bits in the last
+// piece of the longest rows.)
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
 __device__ __forceinline__ u32x4 piece(const T *p, int c, int D) {
     constexpr int V = kVecBytes16<T>;
     u32x4 q = {};
-    if (c + V <= D) {
+    if (c <= D - V) {
         q = __builtin_bit_cast(u32x4, *reinterpret_cast<const Vec<T, V> *>(p + c));
     } else if (c < D) {
 #pragma unroll
@@ -108,7 +109,7 @@ struct Row {
     }
     template <bool PAST = false>
     static __device__ __forceinline__ void put(T *p, int c, int D, const float (&v)[V]) {
-        if (c + V <= D) {
+        if (c <= D - V) {
             vec o;
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = from_f32<T>(v[e]);
@@ -146,7 +147,7 @@ __device__ __forceinline__ void params(float (&v)[V], const void *p, int32_t dt,
     if (!p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = other;
-    } else if (dt == GLIF_F32 && c + V <= D) {
+    } else if (dt == GLIF_F32 && c <= D - V) {
         const Vec<float, 4> *q = reinterpret_cast<const Vec<float, 4> *>(static_cast<const float *>(p) + c);
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = q[e / 4][e % 4];
@@ -160,7 +161,7 @@ __device__ __forceinline__ void params(float (&v)[V], const void *p, int32_t dt,
 template <int V>
 __device__ __forceinline__ void flush(float *part, int c, int D, const float (&v)[V], bool more) {
     typedef Vec<float, 4> f4;
-    if (c + V <= D) {
+    if (c <= D - V) {
 #pragma unroll
         for (int h = 0; h < V; h += 4) {
             f4 o = {v[h], v[h + 1], v[h + 2], v[h + 3]};
@@ -501,7 +502,7 @@ __device__ __forceinline__ void wide_columns(const NormArgs &a, int block, int64
         }
         if (dx) Row<T, 1, 1>::template put<PAST>(dx + r * a.D, c, D, o);
     };
-    if (c + V <= D) {
+    if (c <= D - V) {
 #pragma unroll 2
         for (int64_t r = r0; r < r1; ++r)
             add(*reinterpret_cast<const vec *>(x + r * a.x_stride), *reinterpret_cast<const vec *>(dy + r * a.dy_stride), r);
