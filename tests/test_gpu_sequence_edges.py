@@ -96,6 +96,38 @@ def test_layer_norm_of_the_longest_rows(D):
             near(dx[0, c], r * (gw - sums[0] - xh * sums[1]), r * (gw.abs() + sums[2] * (1 + far) + far * sums[3]), "dx")
 
 
+def test_layer_norm_of_more_rows_than_a_launch_holds():
+    """2^29 rows of two: their threads pass 32 bits.  The last rows are those of a small call."""
+    from v1_glif_model_amd import sequence as seq
+    x = torch.empty(2 ** 29 + 3, 2, dtype=F16, device=DEV)
+    for part in x.split(2 ** 26):
+        part.normal_(generator=torch.Generator(DEV).manual_seed(14))
+    xs = x.requires_grad_(True)
+    y = seq.layer_norm(xs)
+    (dx,) = torch.autograd.grad(y, xs, x.detach())
+    for part in (slice(0, 100), slice(2 ** 28 - 50, 2 ** 28 + 50), slice(-100, None)):
+        own = x.detach()[part].clone().requires_grad_(True)
+        few = seq.layer_norm(own)
+        assert torch.equal(y[part], few) and torch.equal(dx[part], torch.autograd.grad(few, own, own.detach())[0])
+
+
+def test_parameters_of_more_channels_than_a_launch_joins():
+    """The joins of the parameters' sums, 8 threads a sum: one row's and one tick's gradients are products."""
+    from v1_glif_model_amd import sequence as seq
+    D = 2 ** 29 + 77
+    x = torch.empty(1, D, dtype=F16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(15))
+    b = torch.zeros(D, dtype=F16, device=DEV, requires_grad=True)
+    (db,) = torch.autograd.grad(seq.layer_norm(x, None, b), b, x)
+    assert torch.equal(db, x[0])
+    del b, db
+    D = 2 ** 26 + 77
+    x = x[0, :D].reshape(1, 1, D)
+    w = torch.ones(D, 8, dtype=F16, device=DEV, requires_grad=True)
+    y, _ = seq.short_conv(x, w)
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert torch.equal(y, x) and torch.equal(dw[:, 7], x[0, 0]) and not dw[:, :7].any()
+
+
 # ---------------------------------------------------------------------------- linear ----
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("dtype", [BF16, F16])

@@ -267,11 +267,11 @@ __global__ void __launch_bounds__(kBlock) k_conv_bwd(ConvArgs a) {
     }
 }
 
-// dw and db: the parts' sums, 32 columns by 8 threads each, which take the parts in turn.
-__global__ void __launch_bounds__(kBlock) k_conv_join(ConvArgs a) {
+// dw and db: the parts' sums from i0 on, 32 columns by 8 threads each, which take the parts in turn.
+__global__ void __launch_bounds__(kBlock) k_conv_join(ConvArgs a, int64_t i0) {
     __shared__ float sum[8][32];
     const int col = threadIdx.x % 32, lot = threadIdx.x / 32;
-    const int64_t n = static_cast<int64_t>(a.W + 1) * a.D, i = static_cast<int64_t>(blockIdx.x) * 32 + col;
+    const int64_t n = static_cast<int64_t>(a.W + 1) * a.D, i = i0 + static_cast<int64_t>(blockIdx.x) * 32 + col;
     float s = 0.0f;
     if (i < n) {
 #pragma unroll 4
@@ -338,8 +338,10 @@ void shape(ConvArgs &a, int v) {
 }
 
 void join(const ConvArgs &a, hipStream_t s) {
-    if (a.part)
-        hipLaunchKernelGGL(k_conv_join, dim3(static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.W + 1) * a.D, 32))), dim3(kBlock), 0, s, a);
+    constexpr int64_t kMost = blocks_at_once(kBlock) * 32;
+    const int64_t n = static_cast<int64_t>(a.W + 1) * a.D;
+    for (int64_t i = 0; a.part && i < n; i += kMost)
+        hipLaunchKernelGGL(k_conv_join, dim3(static_cast<unsigned>(ceil_div(std::min(kMost, n - i), 32))), dim3(kBlock), 0, s, a, i);
 }
 
 template <typename T, int W>

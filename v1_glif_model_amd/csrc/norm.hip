@@ -538,11 +538,11 @@ __global__ void __launch_bounds__(kWide, 6) k_norm_round(NormArgs a, Round k) {
     }
 }
 
-// The parts' sums: 32 columns by 8 threads each, which take the parts in turn.
-__global__ void __launch_bounds__(kBlock) k_norm_join(NormArgs a) {
+// The parts' sums, from column c0 on: 32 columns by 8 threads each, which take the parts in turn.
+__global__ void __launch_bounds__(kBlock) k_norm_join(NormArgs a, int64_t c0) {
     __shared__ float sum[2][8][32];
     const int col = threadIdx.x % 32, lot = threadIdx.x / 32;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + col;
+    const int64_t c = c0 + static_cast<int64_t>(blockIdx.x) * 32 + col;
     float dw = 0.0f, db = 0.0f;
     if (c < a.D) {
 #pragma unroll 4
@@ -597,10 +597,15 @@ void carve(Carver &c, NormArgs &a, int64_t size, bool param) {
 }
 
 template <typename T, int L, int R>
-void fwd(const NormArgs &a, hipStream_t s) {
-    constexpr int kRows = L > kBlock ? 1 : kBlock / L;
-    hipLaunchKernelGGL((k_norm_fwd<T, L, R>), dim3(static_cast<unsigned>((a.rows + kRows - 1) / kRows)), dim3(L > kBlock ? L : kBlock),
-                       0, s, a);
+void fwd(NormArgs a, hipStream_t s) {
+    constexpr int kThreads = L > kBlock ? L : kBlock, kRows = kThreads / L;
+    constexpr int64_t kMost = blocks_at_once(kThreads) * kRows;
+    const int64_t rows = a.rows;
+    for (int64_t r = 0; r < rows; r += kMost) {
+        a.rows = std::min(kMost, rows - r);
+        hipLaunchKernelGGL((k_norm_fwd<T, L, R>), dim3(static_cast<unsigned>((a.rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, a);
+        a.x = static_cast<const T *>(a.x) + kMost * a.x_stride, a.y = static_cast<T *>(a.y) + kMost * a.D;
+    }
 }
 
 // The threads of a row: as few as hold it in one piece each, up to a wave with four, a block with four, 1024 with four.
@@ -652,8 +657,9 @@ void run_bwd(const NormArgs &a, hipStream_t s) {
             else hipLaunchKernelGGL((k_norm_round<T, false>), dim3(static_cast<unsigned>(blocks)), dim3(kWide), 0, s, a, k);
         }
     }
-    if (a.part)
-        hipLaunchKernelGGL(k_norm_join, dim3(static_cast<unsigned>((a.D + 31) / 32)), dim3(kBlock), 0, s, a);
+    constexpr int64_t kMost = blocks_at_once(kBlock) * 32;
+    for (int64_t c = 0; a.part && c < a.D; c += kMost)
+        hipLaunchKernelGGL(k_norm_join, dim3(static_cast<unsigned>((std::min(kMost, a.D - c) + 31) / 32)), dim3(kBlock), 0, s, a, c);
 }
 
 int check_norm(int64_t rows, int64_t D, int32_t dtype, int32_t pdt, float eps) {

@@ -23,6 +23,9 @@ using Vec = typename VecOf<T, V>::type;
 // kernel itself reads again.
 constexpr int64_t kPastCaches = int64_t(96) << 20;
 
+// Blocks of `threads` that one launch can have: its threads are counted in 32 bits.
+constexpr int64_t blocks_at_once(int threads) { return (int64_t(1) << 31) / threads; }
+
 template <typename T>
 constexpr int kVecBytes16 = 16 / static_cast<int>(sizeof(T));   // elements in a 16-byte access
 
