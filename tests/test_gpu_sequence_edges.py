@@ -288,6 +288,24 @@ def test_scan_of_rates_of_minus_infinity(T):
         near(last[:, dead], want[:, dead].cpu(), want[:, dead].abs().cpu(), "last")
 
 
+def test_scan_of_as_many_groups_as_a_launch_holds():
+    """2^23 groups of two channels are right to the last; 2^24 of one, whose threads pass 32 bits, are refused."""
+    from v1_glif_model_amd import sequence as seq
+    G = 2 ** 23
+    u, delta = rnd(90, 1, 1, 2).repeat(1, 1, G), rnd(91, 1, 1, 2).repeat(1, 1, G)
+    A, maps = -torch.ones(2 * G, 1, device=DEV), torch.ones(1, 1, G, 1, device=DEV)
+    maps[..., -1, :] = 3.0
+    y, last = seq.state_space_scan(u, delta, A, maps, maps)
+    one, end = seq.state_space_scan(u[..., :2].contiguous(), delta[..., :2].contiguous(), A[:2], maps[:, :, :1], maps[:, :, :1])
+    assert torch.equal(y[..., :-2].unflatten(-1, (-1, 2)), one.unsqueeze(-2).expand(1, 1, G - 1, 2))
+    assert torch.equal(y[..., -2:], 3 * (3 * end.view(1, 1, 2))) and torch.equal(last[:, -2:], 3 * end)
+    maps = torch.ones(1, 1, 2 * G, 1, device=DEV)
+    with pytest.raises(ValueError, match="groups"):
+        seq.state_space_scan(u, delta, A, maps, maps)
+    with pytest.raises(ValueError, match="groups"):
+        seq.state_space_step(u[0], torch.zeros(1, 2 * G, 1, device=DEV), delta[0], A, maps[0], maps[0])
+
+
 def test_other_operators_of_an_empty_batch():
     from v1_glif_model_amd import sequence as seq
     x, w, b = (rnd(30, *s).requires_grad_(True) for s in ((7, 0, 12), (12, 4), (12,)))

@@ -713,6 +713,8 @@ int check_scan(const glif_scan *s) {
         s->n_channels > (1 << 24))
         return fail(GLIF_EINVAL, "state space: ticks in [0, 2^20], batch in [0, 65535], channels in [1, 2^24]");
     if (s->n_groups < 1 || s->n_channels % s->n_groups) return fail(GLIF_EINVAL, "state space: the groups must divide the channels");
+    // a launch counts its threads in 32 bits, and a group has a block of them at least
+    if (s->n_groups >= (1 << 24)) return fail(GLIF_EINVAL, "state space: fewer than 2^24 groups");
     if (s->n_state < 1 || s->n_state > 64) return fail(GLIF_EINVAL, "state space: 1 to 64 states");
     return GLIF_OK;
 }
