@@ -347,3 +347,36 @@ def test_forward_mode_derivatives_are_refused(grad):
     assert torch.equal(mem, mem0) and torch.equal(h, h0)
     with torch.no_grad(), forward_ad.dual_level():      # a level alone changes nothing
         assert torch.equal(seq.layer_norm(x), seq.layer_norm(x.clone().requires_grad_(True)).detach())
+
+
+# --------------------------------------------------------------------------- the readout ----
+def small_readout(dtype, **kw):
+    from v1_glif_model_amd.readout import SequenceReadout
+    return SequenceReadout(20, 5, width=16, channels=24, states=4, groups=2, taps=3, rank=3, dtype=dtype, seed=4, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("how", ["step", "load"])
+def test_ticks_go_on_with_the_readout_their_state_was_made_for(dtype, how):
+    """Parameters that change in place between two ticks change nothing for a state that is under way, and all for a new one."""
+    import copy
+    m = small_readout(dtype).eval()
+    old, other = copy.deepcopy(m), small_readout(dtype).eval()
+    with torch.no_grad():
+        for k, p in other.named_parameters():
+            p.add_(0.1 * torch.randn(p.shape, generator=torch.Generator().manual_seed(5)).to(DEV))
+    x = rnd(95, 4, 3, 20)
+    state, want = m.zero_state(3), old.zero_state(3)
+    assert not {t.data_ptr() for t in state.weights.values()} & {p.data_ptr() for p in m.parameters()}
+    assert torch.equal(m.tick(x[0], state), old.tick(x[0], want))
+    if how == "load":
+        m.load_state_dict(other.state_dict())
+    else:
+        with torch.no_grad():
+            for p, q in zip(m.parameters(), other.parameters()):
+                p.copy_(q)
+    for t in range(1, 4):
+        assert torch.equal(m.tick(x[t], state), old.tick(x[t], want)), t
+    new, want = m.zero_state(3), other.zero_state(3)
+    for t in range(4):
+        assert torch.equal(m.tick(x[t], new), other.tick(x[t], want)), t

@@ -24,8 +24,8 @@ __all__ = ["SequenceReadout", "ReadoutState"]
 
 
 class ReadoutState(NamedTuple):
-    """What tick-by-tick reading carries: the last inputs of the convolution, the state space's state, and the weights in
-    the activations' type as they were when the state was made."""
+    """What tick-by-tick reading carries: the last inputs of the convolution, the state space's state, and all of the readout's
+    parameters as they were when the state was made (matrices in the activations' type): training goes on beside it unseen."""
     conv: torch.Tensor      # [B, taps - 1, channels]
     scan: torch.Tensor      # [B, channels, states], float32
     weights: dict
@@ -83,16 +83,22 @@ class SequenceReadout(nn.Module):
         self.norm_out, self.norm_out_bias = filled(1, width), filled(0, width)
         self.head, self.head_bias = matrix(n_outputs, width), filled(0, n_outputs)
 
-    def _weights(self):
-        """The matrices in the activations' type, and the decay rates."""
-        w = {k: getattr(self, k).to(self.dtype) for k in ("embed", "mix_in", "maps", "step", "mix_out", "head")}
+    _MATRICES = ("embed", "mix_in", "maps", "step", "mix_out", "head")
+    _VECTORS = ("norm_in", "norm_in_bias", "embed_bias", "norm_mix", "norm_mix_bias", "conv", "conv_bias", "step_bias", "skip",
+                "mix_out_bias", "norm_out", "norm_out_bias", "head_bias")
+
+    def _weights(self, own: bool = False):
+        """All that the operators read: the matrices in the activations' type, the decay rates, and the rest as it is.  own:
+        none of it shares memory with a parameter."""
+        w = {k: getattr(self, k).to(self.dtype, copy=own) for k in self._MATRICES}
+        w.update((k, getattr(self, k).clone() if own else getattr(self, k)) for k in self._VECTORS)
         w["A"] = -torch.exp(self.log_rate)
         return w
 
     def _into(self, x, w):
         """The residual stream h, and the convolution's input and the gates."""
-        h = linear(layer_norm(x, self.norm_in, self.norm_in_bias), w["embed"], self.embed_bias)
-        c, gate = linear(layer_norm(h, self.norm_mix, self.norm_mix_bias), w["mix_in"]).split(self.channels, -1)
+        h = linear(layer_norm(x, w["norm_in"], w["norm_in_bias"]), w["embed"], w["embed_bias"])
+        c, gate = linear(layer_norm(h, w["norm_mix"], w["norm_mix_bias"]), w["mix_in"]).split(self.channels, -1)
         return h, c, gate
 
     def _maps(self, u, w):
@@ -103,7 +109,7 @@ class SequenceReadout(nn.Module):
         return linear(low, w["step"]), B.unflatten(-1, shape), C.unflatten(-1, shape)
 
     def _out(self, h, w):
-        return linear(layer_norm(h, self.norm_out, self.norm_out_bias), w["head"], self.head_bias)
+        return linear(layer_norm(h, w["norm_out"], w["norm_out_bias"]), w["head"], w["head_bias"])
 
     def _input(self, x, dims):
         if not isinstance(x, torch.Tensor) or x.dim() != dims or x.shape[-1] != self.n_neurons:
@@ -116,10 +122,10 @@ class SequenceReadout(nn.Module):
         and its outputs mean nothing (x must be finite there, and a loss leaves them out)."""
         x, w = self._input(x, 3), self._weights()
         h, c, gate = self._into(x, w)
-        u, _ = short_conv(c, self.conv, self.conv_bias, activation="silu", lengths=lengths)
+        u, _ = short_conv(c, w["conv"], w["conv_bias"], activation="silu", lengths=lengths)
         delta, B, C = self._maps(u, w)
-        y, _ = state_space_scan(u, delta, w["A"], B, C, self.skip, gate, self.step_bias, lengths=lengths)
-        y = linear(y, w["mix_out"], self.mix_out_bias)
+        y, _ = state_space_scan(u, delta, w["A"], B, C, w["skip"], gate, w["step_bias"], lengths=lengths)
+        y = linear(y, w["mix_out"], w["mix_out_bias"])
         if self.training and self.dropout:
             h = dropout(y, self.dropout, self.seed, self.drawn, residual=h)
             self.drawn += y.numel()
@@ -133,17 +139,17 @@ class SequenceReadout(nn.Module):
         dev = self.embed.device
         return ReadoutState(torch.zeros(batch_size, self.taps - 1, self.channels, dtype=self.dtype, device=dev),
                             torch.zeros(batch_size, self.channels, self.states, dtype=torch.float32, device=dev),
-                            self._weights())
+                            self._weights(own=True))
 
     @torch.no_grad()
     def tick(self, x: torch.Tensor, state: ReadoutState) -> torch.Tensor:
         """One tick: x [B, n_neurons] to [B, n_outputs], without dropout or gradient; ``state`` is moved on in place."""
         x, w = self._input(x, 2), state.weights
         h, c, gate = self._into(x, w)
-        u = short_conv_step(c, state.conv, self.conv, self.conv_bias, activation="silu")
+        u = short_conv_step(c, state.conv, w["conv"], w["conv_bias"], activation="silu")
         delta, B, C = self._maps(u, w)
-        y = state_space_step(u, state.scan, delta, w["A"], B, C, self.skip, gate, self.step_bias)
-        return self._out(linear(y, w["mix_out"], self.mix_out_bias, residual=h), w)
+        y = state_space_step(u, state.scan, delta, w["A"], B, C, w["skip"], gate, w["step_bias"])
+        return self._out(linear(y, w["mix_out"], w["mix_out_bias"], residual=h), w)
 
 
 def example(steps: int = 60, ticks: int = 100, batch: int = 16, classes: int = 4, seed: int = 0, say=print):
