@@ -380,3 +380,24 @@ def test_ticks_go_on_with_the_readout_their_state_was_made_for(dtype, how):
     new, want = m.zero_state(3), other.zero_state(3)
     for t in range(4):
         assert torch.equal(m.tick(x[t], new), other.tick(x[t], want)), t
+
+
+def test_training_that_is_resumed_goes_on_with_the_masks(tmp_path):
+    """A readout saved between two steps and loaded again draws the masks that the saved one would have drawn next."""
+    x = rnd(96, 6, 2, 20)
+    m = small_readout(F32, dropout=0.5).train()
+    m(x)
+    torch.save(m.state_dict(), tmp_path / "m.pt")
+    new = small_readout(F32, dropout=0.5).train()
+    new.load_state_dict(torch.load(tmp_path / "m.pt", weights_only=True))
+    assert new.drawn == m.drawn == 6 * 2 * 16
+    assert torch.equal(new(x).detach(), m(x).detach())
+    assert not torch.equal(new(x).detach(), small_readout(F32, dropout=0.5).train()(x).detach())
+    whole = torch.nn.ModuleList([small_readout(F32, dropout=0.5)])
+    whole.load_state_dict({"0." + k: v for k, v in m.state_dict().items()})
+    assert whole[0].drawn == m.drawn
+    named = dict(m.named_parameters())                      # as it was saved before the masks' place was in it
+    new.load_state_dict({k: v.detach() for k, v in named.items()})
+    assert new.drawn == 3 * 6 * 2 * 16
+    with pytest.raises(RuntimeError, match="head_bias"):
+        new.load_state_dict({k: v.detach() for k, v in named.items() if k != "head_bias"})

@@ -37,7 +37,7 @@ class SequenceReadout(nn.Module):
     ``mix`` is a projection to ``channels`` and as many gates, a short convolution of ``taps`` ticks, the state space with
     step, input and output maps projected from the convolved channels (the step through ``rank``), and a projection back.
     Parameters are float32; products run in ``dtype`` (float32, bfloat16 or float16).  ``seed`` sets the first weights and
-    names the stream of the dropout's masks."""
+    names the stream of the dropout's masks; ``drawn``, how much of it training has used, is part of the ``state_dict``."""
 
     def __init__(self, n_neurons: int, n_outputs: int, width: int = 256, channels: int = 512, states: int = 16, groups: int = 1,
                  taps: int = 4, rank: int = 16, dropout: float = 0.1, dtype=torch.bfloat16, seed: int = 0, device="cuda"):
@@ -82,6 +82,18 @@ class SequenceReadout(nn.Module):
         self.mix_out, self.mix_out_bias = matrix(width, channels), filled(0, width)
         self.norm_out, self.norm_out_bias = filled(1, width), filled(0, width)
         self.head, self.head_bias = matrix(n_outputs, width), filled(0, n_outputs)
+
+    def get_extra_state(self):
+        return torch.tensor(self.drawn, dtype=torch.int64)
+
+    def set_extra_state(self, state):
+        self.drawn = int(state)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, *more):
+        """A state without the stream's place leaves it where it is."""
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, *more)
+        if prefix + "_extra_state" in missing_keys:
+            missing_keys.remove(prefix + "_extra_state")
 
     _MATRICES = ("embed", "mix_in", "maps", "step", "mix_out", "head")
     _VECTORS = ("norm_in", "norm_in_bias", "embed_bias", "norm_mix", "norm_mix_bias", "conv", "conv_bias", "step_bias", "skip",
