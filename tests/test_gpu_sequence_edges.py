@@ -401,3 +401,28 @@ def test_training_that_is_resumed_goes_on_with_the_masks(tmp_path):
     assert new.drawn == 3 * 6 * 2 * 16
     with pytest.raises(RuntimeError, match="head_bias"):
         new.load_state_dict({k: v.detach() for k, v in named.items() if k != "head_bias"})
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_activation_checkpointing_draws_one_mask(reentrant):
+    """A forward that is run again in the backward pass: with its place in the stream the gradients are those of one run, bit
+    by bit, whatever ran in between; without it, it is refused."""
+    from torch.utils.checkpoint import checkpoint
+    m, plain = (small_readout(F32, dropout=0.5).train() for _ in range(2))
+    x, y = rnd(97, 6, 2, 20).requires_grad_(True), rnd(98, 7, 2, 20).requires_grad_(True)
+    a = checkpoint(m, x, None, m.draw(6, 2), use_reentrant=reentrant)
+    b = checkpoint(m, y, None, m.draw(7, 2), use_reentrant=reentrant)
+    (a.square().sum() + b.square().sum()).backward()
+    got = [x.grad, y.grad, *(p.grad for p in m.parameters())]
+    x.grad = y.grad = None
+    pa, pb = plain(x), plain(y)
+    assert torch.equal(a, pa) and torch.equal(b, pb) and m.drawn == plain.drawn == 13 * 2 * 16
+    (pa.square().sum() + pb.square().sum()).backward()
+    for g, w in zip(got, [x.grad, y.grad, *(p.grad for p in plain.parameters())]):
+        # a parameter's two gradients are added in either order, and are the same
+        assert torch.equal(g, w)
+    out = checkpoint(m, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="draw"):
+        out.sum().backward()
+    m.eval()
+    checkpoint(m, x, use_reentrant=reentrant).sum().backward()     # no masks, no place

@@ -128,19 +128,33 @@ class SequenceReadout(nn.Module):
             raise ValueError(f"x must be a tensor [{'T, ' * (dims - 2)}B, {self.n_neurons}]")
         return x.to(self.dtype)
 
-    def forward(self, x: torch.Tensor, lengths=None) -> torch.Tensor:
+    def draw(self, ticks: int, batch_size: int) -> int:
+        """Takes the words of one forward off the masks' stream and returns the first: ``drawn`` for a forward that is run
+        more than once, as under activation checkpointing (``checkpoint(readout, z, None, readout.draw(T, B))``)."""
+        first = self.drawn
+        self.drawn += ticks * batch_size * self.width
+        return first
+
+    def forward(self, x: torch.Tensor, lengths=None, drawn=None) -> torch.Tensor:
         """x [T, B, n_neurons] (a rollout's spikes or voltages, any floating type) to [T, B, n_outputs] of ``dtype``.
         ``lengths`` (int32 [B] on the device): the ticks of each batch entry; what is behind them is left out of the mixing
-        and its outputs mean nothing (x must be finite there, and a loss leaves them out)."""
+        and its outputs mean nothing (x must be finite there, and a loss leaves them out).  ``drawn``: the first word of the
+        masks in their stream, from ``draw``; None: the next one, which a forward inside a backward pass (a checkpoint's
+        second) cannot know and refuses."""
         x, w = self._input(x, 3), self._weights()
+        masks = self.training and self.dropout > 0.0
+        if masks and drawn is None:
+            if torch._C._current_graph_task_id() != -1:
+                raise RuntimeError("a readout that is run again in a backward pass needs the masks of its first run: give it "
+                                   "drawn=readout.draw(ticks, batch_size)")
+            drawn = self.draw(x.shape[0], x.shape[1])
         h, c, gate = self._into(x, w)
         u, _ = short_conv(c, w["conv"], w["conv_bias"], activation="silu", lengths=lengths)
         delta, B, C = self._maps(u, w)
         y, _ = state_space_scan(u, delta, w["A"], B, C, w["skip"], gate, w["step_bias"], lengths=lengths)
         y = linear(y, w["mix_out"], w["mix_out_bias"])
-        if self.training and self.dropout:
-            h = dropout(y, self.dropout, self.seed, self.drawn, residual=h)
-            self.drawn += y.numel()
+        if masks:
+            h = dropout(y, self.dropout, self.seed, drawn, residual=h)
         else:
             h = h + y
         return self._out(h, w)
