@@ -301,7 +301,9 @@ int glif_rate_dist_loss(const int32_t *count, int32_t count_rows, int32_t n_neur
  *     Outputs are contiguous.  lengths [B] int32 (NULL: all T ticks; clamped to [0, T]): the ticks of a batch entry from
  *     its length on are not read, give zeros, leave its state alone and take no part in any gradient.
  *   - Sums run in a fixed order: the same call gives the same bits.
- *   - Gradient outputs may be NULL where they are not wanted. */
+ *   - Gradient outputs may be NULL where they are not wanted.
+ *   - Sizes beyond these are refused (GLIF_EINVAL): layer norm 2^31 - 1 rows and columns; linear M and N of 2^21, K of 2^24 - 1;
+ *     sequences of 2^20 ticks, batches of 65535; the scan's 2^24 channels, 2^24 - 1 groups and 64 states. */
 typedef enum { GLIF_F32 = 0, GLIF_BF16 = 1, GLIF_F16 = 2 } glif_dtype;
 typedef enum { GLIF_ACT_NONE = 0, GLIF_ACT_RELU = 1, GLIF_ACT_GELU = 2, GLIF_ACT_SILU = 3 } glif_activation;
 

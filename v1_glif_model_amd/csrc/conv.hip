@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kBlock) k_conv_fwd(ConvArgs a) {
 }
 
 // pre is made again from x rather than kept by the forward: x is read anyway.  The same size: 54 us, 3.7 TB/s (eight channels a
-// thread, whose sums leave half as many waves a SIMD, 104).
+// thread, whose sums leave half as many waves a SIMD, 104).  Ticks behind a length are not read but computed as zeros: trials of
+// half that length take as long.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kBlock) k_conv_bwd(ConvArgs a) {
     typedef Vec<T, V> vec;

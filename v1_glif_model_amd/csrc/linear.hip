@@ -3,9 +3,10 @@
 //   dp = dy act'(pre),  dx = dp W,  dW = dp^T x,  db = sum of dp's rows
 // All three products run on the matrix cores with float32 accumulators (16-bit types 16x16x32, float32 16x16x4).
 //
-// Large products are bound by the matrix cores and what feeds them from LDS (8192^3 bfloat16 837 us, 1314 TFLOP/s of 2500);
-// short ones and ones of few tiles by the fill and drain of their blocks and by the way of their operands from memory (2500 x
-// 66000 x 512 bfloat16 forward 228 us, dx 263, dW 177); single ticks by the stream of the weights.
+// Large products are bound by the matrix cores and what feeds them from LDS (8192^3 bfloat16 802 to 837 us, 1314 to 1370 TFLOP/s
+// of 2500); short ones and ones of few tiles by the fill and drain of their blocks and by the way of their operands from memory
+// (2500 x 66000 x 512 bfloat16, each in a loop of its own: forward 222 us, dx 259, dW 178; after each other in a training step
+// 227, 303 and 202); single ticks by the stream of the weights.
 #include "seq.h"
 
 namespace glif {
@@ -744,7 +745,9 @@ struct Plan {
 // takes, in us, 16-bit 256 x 256 1.7, 128 x 128 1.0, 64 x 64 0.5, and float32, whose products run at 1/16, 128 x 128 3.0, 64
 // x 64 1.1; a step of all of the 1, 2 or 5 blocks that a compute unit holds 1.9, 1.35, 1.2, and 4.3, 2.9 (measured over
 // sweeps of tiles and splits at 15 shapes).  Around the steps go 10, 5 and 3; a split costs its sums' way to memory and back
-// and the launch that adds them.  A float32 sum runs over at most 4096 k's, so that long ones do not lose their last digits.
+// and the launch that adds them.  Tiles of float32 operands sum over at most 4096 k's up to 64 parts (K of 262144), so that long
+// sums do not lose their last digits; few rows are in a wave's parts of k anyway (all-positive float32 terms, K of 66000 with 16500
+// to a wave: 3e-6 of the sum), and 16-bit results keep fewer digits than either.
 Piece piece_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr, double &best) {
     Piece p{};
     best = 0.0;
@@ -856,7 +859,7 @@ void launch_piece(GemmArgs a, const Piece &p, float *part, hipStream_t s) {
         launch_tile<T, 64, 2, 2, PCOL, QCOL>(a, s);
     }
     if (a.splits != 1) {
-        // where the results alone do not fill the chip, lanes over the splits: 5 x 66000 x 512 in 64 parts 14 us -> 4
+        // where the results alone do not fill the chip, lanes over the splits: 5 x 66000 x 512 in 61 parts 14 us -> 4
         const int64_t n4 = a.M * (a.part_ld / 4);
         if (n4 < 32768 && a.splits >= 16)
             hipLaunchKernelGGL((k_gemm_join<T, 16>), dim3(static_cast<unsigned>(ceil_div(n4, kBlock / 16))), dim3(kBlock), 0, s, a);

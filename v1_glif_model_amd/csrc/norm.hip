@@ -398,7 +398,9 @@ __global__ void __launch_bounds__(kWide) k_norm_fwd_wide(NormArgs a) {
 }
 
 // Rows of more than kLongFrom pieces in the registers of one block, which has a compute unit to itself (2500 x 66000 bfloat16
-// 163 us, 4.0 TB/s; gone through twice 197.  2500 x 40000 96 and 87: there several rows a unit come from the L2 again).
+// 172 to 176 us, 3.8 TB/s; gone through twice 201.  2500 x 50000 116 and 112, 2500 x 40000 95 and 87: there several rows a unit
+// come from the L2 again).  Longer ones, as 230,000 columns or 66,000 in float32, are gone through twice (500 x 230000 107 us, 1000
+// x 66000 float32 141: 4.3 and 3.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kLong, 4) k_norm_fwd_long(NormArgs a) {
     typedef Row<T, kLong, kLongR> row;
@@ -571,9 +573,10 @@ int fused_blocks(int64_t rows, int64_t D, int64_t size) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + 4 * per - 1) / (4 * per), 512)));
 }
 
-// A wide backward's rounds of rows: 128 MB of x and dy (2500 x 66000 bfloat16 378 us; 96 and 160 MB 398 and 394), and parts of
-// a round: two blocks a compute unit (272, 408, 544 and 816 blocks 455, 404, 398 and 398 us in rounds of 96 MB), whose sums go
-// on from round to round.
+// A wide backward's rounds of rows: 128 MB of x and dy (96, 128 and 160 MB: 2500 x 66000 bfloat16 386, 380 and 383 us, 1000 x
+// 66000 float32 269, 264 and 307, 2500 x 40000 bfloat16 225, 223 and 233, 500 x 230000, of 5, 4 and 3 rounds, 344, 307 and 272),
+// and parts of a round: two blocks a compute unit (2500 x 66000: 272, 408, 544 and 816 blocks 455, 404, 398 and 398 us in rounds of
+// 96 MB), whose sums go on from round to round.
 int64_t round_rows(int64_t rows, int64_t D, int64_t size) {
     return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t(64) << 20) / (D * size)));
 }

@@ -17,7 +17,8 @@
 //
 // Bound by instruction issue: per state and tick an exponential (a quarter of the rate of the rest) and four products and
 // sums forward, some 24 operations backward; what a channel needs per tick adds about a third (vector units busy 85 to 98
-// percent of the time).  Memory would allow 27 us for 16.4M channels' ticks forward and 55 backward.
+// percent of the time).  Memory would allow 27 us for 16.4M channels' ticks forward and 55 backward.  Ticks behind a length are
+// issued like live ones: over trials of half the ticks, half of that issue is for none.
 #include <cfloat>
 #include <cmath>
 
