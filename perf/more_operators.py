@@ -278,12 +278,12 @@ def _encode(x, held, top, u):
     n = x.numel()
     flat = torch.nn.functional.pad(x.reshape(-1), (0, -n % BLOCK)).reshape(-1, BLOCK)
     most = flat.abs().amax(1)
-    fine = torch.isfinite(most) & (most > 0)
-    part = flat.abs() / most[:, None]
+    fine = torch.isfinite(most) & (most >= torch.finfo(torch.float32).tiny)
+    part = flat.abs() * (1.0 / most)[:, None]
     root = torch.sqrt(part) if top == 127 else torch.sqrt(torch.sqrt(part))
     below = torch.floor(root * top).clamp(max=top - 1)
     a, b = _level(below, top), _level(below + 1.0, top)
-    up = u.reshape(-1, BLOCK) < (part - a) / (b - a) * 65536.0
+    up = u.reshape(-1, BLOCK).float() * (b - a) < (part - a) * 65536.0
     new = below + up
     if top == 255:
         new = torch.where(flat > 0, new.clamp(min=1.0), new)
