@@ -395,6 +395,26 @@ int glif_scan_step(const glif_scan *s, void *y, float *state, void *stream);
 int glif_exp_adam(float *w, float *m, float *v, float *vhat, const float *g, const uint8_t *positive,
                   int64_t n, float alpha, float beta_1, float beta_2, float epsilon, void *stream);
 
+/* AdamW over many variables in one launch (a readout's; no counterpart in the reference, whose optimizer is the one above):
+ *   m = beta_1 m + (1 - beta_1) g;  v = beta_2 v + (1 - beta_2) g^2;  t = iterations + 1
+ *   p = (1 - learning_rate weight_decay) p - learning_rate / (1 - beta_1^t) m / (sqrt(v / (1 - beta_2^t)) + epsilon)
+ * host arrays of n_vars: vars and grads (device pointers; a NULL gradient leaves its variable and moments alone), their types
+ * (glif_dtype; a gradient is float32 or of its variable's type) and sizes.  Variable i's moments begin at element
+ * home(i) = sum over j < i of sizes[j] rounded up to 256, of
+ *   state_bits 32: first, second float32 (first_scale, second_scale not read);
+ *   state_bits 8: first int8, second uint8, with a float32 scale for every 256 elements: m = s (c / 127) |c / 127|,
+ *     v = s (c / 255)^4, rounded to the code below or above by the halves of word (t - 1) home(n_vars) + home(i) + k of the
+ *     Philox stream seed, so that the mean is kept; v > 0 does not become 0.
+ * device: first and second on 16 bytes; iterations [2] int64, the steps done and 0, counted on by the call (by none without
+ * a gradient), so that a captured call goes on.
+ * glif_adamw_values: the values of n (a multiple of 256) codes. */
+int glif_adamw(int32_t n_vars, void *const *vars, const int32_t *var_dtypes, const void *const *grads,
+               const int32_t *grad_dtypes, const int64_t *sizes, int32_t state_bits, void *first, void *second,
+               float *first_scale, float *second_scale, int64_t *iterations, double learning_rate, double beta_1, double beta_2,
+               double epsilon, double weight_decay, uint64_t seed, void *stream);
+int glif_adamw_values(const void *first, const float *first_scale, const void *second, const float *second_scale, int64_t n,
+                      float *first_out, float *second_out, void *stream);
+
 /* ------------------------------------------------------------ input sampling -
  * On-device replacements for the host input streams: LGN spikes (stim_dataset.py:182-197,
  * Bernoulli with p = 1 - exp(-rate * dt / 1000)) and background counts (models.py:865-887,

@@ -1,0 +1,34 @@
+"""What the C entry points of the attention, the gated projection and AdamW refuse before they touch a GPU."""
+import ctypes as C
+
+import pytest
+
+from v1_glif_model_amd import _lib
+
+
+def refused(rc, word=""):
+    assert rc in (_lib.GLIF_EINVAL, _lib.GLIF_ENOMEM), rc
+    assert word in _lib.lib().glif_last_error().decode()
+
+
+def adamw(n=1, var=1 << 20, grad=1 << 21, var_dt=0, grad_dt=0, size=10, bits=32, first=1 << 22, second=1 << 23, scales=1 << 24,
+          count=1 << 25, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, decay=0.0):
+    k = max(n, 1)
+    return _lib.lib().glif_adamw(n, (C.c_void_p * k)(*[var] * k), (C.c_int32 * k)(*[var_dt] * k), (C.c_void_p * k)(*[grad] * k),
+                                 (C.c_int32 * k)(*[grad_dt] * k), (C.c_int64 * k)(*[size] * k), bits, first, second, scales, scales,
+                                 count, lr, b1, b2, eps, decay, 0, None)
+
+
+@pytest.mark.parametrize("kw", [dict(n=-1), dict(bits=16), dict(b1=1.0), dict(b2=-0.5), dict(b1=float("nan")), dict(eps=-1e-9),
+                                dict(decay=float("nan")), dict(size=-1), dict(size=2 ** 36 + 1), dict(var_dt=3), dict(grad_dt=1),
+                                dict(var_dt=1, grad_dt=2), dict(var=None), dict(first=None), dict(count=None),
+                                dict(bits=8, scales=None), dict(first=(1 << 22) + 4)])
+def test_adamw_refuses(kw):
+    refused(adamw(**kw), "NULL" if None in kw.values() else "adamw")
+
+
+def test_adamw_without_work():
+    """No variables, no gradient, no elements: nothing to do, and no GPU needed."""
+    assert adamw(n=0) == 0 and adamw(grad=None) == 0 and adamw(size=0) == 0
+    refused(_lib.lib().glif_adamw_values(None, None, None, None, 255, None, None, None), "256")
+    refused(_lib.lib().glif_adamw_values(None, None, None, None, 256, None, None, None), "NULL")

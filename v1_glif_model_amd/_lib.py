@@ -92,6 +92,9 @@ SIGNATURES = {
                                       C.c_uint64, C.c_uint64, vp, vp, vp, sz, vp]),
     "glif_exp_adam": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, C.c_float, C.c_float, C.c_float, C.c_float,
                                 vp]),
+    "glif_adamw": (C.c_int, [i32, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, C.c_double,
+                             C.c_double, C.c_uint64, vp]),
+    "glif_adamw_values": (C.c_int, [vp, vp, vp, vp, i64, vp, vp, vp]),
     "glif_sample_bernoulli": (C.c_int, [vp, i64, C.c_uint64, C.c_uint64, vp, vp]),
     "glif_sample_poisson": (C.c_int, [C.c_float, C.c_float, i64, C.c_uint64, C.c_uint64, vp, vp]),
     "glif_layer_norm_fwd": (C.c_int, [vp, i64, vp, vp, i32, i32, i64, i64, C.c_float, vp, vp]),

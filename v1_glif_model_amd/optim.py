@@ -1,19 +1,25 @@
 """ExponentiatedAdam and SignedConstraint on the GPU (v1_model_utils/optimizers.py:154-390,
-models.py:419-427).
+models.py:419-427), and AdamW for a readout's variables.
 
 Same names and arguments as the reference.  ``apply_gradients`` runs the dense
 ``update_step`` and then the variable's sign constraint in one libglif kernel
 (``glif_exp_adam``) per variable; the moment slots live on the device beside the
 weights.  Weight vectors are fp32 device tensors updated in place.
+
+``AdamW`` steps all of its variables in one launch, with moments in 32 bits or in 8.
 """
 from __future__ import annotations
+
+import ctypes
+import math
 
 import numpy as np
 import torch
 
 from ._lib import check, lib, ptr, require_gpu, stream_ptr
+from .sequence import DTYPES, _on, _p
 
-__all__ = ["ExponentiatedAdam", "SignedConstraint"]
+__all__ = ["ExponentiatedAdam", "SignedConstraint", "AdamW"]
 
 
 class SignedConstraint:
@@ -93,3 +99,159 @@ class ExponentiatedAdam:
             # copies the synapse tables keep (keyed on the tensor's version) are refreshed
             torch.autograd.graph.increment_version(var)
         self.iterations += 1
+
+
+class AdamW:
+    """Adam with decoupled weight decay over a fixed list of variables, one launch a step (of up to 64 of them):
+
+    ``m = beta_1 m + (1 - beta_1) g``, ``v = beta_2 v + (1 - beta_2) g^2``,
+    ``p = (1 - lr weight_decay) p - lr / (1 - beta_1^t) m / (sqrt(v / (1 - beta_2^t)) + epsilon)``
+
+    ``variables``: contiguous float32, bfloat16 or float16 tensors of one GPU, updated in place (16-bit ones rounded to nearest).
+    ``state_bits``: 32, or 8 for moments of a byte each with a float32 scale for every 256: m as ``s (c / 127) |c / 127|`` and v
+    as ``s (c / 255)^4``, rounded up or down by words of the Philox stream ``seed`` so that their mean is kept.  A gradient that is
+    not finite makes its variable's moments so, in 8 bits those of all 256.
+
+    The count of steps lies on the device: a captured step that is replayed goes on counting.  It keeps the ``learning_rate``
+    that it was captured with; eager steps read the attribute each time."""
+
+    BLOCK = 256
+
+    def __init__(self, variables, learning_rate=0.001, beta_1=0.9, beta_2=0.999, epsilon=1e-8, weight_decay=0.01,
+                 state_bits=32, seed=0, name="AdamW"):
+        require_gpu()
+        self.variables = list(variables)
+        if not self.variables:
+            raise ValueError("there must be at least one variable")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        for what, b in (("beta_1", beta_1), ("beta_2", beta_2)):
+            if not 0.0 <= b < 1.0:
+                raise ValueError(f"{what} must be in [0, 1), got {b}")
+        for what, b in (("epsilon", epsilon), ("weight_decay", weight_decay)):
+            if not 0.0 <= b < math.inf:
+                raise ValueError(f"{what} must be >= 0 and finite, got {b}")
+        dev = getattr(self.variables[0], "device", None)
+        for p in self.variables:
+            self._check(p)
+            if p.device != dev:
+                raise ValueError(f"all variables must be on one device, got {dev} and {p.device}")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.variables if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("two variables share memory")
+        self.learning_rate = learning_rate
+        self.beta_1, self.beta_2, self.epsilon, self.weight_decay = float(beta_1), float(beta_2), float(epsilon), float(weight_decay)
+        self.state_bits, self.seed, self.name, self.device = int(state_bits), int(seed) & (2 ** 64 - 1), name, dev
+        self._types = [p.dtype for p in self.variables]
+        self._shapes = [p.shape for p in self.variables]
+        self._homes = [0]
+        for p in self.variables:
+            self._homes.append(self._homes[-1] + -(-p.numel() // self.BLOCK) * self.BLOCK)
+        n = self._homes[-1]
+
+        def zeros(n, dtype):
+            return torch.zeros(n, dtype=dtype, device=dev)
+
+        if self.state_bits == 32:
+            self._first, self._second = zeros(n, torch.float32), zeros(n, torch.float32)
+            self._scales = None
+        else:
+            self._first, self._second = zeros(n, torch.int8), zeros(n, torch.uint8)
+            self._scales = zeros(n // self.BLOCK, torch.float32), zeros(n // self.BLOCK, torch.float32)
+        self._count = zeros(2, torch.int64)      # steps done; the kernel's own
+        count = len(self.variables)
+        self._sizes = (ctypes.c_int64 * count)(*(p.numel() for p in self.variables))
+        self._codes = (ctypes.c_int32 * count)(*(DTYPES[p.dtype] for p in self.variables))
+        self._pointers = ctypes.c_void_p * count
+        self._ints = ctypes.c_int32 * count
+
+    @staticmethod
+    def _check(p):
+        if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in DTYPES or not p.is_contiguous():
+            raise ValueError("variables must be contiguous float32, bfloat16 or float16 tensors on the GPU")
+
+    @property
+    def iterations(self) -> int:
+        """The steps done (waits for the device)."""
+        return int(self._count[0])
+
+    def apply_gradients(self, gradients=None):
+        """One step.  ``gradients``: one for each variable, float32 or of its type, None for a variable that stays as it is with
+        its moments; by default the variables' ``grad``.  Without any gradient nothing is done or counted."""
+        if gradients is None:
+            gradients = [p.grad for p in self.variables]
+        gradients = list(gradients)
+        if len(gradients) != len(self.variables):
+            raise ValueError(f"there are {len(self.variables)} variables and {len(gradients)} gradients")
+        held, changed = [], []
+        for g, p, dtype, shape in zip(gradients, self.variables, self._types, self._shapes):
+            if p.dtype is not dtype or p.shape != shape or p.device != self.device or not p.is_contiguous():
+                raise ValueError("a variable is not laid out as it was when the optimizer was made")
+            if g is not None:
+                if not isinstance(g, torch.Tensor) or g.device != self.device or g.shape != shape or (
+                        g.dtype is not dtype and g.dtype is not torch.float32):
+                    raise ValueError(f"a gradient must be a tensor of its variable's shape {tuple(shape)} and device, float32 or of its type")
+                g = g if g.is_contiguous() else g.contiguous()
+                changed.append(p)
+            held.append(g)
+        if not changed:
+            return
+        first_scale, second_scale = self._scales or (None, None)
+        with _on(self.device):
+            check(lib().glif_adamw(len(held), self._pointers(*(p.data_ptr() for p in self.variables)), self._codes,
+                                   self._pointers(*(_p(g) for g in held)),
+                                   self._ints(*(0 if g is None else DTYPES[g.dtype] for g in held)), self._sizes, self.state_bits,
+                                   _p(self._first), _p(self._second), _p(first_scale), _p(second_scale), _p(self._count),
+                                   float(self.learning_rate), self.beta_1, self.beta_2, self.epsilon, self.weight_decay, self.seed,
+                                   stream_ptr(self.device)))
+        torch.autograd.graph.increment_version(changed)
+
+    def _views(self, flat, i):
+        return flat[self._homes[i]:self._homes[i] + self._sizes[i]].view(self._shapes[i])
+
+    def moments(self):
+        """The first and the second moments as float32 values, a list of each: the state itself where it is held in 32 bits,
+        what the codes stand for where in 8."""
+        first, second = self._first, self._second
+        if self.state_bits == 8:
+            values = torch.empty((2, first.numel()), dtype=torch.float32, device=self.device)
+            with _on(self.device):
+                check(lib().glif_adamw_values(_p(first), _p(self._scales[0]), _p(second), _p(self._scales[1]), first.numel(),
+                                              _p(values[0]), _p(values[1]), stream_ptr(self.device)))
+            first, second = values
+        count = range(len(self.variables))
+        return [self._views(first, i) for i in count], [self._views(second, i) for i in count]
+
+    def _scale_views(self, k, i):
+        return self._scales[k][self._homes[i] // self.BLOCK:self._homes[i + 1] // self.BLOCK]
+
+    def _state(self, k, i):
+        codes = self._views((self._first, self._second)[k], i)
+        return codes if self.state_bits == 32 else (codes, self._scale_views(k, i))
+
+    def state_dict(self):
+        """``iterations`` and, for each variable, its ``first`` and ``second`` moments (in 8 bits: the codes and their scales),
+        as copies.  The learning rate and the other numbers are the caller's."""
+        def copy(s):
+            return s.clone() if isinstance(s, torch.Tensor) else tuple(t.clone() for t in s)
+        count = range(len(self.variables))
+        return dict(iterations=self.iterations, first=[copy(self._state(0, i)) for i in count],
+                    second=[copy(self._state(1, i)) for i in count])
+
+    def load_state_dict(self, state):
+        """Takes what ``state_dict`` gave for variables of these shapes and the same ``state_bits``."""
+        pairs = []
+        for k, what in enumerate(("first", "second")):
+            if len(state[what]) != len(self.variables):
+                raise ValueError(f"{what} has {len(state[what])} moments for {len(self.variables)} variables")
+            for i, new in enumerate(state[what]):
+                old, new = ([s] if isinstance(s, torch.Tensor) else list(s) for s in (self._state(k, i), new))
+                if len(old) != len(new) or any(a.shape != b.shape or a.dtype is not b.dtype for a, b in zip(old, new)):
+                    raise ValueError(f"{what}[{i}] does not fit the variable and state_bits = {self.state_bits}")
+                pairs += zip(old, new)
+        count = int(state["iterations"])
+        if count < 0:
+            raise ValueError(f"iterations must be >= 0, got {count}")
+        for old, new in pairs:
+            old.copy_(new)
+        self._count.copy_(torch.tensor([count, 0]))
