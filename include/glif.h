@@ -294,7 +294,7 @@ int glif_rate_dist_loss(const int32_t *count, int32_t count_rows, int32_t n_neur
 /* ------------------------------------------------------ sequence operators --
  * What reads a rollout out and is trained with it (the reference's Dense and softmax readouts, models.py:1138-1209,
  * 1213-1392, are Keras layers): layer norm, dropout, a linear map with its epilogue, a short causal convolution and a
- * selective state space scan, each with its backward, and single-tick forms of the last two.
+ * selective state space scan, each with its backward, and single-tick forms of the last two; linear attention likewise.
  *   - Activations are float32, bfloat16 or float16 (glif_dtype); parameters of the small operators (norm weights, taps,
  *     biases) are float32 or of the activations' type (param_dtype).  Sums, statistics and states are float32.
  *   - Sequences are time-major [T][B][D], channels contiguous; strides of ticks and batch entries are in elements.
@@ -381,6 +381,33 @@ size_t glif_scan_bwd_workspace(const glif_scan *s);
 int glif_scan_bwd(const glif_scan *s, const glif_scan_grad *g, const void *keep, void *ws, size_t ws_bytes, void *stream);
 /* One tick: u, delta, z [B][D], B and C [B][G][N] (s->n_ticks 1, tick strides unused); state [B][D][N] in place. */
 int glif_scan_step(const glif_scan *s, void *y, float *state, void *stream);
+
+/* Linear attention with a decay for each head; k and v are shared by the n_heads / n_groups heads of a group:
+ *   S[t] = exp(log_decay[h]) S[t - 1] + k[t] v[t]^T,   y[t] = scale q[t] S[t]
+ * S [d_key][d_value] float32, both at most 128.  exp(-infinity) is 0: nothing is remembered.  log_decay has no gradient. */
+typedef struct {
+    const void *q, *k, *v;           /* [T][B][n_heads][d_key], [T][B][n_groups][d_key], .. [d_value], channels contiguous */
+    const float *log_decay;          /* [n_heads] */
+    const float *state;              /* [B][n_heads][d_key][d_value] before the first tick, NULL: zeros */
+    const int32_t *lengths;
+    int64_t q_st, q_sb, q_sh, k_st, k_sb, k_sh, v_st, v_sb, v_sh;
+    float scale;
+    int32_t dtype, n_ticks, n_batch, n_heads, n_groups, d_key, d_value;
+} glif_attention;
+/* y [T][B][n_heads][d_value]; last (may be NULL): the states after each length. */
+size_t glif_attention_fwd_workspace(const glif_attention *s);
+int glif_attention_fwd(const glif_attention *s, void *y, float *last, void *ws, size_t ws_bytes, void *stream);
+typedef struct {
+    const void *dy;                  /* [T][B][n_heads][d_value], channels contiguous */
+    int64_t dy_st, dy_sb, dy_sh;
+    const float *dlast;              /* like state, or NULL */
+    void *dq, *dk, *dv;              /* contiguous, of dtype */
+    float *dstate;
+} glif_attention_grad;
+size_t glif_attention_bwd_workspace(const glif_attention *s);
+int glif_attention_bwd(const glif_attention *s, const glif_attention_grad *g, void *ws, size_t ws_bytes, void *stream);
+/* One tick: q [B][n_heads][d_key] and so on (tick strides, lengths and s->state unused); state in place. */
+int glif_attention_step(const glif_attention *s, void *y, float *state, void *stream);
 
 /* ------------------------------------------------------------- optimizer ------
  * Replaces ExponentiatedAdam.update_step, dense branch (v1_model_utils/optimizers.py:

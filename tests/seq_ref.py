@@ -107,3 +107,18 @@ def near(out, ref, terms, what, more=0.0):
     over = ((o - r).abs() - bound)
     bad = ~(over <= 0)
     assert not bool(bad.any()), (what, int(bad.sum()), float((o - r).abs().max()), float(over.max()))
+
+
+def linear_attention(q, k, v, decay, scale, state=None, lengths=None):
+    """y and the last state, by ticks; of non-negative inputs autograd gives the sums of the gradients' absolute terms."""
+    T, B, H, K = q.shape
+    k, v = (t.repeat_interleave(H // t.shape[2], 2) for t in (k, v))
+    h = torch.zeros(B, H, K, v.shape[-1], dtype=q.dtype) if state is None else state
+    lam = torch.exp(decay)[:, None, None]
+    end = torch.full((B,), T) if lengths is None else lengths.clamp(0, T)
+    ys = []
+    for t in range(T):
+        on = (t < end)[:, None, None, None]
+        h = torch.where(on, lam * h + k[t][..., None] * v[t][..., None, :], h)
+        ys.append(torch.where(on[..., 0], scale * (q[t][..., None] * h).sum(-2), torch.zeros((), dtype=q.dtype)))
+    return torch.stack(ys) if T else torch.zeros(0, B, H, v.shape[-1], dtype=q.dtype), h

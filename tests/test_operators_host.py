@@ -32,3 +32,35 @@ def test_adamw_without_work():
     assert adamw(n=0) == 0 and adamw(grad=None) == 0 and adamw(size=0) == 0
     refused(_lib.lib().glif_adamw_values(None, None, None, None, 255, None, None, None), "256")
     refused(_lib.lib().glif_adamw_values(None, None, None, None, 256, None, None, None), "NULL")
+
+
+def attention(**kw):
+    s = _lib.Attention()
+    for n in ("q", "k", "v", "log_decay"):
+        setattr(s, n, 1 << 20)
+    s.n_ticks, s.n_batch, s.n_heads, s.n_groups, s.d_key, s.d_value = 4, 2, 4, 2, 8, 8
+    for n, x in kw.items():
+        setattr(s, n, x)
+    return C.byref(s)
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=3), dict(n_ticks=-1), dict(n_ticks=2 ** 20 + 1), dict(n_batch=65536), dict(n_heads=4097),
+                                dict(n_groups=3), dict(n_groups=0), dict(d_key=0), dict(d_key=129), dict(d_value=129), dict(q=None),
+                                dict(log_decay=None), dict(n_batch=65535, n_heads=4096, n_groups=1)])
+def test_attention_refuses(kw):
+    L, g = _lib.lib(), _lib.AttentionGrad(dy=1 << 21)
+    refused(L.glif_attention_fwd(attention(**kw), 1 << 22, None, None, 0, None))
+    refused(L.glif_attention_bwd(attention(**kw), C.byref(g), None, 0, None))
+    refused(L.glif_attention_step(attention(**kw), 1 << 22, 1 << 23, None))
+
+
+def test_attention_refuses_missing_outputs_and_workspaces():
+    L, g = _lib.lib(), _lib.AttentionGrad(dq=1 << 21)
+    refused(L.glif_attention_fwd(attention(), None, None, None, 0, None), "NULL")
+    refused(L.glif_attention_bwd(attention(), C.byref(g), None, 0, None), "NULL")
+    refused(L.glif_attention_bwd(attention(), None, None, 0, None), "NULL")
+    refused(L.glif_attention_step(attention(), 1 << 22, None, None), "NULL")
+    long = attention(n_ticks=4096)
+    assert L.glif_attention_fwd_workspace(long) > 0
+    refused(L.glif_attention_fwd(long, 1 << 22, None, None, 0, None), "workspace")
+    assert L.glif_attention_fwd(attention(n_batch=0), None, None, None, 0, None) == 0

@@ -53,6 +53,20 @@ class ScanGrad(C.Structure):
                 + [(n, vp) for n in ("dlast", "du", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias", "dstate")])
 
 
+class Attention(C.Structure):
+    """glif_attention."""
+    _fields_ = ([(n, vp) for n in ("q", "k", "v", "log_decay", "state", "lengths")]
+                + [(n, C.c_int64) for n in ("q_st", "q_sb", "q_sh", "k_st", "k_sb", "k_sh", "v_st", "v_sb", "v_sh")]
+                + [("scale", C.c_float)]
+                + [(n, C.c_int32) for n in ("dtype", "n_ticks", "n_batch", "n_heads", "n_groups", "d_key", "d_value")])
+
+
+class AttentionGrad(C.Structure):
+    """glif_attention_grad."""
+    _fields_ = ([("dy", vp)] + [(n, C.c_int64) for n in ("dy_st", "dy_sb", "dy_sh")]
+                + [(n, vp) for n in ("dlast", "dq", "dk", "dv", "dstate")])
+
+
 SIGNATURES = {
     "glif_last_error": (C.c_char_p, []),
     "glif_version": (C.c_int, []),
@@ -92,6 +106,11 @@ SIGNATURES = {
                                       C.c_uint64, C.c_uint64, vp, vp, vp, sz, vp]),
     "glif_exp_adam": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, C.c_float, C.c_float, C.c_float, C.c_float,
                                 vp]),
+    "glif_attention_fwd_workspace": (sz, [C.POINTER(Attention)]),
+    "glif_attention_fwd": (C.c_int, [C.POINTER(Attention), vp, vp, vp, sz, vp]),
+    "glif_attention_bwd_workspace": (sz, [C.POINTER(Attention)]),
+    "glif_attention_bwd": (C.c_int, [C.POINTER(Attention), C.POINTER(AttentionGrad), vp, sz, vp]),
+    "glif_attention_step": (C.c_int, [C.POINTER(Attention), vp, vp, vp]),
     "glif_adamw": (C.c_int, [i32, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, C.c_double,
                              C.c_double, C.c_uint64, vp]),
     "glif_adamw_values": (C.c_int, [vp, vp, vp, vp, i64, vp, vp, vp]),

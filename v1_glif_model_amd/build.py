@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libglif.so")
 OBJ_DIR = os.path.join(HERE, "_build")
 SOURCES = ["table.hip", "compact.hip", "syn.hip", "cell.hip", "optim.hip", "sample.hip", "loss.hip", "prof.hip",
-           "norm.hip", "dropout.hip", "linear.hip", "conv.hip", "scan.hip"]
+           "norm.hip", "dropout.hip", "linear.hip", "conv.hip", "scan.hip", "attention.hip"]
 
 HIPCC_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",

@@ -1,0 +1,733 @@
+// Linear attention with a decay for each head, its backward, and its form for single ticks:
+//   S[t] = lam S[t-1] + k[t] v[t]^T,   y[t] = scale q[t] S[t],   lam = exp(log_decay[h]),   S [K][V] float32
+//
+// Everything but the step is one function of three sequences, F(a, b, c; X): over the ticks of a chunk, counted from 0,
+//   out_i = sum over j <= i of lam^(i-j) (a_i . b_j) c_j  +  lam^(i+lead) a_i X
+//   X    <- lam^n X + sum over j of lam^(n-lead-j) b_j c_j^T                        (n ticks in the chunk)
+//   y  = scale F(q, k, v; S0)                    lead 1
+//   dq = scale F(dy, v, k; S0^T)                 lead 1
+//   dk = F(v, dy, scale q; dS^T)                 lead 0, time backwards: the gradient of the last state comes undecayed to the
+//   dv = F(k, scale q, dy; dS)                   last tick, and what is left behind the first is dS0
+// No power is of a negative exponent, so no decay, 0 among them, can overflow.
+#include <type_traits>
+
+#include "mma.h"
+
+namespace glif {
+namespace {
+
+struct AttSeq {
+    const void *p;
+    int64_t st, sb, sh;   // strides of ticks, batch entries and heads
+    int32_t share, d;     // heads of the attention that share one of it; channels
+};
+
+struct AttPass {
+    AttSeq a, b, c;
+    void *out;                     // [T][B][H][c.d], or NULL
+    int32_t wide;                  // out is float32, to be added up over shared heads
+    int32_t back, lead;
+    float out_scale, in_scale;
+    const float *x;                // the state before the first tick, or NULL: strides of (segment, entry and head, b's and c's channels)
+    int64_t x_seg, x_bh, x_b, x_c;
+    float *x_out;                  // the state after the last, likewise, or NULL
+};
+
+struct AttArgs {
+    AttPass pass[3];
+    int32_t passes, tiles;         // tiles of c's channels
+    const float *log_decay;
+    const int32_t *lengths;
+    int32_t T, B, H, segments, seg_ticks;
+};
+
+// lam^n for n >= 0: 1 for n = 0 whatever the decay is
+__device__ __forceinline__ float power(float rate, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(rate * static_cast<float>(n)); }
+
+__device__ __forceinline__ int live_ticks(const int32_t *lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }
+
+#ifdef __HIP_DEVICE_COMPILE__   // the host's pass does not know the builtins
+// 16-bit products of bfloat16, and float32 ones for float32 and for float16: states and scores of float16 sequences do not
+// stay within its range.
+template <typename T>
+struct Form {
+    using C = float;
+    static constexpr int kTicks = 32, kStep = 16, kPer = 4;   // ticks of a chunk, terms of a matrix product, those of a lane
+};
+template <>
+struct Form<bf16> {
+    using C = bf16;
+    static constexpr int kTicks = 64, kStep = 32, kPer = 8;
+};
+
+// kTicks x W of a sequence from memory to rows of LDS, in two steps.
+template <typename T, int W>
+struct Tile {
+    using F = Form<T>;
+    using C = typename F::C;
+    static constexpr int kV = kVecBytes16<T>, kRow = W * static_cast<int>(sizeof(C)) + 16, kBytes = F::kTicks * kRow;
+    static constexpr int kPieces = F::kTicks * W / kV, kN = (kPieces + kBlock - 1) / kBlock;
+    typedef Vec<T, kV> vec;
+    vec r[kN];
+
+    // ticks `first`, first + step, ...: n of them; channels from c0 on, of which there are d
+    __device__ __forceinline__ void load(const T *p, int64_t st, int64_t first, int step, int n, int c0, int d) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int u = threadIdx.x + i * kBlock, row = u / (W / kV), at = c0 + u % (W / kV) * kV;
+            vec v = {};
+            if (row < n && at < d) {
+                const T *q = p + (first + static_cast<int64_t>(row) * step) * st + at;
+                if (at + kV <= d) {
+                    v = *reinterpret_cast<const vec *>(q);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kV; ++e)
+                        if (at + e < d) v[e] = q[e];
+                }
+            }
+            r[i] = v;
+        }
+    }
+    __device__ __forceinline__ void store(char *lds) const {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int u = threadIdx.x + i * kBlock;
+            if (kPieces % kBlock && u >= kPieces) break;
+            C *to = reinterpret_cast<C *>(lds + u / (W / kV) * kRow) + u % (W / kV) * kV;
+            constexpr int kE = 16 / static_cast<int>(sizeof(C));
+            typedef C out __attribute__((ext_vector_type(16 / sizeof(C))));
+#pragma unroll
+            for (int s = 0; s < kV / kE; ++s) {
+                out o;
+#pragma unroll
+                for (int e = 0; e < kE; ++e) o[e] = static_cast<C>(r[i][s * kE + e]);
+                *reinterpret_cast<out *>(to + s * kE) = o;
+            }
+        }
+    }
+    __device__ __forceinline__ bool finite() const {
+        bool f = true;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+#pragma unroll
+            for (int e = 0; e < kV; ++e) f = f && fabsf(to_f32(static_cast<T>(r[i][e]))) < __builtin_inff();
+        return f;
+    }
+};
+
+// Operands: lane l holds row l % 16 and the kPer terms from kPer (l / 16) on.
+template <typename C, int ROW>
+__device__ __forceinline__ typename Mma<C>::frag rows_of(const char *lds, int row0, int k0, int lane) {
+    constexpr int kPer = 16 / static_cast<int>(sizeof(C));
+    return *reinterpret_cast<const typename Mma<C>::frag *>(lds + (row0 + lane % 16) * ROW + (k0 + lane / 16 * kPer) * static_cast<int>(sizeof(C)));
+}
+
+// The tile's columns as rows, its ticks k0, .. as terms.  Four columns from each of c0, c0 + GAP, c0 + 2 GAP and c0 + 3 GAP.
+template <typename C, int ROW, int GAP>
+__device__ __forceinline__ typename Mma<C>::frag columns_of(const char *lds, int c0, int k0, int lane) {
+    const int r16 = lane % 16, kq = lane / 16;
+    if constexpr (sizeof(C) == 2) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4 *l4;
+        const char *p = lds + (k0 + 8 * kq + (r16 >> 2)) * ROW + (c0 + (r16 & 3) * GAP) * 2;
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(p));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(p + 4 * ROW));
+        return __builtin_bit_cast(typename Mma<C>::frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+        static_assert(GAP == 4, "columns in order");
+        typename Mma<C>::frag v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const C *>(lds + (k0 + 4 * kq + e) * ROW + (c0 + r16) * 4);
+        return v;
+    }
+}
+#endif
+
+// A block takes one entry and head, 4 WC of c's channels and one segment of the ticks, chunk by chunk; each of its waves keeps
+// the state of its WC channels in registers, as a matrix product's result and the next one's operand (which of b's
+// channels a row of it is, is chosen so that a lane's values are kPer neighbours).  STATES: no outputs, only the state that
+// the segment adds to nothing.
+template <typename T, int D, int WC, bool STATES>
+__global__ void __launch_bounds__(kBlock, 2) k_attention(AttArgs args) {
+#ifdef __HIP_DEVICE_COMPILE__
+    using F = Form<T>;
+    using C = typename F::C;
+    using M = Mma<C>;
+    typedef typename M::frag frag;
+    constexpr int kTicks = F::kTicks, kStep = F::kStep, kPer = F::kPer, TI = kTicks / 16, KT = kTicks / kStep, KD = D / kStep;
+    constexpr int XT = D / 16, CT = WC / 16, GAP = kPer == 8 ? 8 : 4;
+    using TD = Tile<T, D>;
+    using TC = Tile<T, 4 * WC>;
+    constexpr int kRow = TD::kRow, kRowC = TC::kRow, kRowP = kTicks * static_cast<int>(sizeof(C)) + 16;
+    __shared__ __attribute__((aligned(16))) char lds_a[STATES ? 16 : TD::kBytes];
+    __shared__ __attribute__((aligned(16))) char lds_b[TD::kBytes];
+    __shared__ __attribute__((aligned(16))) char lds_c[TC::kBytes];
+    __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * kRowP];
+    __shared__ int odd[2];   // whether c is not finite somewhere in this chunk, and in the next
+
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
+    // The blocks that read the same sequences are on one XCD (block id mod 8), after each other.
+    const int kin = args.tiles * args.passes, slot = static_cast<int>(blockIdx.x >> 3);
+    const int64_t group = static_cast<int64_t>(slot / kin) * 8 + (blockIdx.x & 7);
+    if (group >= static_cast<int64_t>(args.B) * args.H * args.segments) return;
+    const AttPass &p = args.pass[slot % kin / args.tiles];
+    const int tile = slot % args.tiles, seg = static_cast<int>(group % args.segments);
+    const int bh = static_cast<int>(group / args.segments), b = bh / args.H, h = bh % args.H;
+    const int c0 = tile * 4 * WC, dc = p.c.d, db = p.b.d;
+    if (c0 >= dc) return;
+    const int len = live_ticks(args.lengths, b, args.T);
+    const int begin = min(seg * args.seg_ticks, len), end = min(begin + args.seg_ticks, len);
+    const float rate = args.log_decay[h] * 1.4426950408889634f;
+    const int wc = c0 + wave * WC;       // the wave's first channel
+    const bool active = wc < dc;
+
+    const T *pa = static_cast<const T *>(p.a.p) + b * p.a.sb + h / p.a.share * p.a.sh;
+    const T *pb = static_cast<const T *>(p.b.p) + b * p.b.sb + h / p.b.share * p.b.sh;
+    const T *pc = static_cast<const T *>(p.c.p) + b * p.c.sb + h / p.c.share * p.c.sh;
+    const int64_t out_st = static_cast<int64_t>(args.B) * args.H * dc;
+    const int64_t out_at = static_cast<int64_t>(bh) * dc;
+
+    // state: x[i][j][r] is of b's channel row(i) + r and c's channel wc + 16 j + r16
+    auto row = [&](int i) { return kPer == 8 ? 32 * (i / 2) + 8 * kq + 4 * (i % 2) : 16 * i + 4 * kq; };
+    f32x4 x[XT][CT] = {};
+    auto at_state = [&](const float *q, int i, int j, int r) {
+        return q + seg * p.x_seg + bh * p.x_bh + (row(i) + r) * p.x_b + (wc + 16 * j + r16) * p.x_c;
+    };
+    if (!STATES && p.x)
+#pragma unroll
+        for (int i = 0; i < XT; ++i)
+#pragma unroll
+            for (int j = 0; j < CT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row(i) + r < db && wc + 16 * j + r16 < dc) x[i][j][r] = *at_state(p.x, i, j, r);
+
+    // decays within a 16 x 16 tile of scores (tick i in the lane, ticks j = 4 kq + r) on the diagonal and below it
+    float on[4], below[4], weight[KT][kPer];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int n = r16 - 4 * kq - r;
+        on[r] = n < 0 ? 0.0f : power(rate, n) * p.in_scale;
+        below[r] = power(rate, 16 + n) * p.in_scale;
+    }
+    auto weigh = [&](int hi) {   // of tick j in a state after tick hi - 1
+#pragma unroll
+        for (int s = 0; s < KT; ++s)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const int j = s * kStep + kq * kPer + e;
+                weight[s][e] = j < hi ? power(rate, hi - p.lead - j) * p.in_scale : 0.0f;
+            }
+    };
+    weigh(kTicks);
+    if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
+        for (int u = threadIdx.x; u < kTicks * kRowP / 4; u += kBlock) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
+    }
+    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+
+    TD ra, rb;
+    TC rc;
+    auto fetch = [&](int at) {
+        const int n = min(end - at, kTicks), step = p.back ? -1 : 1;
+        const int64_t first = p.back ? len - 1 - at : at;
+        if (!STATES) ra.load(pa, p.a.st, first, step, n, 0, p.a.d);
+        rb.load(pb, p.b.st, first, step, n, 0, db);
+        rc.load(pc, p.c.st, first, step, n, c0, dc);
+    };
+    auto only = [&](frag &f, int s, int tick) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            if (s * kStep + kq * kPer + e != tick) f[e] = static_cast<C>(0.0f);
+    };
+    // Outputs of the ticks lo .. hi - 1 of the chunk at `at`, and the state after them; ONE: hi = lo + 1, and no other tick is
+    // multiplied with anything.
+    auto advance = [&](auto one, int at, int lo, int hi) {
+        constexpr bool ONE = decltype(one)::value;
+        frag fc[KT][CT];
+#pragma unroll
+        for (int s = 0; s < KT; ++s)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                fc[s][j] = columns_of<C, kRowC, 4>(lds_c, wave * WC + 16 * j, s * kStep, lane);
+                if (ONE) only(fc[s][j], s, lo);
+            }
+        if (!STATES && p.out) {
+            frag fx[KD][CT];
+#pragma unroll
+            for (int k = 0; k < KD; ++k)
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) fx[k][j][e] = static_cast<C>(x[k * (kPer / 4) + e / 4][j][e % 4]);
+#pragma unroll
+            for (int it = 0; it < TI; ++it) {
+                if (16 * it >= hi || 16 * it + 16 <= lo) continue;
+                f32x4 o[CT] = {};
+#pragma unroll
+                for (int k = 0; k < KD; ++k) {
+                    const frag fa = rows_of<C, kRow>(lds_a, 16 * it, k * kStep, lane);
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) o[j] = M::run(fx[k][j], fa, o[j]);
+                }
+                const int i = 16 * it + r16;
+                const float f = power(rate, max(i - lo, 0) + p.lead);
+#pragma unroll
+                for (int j = 0; j < CT; ++j) o[j] *= f;
+#pragma unroll
+                for (int s = 0; s < KT; ++s) {
+                    if (s * kStep > 16 * it + 15) break;
+                    const frag fp = rows_of<C, kRowP>(lds_p, 16 * it, s * kStep, lane);
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) o[j] = M::run(fc[s][j], fp, o[j]);
+                }
+                if (i < lo || i >= hi) continue;
+                const int64_t t = p.back ? len - 1 - at - i : at + i;
+#pragma unroll
+                for (int j = 0; j < CT; ++j) {
+                    const int ch = wc + 16 * j + 4 * kq, have = dc - ch;
+                    if (have <= 0) continue;
+                    const f32x4 v = o[j] * p.out_scale;
+                    const int64_t to = t * out_st + out_at + ch;
+                    if (p.wide) {
+                        float *q = static_cast<float *>(p.out) + to;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (e < have) q[e] = v[e];
+                    } else {
+                        T *q = static_cast<T *>(p.out) + to;
+                        if (have >= 4) {
+                            *reinterpret_cast<Vec<T, 4> *>(q) = __builtin_convertvector(v, Vec<T, 4>);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (e < have) q[e] = from_f32<T>(v[e]);
+                        }
+                    }
+                }
+            }
+        }
+        const float f = power(rate, hi - lo);
+#pragma unroll
+        for (int i = 0; i < XT; ++i)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) x[i][j] *= f;
+        // The state is float32, but what a matrix instruction multiplies is not: a weighted value is three bfloat16
+        // ones, 24 bits together.
+        constexpr int kParts = sizeof(C) == 2 ? 3 : 1;
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+            frag part[CT][kParts];
+#pragma unroll
+            for (int j = 0; j < CT; ++j)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    float v = static_cast<float>(fc[s][j][e]) * weight[s][e];
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) {
+                        part[j][q][e] = static_cast<C>(v);
+                        v -= static_cast<float>(part[j][q][e]);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < XT; ++i) {
+                frag fb = columns_of<C, kRow, GAP>(lds_b, kPer == 8 ? 32 * (i / 2) + 4 * (i % 2) : 16 * i, s * kStep, lane);
+                if (ONE) only(fb, s, lo);
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) x[i][j] = M::run(fb, part[j][q], x[i][j]);
+            }
+        }
+    };
+    if (begin < end) fetch(begin);
+    for (int at = begin, turn = 0; at < end; at += kTicks, turn ^= 1) {
+        const int n = min(end - at, kTicks);
+        __syncthreads();   // the last chunk's tiles have been read
+        if (!STATES) ra.store(lds_a);
+        rb.store(lds_b);
+        rc.store(lds_c);
+        if (!STATES && !rc.finite()) odd[turn] = 1;
+        if (threadIdx.x == 0) odd[turn ^ 1] = 0;
+        __syncthreads();
+        if (at + kTicks < end) fetch(at + kTicks);
+        const bool single = !STATES && odd[turn] != 0;
+        if (!STATES) {
+            // scores: rows j, columns i
+#pragma unroll
+            for (int u = 0; u < TI * TI / 4; ++u) {
+                const int it = TI == 4 ? wave : wave / 2, jt = TI == 4 ? u : wave % 2;
+                if (jt > it) continue;
+                f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < KD; ++k)
+                    s = M::run(rows_of<C, kRow>(lds_b, 16 * jt, k * kStep, lane), rows_of<C, kRow>(lds_a, 16 * it, k * kStep, lane), s);
+                typedef C four __attribute__((ext_vector_type(4)));
+                four o;
+                const float far = it == jt ? 1.0f : power(rate, 16 * (it - jt - 1));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float f = it == jt ? (4 * kq + r <= r16 ? s[r] * on[r] : 0.0f) : s[r] * below[r] * far;
+                    o[r] = static_cast<C>(f);
+                }
+                *reinterpret_cast<four *>(lds_p + (16 * it + r16) * kRowP + (16 * jt + 4 * kq) * static_cast<int>(sizeof(C))) = o;
+            }
+            __syncthreads();
+        }
+        if (!active) continue;
+        // A product with a later tick's 0 is NaN where that tick's c is not finite: such a chunk goes tick by tick.
+        if (single) {
+            for (int i = 0; i < n; ++i) {
+                weigh(i + 1);
+                advance(std::true_type{}, at, i, i + 1);
+            }
+        } else {
+            if (n < kTicks) weigh(n);
+            advance(std::false_type{}, at, 0, n);
+        }
+    }
+    // Ticks behind the length are 0.
+    if (!STATES && p.out) {
+        const int t0 = max(len, seg * args.seg_ticks), t1 = min(args.T, (seg + 1) * args.seg_ticks), w = min(4 * WC, dc - c0);
+        for (int u = threadIdx.x; u < (t1 - t0) * w; u += kBlock) {
+            const int64_t to = (t0 + u / w) * out_st + out_at + c0 + u % w;
+            if (p.wide) static_cast<float *>(p.out)[to] = 0.0f;
+            else static_cast<T *>(p.out)[to] = T(0.0f);
+        }
+    }
+    if (p.x_out && active)
+#pragma unroll
+        for (int i = 0; i < XT; ++i)
+#pragma unroll
+            for (int j = 0; j < CT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row(i) + r < db && wc + 16 * j + r16 < dc) *const_cast<float *>(at_state(p.x_out, i, j, r)) = x[i][j][r];
+#endif
+}
+
+struct JoinArgs {
+    float *states;          // [segments][B H][n]: what each segment adds; becomes the state before each
+    const float *x;         // [B H][n] before the first, or NULL
+    float *x_out;           // after the last, or NULL
+    const float *log_decay;
+    const int32_t *lengths;
+    int32_t T, H, segments, seg_ticks;
+    int64_t bh, n;
+};
+
+__global__ void __launch_bounds__(kBlock) k_attention_join(JoinArgs a) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+    if (i >= a.bh * a.n) return;
+    const int bh = static_cast<int>(i / a.n), len = live_ticks(a.lengths, bh / a.H, a.T);
+    const float rate = a.log_decay[bh % a.H] * 1.4426950408889634f;
+    float x = a.x ? a.x[i] : 0.0f;
+    for (int s = 0; s < a.segments; ++s) {
+        const int ticks = min(max(len - s * a.seg_ticks, 0), a.seg_ticks);
+        float *p = a.states + s * a.bh * a.n + i;
+        const float more = *p;
+        *p = x;
+        if (ticks) x = x * power(rate, ticks) + more;
+    }
+    if (a.x_out) a.x_out[i] = x;
+}
+
+// out[row][g][d] = the sum of in[row][g share + i][d] over i, in their order
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_attention_share(const float *in, int64_t rows, int groups, int share, int d, T *out) {
+    const int64_t n = rows * groups * d;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+        const float *p = in + i / d * share * d + i % d;
+        float s = 0.0f;
+        for (int k = 0; k < share; ++k) s += p[static_cast<int64_t>(k) * d];
+        out[i] = from_f32<T>(s);
+    }
+}
+
+template <typename T, int D, int WC>
+void run_pass(AttArgs a, bool states, hipStream_t s) {
+    int widest = 0;
+    for (int i = 0; i < a.passes; ++i) widest = std::max(widest, a.pass[i].c.d);
+    a.tiles = ceil_div(widest, 4 * WC);
+    const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
+    const dim3 grid(static_cast<unsigned>(groups * a.tiles * a.passes));
+    if (states) hipLaunchKernelGGL((k_attention<T, D, WC, true>), grid, dim3(kBlock), 0, s, a);
+    else hipLaunchKernelGGL((k_attention<T, D, WC, false>), grid, dim3(kBlock), 0, s, a);
+}
+
+template <typename T>
+void run_passes(const AttArgs &a, bool states, hipStream_t s) {
+    int da = 0, dc = 0;
+    for (int i = 0; i < a.passes; ++i) da = std::max(da, a.pass[i].b.d), dc = std::max(dc, a.pass[i].c.d);
+    if (dc <= 64) {
+        if (da <= 32) run_pass<T, 32, 16>(a, states, s);
+        else if (da <= 64) run_pass<T, 64, 16>(a, states, s);
+        else run_pass<T, 128, 16>(a, states, s);
+    } else {
+        if (da <= 32) run_pass<T, 32, 32>(a, states, s);
+        else if (da <= 64) run_pass<T, 64, 32>(a, states, s);
+        else run_pass<T, 128, 32>(a, states, s);
+    }
+}
+
+template <typename T>
+void run_share(const float *in, int64_t rows, int groups, int share, int d, void *out, hipStream_t s) {
+    const int64_t n = rows * groups * d;
+    if (n == 0) return;
+    hipLaunchKernelGGL(k_attention_share<T>, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n, kBlock), 16384))), dim3(kBlock), 0, s,
+                       in, rows, groups, share, d, static_cast<T *>(out));
+}
+
+// One tick: a block takes 32 of v's channels of an entry and head, 8 lanes by 32 lots of k's channels.
+struct StepArgs {
+    const void *q, *k, *v;
+    int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
+    const float *log_decay;
+    float *state;
+    void *y;
+    int32_t H, share, K, V, tiles;
+    float scale;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_attention_step(StepArgs a) {
+    __shared__ float sums[kBlock / kWave][32];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int tile = blockIdx.x % a.tiles, bh = blockIdx.x / a.tiles, b = bh / a.H, h = bh % a.H;
+    const int c = tile * 32 + threadIdx.x % 8 * 4, have = a.V - c;
+    const T *q = static_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh;
+    const T *k = static_cast<const T *>(a.k) + b * a.k_sb + h / a.share * a.k_sh;
+    const T *v = static_cast<const T *>(a.v) + b * a.v_sb + h / a.share * a.v_sh;
+    const float lam = __builtin_amdgcn_exp2f(a.log_decay[h] * 1.4426950408889634f);
+    float *state = a.state + static_cast<int64_t>(bh) * a.K * a.V + c;
+    f32x4 vv = {0.0f, 0.0f, 0.0f, 0.0f}, sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < have) vv[e] = to_f32(v[c + e]);
+#pragma unroll 4
+    for (int d = threadIdx.x / 8; d < a.K; d += 32) {
+        const float kd = to_f32(k[d]), qd = to_f32(q[d]);
+        float *p = state + static_cast<int64_t>(d) * a.V;
+        if (have >= 4) {
+            const f32x4 x = *reinterpret_cast<const Vec<f32, 4> *>(p) * lam + vv * kd;
+            *reinterpret_cast<Vec<f32, 4> *>(p) = x;
+            sum += x * qd;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < have) {
+                    const float x = p[e] * lam + vv[e] * kd;
+                    p[e] = x;
+                    sum[e] += x * qd;
+                }
+        }
+    }
+#pragma unroll
+    for (int m = 8; m < kWave; m <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], m, kWave);
+    if (lane < 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[wave][lane * 4 + e] = sum[e];
+    __syncthreads();
+    const int ch = tile * 32 + threadIdx.x;
+    if (threadIdx.x >= 32 || ch >= a.V) return;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kBlock / kWave; ++w) s += sums[w][threadIdx.x];
+    static_cast<T *>(a.y)[static_cast<int64_t>(bh) * a.V + ch] = from_f32<T>(s * a.scale);
+}
+
+template <typename T>
+void run_step(const StepArgs &a, int64_t blocks, hipStream_t s) {
+    hipLaunchKernelGGL(k_attention_step<T>, dim3(static_cast<unsigned>(blocks)), dim3(kBlock), 0, s, a);
+}
+
+int check_attention(const glif_attention *a, bool step) {
+    if (!a) return fail(GLIF_EINVAL, "NULL argument");
+    if (!known_dtype(a->dtype)) return fail(GLIF_EINVAL, "attention: unknown type");
+    if (a->n_ticks < 0 || a->n_ticks > (1 << 20) || a->n_batch < 0 || a->n_batch > 65535 || a->n_heads < 0 || a->n_heads > 4096)
+        return fail(GLIF_EINVAL, "attention: at most 2^20 ticks, a batch of 65535 and 4096 heads");
+    if (a->n_groups < 1 || a->n_heads % a->n_groups) return fail(GLIF_EINVAL, "attention: n_groups must divide n_heads");
+    if (a->d_key < 1 || a->d_key > 128 || a->d_value < 1 || a->d_value > 128)
+        return fail(GLIF_EINVAL, "attention: keys and values have 1 to 128 channels");
+    if (static_cast<int64_t>(a->n_batch) * a->n_heads > (1 << 20))
+        return fail(GLIF_EINVAL, "attention: at most 2^20 heads in a batch");
+    const bool some = static_cast<int64_t>(a->n_batch) * a->n_heads != 0;
+    if (some && (!a->log_decay || ((step || a->n_ticks) && (!a->q || !a->k || !a->v)))) return fail(GLIF_EINVAL, "NULL argument");
+    return GLIF_OK;
+}
+
+// Ticks in segments where there are too few blocks for the chip: a first launch gives the state that each segment adds,
+// a second joins them, and then all segments go at once.  The first reads two of three sequences again.
+void cut(AttArgs &a, int64_t blocks, int ticks) {
+    a.segments = 1, a.seg_ticks = std::max((a.T + ticks - 1) / ticks, 1) * ticks;
+    if (blocks == 0 || blocks >= 256) return;
+    const int64_t chunks = (a.T + ticks - 1) / ticks, want = std::min<int64_t>((512 + blocks - 1) / blocks, chunks / 4);
+    if (want < 2) return;
+    a.seg_ticks = static_cast<int>((chunks + want - 1) / want) * ticks;
+    a.segments = (a.T + a.seg_ticks - 1) / a.seg_ticks;
+}
+
+int chunk_ticks(int32_t dtype) { return dtype == GLIF_BF16 ? 64 : 32; }
+
+AttArgs common(const glif_attention *s) {
+    AttArgs a{};
+    a.log_decay = s->log_decay, a.lengths = s->lengths, a.T = s->n_ticks, a.B = s->n_batch, a.H = s->n_heads;
+    return a;
+}
+
+AttArgs forward_args(const glif_attention *s) {
+    AttArgs a = common(s);
+    const int64_t tiles = s->d_value <= 64 ? 1 : (s->d_value + 127) / 128;
+    cut(a, static_cast<int64_t>(a.B) * a.H * tiles, chunk_ticks(s->dtype));
+    return a;
+}
+
+AttArgs backward_args(const glif_attention *s) {
+    AttArgs a = common(s);
+    cut(a, static_cast<int64_t>(a.B) * a.H * 3, chunk_ticks(s->dtype));
+    return a;
+}
+
+size_t state_floats(const AttArgs &a, const glif_attention *s) {
+    return a.segments > 1 ? static_cast<size_t>(a.segments) * a.B * a.H * s->d_key * s->d_value : 0;
+}
+
+struct AttBack {
+    float *forward, *backward;   // states of the segments, each way
+    float *dk, *dv;              // of every head, where heads share theirs
+};
+
+void carve(Carver &c, AttBack &b, const AttArgs &a, const glif_attention *s) {
+    if (const size_t n = state_floats(a, s)) b.forward = c.take<float>(n), b.backward = c.take<float>(n);
+    if (s->n_groups < s->n_heads) {
+        const size_t rows = static_cast<size_t>(a.T) * a.B * a.H;
+        b.dk = c.take<float>(rows * s->d_key), b.dv = c.take<float>(rows * s->d_value);
+    }
+}
+
+// The states before every segment, [segments][B H][d_key][d_value].
+void segment_states(const AttArgs &of, const AttSeq &b, const AttSeq &c, bool back, float in_scale, const float *x, float *x_out, float *states,
+                    int32_t dtype, hipStream_t s) {
+    AttArgs a = of;
+    const int64_t n = static_cast<int64_t>(b.d) * c.d, bh = static_cast<int64_t>(a.B) * a.H;
+    AttPass &p = a.pass[0];
+    a.passes = 1;
+    p = AttPass{};
+    p.a = p.b = b, p.c = c, p.back = back, p.lead = back ? 0 : 1, p.in_scale = in_scale;
+    p.x_out = states, p.x_seg = bh * n, p.x_bh = n, p.x_b = c.d, p.x_c = 1;
+    GLIF_BY_DTYPE(dtype, run_passes, a, true, s);
+    const JoinArgs j{states, x, x_out, a.log_decay, a.lengths, a.T, a.H, a.segments, a.seg_ticks, bh, n};
+    hipLaunchKernelGGL(k_attention_join, dim3(static_cast<unsigned>(ceil_div(bh * n, kBlock))), dim3(kBlock), 0, s, j);
+}
+
+}  // namespace
+}  // namespace glif
+
+using namespace glif;
+
+extern "C" {
+
+size_t glif_attention_fwd_workspace(const glif_attention *s) {
+    if (check_attention(s, false)) return 0;
+    const AttArgs a = forward_args(s);
+    Carver c(nullptr, 0);
+    if (const size_t n = state_floats(a, s)) c.take<float>(n);
+    return c.off;
+}
+
+int glif_attention_fwd(const glif_attention *s, void *y, float *last, void *ws, size_t ws_bytes, void *stream) {
+    if (int rc = check_attention(s, false)) return rc;
+    AttArgs a = forward_args(s);
+    if (static_cast<int64_t>(a.B) * a.H == 0) return GLIF_OK;
+    if (a.T && !y) return fail(GLIF_EINVAL, "NULL argument");
+    Carver c(ws, ws_bytes);
+    const size_t n = state_floats(a, s);
+    float *states = n ? c.take<float>(n) : nullptr;
+    if (!c.ok() || (n && !ws)) return fail(GLIF_ENOMEM, "attention: workspace too small");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int32_t share = s->n_heads / s->n_groups;
+    const AttSeq q{s->q, s->q_st, s->q_sb, s->q_sh, 1, s->d_key}, k{s->k, s->k_st, s->k_sb, s->k_sh, share, s->d_key};
+    const AttSeq v{s->v, s->v_st, s->v_sb, s->v_sh, share, s->d_value};
+    if (n) segment_states(a, k, v, false, 1.0f, s->state, last, states, s->dtype, st);
+    AttPass &p = a.pass[0];
+    a.passes = 1;
+    p.a = q, p.b = k, p.c = v, p.out = y, p.lead = 1, p.out_scale = s->scale, p.in_scale = 1.0f;
+    const int64_t each = static_cast<int64_t>(s->d_key) * s->d_value;
+    p.x = n ? states : s->state, p.x_seg = n ? each * a.B * a.H : 0, p.x_bh = each, p.x_b = s->d_value, p.x_c = 1;
+    p.x_out = n ? nullptr : last;
+    GLIF_BY_DTYPE(s->dtype, run_passes, a, false, st);
+    GLIF_HIP(hipGetLastError());
+    return GLIF_OK;
+}
+
+size_t glif_attention_bwd_workspace(const glif_attention *s) {
+    if (check_attention(s, false)) return 0;
+    const AttArgs a = backward_args(s);
+    Carver c(nullptr, 0);
+    AttBack b{};
+    carve(c, b, a, s);
+    return c.off;
+}
+
+int glif_attention_bwd(const glif_attention *s, const glif_attention_grad *g, void *ws, size_t ws_bytes, void *stream) {
+    if (int rc = check_attention(s, false)) return rc;
+    if (!g) return fail(GLIF_EINVAL, "NULL argument");
+    AttArgs a = backward_args(s);
+    if (static_cast<int64_t>(a.B) * a.H == 0) return GLIF_OK;
+    if (a.T && !g->dy) return fail(GLIF_EINVAL, "NULL argument");
+    Carver c(ws, ws_bytes);
+    AttBack w{};
+    carve(c, w, a, s);
+    if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "attention: workspace too small");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int32_t share = s->n_heads / s->n_groups;
+    const bool shared = share > 1, cut = a.segments > 1;
+    const AttSeq q{s->q, s->q_st, s->q_sb, s->q_sh, 1, s->d_key}, k{s->k, s->k_st, s->k_sb, s->k_sh, share, s->d_key};
+    const AttSeq v{s->v, s->v_st, s->v_sb, s->v_sh, share, s->d_value}, dy{g->dy, g->dy_st, g->dy_sb, g->dy_sh, 1, s->d_value};
+    const int64_t each = static_cast<int64_t>(s->d_key) * s->d_value, seg = cut ? each * a.B * a.H : 0;
+    const bool back = g->dk || g->dv || g->dstate;
+    if (cut && g->dq) segment_states(a, k, v, false, 1.0f, s->state, nullptr, w.forward, s->dtype, st);
+    if (cut && back) segment_states(a, q, dy, true, s->scale, g->dlast, g->dstate, w.backward, s->dtype, st);
+    if (g->dq) {
+        AttPass &p = a.pass[a.passes++];
+        p.a = dy, p.b = v, p.c = k, p.out = g->dq, p.lead = 1, p.out_scale = s->scale, p.in_scale = 1.0f;
+        p.x = cut ? w.forward : s->state, p.x_seg = seg, p.x_bh = each, p.x_b = 1, p.x_c = s->d_value;
+    }
+    if (g->dk) {
+        AttPass &p = a.pass[a.passes++];
+        p.a = v, p.b = dy, p.c = q, p.out = shared ? w.dk : g->dk, p.wide = shared, p.back = 1, p.out_scale = 1.0f, p.in_scale = s->scale;
+        p.x = cut ? w.backward : g->dlast, p.x_seg = seg, p.x_bh = each, p.x_b = 1, p.x_c = s->d_value;
+    }
+    if (g->dv || (g->dstate && !cut)) {
+        AttPass &p = a.pass[a.passes++];
+        p.a = k, p.b = q, p.c = dy, p.out = !g->dv ? nullptr : shared ? w.dv : g->dv, p.wide = shared, p.back = 1, p.out_scale = 1.0f;
+        p.in_scale = s->scale;
+        p.x = cut ? w.backward : g->dlast, p.x_seg = seg, p.x_bh = each, p.x_b = s->d_value, p.x_c = 1;
+        p.x_out = cut ? nullptr : g->dstate;
+    }
+    if (a.passes) GLIF_BY_DTYPE(s->dtype, run_passes, a, false, st);
+    if (shared) {
+        const int64_t rows = static_cast<int64_t>(a.T) * a.B;
+        if (g->dk) GLIF_BY_DTYPE(s->dtype, run_share, w.dk, rows, s->n_groups, share, s->d_key, g->dk, st);
+        if (g->dv) GLIF_BY_DTYPE(s->dtype, run_share, w.dv, rows, s->n_groups, share, s->d_value, g->dv, st);
+    }
+    GLIF_HIP(hipGetLastError());
+    return GLIF_OK;
+}
+
+int glif_attention_step(const glif_attention *s, void *y, float *state, void *stream) {
+    if (int rc = check_attention(s, true)) return rc;
+    const int64_t bh = static_cast<int64_t>(s->n_batch) * s->n_heads;
+    if (bh == 0) return GLIF_OK;
+    if (!y || !state) return fail(GLIF_EINVAL, "NULL argument");
+    const int tiles = (s->d_value + 31) / 32;
+    const StepArgs a{s->q, s->k, s->v, s->q_sb, s->q_sh, s->k_sb, s->k_sh, s->v_sb, s->v_sh, s->log_decay, state, y,
+                     s->n_heads, s->n_heads / s->n_groups, s->d_key, s->d_value, tiles, s->scale};
+    GLIF_BY_DTYPE(s->dtype, run_step, a, bh * tiles, static_cast<hipStream_t>(stream));
+    GLIF_HIP(hipGetLastError());
+    return GLIF_OK;
+}
+
+}  // extern "C"

@@ -7,12 +7,10 @@
 // of 2500); short ones and ones of few tiles by the fill and drain of their blocks and by the way of their operands from memory
 // (2500 x 66000 x 512 bfloat16, each in a loop of its own: forward 222 us, dx 259, dW 178; after each other in a training step
 // 227, 303 and 202); single ticks by the stream of the weights.
-#include "seq.h"
+#include "mma.h"
 
 namespace glif {
 namespace {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // C[m][n] = sum_k P(m, k) Q(n, k): P(m, k) is p[m * p_ld + k], or p[k * p_ld + m] where its columns are contiguous;
 // likewise Q.
@@ -59,31 +57,6 @@ __device__ __forceinline__ float slope_of(float p, int act) {
         default: return 1.0f;
     }
 }
-
-// One matrix instruction's operands from a row-major LDS row of 32 k's: 16-bit types take 8 consecutive k's a lane.
-template <typename T>
-struct Mma;
-template <>
-struct Mma<bf16> {
-    typedef bf16 frag __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-};
-template <>
-struct Mma<f16> {
-    typedef f16 frag __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-};
-// float32: lane l holds four consecutive k's, element i of every lane makes one 16x16x4 product (the order of the k's in
-// a sum is free, as long as both operands have it)
-template <>
-struct Mma<f32> {
-    typedef f32 frag __attribute__((ext_vector_type(4)));
-    static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-        return c;
-    }
-};
 
 // ---- tiles in LDS -----------------------------------------------------------------------------------------------------
 // An operand's tile is ROWS rows (of m or n) of 128 bytes of k: 64 16-bit values or 32 float32.  LDS gives 256 bytes a clock:

@@ -2,8 +2,8 @@
 // dense branch :354-376, models.py:419-427): one streaming pass over a weight vector; and AdamW over many tensors at once.
 #include <cmath>
 
+#include "mma.h"
 #include "philox.h"
-#include "seq.h"
 
 namespace glif {
 
@@ -50,7 +50,6 @@ __global__ void __launch_bounds__(kBlock)
 // its mean is the value: moments that move by less than a code's step each time still move.  What is not 0 of v does not
 // become 0, as the step divides by its root.  The random numbers of element i of all variables' blocks are the two halves of word
 // (t - 1) P + i of the Philox stream `seed`, P the elements of all blocks.
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kUnit = 256;          // elements that a wave takes at once, and that share a scale
 constexpr int kUnitsPerBlock = 16;  // that a block takes at once
 constexpr int kMostTensors = 64;    // of a launch

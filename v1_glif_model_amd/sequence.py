@@ -7,7 +7,8 @@ these are the operators of a trained readout over whole training windows and, ti
 * ``dropout``                                       its mask drawn from the Philox streams of ``inputs`` and never stored;
 * ``linear``                                        with bias, activation and residual in one kernel;
 * ``short_conv``, ``short_conv_step``               a causal convolution of a few ticks per channel;
-* ``state_space_scan``, ``state_space_step``        a selective state space.
+* ``state_space_scan``, ``state_space_step``        a selective state space;
+* ``linear_attention``, ``linear_attention_step``   linear attention with a decay for each head.
 
 Activations are float32, bfloat16 or float16 tensors on the GPU; statistics, sums and states are float32 and every output
 is rounded once.  Sequences are time-major ``[T, B, D]`` like the rollouts.  ``lengths`` (int32 ``[B]``, on the device)
@@ -26,7 +27,8 @@ from torch.autograd import forward_ad
 from . import _lib
 from ._lib import check, lib
 
-__all__ = ["layer_norm", "dropout", "linear", "short_conv", "short_conv_step", "state_space_scan", "state_space_step"]
+__all__ = ["layer_norm", "dropout", "linear", "short_conv", "short_conv_step", "state_space_scan", "state_space_step",
+           "linear_attention", "linear_attention_step"]
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -534,3 +536,111 @@ def _tick(t):
     if t is None or t.is_contiguous():
         return t
     return t if t[:1].is_contiguous() else t.contiguous()
+
+
+# ------------------------------------------------------------------- linear attention ----
+def _heads(t):
+    """t [..., heads, channels] with the channels contiguous."""
+    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _attention_struct(q, k, v, log_decay, state, lengths, scale, ticks):
+    """glif_attention of tensors with contiguous channels (held by the caller)."""
+    strides = [n for t in (q, k, v) for n in (t.stride()[:3] if ticks else (0, *t.stride()[:2]))]
+    return _lib.Attention(_p(q), _p(k), _p(v), _p(log_decay), _p(state), _p(lengths), *strides, scale, DTYPES[q.dtype],
+                          q.shape[0] if ticks else 1, q.shape[-3], q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1])
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, lengths, scale):
+        ctx.set_materialize_grads(False)
+        (T, B, H, K), V, dev = q.shape, v.shape[-1], q.device
+        held = [_heads(q), _heads(k), _heads(v), _dense(log_decay), _dense(state), lengths]
+        s = _attention_struct(*held, scale, True)
+        y = torch.empty((T, B, H, V), dtype=q.dtype, device=dev)
+        last = torch.empty((B, H, K, V), dtype=torch.float32, device=dev)
+        L = lib()
+        ws = _workspace(L.glif_attention_fwd_workspace(byref(s)), dev)
+        with _on(dev):
+            check(L.glif_attention_fwd(byref(s), _p(y), _p(last), _p(ws), _size(ws), _stream(dev)))
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.scale = scale
+        return y, last
+
+    @staticmethod
+    def backward(ctx, dy, dlast):
+        _first_only("linear_attention")
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        (T, B, H, K), V, dev = q.shape, v.shape[-1], q.device
+        held = [_heads(q), _heads(k), _heads(v), _dense(log_decay), _dense(state), lengths]
+        s = _attention_struct(*held, ctx.scale, True)
+        dy = _heads(dy) if dy is not None else torch.zeros((T, B, H, V), dtype=q.dtype, device=dev)
+        dlast = _dense(dlast)
+        wants = ctx.needs_input_grad
+        dq, dk, dv, dstate = (torch.empty(t.shape, dtype=t.dtype, device=dev) if w else None
+                              for t, w in ((q, wants[0]), (k, wants[1]), (v, wants[2]), (state, wants[4])))
+        g = _lib.AttentionGrad(_p(dy), *dy.stride()[:3], _p(dlast), _p(dq), _p(dk), _p(dv), _p(dstate))
+        L = lib()
+        ws = _workspace(L.glif_attention_bwd_workspace(byref(s)), dev)
+        with _on(dev):
+            check(L.glif_attention_bwd(byref(s), byref(g), _p(ws), _size(ws), _stream(dev)))
+        return dq, dk, dv, None, dstate, None, None
+
+
+def _attention_args(q, k, v, log_decay, scale):
+    _activations(q, "q")
+    lead, (H, K) = tuple(q.shape[:-2]), q.shape[-2:]
+    _need(k, "k", (*lead, None, K), q.dtype, q.device)
+    G = k.shape[-2]
+    _need(v, "v", (*lead, G, None), q.dtype, q.device)
+    V = v.shape[-1]
+    if not 1 <= K <= 128 or not 1 <= V <= 128:
+        raise ValueError(f"q, k and v must have 1 to 128 channels a head, got {K} and {V}")
+    if G < 1 or H < 1 or H % G:
+        raise ValueError(f"the heads of k and v ({G}) must divide those of q ({H})")
+    _need(log_decay, "log_decay", (H,), torch.float32, q.device)
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError("log_decay has no gradient: each head's decay is a constant")
+    return float(K ** -0.5 if scale is None else scale)
+
+
+def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths=None):
+    """Attention without a softmax, whose heads forget each at its own rate:
+
+    ``S[t] = exp(log_decay) * S[t - 1] + k[t][:, None] * v[t]``, ``y[t] = scale * q[t] @ S[t]``
+
+    q [T, B, H, K], k [T, B, G, K], v [T, B, G, V] (K and V at most 128; H / G heads share a k and a v); log_decay [H]
+    float32, at most 0, -inf for a head that sees only its own tick, a constant without a gradient; ``scale`` K^-0.5 if None;
+    initial_state [B, H, K, V] float32 or None.  Returns y [T, B, H, V] and the state [B, H, K, V] after each batch entry's
+    last tick.
+
+    Ticks are taken in chunks, as matrix products.  Those of bfloat16 sequences multiply scores and states rounded to bfloat16
+    (their sums, and the states themselves, are float32); those of float16 ones are float32, as states and scores go beyond
+    float16's range."""
+    if torch.is_tensor(q) and q.dim() != 4:
+        raise ValueError(f"q must be [T, B, H, K], got shape {tuple(q.shape)}")
+    scale = _attention_args(q, k, v, log_decay, scale)
+    if initial_state is not None:
+        _need(initial_state, "initial_state", (*q.shape[1:], v.shape[-1]), torch.float32, q.device)
+    lengths = _lengths(lengths, q, q.shape[1])
+    return _apply(_Attention, _wants_grad(q, k, v, log_decay, initial_state), q, k, v, log_decay, initial_state, lengths, scale)
+
+
+def linear_attention_step(q, k, v, state, log_decay, scale=None) -> torch.Tensor:
+    """One tick of ``linear_attention``: q [B, H, K], k [B, G, K], v [B, G, V]; ``state`` [B, H, K, V] is moved on in place.
+    No gradient."""
+    if torch.is_tensor(q) and q.dim() != 3:
+        raise ValueError(f"q must be [B, H, K], got shape {tuple(q.shape)}")
+    scale = _attention_args(q, k, v, log_decay, scale)
+    _need(state, "state", (*q.shape, v.shape[-1]), torch.float32, q.device)
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous: it is written in place")
+    _refuse_grad("linear_attention_step", q, state, k, v, log_decay)
+    held = [_heads(q), _heads(k), _heads(v), _dense(log_decay), None, None]
+    s = _attention_struct(*held, scale, False)
+    y = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
+    with _on(q.device):
+        check(lib().glif_attention_step(byref(s), _p(y), _p(state), _stream(q.device)))
+    torch.autograd.graph.increment_version(state)
+    return y
