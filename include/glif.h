@@ -337,6 +337,19 @@ int glif_linear_bwd(const void *dy, int64_t lddy, const float *pre, const void *
                     int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
                     void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream);
 
+/* Both projections of a gated feed-forward block, the activation and the product: y = act(x Wg^T + bg) (x Wu^T + bu), weight
+ * [2N][K] of Wg's rows, then Wu's, bias [2N] or NULL likewise, y [M][N]; pre [M][2N] (NULL: not kept) takes both arguments for the
+ * backward, in float32.  dpg = dy u act'(g), dpu = dy act(g); the rest as above with dp = (dpg, dpu).  N is at most 2^20, a
+ * weight's first N rows below 4 GiB. */
+size_t glif_gated_linear_fwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K);
+int glif_gated_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int32_t dtype,
+                          int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation, void *y, float *pre, void *ws,
+                          size_t ws_bytes, void *stream);
+size_t glif_gated_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t unaligned);
+int glif_gated_linear_bwd(const void *dy, int64_t lddy, const float *pre, const void *x, int64_t ldx, const void *weight,
+                          int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
+                          void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream);
+
 /* Causal convolution with W <= 8 taps per channel: y[t] = act(bias + sum_k weight[d][k] x[t - (W - 1) + k]), act the
  * identity or silu.  state [B][W - 1][D] (NULL: zeros) holds the ticks before 0, last (may be NULL) the last W - 1 ones
  * before each length.  The step moves `state` on in place. */

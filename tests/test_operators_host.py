@@ -64,3 +64,25 @@ def test_attention_refuses_missing_outputs_and_workspaces():
     assert L.glif_attention_fwd_workspace(long) > 0
     refused(L.glif_attention_fwd(long, 1 << 22, None, None, 0, None), "workspace")
     assert L.glif_attention_fwd(attention(n_batch=0), None, None, None, 0, None) == 0
+
+
+def gated(dtype=0, bias_dtype=0, M=4, N=8, K=16, act=3, ldx=16, ldw=16, x=1 << 20, w=1 << 21, y=1 << 22):
+    return _lib.lib().glif_gated_linear_fwd(x, ldx, w, ldw, None, dtype, bias_dtype, M, N, K, act, y, None, None, 0, None)
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=3), dict(bias_dtype=1), dict(M=-1), dict(N=2 ** 20 + 1), dict(N=-1), dict(K=2 ** 24), dict(act=4),
+                                dict(ldx=2 ** 24), dict(ldw=2 ** 24), dict(x=None), dict(w=None), dict(y=None),
+                                dict(N=2 ** 20, K=1024, ldw=1024)])
+def test_gated_linear_refuses(kw):
+    refused(gated(**kw))
+
+
+def test_gated_linear_refuses_missing_workspaces_and_arguments():
+    L = _lib.lib()
+    assert gated(M=0) == 0 and gated(N=0) == 0
+    assert L.glif_gated_linear_fwd_workspace(0, 4, 8, 2 ** 20) > 0
+    refused(gated(K=2 ** 20, ldx=2 ** 20, ldw=2 ** 20), "workspace")
+    a = (1 << 20, 16, 0, 0, 4, 8, 16, 3, 1 << 21, None, None, None, 0, None)
+    refused(L.glif_gated_linear_bwd(1 << 22, 8, None, 1 << 23, 16, *a), "NULL")
+    refused(L.glif_gated_linear_bwd(1 << 22, 8, 1 << 24, 1 << 23, 16, *a), "workspace")
+    refused(L.glif_gated_linear_bwd(None, 8, 1 << 24, 1 << 23, 16, *a), "NULL")

@@ -124,6 +124,10 @@ SIGNATURES = {
     "glif_linear_fwd": (C.c_int, [vp, i64, vp, i64, vp, vp, i64, i32, i32, i64, i64, i64, i32, vp, vp, vp, sz, vp]),
     "glif_linear_bwd_workspace": (sz, [i32, i64, i64, i64, i32, i32]),
     "glif_linear_bwd": (C.c_int, [vp, i64, vp, vp, i64, vp, i64, i32, i32, i64, i64, i64, i32, vp, vp, vp, vp, sz, vp]),
+    "glif_gated_linear_fwd_workspace": (sz, [i32, i64, i64, i64]),
+    "glif_gated_linear_fwd": (C.c_int, [vp, i64, vp, i64, vp, i32, i32, i64, i64, i64, i32, vp, vp, vp, sz, vp]),
+    "glif_gated_linear_bwd_workspace": (sz, [i32, i64, i64, i64, i32]),
+    "glif_gated_linear_bwd": (C.c_int, [vp, i64, vp, vp, i64, vp, i64, i32, i32, i64, i64, i64, i32, vp, vp, vp, vp, sz, vp]),
     "glif_short_conv_fwd": (C.c_int, [vp, i64, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
     "glif_short_conv_bwd_workspace": (sz, [i32, i32, i32, i32, i32]),
     "glif_short_conv_bwd": (C.c_int, [vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp,

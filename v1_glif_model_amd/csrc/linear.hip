@@ -34,7 +34,15 @@ struct GemmArgs {
     int64_t ldr;
     int32_t bias_dt, act;
     int32_t past;              // results go past the caches, which keep the operands
+    // Gated: q's rows are taken in turns of 16, of its first `half` (the gates) and of those from `half` on, and N counts both
+    // (whole turns); c, with `outs` columns, is act(gate) times the other.  pre has 2 half columns, bias 2 half values.
+    int64_t half, outs, pre_ld;
 };
+
+// The row of q behind column v of a gated product; those of a turn's end past the last repeat it.
+__device__ __forceinline__ int64_t gated_row(const GemmArgs &a, int64_t v) {
+    return min(v / 32 * 16 + v % 16, a.outs - 1) + (v / 16 % 2) * a.half;
+}
 
 __device__ __forceinline__ float act_of(float p, int act) {
     switch (act) {
@@ -86,6 +94,13 @@ struct Stage {
         for (int i = 0; i < kN; ++i) {
             const int u = threadIdx.x + i * NT;
             at[i] = p + min(row0 + (u >> 3), rows - 1) * ld + k0 + (u & 7) * kV;
+        }
+    }
+    __device__ __forceinline__ void init_gated(const GemmArgs &a, int64_t row0, int64_t k0) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int u = threadIdx.x + i * NT;
+            at[i] = static_cast<const T *>(a.q) + gated_row(a, row0 + (u >> 3)) * a.q_ld + k0 + (u & 7) * kV;
         }
     }
     // left: the k's from the tile's first one on
@@ -155,7 +170,7 @@ struct Finish {
     }
     __device__ __forceinline__ void operator()(const GemmArgs &a, int64_t m, f32x4 v, vec res) const {
         v += bias;
-        if (a.pre) write(a.pre + m * a.ldc + n, v, have, a.past);
+        if (a.pre) write(a.pre + m * a.pre_ld + n, v, have, a.past);
         if (a.act != GLIF_ACT_NONE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = act_of(v[e], a.act);
@@ -165,9 +180,33 @@ struct Finish {
     }
 };
 
+// Likewise four neighbouring results of a gated product.
+template <typename T>
+struct FinishGated {
+    f32x4 gate = {0.0f, 0.0f, 0.0f, 0.0f}, other = {0.0f, 0.0f, 0.0f, 0.0f};   // bias
+    int64_t n;
+    int have;
+    __device__ __forceinline__ FinishGated(const GemmArgs &a, int64_t col) : n(col), have(static_cast<int>(min(static_cast<int64_t>(4), a.outs - col))) {
+        if (a.bias)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < have) gate[e] = load_param(a.bias, a.bias_dt, n + e), other[e] = load_param(a.bias, a.bias_dt, a.half + n + e);
+    }
+    __device__ __forceinline__ void operator()(const GemmArgs &a, int64_t m, f32x4 g, f32x4 u) const {
+        g += gate, u += other;
+        if (a.pre) {
+            Finish<T>::write(a.pre + m * a.pre_ld + n, g, have, a.past);
+            Finish<T>::write(a.pre + m * a.pre_ld + a.half + n, u, have, a.past);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] *= act_of(g[e], a.act);
+        Finish<T>::write(static_cast<T *>(a.c) + m * a.ldc + n, u, have, a.past);
+    }
+};
+
 // A wave's TM x TN results by way of a slab of its own in LDS: rows come out whole, and the epilogue stands once.  Quad q of
 // row r lies at q ^ r mod the row's quads.
-template <typename T, int TM, int TN, int SLAB>
+template <typename T, int TM, int TN, int SLAB, bool GATED>
 __device__ __forceinline__ void put(const GemmArgs &a, f32x4 (&acc)[TM / 16][TN / 16], char *lds, int64_t m0, int64_t n0, int split) {
     constexpr int kQuads = TN / 4, kRows = SLAB / (TN * 4) < TM ? SLAB / (TN * 4) : TM;
     constexpr int kStep = kWave / kQuads, kAhead = 4;
@@ -185,8 +224,31 @@ __device__ __forceinline__ void put(const GemmArgs &a, f32x4 (&acc)[TM / 16][TN 
                 const int r = 16 * i + r16, q = 4 * j + kq;
                 slab[r * kQuads + (q ^ (r & (kQuads - 1)))] = acc[h * (kRows / 16) + i][j];
             }
-        if (n >= a.N) continue;
         const int left = static_cast<int>(min(a.M - m0 - h * kRows, static_cast<int64_t>(kRows)));
+        if constexpr (GATED) {
+            if (a.splits == 1) {   // quads of gates and, four on, of what they multiply
+                constexpr int kOuts = kQuads / 2, kLanes = kWave / kOuts;
+                static_assert(kRows % (2 * kLanes) == 0, "slab");
+                const int o = lane % kOuts, g = o / 4 * 8 + o % 4;
+                const int64_t col = n0 / 2 + o * 4;
+                if (col >= a.outs) continue;
+                const FinishGated<T> end(a, col);
+#pragma unroll 1
+                for (int r = lane / kOuts; r < kRows; r += 2 * kLanes) {
+                    f32x4 v[2][2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int at = r + u * kLanes, key = at & (kQuads - 1);
+                        v[u][0] = slab[at * kQuads + (g ^ key)], v[u][1] = slab[at * kQuads + ((g + 4) ^ key)];
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        if (r + u * kLanes < left) end(a, m0 + h * kRows + r + u * kLanes, v[u][0], v[u][1]);
+                }
+                continue;
+            }
+        }
+        if (n >= a.N) continue;
 #pragma unroll 1
         for (int r = lane / kQuads; r < kRows; r += kStep * kAhead) {
             f32x4 v[kAhead];
@@ -224,7 +286,7 @@ __device__ __forceinline__ void my_tile(const GemmArgs &a, int &tm, int &tn, int
 // BM x BN of C by WM x WN waves, of k in the split's part, for operands of 16-bit rows of k that start anywhere.  Two tiles of
 // each operand in LDS: while one is multiplied, the next comes into registers, and from there into the other (2500 x 66000 x
 // 512 bfloat16 forward 264 us; straight into LDS, below, 230).
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, bool GATED = false>
 __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
     using M = Mma<T>;
     constexpr int NT = WM * WN * kWave, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
@@ -239,7 +301,8 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
     Stage<T, BM, NT> sp;
     Stage<T, BN, NT> sq;
     sp.init(static_cast<const T *>(a.p), a.p_ld, m0, a.M, k0);
-    sq.init(static_cast<const T *>(a.q), a.q_ld, n0, a.N, k0);
+    if constexpr (GATED) sq.init_gated(a, n0, k0);
+    else sq.init(static_cast<const T *>(a.q), a.q_ld, n0, a.N, k0);
     f32x4 acc[FM][FN] = {};
     const int steps = static_cast<int>((k1 - k0 + BK - 1) / BK);
     if (steps > 0) {
@@ -278,7 +341,7 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm(GemmArgs a) {
         }
         __syncthreads();
     }
-    put<T, TM, TN, 2 * kTile / (WM * WN)>(a, acc, lds + wave * (2 * kTile / (WM * WN)), m0 + wm, n0 + wn, split);
+    put<T, TM, TN, 2 * kTile / (WM * WN), GATED>(a, acc, lds + wave * (2 * kTile / (WM * WN)), m0 + wm, n0 + wn, split);
 }
 
 #ifdef __HIP_DEVICE_COMPILE__   // the host's pass does not know the builtins
@@ -324,6 +387,19 @@ struct Direct {
             int r, at;
             place(wave, lane, i, r, at);
             off[i] = COL ? r * ld + min(at, have * kSize - PB) : min(r, have - 1) * ld + at;
+        }
+    }
+
+    // q of a gated product: the way from a gate's row to the other's is within 32 bits
+    __device__ __forceinline__ void init_gated(const GemmArgs &a, int64_t row0, int64_t k0, int wave, int lane) {
+        ld = static_cast<uint32_t>(a.q_ld * kSize);
+        base = static_cast<const char *>(a.q) + (row0 / 2 * a.q_ld + k0) * kSize;
+        range = -1;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            int r, at;
+            place(wave, lane, i, r, at);
+            off[i] = static_cast<uint32_t>(gated_row(a, row0 + r) - row0 / 2) * ld + at;
         }
     }
 
@@ -400,7 +476,7 @@ struct Direct {
 // BM x BN of C by WM x WN waves, of k in the split's part.  Two tiles of each operand in LDS; the second half of a tile's
 // operands is in registers before the barrier at which the tile's LDS is given to the loads of the tile after next, and the
 // first half of the next tile's is read while that second half is multiplied.
-template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL, int PB>
+template <typename T, int BM, int BN, int WM, int WN, bool PCOL, bool QCOL, int PB, bool GATED = false>
 __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
 #ifdef __HIP_DEVICE_COMPILE__
     using M = Mma<T>;
@@ -421,7 +497,8 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
     P p;
     Q q;
     p.init(a.p, a.p_ld, m0, a.p_rows, k0, wave, lane);
-    q.init(a.q, a.q_ld, n0, a.q_rows, k0, wave, lane);
+    if constexpr (GATED) q.init_gated(a, n0, k0, wave, lane);
+    else q.init(a.q, a.q_ld, n0, a.q_rows, k0, wave, lane);
     const typename P::Reader rp(wm, r16, kq);
     const typename Q::Reader rq(wn, r16, kq);
     f32x4 acc[FM][FN] = {};
@@ -494,7 +571,7 @@ __global__ void __launch_bounds__(WM *WN *kWave) k_gemm_direct(GemmArgs a) {
     __syncthreads();
     constexpr int kSlab = 2 * kTile / W;
     char *slab = wave < W / 2 ? lds0 + wave * kSlab : lds1 + (wave - W / 2) * kSlab;
-    put<T, TM, TN, kSlab>(a, acc, slab, m0 + wm, n0 + wn, split);
+    put<T, TM, TN, kSlab, GATED>(a, acc, slab, m0 + wm, n0 + wn, split);
 #endif
 }
 
@@ -567,6 +644,84 @@ __global__ void __launch_bounds__(kBlock) k_few(GemmArgs a) {
     }
 }
 
+// The gated product of at most 16 MT rows (m): a block streams 16 gates' rows and the 16 others'.
+template <typename T, int MT>
+__global__ void __launch_bounds__(kBlock) k_few_gated(GemmArgs a) {
+    using M = Mma<T>;
+    constexpr int kV = 16 / static_cast<int>(sizeof(T)), KS = 4 * kV, U = 4, kWaves = kBlock / kWave;
+    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    __shared__ f32x4 sums[kWaves][MT][2][kWave];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r16 = lane % 16, kq = lane / 16;
+    const int groups = a.tiles_n, split = blockIdx.x / groups;
+    const int64_t col0 = static_cast<int64_t>(blockIdx.x - split * groups) * 16;
+    const int64_t b0 = split * a.k_part, b1 = min(a.K, b0 + a.k_part), part = (b1 - b0 + kWaves * KS - 1) / (kWaves * KS) * KS;
+    const int64_t k0 = min(b0 + wave * part, b1), k1 = min(k0 + part, b1);
+    const T *pw[2], *pf[MT];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) pw[h] = static_cast<const T *>(a.q) + gated_row(a, 2 * col0 + 16 * h + r16) * a.q_ld + kq * kV;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) pf[i] = static_cast<const T *>(a.p) + min(static_cast<int64_t>(16 * i + r16), a.M - 1) * a.p_ld + kq * kV;
+    f32x4 acc[MT][2] = {};
+    int64_t k = k0;
+    for (; k + U * KS <= k1; k += U * KS) {
+        vec w[U][2], f[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[u][h] = *reinterpret_cast<const vec *>(pw[h] + k + u * KS);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) f[u][i] = *reinterpret_cast<const vec *>(pf[i] + k + u * KS);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) acc[i][h] = M::run(w[u][h], f[u][i], acc[i][h]);
+    }
+    for (; k < k1; k += KS) {
+        const int64_t left = k1 - k - kq * kV;
+        auto load = [&](const T *p) {
+            if (left >= kV) return *reinterpret_cast<const vec *>(p + k);
+            vec v;
+#pragma unroll
+            for (int e = 0; e < kV; ++e) v[e] = e < left ? p[k + e] : T(0.0f);
+            return v;
+        };
+        const vec w[2] = {load(pw[0]), load(pw[1])};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const vec f = load(pf[i]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[i][h] = M::run(w[h], f, acc[i][h]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) sums[wave][i][h][lane] = acc[i][h];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4 v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        v[h] = sums[0][wave][h][lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) v[h] += sums[w][wave][h][lane];
+    }
+    const int64_t m = 16 * wave + r16, n = col0 + kq * 4;
+    if (m >= a.M) return;
+    if (a.splits > 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<f32x4 *>(a.part + (split * a.M + m) * a.part_ld + 2 * col0 + 16 * h + kq * 4) = v[h];
+    } else if (n < a.outs) {
+        const FinishGated<T> finish(a, n);
+        finish(a, m, v[0], v[1]);
+    }
+}
+
 // The splits' sums and the epilogue: four results by G lanes, which take the splits in turn (their sums are joined by a fixed
 // tree).
 template <typename T, int G>
@@ -586,6 +741,33 @@ __global__ void __launch_bounds__(kBlock) k_gemm_join(GemmArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], x, kWave);
         if (g == 0) finish(a, m, v, res);
+    }
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kBlock) k_gemm_join_gated(GemmArgs a) {
+    const int64_t quads = (a.outs + 3) / 4, n4 = a.M * quads, step = static_cast<int64_t>(gridDim.x) * (kBlock / G);
+    const int g = threadIdx.x % G;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kBlock / G) + threadIdx.x / G; i < n4; i += step) {
+        const int64_t m = i / quads, n = (i - m * quads) * 4;
+        f32x4 v[2] = {};
+        const float *p = a.part + (g * a.M + m) * a.part_ld + n / 16 * 32 + n % 16;
+#pragma unroll 4
+        for (int s = g; s < a.splits; s += G, p += G * a.M * a.part_ld) {
+            v[0] += *reinterpret_cast<const f32x4 *>(p);
+            v[1] += *reinterpret_cast<const f32x4 *>(p + 16);
+        }
+#pragma unroll
+        for (int x = 1; x < G; x <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[0][e] += __shfl_xor(v[0][e], x, kWave);
+                v[1][e] += __shfl_xor(v[1][e], x, kWave);
+            }
+        if (g == 0) {
+            const FinishGated<T> finish(a, n);
+            finish(a, m, v[0], v[1]);
+        }
     }
 }
 
@@ -659,6 +841,69 @@ __global__ void __launch_bounds__(kBlock) k_slope(SlopeArgs a) {
     }
 }
 
+// Of a gated product: dp's first N columns are dy u act'(g), the others dy act(g), as above rounded for the products and summed
+// by columns before.
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_gate_slope(SlopeArgs a) {
+    constexpr int V = kVecBytes16<T>;
+    typedef Vec<T, V> vec;
+    typedef Vec<float, V> wide;
+    __shared__ float sum[2][kSlopeLots][kSlopeCols * V + 4];
+    const int col = threadIdx.x % kSlopeCols, lot = threadIdx.x / kSlopeCols;
+    const int64_t n = (static_cast<int64_t>(blockIdx.x) * kSlopeCols + col) * V;
+    const int64_t r0 = a.M * blockIdx.y / a.parts, r1 = a.M * (blockIdx.y + 1) / a.parts;
+    const int have = static_cast<int>(max(min(a.N - n, static_cast<int64_t>(V)), static_cast<int64_t>(0)));
+    float sg[V] = {}, su[V] = {};
+#pragma unroll 2
+    for (int64_t m = r0 + lot; m < r1; m += kSlopeLots) {
+        const T *dy = static_cast<const T *>(a.dy) + m * a.lddy + n;
+        const float *pre = a.pre + m * 2 * a.N + n;
+        T *dp = static_cast<T *>(a.dp) + m * a.lddp + n;
+        vec d = {}, og, ou;
+        wide g = {}, u = {};
+        if (have == V) {
+            d = *reinterpret_cast<const vec *>(dy);
+            g = *reinterpret_cast<const wide *>(pre);
+            u = *reinterpret_cast<const wide *>(pre + a.N);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e < have) d[e] = dy[e], g[e] = pre[e], u[e] = pre[a.N + e];
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float f = to_f32(static_cast<T>(d[e])), vg = f * u[e] * slope_of(g[e], a.act), vu = f * act_of(g[e], a.act);
+            og[e] = from_f32<T>(vg), ou[e] = from_f32<T>(vu);
+            sg[e] += vg, su[e] += vu;
+        }
+        if (!a.dp) continue;
+        if (have == V) {
+            *reinterpret_cast<vec *>(dp) = og;
+            *reinterpret_cast<vec *>(dp + a.N) = ou;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e < have) dp[e] = og[e], dp[a.N + e] = ou[e];
+        }
+    }
+    // the columns that fill dp's rows up
+    if (a.dp && blockIdx.x == 0 && threadIdx.x < a.lddp - 2 * a.N)
+        for (int64_t m = r0; m < r1; ++m) static_cast<T *>(a.dp)[m * a.lddp + 2 * a.N + threadIdx.x] = T(0.0f);
+    if (!a.part) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[0][lot][col * V + e] = sg[e], sum[1][lot][col * V + e] = su[e];
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSlopeCols * V;
+    for (int c = threadIdx.x; c < 2 * kSlopeCols * V; c += kBlock) {
+        const int h = c / (kSlopeCols * V), at = c % (kSlopeCols * V);
+        if (first + at >= a.N) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSlopeLots; ++i) s += sum[h][i][at];
+        a.part[static_cast<int64_t>(blockIdx.y) * 2 * a.N + h * a.N + first + at] = s;
+    }
+}
+
 // 16-bit rows onto 16-byte addresses: out [rows][ldo], ldo a multiple of 8, zeros past cols.
 __global__ void __launch_bounds__(kBlock) k_repack(const uint16_t *in, int64_t ld, int64_t rows, int64_t cols, uint16_t *out, int64_t ldo) {
     typedef Vec<uint16_t, 8> vec;
@@ -723,7 +968,7 @@ struct Plan {
 // and the launch that adds them.  Tiles of float32 operands sum over at most 4096 k's up to 64 parts (K of 262144), so that long
 // sums do not lose their last digits; few rows are in a wave's parts of k anyway (all-positive float32 terms, K of 66000 with 16500
 // to a wave: 3e-6 of the sum), and 16-bit results keep fewer digits than either.
-Piece piece_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr, double &best) {
+Piece piece_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr, bool gated, double &best) {
     Piece p{};
     best = 0.0;
     p.rows = M, p.part_ld = (N + 3) / 4 * 4, p.splits = 1, p.kind = kTile128;
@@ -732,9 +977,10 @@ Piece piece_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr, double 
     if (M <= 0 || N <= 0) return p;
     const int64_t few = std::min(M, N), many = std::max(M, N);
     int64_t splits = 1;
-    if (rr && few <= 32) {
+    if (rr && few <= 32 && !(gated && N < M)) {
         p.kind = few <= 16 ? kFew16 : kFew32;
-        splits = std::max<int64_t>(1, std::min<int64_t>(2048 / ((many + 15) / 16), K / 512));
+        const int64_t each = gated ? 32 : 16;   // rows of a block
+        splits = std::max<int64_t>(1, std::min<int64_t>(2048 / ((many + each - 1) / each), K / 512));
         p.k_part = (steps + splits - 1) / splits * bk;
         best = 10.0 + static_cast<double>(many * K * size) / 4e6;   // the stream at 4 TB/s
     } else {
@@ -765,10 +1011,10 @@ Piece piece_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr, double 
 // Tiles that are a few more than whole rounds of the chip's blocks cost one round more.  Where it is cheaper, and by more than
 // a launch, the whole rounds are one piece, and the rest, as short tiles or with k in parts, is another (2500 x 66000 x 512
 // bfloat16, dW of 516 tiles of 256 x 256, 226 us in one, 177 in two).
-Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
+Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr, bool gated = false) {
     Plan p{};
     double best;
-    p.one = piece_for(dtype, M, N, K, rr, best);
+    p.one = piece_for(dtype, M, N, K, rr, gated, best);
     p.cut_m = M > N;
     const int64_t across = std::min(M, N), along = std::max(M, N);
     if (across <= 32) return p;
@@ -778,8 +1024,8 @@ Plan plan_for(int32_t dtype, int64_t M, int64_t N, int64_t K, bool rr) {
         const int64_t cut = wide * ((along + tile - 1) / tile) / slots * slots / wide * tile;
         if (cut == 0 || cut >= along) continue;
         double first, rest;
-        const Piece one = p.cut_m ? piece_for(dtype, cut, N, K, rr, first) : piece_for(dtype, M, cut, K, rr, first);
-        const Piece two = p.cut_m ? piece_for(dtype, M - cut, N, K, rr, rest) : piece_for(dtype, M, N - cut, K, rr, rest);
+        const Piece one = p.cut_m ? piece_for(dtype, cut, N, K, rr, gated, first) : piece_for(dtype, M, cut, K, rr, gated, first);
+        const Piece two = p.cut_m ? piece_for(dtype, M - cut, N, K, rr, gated, rest) : piece_for(dtype, M, N - cut, K, rr, gated, rest);
         if (first + rest + 4.0 < best) best = first + rest + 4.0, p.one = one, p.two = two, p.cut = cut;
     }
     return p;
@@ -793,22 +1039,27 @@ bool on_16(const void *p, int64_t ld, int64_t along, size_t size) {
 
 // float32 rows may start on any float32; 16-bit rows of k that do not lie on 16 bytes come by way of registers (16-bit
 // operands of columns have been put on 16 bytes).
-template <typename T, int TILE, int WM, int WN, bool PCOL, bool QCOL>
+template <typename T, int TILE, int WM, int WN, bool PCOL, bool QCOL, bool GATED>
 void launch_tile(GemmArgs &a, hipStream_t s) {
     a.tiles_m = ceil_div(a.M, TILE), a.tiles_n = ceil_div(a.N, TILE);
     const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n * a.splits)), block(WM * WN * kWave);
     if (on_16(a.p, a.p_ld, PCOL ? a.p_rows : a.k_cols, sizeof(T)) && on_16(a.q, a.q_ld, QCOL ? a.q_rows : a.k_cols, sizeof(T))) {
-        hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL, 16>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL, 16, GATED>), grid, block, 0, s, a);
     } else if constexpr (sizeof(T) == 4) {
-        hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL, 4>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((k_gemm_direct<T, TILE, TILE, WM, WN, PCOL, QCOL, 4, GATED>), grid, block, 0, s, a);
     } else if constexpr (!PCOL && !QCOL) {
-        if constexpr (TILE == 64) hipLaunchKernelGGL((k_gemm<T, 64, 64, 2, 1>), grid, dim3(2 * kWave), 0, s, a);
-        else hipLaunchKernelGGL((k_gemm<T, TILE, TILE, WM, WN>), grid, block, 0, s, a);
+        if constexpr (TILE == 64) hipLaunchKernelGGL((k_gemm<T, 64, 64, 2, 1, GATED>), grid, dim3(2 * kWave), 0, s, a);
+        else hipLaunchKernelGGL((k_gemm<T, TILE, TILE, WM, WN, GATED>), grid, block, 0, s, a);
     }
 }
 
-template <typename T, int MT>
+template <typename T, int MT, bool GATED>
 void launch_few(GemmArgs &a, hipStream_t s) {
+    if constexpr (GATED) {
+        a.tiles_n = ceil_div(a.N, 32);
+        hipLaunchKernelGGL((k_few_gated<T, MT>), dim3(static_cast<unsigned>(a.tiles_n * a.splits)), dim3(kBlock), 0, s, a);
+        return;
+    }
     const bool nfew = a.N < a.M;
     a.tiles_m = ceil_div(a.M, 16), a.tiles_n = ceil_div(a.N, 16);
     const dim3 grid(static_cast<unsigned>((nfew ? a.tiles_m : a.tiles_n) * a.splits));
@@ -816,7 +1067,7 @@ void launch_few(GemmArgs &a, hipStream_t s) {
     else hipLaunchKernelGGL((k_few<T, MT, false>), grid, dim3(kBlock), 0, s, a);
 }
 
-template <typename T, bool PCOL, bool QCOL>
+template <typename T, bool PCOL, bool QCOL, bool GATED>
 void launch_piece(GemmArgs a, const Piece &p, float *part, hipStream_t s) {
     a.splits = p.splits, a.k_part = p.k_part, a.part_ld = p.part_ld, a.part = part;
     // a tile's rows of k within 32-bit offsets
@@ -825,18 +1076,24 @@ void launch_piece(GemmArgs a, const Piece &p, float *part, hipStream_t s) {
     if (a.K == 0) {
         a.splits = 0;   // the epilogue of empty sums (the tile kernels load a first tile whatever there is)
     } else if (p.kind == kFew16 || p.kind == kFew32) {
-        if constexpr (!PCOL && !QCOL) p.kind == kFew16 ? launch_few<T, 1>(a, s) : launch_few<T, 2>(a, s);
+        if constexpr (!PCOL && !QCOL) p.kind == kFew16 ? launch_few<T, 1, GATED>(a, s) : launch_few<T, 2, GATED>(a, s);
     } else if (sizeof(T) == 2 && p.kind == kTile256 && most >= 256) {
-        if constexpr (sizeof(T) == 2) launch_tile<T, 256, 2, 4, PCOL, QCOL>(a, s);
+        if constexpr (sizeof(T) == 2) launch_tile<T, 256, 2, 4, PCOL, QCOL, GATED>(a, s);
     } else if (p.kind != kTile64 && most >= 128) {
-        launch_tile<T, 128, 2, 2, PCOL, QCOL>(a, s);
+        launch_tile<T, 128, 2, 2, PCOL, QCOL, GATED>(a, s);
     } else {
-        launch_tile<T, 64, 2, 2, PCOL, QCOL>(a, s);
+        launch_tile<T, 64, 2, 2, PCOL, QCOL, GATED>(a, s);
     }
     if (a.splits != 1) {
         // where the results alone do not fill the chip, lanes over the splits: 5 x 66000 x 512 in 61 parts 14 us -> 4
-        const int64_t n4 = a.M * (a.part_ld / 4);
-        if (n4 < 32768 && a.splits >= 16)
+        const int64_t n4 = a.M * (GATED ? (a.outs + 3) / 4 : a.part_ld / 4);
+        if constexpr (GATED) {
+            if (n4 < 32768 && a.splits >= 16)
+                hipLaunchKernelGGL((k_gemm_join_gated<T, 16>), dim3(static_cast<unsigned>(ceil_div(n4, kBlock / 16))), dim3(kBlock), 0, s, a);
+            else
+                hipLaunchKernelGGL((k_gemm_join_gated<T, 1>), dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))),
+                                   dim3(kBlock), 0, s, a);
+        } else if (n4 < 32768 && a.splits >= 16)
             hipLaunchKernelGGL((k_gemm_join<T, 16>), dim3(static_cast<unsigned>(ceil_div(n4, kBlock / 16))), dim3(kBlock), 0, s, a);
         else
             hipLaunchKernelGGL((k_gemm_join<T, 1>), dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(n4, kBlock), 8192))),
@@ -844,14 +1101,14 @@ void launch_piece(GemmArgs a, const Piece &p, float *part, hipStream_t s) {
     }
 }
 
-template <typename T, bool PCOL, bool QCOL>
+template <typename T, bool PCOL, bool QCOL, bool GATED = false>
 int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return GLIF_OK;
     // (8192^3 bfloat16 1009 us -> 846; 2500 x 512 x 66000, 330 MB of results, 292 -> 271; 2500 x 512 x 12007, 60 MB, 57 and 63)
-    a.past = a.M * a.N * static_cast<int64_t>(sizeof(T)) > kPastCaches;
-    a.ldc = a.N;
+    a.ldc = GATED ? a.half : a.N, a.pre_ld = GATED ? 2 * a.half : a.N;
+    a.past = a.M * a.ldc * static_cast<int64_t>(sizeof(T)) > kPastCaches;
     if (p.cut == 0) {
-        launch_piece<T, PCOL, QCOL>(a, p.one, part, s);
+        launch_piece<T, PCOL, QCOL, GATED>(a, p.one, part, s);
         return GLIF_OK;
     }
     GemmArgs b = a;
@@ -861,16 +1118,18 @@ int launch_gemm(GemmArgs a, const Plan &p, float *part, hipStream_t s) {
         a.M = p.cut, b.M -= p.cut, b.p_rows -= p.cut;
         on(b.p, p.cut * size * (PCOL ? 1 : b.p_ld));
         on(b.c, p.cut * size * b.ldc), on(b.residual, p.cut * size * b.ldr);
-        if (b.pre) b.pre += p.cut * b.ldc;
+        if (b.pre) b.pre += p.cut * b.pre_ld;
     } else {
+        const int64_t cols = GATED ? p.cut / 2 : p.cut;   // results: a turn of 32 gives 16, and tiles are whole turns
         a.N = p.cut, b.N -= p.cut, b.q_rows -= p.cut;
-        on(b.q, p.cut * size * (QCOL ? 1 : b.q_ld));
-        on(b.c, p.cut * size), on(b.residual, p.cut * size);
-        if (b.pre) b.pre += p.cut;
-        on(b.bias, p.cut * static_cast<int64_t>(dtype_size(b.bias_dt)));
+        if (GATED) a.outs = cols, b.outs -= cols;
+        on(b.q, cols * size * (QCOL ? 1 : b.q_ld));
+        on(b.c, cols * size), on(b.residual, cols * size);
+        if (b.pre) b.pre += cols;
+        on(b.bias, cols * static_cast<int64_t>(dtype_size(b.bias_dt)));
     }
-    launch_piece<T, PCOL, QCOL>(a, p.one, part, s);
-    launch_piece<T, PCOL, QCOL>(b, p.two, part, s);
+    launch_piece<T, PCOL, QCOL, GATED>(a, p.one, part, s);
+    launch_piece<T, PCOL, QCOL, GATED>(b, p.two, part, s);
     return GLIF_OK;
 }
 
@@ -880,6 +1139,15 @@ template <typename T>
 int gemm_rc(const GemmArgs &a, const Plan &p, float *part, hipStream_t s) { return launch_gemm<T, false, true>(a, p, part, s); }
 template <typename T>
 int gemm_cc(const GemmArgs &a, const Plan &p, float *part, hipStream_t s) { return launch_gemm<T, true, true>(a, p, part, s); }
+
+template <typename T>
+int gemm_gated(const GemmArgs &a, const Plan &p, float *part, hipStream_t s) { return launch_gemm<T, false, false, true>(a, p, part, s); }
+
+template <typename T>
+void run_gate_slope(const SlopeArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL(k_gate_slope<T>, dim3(static_cast<unsigned>(ceil_div(a.N, kSlopeCols * kVecBytes16<T>)), static_cast<unsigned>(a.parts)),
+                       dim3(kBlock), 0, s, a);
+}
 
 template <typename T>
 void run_slope(const SlopeArgs &a, hipStream_t s) {
@@ -938,6 +1206,69 @@ void run_repack(const void *in, int64_t ld, int64_t rows, int64_t cols, void *ou
                        static_cast<const uint16_t *>(in), ld, rows, cols, static_cast<uint16_t *>(out), ldo);
 }
 
+// Columns of a gated product: whole turns of 16 gates and the 16 others.
+int64_t turns(int64_t N) { return (N + 15) / 16 * 32; }
+
+int check_gated(int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t act, int64_t ldw) {
+    if (N < 0 || N > (1 << 20)) return fail(GLIF_EINVAL, "linear: a gated product has at most 2^20 columns");
+    if (int rc = check_linear(dtype, bias_dtype, M, turns(N), K, act)) return rc;
+    if ((N + 256) * std::max<int64_t>(ldw, K) * static_cast<int64_t>(dtype_size(dtype)) >= int64_t(1) << 32)
+        return fail(GLIF_EINVAL, "linear: the gates' rows of a weight must be below 4 GiB");
+    return GLIF_OK;
+}
+
+// gated: N counts the weight's rows, dy has half as many columns.
+int linear_bwd(bool gated, const void *dy, int64_t lddy, const float *pre, const void *x, int64_t ldx, const void *weight, int64_t ldw,
+               int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation, void *dx, void *dweight,
+               void *dbias, void *ws, size_t ws_bytes, hipStream_t s) {
+    if (int rc = check_linear(dtype, bias_dtype, M, N, K, activation)) return rc;
+    if (int rc = check_strides(lddy, ldx, ldw)) return rc;
+    const bool some = M && N;
+    if (some && (!dy || ((gated || activation != GLIF_ACT_NONE) && !pre) || (dx && K && !weight) || (dweight && K && !x)))
+        return fail(GLIF_EINVAL, "NULL argument");
+    const size_t size = dtype_size(dtype);
+    const bool half = size == 2;
+    const bool move_dy = !gated && half && (dx || dweight) && !on_16(dy, lddy, N, size);
+    const bool move_w = half && dx && !on_16(weight, ldw, K, size), move_x = half && dweight && !on_16(x, ldx, K, size);
+    Back b{};
+    Carver c(ws, ws_bytes);
+    carve(c, b, dtype, M, N, K, gated ? GLIF_ACT_SILU : activation, move_dy || move_w || move_x);
+    if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "linear: workspace too small");
+    const void *dp = dy;
+    int64_t lddp = lddy, n_cols = N, k_cols = K;
+    const bool own_dp = gated || activation != GLIF_ACT_NONE || move_dy;
+    if (own_dp || dbias) {
+        SlopeArgs a{dy, pre, lddy, M, N, own_dp ? b.dp : nullptr, b.np, dbias ? b.sums : nullptr, activation, b.parts};
+        if (gated) {
+            a.N = N / 2;
+            if (N) GLIF_BY_DTYPE(dtype, run_gate_slope, a, s);   // sums of no rows are 0
+        } else {
+            GLIF_BY_DTYPE(dtype, run_slope, a, s);
+        }
+        if (own_dp) dp = b.dp, lddp = n_cols = b.np;
+        if (dbias && N)
+            hipLaunchKernelGGL(k_bias_join, dim3(static_cast<unsigned>(ceil_div(N, kSlopeCols))), dim3(kBlock), 0, s, b.sums, b.parts,
+                               N, dbias, bias_dtype);
+    }
+    if (dx) {
+        GemmArgs a{};
+        if (move_w) run_repack(weight, ldw, N, K, b.w, b.kp, s), weight = b.w, ldw = k_cols = b.kp;
+        a.p = dp, a.p_ld = lddp, a.q = weight, a.q_ld = ldw, a.M = a.p_rows = M, a.N = K, a.q_rows = k_cols, a.K = N, a.k_cols = n_cols;
+        a.c = dx;
+        if (int rc = GLIF_BY_DTYPE(dtype, gemm_rc, a, b.dx, b.part, s)) return rc;
+    }
+    if (dweight) {
+        GemmArgs a{};
+        k_cols = K;
+        if (move_x) run_repack(x, ldx, M, K, b.x, b.kp, s), x = b.x, ldx = k_cols = b.kp;
+        a.p = dp, a.p_ld = lddp, a.q = x, a.q_ld = ldx, a.M = N, a.p_rows = n_cols, a.N = K, a.q_rows = k_cols, a.K = a.k_cols = M;
+        a.c = dweight;
+        if (int rc = GLIF_BY_DTYPE(dtype, gemm_cc, a, b.dw, b.part, s)) return rc;
+    }
+    GLIF_HIP(hipGetLastError());
+    return GLIF_OK;
+}
+
 }  // namespace
 }  // namespace glif
 
@@ -982,48 +1313,50 @@ size_t glif_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K,
 int glif_linear_bwd(const void *dy, int64_t lddy, const float *pre, const void *x, int64_t ldx, const void *weight,
                     int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
                     void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream) {
-    if (int rc = check_linear(dtype, bias_dtype, M, N, K, activation)) return rc;
-    if (int rc = check_strides(lddy, ldx, ldw)) return rc;
-    const bool some = M && N;
-    if (some && (!dy || (activation != GLIF_ACT_NONE && !pre) || (dx && K && !weight) || (dweight && K && !x)))
-        return fail(GLIF_EINVAL, "NULL argument");
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const size_t size = dtype_size(dtype);
-    const bool half = size == 2;
-    const bool move_dy = half && (dx || dweight) && !on_16(dy, lddy, N, size);
-    const bool move_w = half && dx && !on_16(weight, ldw, K, size), move_x = half && dweight && !on_16(x, ldx, K, size);
-    Back b{};
+    return linear_bwd(false, dy, lddy, pre, x, ldx, weight, ldw, dtype, bias_dtype, M, N, K, activation, dx, dweight, dbias, ws,
+                      ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+size_t glif_gated_linear_fwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K) {
+    if (check_gated(dtype, dtype, M, N, K, 0, K)) return 0;
+    Carver c(nullptr, 0);
+    if (const size_t n = plan_for(dtype, M, turns(N), K, true, true).floats()) c.take<float>(n);
+    return c.off;
+}
+
+int glif_gated_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int32_t dtype,
+                          int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation, void *y, float *pre, void *ws,
+                          size_t ws_bytes, void *stream) {
+    if (int rc = check_gated(dtype, bias_dtype, M, N, K, activation, ldw)) return rc;
+    if (int rc = check_strides(ldx, ldw, 0)) return rc;
+    if (M == 0 || N == 0) return GLIF_OK;
+    if (!y || (K && (!x || !weight))) return fail(GLIF_EINVAL, "NULL argument");
+    GemmArgs a{};
+    a.p = x, a.p_ld = ldx, a.q = weight, a.q_ld = ldw, a.M = a.p_rows = M, a.N = a.q_rows = turns(N), a.K = a.k_cols = K;
+    a.c = y, a.pre = pre, a.bias = bias, a.bias_dt = bias_dtype, a.act = activation, a.half = a.outs = N;
+    const Plan p = plan_for(dtype, M, a.N, K, true, true);
     Carver c(ws, ws_bytes);
-    carve(c, b, dtype, M, N, K, activation, move_dy || move_w || move_x);
-    if (!c.ok() || (c.off && !ws)) return fail(GLIF_ENOMEM, "linear: workspace too small");
-    const void *dp = dy;
-    int64_t lddp = lddy, n_cols = N, k_cols = K;
-    const bool own_dp = activation != GLIF_ACT_NONE || move_dy;
-    if (own_dp || dbias) {
-        SlopeArgs a{dy, pre, lddy, M, N, own_dp ? b.dp : nullptr, b.np, dbias ? b.sums : nullptr, activation, b.parts};
-        GLIF_BY_DTYPE(dtype, run_slope, a, s);
-        if (own_dp) dp = b.dp, lddp = n_cols = b.np;
-        if (dbias && N)
-            hipLaunchKernelGGL(k_bias_join, dim3(static_cast<unsigned>(ceil_div(N, kSlopeCols))), dim3(kBlock), 0, s, b.sums, b.parts,
-                               N, dbias, bias_dtype);
-    }
-    if (dx) {
-        GemmArgs a{};
-        if (move_w) run_repack(weight, ldw, N, K, b.w, b.kp, s), weight = b.w, ldw = k_cols = b.kp;
-        a.p = dp, a.p_ld = lddp, a.q = weight, a.q_ld = ldw, a.M = a.p_rows = M, a.N = K, a.q_rows = k_cols, a.K = N, a.k_cols = n_cols;
-        a.c = dx;
-        if (int rc = GLIF_BY_DTYPE(dtype, gemm_rc, a, b.dx, b.part, s)) return rc;
-    }
-    if (dweight) {
-        GemmArgs a{};
-        k_cols = K;
-        if (move_x) run_repack(x, ldx, M, K, b.x, b.kp, s), x = b.x, ldx = k_cols = b.kp;
-        a.p = dp, a.p_ld = lddp, a.q = x, a.q_ld = ldx, a.M = N, a.p_rows = n_cols, a.N = K, a.q_rows = k_cols, a.K = a.k_cols = M;
-        a.c = dweight;
-        if (int rc = GLIF_BY_DTYPE(dtype, gemm_cc, a, b.dw, b.part, s)) return rc;
-    }
+    float *part = c.take<float>(p.floats());
+    if (!c.ok() || (p.floats() && !ws)) return fail(GLIF_ENOMEM, "linear: workspace too small");
+    if (int rc = GLIF_BY_DTYPE(dtype, gemm_gated, a, p, part, static_cast<hipStream_t>(stream))) return rc;
     GLIF_HIP(hipGetLastError());
     return GLIF_OK;
+}
+
+size_t glif_gated_linear_bwd_workspace(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t unaligned) {
+    if (check_gated(dtype, dtype, M, N, K, 0, K)) return 0;
+    Carver c(nullptr, 0);
+    Back b{};
+    carve(c, b, dtype, M, 2 * N, K, GLIF_ACT_SILU, unaligned != 0);
+    return c.mark();
+}
+
+int glif_gated_linear_bwd(const void *dy, int64_t lddy, const float *pre, const void *x, int64_t ldx, const void *weight,
+                          int64_t ldw, int32_t dtype, int32_t bias_dtype, int64_t M, int64_t N, int64_t K, int32_t activation,
+                          void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes, void *stream) {
+    if (int rc = check_gated(dtype, bias_dtype, M, N, K, activation, ldw)) return rc;
+    return linear_bwd(true, dy, lddy, pre, x, ldx, weight, ldw, dtype, bias_dtype, M, 2 * N, K, activation, dx, dweight, dbias, ws,
+                      ws_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -6,6 +6,7 @@ these are the operators of a trained readout over whole training windows and, ti
 * ``layer_norm``                                    over the last axis;
 * ``dropout``                                       its mask drawn from the Philox streams of ``inputs`` and never stored;
 * ``linear``                                        with bias, activation and residual in one kernel;
+* ``gated_linear``                                  both projections of a gated feed-forward block, activation and product;
 * ``short_conv``, ``short_conv_step``               a causal convolution of a few ticks per channel;
 * ``state_space_scan``, ``state_space_step``        a selective state space;
 * ``linear_attention``, ``linear_attention_step``   linear attention with a decay for each head.
@@ -27,7 +28,7 @@ from torch.autograd import forward_ad
 from . import _lib
 from ._lib import check, lib
 
-__all__ = ["layer_norm", "dropout", "linear", "short_conv", "short_conv_step", "state_space_scan", "state_space_step",
+__all__ = ["layer_norm", "dropout", "linear", "gated_linear", "short_conv", "short_conv_step", "state_space_scan", "state_space_step",
            "linear_attention", "linear_attention_step"]
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -329,6 +330,70 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias=None, activation=None, re
     if residual is not None:
         _need(residual, "residual", (*x.shape[:-1], N), x.dtype, x.device)
     return _apply(_Linear, _wants_grad(x, weight, bias, residual), x, weight, bias, residual, ACTIVATIONS[activation], bdt)
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, bdt):
+        N, K = weight.shape[0] // 2, weight.shape[1]
+        dt = DTYPES[x.dtype]
+        M = math.prod(x.shape[:-1])
+        xr, ldx = _rows(x, K) if K else (x, 0)
+        wr, ldw = _rows(weight, K) if K else (weight, 0)
+        b = _dense(bias)
+        y = x.new_empty((*x.shape[:-1], N))
+        pre = torch.empty((M, 2 * N), dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad[:3]) else None
+        L, dev = lib(), x.device
+        n = L.glif_gated_linear_fwd_workspace(dt, M, N, K)
+        ws = _workspace(n, dev)
+        with _on(dev):
+            check(L.glif_gated_linear_fwd(_p(xr), ldx, _p(wr), ldw, _p(b), dt, DTYPES[bdt], M, N, K, act, _p(y), _p(pre), _p(ws), n,
+                                          _stream(dev)))
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act, ctx.bdt, ctx.M = act, bdt, M
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _first_only("gated_linear")
+        x, weight, pre = ctx.saved_tensors
+        N, K = weight.shape[0] // 2, weight.shape[1]
+        M, dt, dev = ctx.M, DTYPES[x.dtype], x.device
+        xr, ldx = _rows(x, K) if K else (x, 0)
+        wr, ldw = _rows(weight, K) if K else (weight, 0)
+        gr, ldg = _rows(dy, N) if N else (dy, 0)
+        wx, ww, wb = ctx.needs_input_grad[:3]
+        dx = x.new_empty(x.shape) if wx else None
+        dw = x.new_empty((2 * N, K)) if ww else None
+        db = torch.empty(2 * N, dtype=ctx.bdt, device=dev) if wb else None
+        L, V = lib(), 16 // x.element_size()
+        px, pw = xr.data_ptr(), wr.data_ptr()
+        odd = (ldx % V or ldw % V or K % V or (px | pw) % 16) != 0
+        n = L.glif_gated_linear_bwd_workspace(dt, M, N, K, odd)
+        ws = _workspace(n, dev)
+        with _on(dev):
+            check(L.glif_gated_linear_bwd(_p(gr), ldg, _p(pre), px, ldx, pw, ldw, dt, DTYPES[ctx.bdt], M, N, K, ctx.act, _p(dx),
+                                          _p(dw), _p(db), _p(ws), n, _stream(dev)))
+        return dx, dw, db, None, None
+
+
+def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias=None, activation="silu") -> torch.Tensor:
+    """``act(x @ weight[:N].T + bias[:N]) * (x @ weight[N:].T + bias[N:])``: the first half of a gated feed-forward block, whose
+    second is a ``linear`` with the residual.  x [..., K], weight [2 N, K] of x's type, bias [2 N] float32 or of x's type;
+    ``activation``: None, "relu", "gelu" (the error function's) or "silu".
+
+    For the gradient both products are kept in float32; what reaches them is rounded to x's type for the products that give the
+    gradients of x and weight, as in ``linear``, and summed in float32 for the bias's."""
+    _activations(x, "x")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {[a for a in ACTIVATIONS]}, got {activation!r}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one axis")
+    _need(weight, "weight", (None, x.shape[-1]), x.dtype, x.device)
+    if weight.shape[0] % 2:
+        raise ValueError(f"weight must have an even number of rows, got {weight.shape[0]}")
+    bdt = _params(x, None, None, bias, (weight.shape[0],))
+    return _apply(_GatedLinear, _wants_grad(x, weight, bias), x, weight, bias, ACTIVATIONS[activation], bdt)
 
 
 # ----------------------------------------------------------------- short convolution ----
