@@ -9,8 +9,6 @@
 //   dk = F(v, dy, scale q; dS^T)                 lead 0, time backwards: the gradient of the last state comes undecayed to the
 //   dv = F(k, scale q, dy; dS)                   last tick, and what is left behind the first is dS0
 // No power is of a negative exponent, so no decay, 0 among them, can overflow.
-#include <type_traits>
-
 #include "mma.h"
 
 namespace glif {
@@ -61,12 +59,12 @@ struct Form<bf16> {
 };
 
 // kTicks x W of a sequence from memory to rows of LDS, in two steps.
-template <typename T, int W>
+template <typename T, int W, int NT>
 struct Tile {
     using F = Form<T>;
     using C = typename F::C;
     static constexpr int kV = kVecBytes16<T>, kRow = W * static_cast<int>(sizeof(C)) + 16, kBytes = F::kTicks * kRow;
-    static constexpr int kPieces = F::kTicks * W / kV, kN = (kPieces + kBlock - 1) / kBlock;
+    static constexpr int kPieces = F::kTicks * W / kV, kN = (kPieces + NT - 1) / NT;
     typedef Vec<T, kV> vec;
     vec r[kN];
 
@@ -74,7 +72,7 @@ struct Tile {
     __device__ __forceinline__ void load(const T *p, int64_t st, int64_t first, int step, int n, int c0, int d) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int u = threadIdx.x + i * kBlock, row = u / (W / kV), at = c0 + u % (W / kV) * kV;
+            const int u = threadIdx.x + i * NT, row = u / (W / kV), at = c0 + u % (W / kV) * kV;
             vec v = {};
             if (row < n && at < d) {
                 const T *q = p + (first + static_cast<int64_t>(row) * step) * st + at;
@@ -92,8 +90,8 @@ struct Tile {
     __device__ __forceinline__ void store(char *lds) const {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int u = threadIdx.x + i * kBlock;
-            if (kPieces % kBlock && u >= kPieces) break;
+            const int u = threadIdx.x + i * NT;
+            if (kPieces % NT && u >= kPieces) break;
             C *to = reinterpret_cast<C *>(lds + u / (W / kV) * kRow) + u % (W / kV) * kV;
             constexpr int kE = 16 / static_cast<int>(sizeof(C));
             typedef C out __attribute__((ext_vector_type(16 / sizeof(C))));
@@ -144,27 +142,28 @@ __device__ __forceinline__ typename Mma<C>::frag columns_of(const char *lds, int
 }
 #endif
 
-// A block takes one entry and head, 4 WC of c's channels and one segment of the ticks, chunk by chunk; each of its waves keeps
-// the state of its WC channels in registers, as a matrix product's result and the next one's operand (which of b's
-// channels a row of it is, is chosen so that a lane's values are kPer neighbours).  STATES: no outputs, only the state that
-// the segment adds to nothing.
-template <typename T, int D, int WC, bool STATES>
-__global__ void __launch_bounds__(kBlock, 2) k_attention(AttArgs args) {
+// A block takes one entry and head, 16 of c's channels a wave and one segment of the ticks, chunk by chunk; each wave keeps the
+// state of its channels in registers, as a matrix product's result and the next one's operand (which of b's channels a row of it
+// is, is chosen so that a lane's values are kPer neighbours).  STATES: no outputs, only the state that the segment adds to
+// nothing.
+template <typename T, int D, int NW, bool STATES>
+__global__ void __launch_bounds__(NW *kWave, NW == 8 ? 4 : 2) k_attention(AttArgs args) {
 #ifdef __HIP_DEVICE_COMPILE__
     using F = Form<T>;
     using C = typename F::C;
     using M = Mma<C>;
     typedef typename M::frag frag;
     constexpr int kTicks = F::kTicks, kStep = F::kStep, kPer = F::kPer, TI = kTicks / 16, KT = kTicks / kStep, KD = D / kStep;
-    constexpr int XT = D / 16, CT = WC / 16, GAP = kPer == 8 ? 8 : 4;
-    using TD = Tile<T, D>;
-    using TC = Tile<T, 4 * WC>;
-    constexpr int kRow = TD::kRow, kRowC = TC::kRow, kRowP = kTicks * static_cast<int>(sizeof(C)) + 16;
+    constexpr int NT = NW * kWave, W = NW * 16, XT = D / 16, GAP = kPer == 8 ? 8 : 4, kSize = static_cast<int>(sizeof(C));
+    using TD = Tile<T, D, NT>;
+    using TC = Tile<T, W, NT>;
+    constexpr int kRow = TD::kRow, kRowC = TC::kRow, kRowP = kTicks * kSize + 16;
     __shared__ __attribute__((aligned(16))) char lds_a[STATES ? 16 : TD::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_b[TD::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_c[TC::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * kRowP];
-    __shared__ int odd[2];   // whether c is not finite somewhere in this chunk, and in the next
+    __shared__ float weight[kTicks];   // of tick j in the state after the chunk
+    __shared__ int odd[2];             // whether c is not finite somewhere in this chunk, and in the next
 
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
     // The blocks that read the same sequences are on one XCD (block id mod 8), after each other.
@@ -174,12 +173,12 @@ __global__ void __launch_bounds__(kBlock, 2) k_attention(AttArgs args) {
     const AttPass &p = args.pass[slot % kin / args.tiles];
     const int tile = slot % args.tiles, seg = static_cast<int>(group % args.segments);
     const int bh = static_cast<int>(group / args.segments), b = bh / args.H, h = bh % args.H;
-    const int c0 = tile * 4 * WC, dc = p.c.d, db = p.b.d;
+    const int c0 = tile * W, dc = p.c.d, db = p.b.d;
     if (c0 >= dc) return;
     const int len = live_ticks(args.lengths, b, args.T);
     const int begin = min(seg * args.seg_ticks, len), end = min(begin + args.seg_ticks, len);
     const float rate = args.log_decay[h] * 1.4426950408889634f;
-    const int wc = c0 + wave * WC;       // the wave's first channel
+    const int wc = c0 + wave * 16;       // the wave's first channel
     const bool active = wc < dc;
 
     const T *pa = static_cast<const T *>(p.a.p) + b * p.a.sb + h / p.a.share * p.a.sh;
@@ -188,176 +187,77 @@ __global__ void __launch_bounds__(kBlock, 2) k_attention(AttArgs args) {
     const int64_t out_st = static_cast<int64_t>(args.B) * args.H * dc;
     const int64_t out_at = static_cast<int64_t>(bh) * dc;
 
-    // state: x[i][j][r] is of b's channel row(i) + r and c's channel wc + 16 j + r16
+    // state: x[i][r] is of b's channel row(i) + r and c's channel wc + r16
     auto row = [&](int i) { return kPer == 8 ? 32 * (i / 2) + 8 * kq + 4 * (i % 2) : 16 * i + 4 * kq; };
-    f32x4 x[XT][CT] = {};
-    auto at_state = [&](const float *q, int i, int j, int r) {
-        return q + seg * p.x_seg + bh * p.x_bh + (row(i) + r) * p.x_b + (wc + 16 * j + r16) * p.x_c;
+    f32x4 x[XT] = {};
+    auto at_state = [&](const float *q, int i, int r) {
+        return q + seg * p.x_seg + bh * p.x_bh + (row(i) + r) * p.x_b + (wc + r16) * p.x_c;
     };
     if (!STATES && p.x)
 #pragma unroll
         for (int i = 0; i < XT; ++i)
 #pragma unroll
-            for (int j = 0; j < CT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (row(i) + r < db && wc + 16 * j + r16 < dc) x[i][j][r] = *at_state(p.x, i, j, r);
+            for (int r = 0; r < 4; ++r)
+                if (row(i) + r < db && wc + r16 < dc) x[i][r] = *at_state(p.x, i, r);
 
     // decays within a 16 x 16 tile of scores (tick i in the lane, ticks j = 4 kq + r) on the diagonal and below it
-    float on[4], below[4], weight[KT][kPer];
+    float on[4], below[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int n = r16 - 4 * kq - r;
         on[r] = n < 0 ? 0.0f : power(rate, n) * p.in_scale;
         below[r] = power(rate, 16 + n) * p.in_scale;
     }
-    auto weigh = [&](int hi) {   // of tick j in a state after tick hi - 1
-#pragma unroll
-        for (int s = 0; s < KT; ++s)
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const int j = s * kStep + kq * kPer + e;
-                weight[s][e] = j < hi ? power(rate, hi - p.lead - j) * p.in_scale : 0.0f;
-            }
-    };
-    weigh(kTicks);
     if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
-        for (int u = threadIdx.x; u < kTicks * kRowP / 4; u += kBlock) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
+        for (int u = threadIdx.x; u < kTicks * kRowP / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
     }
     if (threadIdx.x < 2) odd[threadIdx.x] = 0;
 
     TD ra, rb;
     TC rc;
-    auto fetch = [&](int at) {
-        const int n = min(end - at, kTicks), step = p.back ? -1 : 1;
+    auto fetch = [&](int at, int n) {
+        const int step = p.back ? -1 : 1;
         const int64_t first = p.back ? len - 1 - at : at;
         if (!STATES) ra.load(pa, p.a.st, first, step, n, 0, p.a.d);
         rb.load(pb, p.b.st, first, step, n, 0, db);
         rc.load(pc, p.c.st, first, step, n, c0, dc);
     };
-    auto only = [&](frag &f, int s, int tick) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            if (s * kStep + kq * kPer + e != tick) f[e] = static_cast<C>(0.0f);
-    };
-    // Outputs of the ticks lo .. hi - 1 of the chunk at `at`, and the state after them; ONE: hi = lo + 1, and no other tick is
-    // multiplied with anything.
-    auto advance = [&](auto one, int at, int lo, int hi) {
-        constexpr bool ONE = decltype(one)::value;
-        frag fc[KT][CT];
-#pragma unroll
-        for (int s = 0; s < KT; ++s)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) {
-                fc[s][j] = columns_of<C, kRowC, 4>(lds_c, wave * WC + 16 * j, s * kStep, lane);
-                if (ONE) only(fc[s][j], s, lo);
-            }
-        if (!STATES && p.out) {
-            frag fx[KD][CT];
-#pragma unroll
-            for (int k = 0; k < KD; ++k)
-#pragma unroll
-                for (int j = 0; j < CT; ++j)
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e) fx[k][j][e] = static_cast<C>(x[k * (kPer / 4) + e / 4][j][e % 4]);
-#pragma unroll
-            for (int it = 0; it < TI; ++it) {
-                if (16 * it >= hi || 16 * it + 16 <= lo) continue;
-                f32x4 o[CT] = {};
-#pragma unroll
-                for (int k = 0; k < KD; ++k) {
-                    const frag fa = rows_of<C, kRow>(lds_a, 16 * it, k * kStep, lane);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) o[j] = M::run(fx[k][j], fa, o[j]);
-                }
-                const int i = 16 * it + r16;
-                const float f = power(rate, max(i - lo, 0) + p.lead);
-#pragma unroll
-                for (int j = 0; j < CT; ++j) o[j] *= f;
-#pragma unroll
-                for (int s = 0; s < KT; ++s) {
-                    if (s * kStep > 16 * it + 15) break;
-                    const frag fp = rows_of<C, kRowP>(lds_p, 16 * it, s * kStep, lane);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) o[j] = M::run(fc[s][j], fp, o[j]);
-                }
-                if (i < lo || i >= hi) continue;
-                const int64_t t = p.back ? len - 1 - at - i : at + i;
-#pragma unroll
-                for (int j = 0; j < CT; ++j) {
-                    const int ch = wc + 16 * j + 4 * kq, have = dc - ch;
-                    if (have <= 0) continue;
-                    const f32x4 v = o[j] * p.out_scale;
-                    const int64_t to = t * out_st + out_at + ch;
-                    if (p.wide) {
-                        float *q = static_cast<float *>(p.out) + to;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < have) q[e] = v[e];
-                    } else {
-                        T *q = static_cast<T *>(p.out) + to;
-                        if (have >= 4) {
-                            *reinterpret_cast<Vec<T, 4> *>(q) = __builtin_convertvector(v, Vec<T, 4>);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (e < have) q[e] = from_f32<T>(v[e]);
-                        }
-                    }
-                }
-            }
-        }
-        const float f = power(rate, hi - lo);
-#pragma unroll
-        for (int i = 0; i < XT; ++i)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) x[i][j] *= f;
-        // The state is float32, but what a matrix instruction multiplies is not: a weighted value is three bfloat16
-        // ones, 24 bits together.
-        constexpr int kParts = sizeof(C) == 2 ? 3 : 1;
-#pragma unroll
-        for (int s = 0; s < KT; ++s) {
-            frag part[CT][kParts];
-#pragma unroll
-            for (int j = 0; j < CT; ++j)
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    float v = static_cast<float>(fc[s][j][e]) * weight[s][e];
-#pragma unroll
-                    for (int q = 0; q < kParts; ++q) {
-                        part[j][q][e] = static_cast<C>(v);
-                        v -= static_cast<float>(part[j][q][e]);
-                    }
-                }
-#pragma unroll
-            for (int i = 0; i < XT; ++i) {
-                frag fb = columns_of<C, kRow, GAP>(lds_b, kPer == 8 ? 32 * (i / 2) + 4 * (i % 2) : 16 * i, s * kStep, lane);
-                if (ONE) only(fb, s, lo);
-#pragma unroll
-                for (int j = 0; j < CT; ++j)
-#pragma unroll
-                    for (int q = 0; q < kParts; ++q) x[i][j] = M::run(fb, part[j][q], x[i][j]);
-            }
-        }
-    };
-    if (begin < end) fetch(begin);
-    for (int at = begin, turn = 0; at < end; at += kTicks, turn ^= 1) {
-        const int n = min(end - at, kTicks);
+    // A product with a later tick's 0 is NaN where that tick's c is not finite: such a chunk is fetched again, as chunks of one
+    // tick, up to `careful`.
+    int weighed = 0, careful = begin;
+    if (begin < end) fetch(begin, min(end - begin, kTicks));
+    for (int at = begin, turn = 0; at < end;) {
+        const int n = at < careful ? 1 : min(end - at, kTicks);
         __syncthreads();   // the last chunk's tiles have been read
         if (!STATES) ra.store(lds_a);
         rb.store(lds_b);
         rc.store(lds_c);
-        if (!STATES && !rc.finite()) odd[turn] = 1;
+        if (n != weighed) {
+            if (threadIdx.x < kTicks) {
+                const int j = threadIdx.x;
+                weight[j] = j < n ? power(rate, n - p.lead - j) * p.in_scale : 0.0f;
+            }
+            weighed = n;
+        }
+        if (!STATES && n > 1 && !rc.finite()) odd[turn] = 1;
         if (threadIdx.x == 0) odd[turn ^ 1] = 0;
         __syncthreads();
-        if (at + kTicks < end) fetch(at + kTicks);
-        const bool single = !STATES && odd[turn] != 0;
+        if (!STATES) {
+            const bool again = odd[turn] != 0;
+            turn ^= 1;
+            if (again) {
+                careful = at + n;
+                fetch(at, 1);
+                continue;
+            }
+        }
+        const int here = at;
+        at += n;
+        if (at < end) fetch(at, at < careful ? 1 : min(end - at, kTicks));
         if (!STATES) {
             // scores: rows j, columns i
-#pragma unroll
-            for (int u = 0; u < TI * TI / 4; ++u) {
-                const int it = TI == 4 ? wave : wave / 2, jt = TI == 4 ? u : wave % 2;
-                if (jt > it) continue;
+            for (int u = wave; u < TI * (TI + 1) / 2; u += NW) {
+                const int it = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, jt = u - it * (it + 1) / 2;
                 f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < KD; ++k)
@@ -370,26 +270,86 @@ __global__ void __launch_bounds__(kBlock, 2) k_attention(AttArgs args) {
                     const float f = it == jt ? (4 * kq + r <= r16 ? s[r] * on[r] : 0.0f) : s[r] * below[r] * far;
                     o[r] = static_cast<C>(f);
                 }
-                *reinterpret_cast<four *>(lds_p + (16 * it + r16) * kRowP + (16 * jt + 4 * kq) * static_cast<int>(sizeof(C))) = o;
+                *reinterpret_cast<four *>(lds_p + (16 * it + r16) * kRowP + (16 * jt + 4 * kq) * kSize) = o;
             }
             __syncthreads();
         }
         if (!active) continue;
-        // A product with a later tick's 0 is NaN where that tick's c is not finite: such a chunk goes tick by tick.
-        if (single) {
-            for (int i = 0; i < n; ++i) {
-                weigh(i + 1);
-                advance(std::true_type{}, at, i, i + 1);
+        frag fc[KT];
+#pragma unroll
+        for (int s = 0; s < KT; ++s) fc[s] = columns_of<C, kRowC, 4>(lds_c, wave * 16, s * kStep, lane);
+        if (!STATES && p.out) {
+            // rows c's channels, columns i
+            f32x4 o[TI] = {};
+#pragma unroll
+            for (int k = 0; k < KD; ++k) {
+                frag fx;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) fx[e] = static_cast<C>(x[k * (kPer / 4) + e / 4][e % 4]);
+#pragma unroll
+                for (int it = 0; it < TI; ++it) o[it] = M::run(fx, rows_of<C, kRow>(lds_a, 16 * it, k * kStep, lane), o[it]);
             }
-        } else {
-            if (n < kTicks) weigh(n);
-            advance(std::false_type{}, at, 0, n);
+#pragma unroll
+            for (int it = 0; it < TI; ++it) o[it] *= power(rate, 16 * it + r16 + p.lead);
+#pragma unroll
+            for (int s = 0; s < KT; ++s)
+#pragma unroll
+                for (int it = 0; it < TI; ++it)
+                    if (s * kStep <= 16 * it + 15) o[it] = M::run(fc[s], rows_of<C, kRowP>(lds_p, 16 * it, s * kStep, lane), o[it]);
+#pragma unroll
+            for (int it = 0; it < TI; ++it) {
+                const int i = 16 * it + r16, ch = wc + 4 * kq, have = dc - ch;
+                if (i >= n || have <= 0) continue;
+                const int64_t tick = p.back ? len - 1 - here - i : here + i;
+                const f32x4 v = o[it] * p.out_scale;
+                const int64_t to = tick * out_st + out_at + ch;
+                if (p.wide) {
+                    float *q = static_cast<float *>(p.out) + to;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < have) q[e] = v[e];
+                } else {
+                    T *q = static_cast<T *>(p.out) + to;
+                    if (have >= 4) {
+                        *reinterpret_cast<Vec<T, 4> *>(q) = __builtin_convertvector(v, Vec<T, 4>);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (e < have) q[e] = from_f32<T>(v[e]);
+                    }
+                }
+            }
+        }
+        const float f = power(rate, n);
+#pragma unroll
+        for (int i = 0; i < XT; ++i) x[i] *= f;
+        // The state is float32, but what a matrix instruction multiplies is not: a weighted value is three bfloat16 ones, 24
+        // bits together.
+        constexpr int kParts = kSize == 2 ? 3 : 1;
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+            frag part[kParts];
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                float v = static_cast<float>(fc[s][e]) * weight[s * kStep + kq * kPer + e];
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    part[q][e] = static_cast<C>(v);
+                    v -= static_cast<float>(part[q][e]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < XT; ++i) {
+                const frag fb = columns_of<C, kRow, GAP>(lds_b, kPer == 8 ? 32 * (i / 2) + 4 * (i % 2) : 16 * i, s * kStep, lane);
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) x[i] = M::run(fb, part[q], x[i]);
+            }
         }
     }
     // Ticks behind the length are 0.
     if (!STATES && p.out) {
-        const int t0 = max(len, seg * args.seg_ticks), t1 = min(args.T, (seg + 1) * args.seg_ticks), w = min(4 * WC, dc - c0);
-        for (int u = threadIdx.x; u < (t1 - t0) * w; u += kBlock) {
+        const int t0 = max(len, seg * args.seg_ticks), t1 = min(args.T, (seg + 1) * args.seg_ticks), w = min(W, dc - c0);
+        for (int u = threadIdx.x; u < (t1 - t0) * w; u += NT) {
             const int64_t to = (t0 + u / w) * out_st + out_at + c0 + u % w;
             if (p.wide) static_cast<float *>(p.out)[to] = 0.0f;
             else static_cast<T *>(p.out)[to] = T(0.0f);
@@ -399,10 +359,8 @@ __global__ void __launch_bounds__(kBlock, 2) k_attention(AttArgs args) {
 #pragma unroll
         for (int i = 0; i < XT; ++i)
 #pragma unroll
-            for (int j = 0; j < CT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (row(i) + r < db && wc + 16 * j + r16 < dc) *const_cast<float *>(at_state(p.x_out, i, j, r)) = x[i][j][r];
+            for (int r = 0; r < 4; ++r)
+                if (row(i) + r < db && wc + r16 < dc) *const_cast<float *>(at_state(p.x_out, i, r)) = x[i][r];
 #endif
 }
 
@@ -444,15 +402,15 @@ __global__ void __launch_bounds__(kBlock) k_attention_share(const float *in, int
     }
 }
 
-template <typename T, int D, int WC>
+template <typename T, int D, int NW>
 void run_pass(AttArgs a, bool states, hipStream_t s) {
     int widest = 0;
     for (int i = 0; i < a.passes; ++i) widest = std::max(widest, a.pass[i].c.d);
-    a.tiles = ceil_div(widest, 4 * WC);
+    a.tiles = ceil_div(widest, 16 * NW);
     const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
-    const dim3 grid(static_cast<unsigned>(groups * a.tiles * a.passes));
-    if (states) hipLaunchKernelGGL((k_attention<T, D, WC, true>), grid, dim3(kBlock), 0, s, a);
-    else hipLaunchKernelGGL((k_attention<T, D, WC, false>), grid, dim3(kBlock), 0, s, a);
+    const dim3 grid(static_cast<unsigned>(groups * a.tiles * a.passes)), block(NW * kWave);
+    if (states) hipLaunchKernelGGL((k_attention<T, D, NW, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_attention<T, D, NW, false>), grid, block, 0, s, a);
 }
 
 template <typename T>
@@ -460,13 +418,13 @@ void run_passes(const AttArgs &a, bool states, hipStream_t s) {
     int da = 0, dc = 0;
     for (int i = 0; i < a.passes; ++i) da = std::max(da, a.pass[i].b.d), dc = std::max(dc, a.pass[i].c.d);
     if (dc <= 64) {
-        if (da <= 32) run_pass<T, 32, 16>(a, states, s);
-        else if (da <= 64) run_pass<T, 64, 16>(a, states, s);
-        else run_pass<T, 128, 16>(a, states, s);
+        if (da <= 32) run_pass<T, 32, 4>(a, states, s);
+        else if (da <= 64) run_pass<T, 64, 4>(a, states, s);
+        else run_pass<T, 128, 4>(a, states, s);
     } else {
-        if (da <= 32) run_pass<T, 32, 32>(a, states, s);
-        else if (da <= 64) run_pass<T, 64, 32>(a, states, s);
-        else run_pass<T, 128, 32>(a, states, s);
+        if (da <= 32) run_pass<T, 32, 8>(a, states, s);
+        else if (da <= 64) run_pass<T, 64, 8>(a, states, s);
+        else run_pass<T, 128, 8>(a, states, s);
     }
 }
 
