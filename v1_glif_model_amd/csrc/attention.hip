@@ -9,6 +9,8 @@
 //   dk = F(v, dy, scale q; dS^T)                 lead 0, time backwards: the gradient of the last state comes undecayed to the
 //   dv = F(k, scale q, dy; dS)                   last tick, and what is left behind the first is dS0
 // No power is of a negative exponent, so no decay, 0 among them, can overflow.
+#include <type_traits>
+
 #include "mma.h"
 
 namespace glif {
@@ -44,6 +46,9 @@ __device__ __forceinline__ float power(float rate, int n) { return n == 0 ? 1.0f
 
 __device__ __forceinline__ int live_ticks(const int32_t *lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+
 #ifdef __HIP_DEVICE_COMPILE__   // the host's pass does not know the builtins
 // 16-bit products of bfloat16, and float32 ones for float32 and for float16: states and scores of float16 sequences do not
 // stay within its range.
@@ -58,96 +63,177 @@ struct Form<bf16> {
     static constexpr int kTicks = 64, kStep = 32, kPer = 8;
 };
 
-// kTicks x W of a sequence from memory to rows of LDS, in two steps.
-template <typename T, int W, int NT>
+// Rows of W values in LDS.  16-bit ones are read by 16 rows of the same 16 bytes, and, turned, by four rows of 8 bytes from each
+// of four neighbouring 16: the 16-byte pieces of a row are permuted so that either goes to all banks.  float32 rows are 16 bytes
+// apart for the first, and their columns lie apart anyway.
+template <typename C, int W>
+struct Rows {
+    static constexpr bool kTurned = sizeof(C) == 2;
+    static constexpr int kSize = static_cast<int>(sizeof(C)), kBytes = W * kSize + (kTurned ? 0 : 16);
+    static __device__ __forceinline__ int key(int row) {
+        return !kTurned ? 0 : W == 128 ? (row & 3) << 2 | (row >> 2 & 3) : W == 64 ? (row & 2) << 1 | (row >> 2 & 3) : row >> 2 & 3;
+    }
+    // of value i of a row
+    static __device__ __forceinline__ int at(int row, int i) {
+        const int byte = i * kSize;
+        return row * kBytes + ((byte >> 4 ^ key(row)) << 4 | (byte & 15));
+    }
+    // Operands: lane l holds row l % 16 and the 16 bytes' terms from the (l / 16)th on.
+    static __device__ __forceinline__ typename Mma<C>::frag rows(const char *lds, int row0, int k0, int lane) {
+        return *reinterpret_cast<const typename Mma<C>::frag *>(lds + at(row0 + lane % 16, k0 + lane / 16 * (16 / kSize)));
+    }
+    // Columns as rows, rows k0, .. as terms.  Four columns from each of c0, c0 + GAP, c0 + 2 GAP and c0 + 3 GAP.
+    template <int GAP>
+    static __device__ __forceinline__ typename Mma<C>::frag columns(const char *lds, int c0, int k0, int lane) {
+        const int r16 = lane % 16, kq = lane / 16;
+        if constexpr (kTurned) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s4 *l4;
+            const int row = k0 + 8 * kq + (r16 >> 2), col = c0 + (r16 & 3) * GAP;
+            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(lds + at(row, col)));
+            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(lds + at(row + 4, col)));
+            return __builtin_bit_cast(typename Mma<C>::frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            static_assert(GAP == 4, "columns in order");
+            typename Mma<C>::frag v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const C *>(lds + at(k0 + 4 * kq + e, c0 + r16));
+            return v;
+        }
+    }
+};
+
+// kTicks x W of a sequence from memory to rows of LDS, in two steps: thread by thread the same 16 bytes of rows kRows apart, so
+// that of a whole chunk of whole rows one address and nothing else is a lane's.  No load waits for a condition: ticks and
+// channels that are not there repeat others, and are put away as zeros (channels never: init() clears them).
+// WHOLE: all W channels are there.
+template <typename T, int W, int NT, bool WHOLE>
 struct Tile {
     using F = Form<T>;
     using C = typename F::C;
-    static constexpr int kV = kVecBytes16<T>, kRow = W * static_cast<int>(sizeof(C)) + 16, kBytes = F::kTicks * kRow;
-    static constexpr int kPieces = F::kTicks * W / kV, kN = (kPieces + NT - 1) / NT;
+    static constexpr int kSize = static_cast<int>(sizeof(T)), kV = kVecBytes16<T>;
+    using R = Rows<C, W>;
+    static constexpr int kBytes = F::kTicks * R::kBytes, kAcross = W / kV, kRows = NT / kAcross, kN = (F::kTicks + kRows - 1) / kRows;
+    static_assert(NT % kAcross == 0, "a thread keeps to its channels");
     typedef Vec<T, kV> vec;
     vec r[kN];
+    const char *base;     // of the sequence's channels
+    int64_t step;         // bytes from a tick to the next, in their order
+    int row, at;          // the thread's first row and channel
+    int d;                // channels
+    uint32_t off;         // its first bytes in a whole chunk, from the lowest tick
 
-    // ticks `first`, first + step, ...: n of them; channels from c0 on, of which there are d
-    __device__ __forceinline__ void load(const T *p, int64_t st, int64_t first, int step, int n, int c0, int d) {
+    static __device__ __forceinline__ int least(int a, int b) { return a < b ? a : b; }
+    // the first channel that is read: the last piece is moved back to end with them
+    __device__ __forceinline__ int from() const { return WHOLE ? at : d < kV ? 0 : least(at, d - kV); }
+
+    __device__ __forceinline__ void init(char *lds, const T *p, int64_t st, bool back, int channels) {
+        base = reinterpret_cast<const char *>(p), step = back ? -st * kSize : st * kSize, d = channels;
+        row = threadIdx.x / kAcross, at = threadIdx.x % kAcross * kV;
+        const int first = least(row, F::kTicks - 1);
+        off = static_cast<uint32_t>(back ? F::kTicks - 1 - first : first) * static_cast<uint32_t>(st * kSize) + static_cast<uint32_t>(from() * kSize);
+        for (int u = threadIdx.x; u < kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds)[u] = 0u;
+    }
+    // n ticks, the first of them `first`
+    __device__ __forceinline__ void load(int64_t first, int n) {
+        const bool back = step < 0;
+        const int64_t apart = back ? -step : step;
+        const char *low = base + (back ? first - (n - 1) : first) * apart;
+        if (n == F::kTicks && (WHOLE || d >= kV)) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                r[i] = *reinterpret_cast<const vec *>(low + i * kRows * step + off);
+            }
+            return;
+        }
+        int mine = row;
+        asm volatile("" : "+v"(mine));   // what follows is for the few other chunks: it must not take registers of the loop
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int u = threadIdx.x + i * NT, row = u / (W / kV), at = c0 + u % (W / kV) * kV;
-            vec v = {};
-            if (row < n && at < d) {
-                const T *q = p + (first + static_cast<int64_t>(row) * step) * st + at;
-                if (at + kV <= d) {
-                    v = *reinterpret_cast<const vec *>(q);
-                } else {
+            const int at_row = least(mine + i * kRows, n - 1);
+            const char *q = low + (static_cast<uint32_t>(back ? n - 1 - at_row : at_row) * static_cast<uint32_t>(apart) + static_cast<uint32_t>(from() * kSize));
+            if (WHOLE || d >= kV) {
+                r[i] = *reinterpret_cast<const vec *>(q);
+            } else {
 #pragma unroll
-                    for (int e = 0; e < kV; ++e)
-                        if (at + e < d) v[e] = q[e];
-                }
+                for (int e = 0; e < kV; ++e) r[i][e] = e < d ? reinterpret_cast<const T *>(q)[least(e, d - 1)] : T(0.0f);
             }
-            r[i] = v;
         }
     }
-    __device__ __forceinline__ void store(char *lds) const {
+    __device__ __forceinline__ void store(char *lds, int n) const {
+        constexpr int kE = 16 / static_cast<int>(sizeof(C));
+        typedef C out __attribute__((ext_vector_type(16 / sizeof(C))));
+        if (n == F::kTicks && (WHOLE || d == W)) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                if (kN * kRows > F::kTicks && row + i * kRows >= F::kTicks) break;
+#pragma unroll
+                for (int s = 0; s < kV / kE; ++s) {
+                    out o;
+#pragma unroll
+                    for (int e = 0; e < kE; ++e) o[e] = static_cast<C>(r[i][s * kE + e]);
+                    *reinterpret_cast<out *>(lds + R::at(row + i * kRows, at + s * kE)) = o;
+                }
+            }
+            return;
+        }
+        int mine = row;
+        asm volatile("" : "+v"(mine));
+        // the piece that was moved back moves on again; behind the channels are zeros
+        const int bits = WHOLE ? 0 : least(at - from(), kV) * kSize * 8;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int u = threadIdx.x + i * NT;
-            if (kPieces % NT && u >= kPieces) break;
-            C *to = reinterpret_cast<C *>(lds + u / (W / kV) * kRow) + u % (W / kV) * kV;
-            constexpr int kE = 16 / static_cast<int>(sizeof(C));
-            typedef C out __attribute__((ext_vector_type(16 / sizeof(C))));
+            const int to_row = mine + i * kRows;
+            if (kN * kRows > F::kTicks && to_row >= F::kTicks) break;
+            u64x2 w = __builtin_bit_cast(u64x2, r[i]);
+            if (bits >= 128 || to_row >= n) w = u64x2{0, 0};
+            else if (bits >= 64) w = u64x2{w[1] >> (bits - 64), 0};
+            else if (bits > 0) w = u64x2{w[0] >> bits | w[1] << (64 - bits), w[1] >> bits};
+            const vec v = __builtin_bit_cast(vec, w);
 #pragma unroll
             for (int s = 0; s < kV / kE; ++s) {
                 out o;
 #pragma unroll
-                for (int e = 0; e < kE; ++e) o[e] = static_cast<C>(r[i][s * kE + e]);
-                *reinterpret_cast<out *>(to + s * kE) = o;
+                for (int e = 0; e < kE; ++e) o[e] = static_cast<C>(v[s * kE + e]);
+                *reinterpret_cast<out *>(lds + R::at(to_row, at + s * kE)) = o;
             }
         }
     }
     __device__ __forceinline__ bool finite() const {
-        bool f = true;
+        if constexpr (kSize == 2) {
+            typedef uint16_t pair __attribute__((ext_vector_type(2)));
+            pair most = {0, 0};
 #pragma unroll
-        for (int i = 0; i < kN; ++i)
+            for (int i = 0; i < kN; ++i) {
+                const u32x4 w = __builtin_bit_cast(u32x4, r[i]);
 #pragma unroll
-            for (int e = 0; e < kV; ++e) f = f && fabsf(to_f32(static_cast<T>(r[i][e]))) < __builtin_inff();
-        return f;
+                for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(pair, w[e] & 0x7fff7fffu));
+            }
+            const uint16_t inf = std::is_same_v<T, bf16> ? 0x7f80 : 0x7c00;
+            return (most[0] > most[1] ? most[0] : most[1]) < inf;
+        } else {
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int e = 0; e < kV; ++e) {
+                    const uint32_t w = __builtin_bit_cast(uint32_t, static_cast<float>(r[i][e])) & 0x7fffffffu;
+                    most = most > w ? most : w;
+                }
+            return most < 0x7f800000u;
+        }
     }
 };
 
-// Operands: lane l holds row l % 16 and the kPer terms from kPer (l / 16) on.
-template <typename C, int ROW>
-__device__ __forceinline__ typename Mma<C>::frag rows_of(const char *lds, int row0, int k0, int lane) {
-    constexpr int kPer = 16 / static_cast<int>(sizeof(C));
-    return *reinterpret_cast<const typename Mma<C>::frag *>(lds + (row0 + lane % 16) * ROW + (k0 + lane / 16 * kPer) * static_cast<int>(sizeof(C)));
-}
-
-// The tile's columns as rows, its ticks k0, .. as terms.  Four columns from each of c0, c0 + GAP, c0 + 2 GAP and c0 + 3 GAP.
-template <typename C, int ROW, int GAP>
-__device__ __forceinline__ typename Mma<C>::frag columns_of(const char *lds, int c0, int k0, int lane) {
-    const int r16 = lane % 16, kq = lane / 16;
-    if constexpr (sizeof(C) == 2) {
-        typedef short s4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s4 *l4;
-        const char *p = lds + (k0 + 8 * kq + (r16 >> 2)) * ROW + (c0 + (r16 & 3) * GAP) * 2;
-        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(p));
-        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4)(p + 4 * ROW));
-        return __builtin_bit_cast(typename Mma<C>::frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    } else {
-        static_assert(GAP == 4, "columns in order");
-        typename Mma<C>::frag v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const C *>(lds + (k0 + 4 * kq + e) * ROW + (c0 + r16) * 4);
-        return v;
-    }
-}
 #endif
 
 // A block takes one entry and head, 16 of c's channels a wave and one segment of the ticks, chunk by chunk; each wave keeps the
 // state of its channels in registers, as a matrix product's result and the next one's operand (which of b's channels a row of it
 // is, is chosen so that a lane's values are kPer neighbours).  STATES: no outputs, only the state that the segment adds to
 // nothing.
-template <typename T, int D, int NW, bool STATES>
-__global__ void __launch_bounds__(NW *kWave, NW == 8 ? 4 : 2) k_attention(AttArgs args) {
+// WHOLE: all heads have D channels in b and 16 NW in c, and outputs are of type T.
+template <typename T, int D, int NW, bool STATES, bool WHOLE>
+__global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
 #ifdef __HIP_DEVICE_COMPILE__
     using F = Form<T>;
     using C = typename F::C;
@@ -155,14 +241,16 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 ? 4 : 2) k_attention(AttArg
     typedef typename M::frag frag;
     constexpr int kTicks = F::kTicks, kStep = F::kStep, kPer = F::kPer, TI = kTicks / 16, KT = kTicks / kStep, KD = D / kStep;
     constexpr int NT = NW * kWave, W = NW * 16, XT = D / 16, GAP = kPer == 8 ? 8 : 4, kSize = static_cast<int>(sizeof(C));
-    using TD = Tile<T, D, NT>;
-    using TC = Tile<T, W, NT>;
-    constexpr int kRow = TD::kRow, kRowC = TC::kRow, kRowP = kTicks * kSize + 16;
+    using TD = Tile<T, D, NT, WHOLE>;
+    using TC = Tile<T, W, NT, WHOLE>;
+    using RD = Rows<C, D>;
+    using RC = Rows<C, W>;
+    using RP = Rows<C, kTicks>;
     __shared__ __attribute__((aligned(16))) char lds_a[STATES ? 16 : TD::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_b[TD::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_c[TC::kBytes];
-    __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * kRowP];
-    __shared__ float weight[kTicks];   // of tick j in the state after the chunk
+    __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * RP::kBytes];
+    __shared__ __attribute__((aligned(32))) float weight[kTicks];   // of tick j in the state after the chunk
     __shared__ int odd[2];             // whether c is not finite somewhere in this chunk, and in the next
 
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
@@ -170,72 +258,85 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 ? 4 : 2) k_attention(AttArg
     const int kin = args.tiles * args.passes, slot = static_cast<int>(blockIdx.x >> 3);
     const int64_t group = static_cast<int64_t>(slot / kin) * 8 + (blockIdx.x & 7);
     if (group >= static_cast<int64_t>(args.B) * args.H * args.segments) return;
-    const AttPass &p = args.pass[slot % kin / args.tiles];
+    const AttPass &pass = args.pass[slot % kin / args.tiles];
     const int tile = slot % args.tiles, seg = static_cast<int>(group % args.segments);
     const int bh = static_cast<int>(group / args.segments), b = bh / args.H, h = bh % args.H;
-    const int c0 = tile * W, dc = p.c.d, db = p.b.d;
+    const int c0 = WHOLE ? 0 : tile * W, dc = WHOLE ? W : pass.c.d, db = WHOLE ? D : pass.b.d;
     if (c0 >= dc) return;
-    const int len = live_ticks(args.lengths, b, args.T);
-    const int begin = min(seg * args.seg_ticks, len), end = min(begin + args.seg_ticks, len);
+    const int T_ = args.T, len = live_ticks(args.lengths, b, T_), seg_first = seg * args.seg_ticks, seg_end = min(T_, seg_first + args.seg_ticks);
+    const int begin = min(seg_first, len), end = min(seg_end, len);
     const float rate = args.log_decay[h] * 1.4426950408889634f;
     const int wc = c0 + wave * 16;       // the wave's first channel
-    const bool active = wc < dc;
-
-    const T *pa = static_cast<const T *>(p.a.p) + b * p.a.sb + h / p.a.share * p.a.sh;
-    const T *pb = static_cast<const T *>(p.b.p) + b * p.b.sb + h / p.b.share * p.b.sh;
-    const T *pc = static_cast<const T *>(p.c.p) + b * p.c.sb + h / p.c.share * p.c.sh;
+    const bool active = wc < dc, back = pass.back, wide = !WHOLE && pass.wide;
+    const int lead = pass.lead;
+    const float in_scale = pass.in_scale, out_scale = pass.out_scale;
     const int64_t out_st = static_cast<int64_t>(args.B) * args.H * dc;
-    const int64_t out_at = static_cast<int64_t>(bh) * dc;
+    // out: the lane's four channels of tick r16, in ticks from the segment's first
+    void *const out = pass.out;
+    const int64_t out_lane = static_cast<int64_t>(bh) * dc + wc + 4 * kq;
+    const int have = dc - wc - 4 * kq;
+
+    TD ra, rb;
+    TC rc;
+    if (!STATES) ra.init(lds_a, static_cast<const T *>(pass.a.p) + b * pass.a.sb + h / pass.a.share * pass.a.sh, pass.a.st, back, db);
+    rb.init(lds_b, static_cast<const T *>(pass.b.p) + b * pass.b.sb + h / pass.b.share * pass.b.sh, pass.b.st, back, db);
+    rc.init(lds_c, static_cast<const T *>(pass.c.p) + b * pass.c.sb + h / pass.c.share * pass.c.sh + c0, pass.c.st, back, min(dc - c0, W));
+    auto fetch = [&](int at, int n) {
+        const int64_t first = back ? len - 1 - at : at;
+        if (!STATES) ra.load(first, n);
+        rb.load(first, n);
+        rc.load(first, n);
+    };
+    if (begin < end) fetch(begin, min(end - begin, kTicks));
 
     // state: x[i][r] is of b's channel row(i) + r and c's channel wc + r16
     auto row = [&](int i) { return kPer == 8 ? 32 * (i / 2) + 8 * kq + 4 * (i % 2) : 16 * i + 4 * kq; };
     f32x4 x[XT] = {};
-    auto at_state = [&](const float *q, int i, int r) {
-        return q + seg * p.x_seg + bh * p.x_bh + (row(i) + r) * p.x_b + (wc + r16) * p.x_c;
-    };
-    if (!STATES && p.x)
+    if (!STATES && pass.x && active) {
+        const int64_t x_b = pass.x_b;
+        const float *from = pass.x + seg * pass.x_seg + bh * pass.x_bh + min(wc + r16, dc - 1) * pass.x_c;
+#pragma unroll
+        for (int i = 0; i < XT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[i][r] = from[min(row(i) + r, db - 1) * x_b];
 #pragma unroll
         for (int i = 0; i < XT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (row(i) + r < db && wc + r16 < dc) x[i][r] = *at_state(p.x, i, r);
+                if (row(i) + r >= db || wc + r16 >= dc) x[i][r] = 0.0f;
+    }
 
     // decays within a 16 x 16 tile of scores (tick i in the lane, ticks j = 4 kq + r) on the diagonal and below it
     float on[4], below[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int n = r16 - 4 * kq - r;
-        on[r] = n < 0 ? 0.0f : power(rate, n) * p.in_scale;
-        below[r] = power(rate, 16 + n) * p.in_scale;
+        on[r] = n < 0 ? 0.0f : power(rate, n) * in_scale * out_scale;
+        below[r] = power(rate, 16 + n) * in_scale * out_scale;
     }
     if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
-        for (int u = threadIdx.x; u < kTicks * kRowP / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
+        for (int u = threadIdx.x; u < kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
     }
     if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+    float across[TI];   // decays of the state in tick 16 it + r16
+#pragma unroll
+    for (int it = 0; it < TI; ++it) across[it] = power(rate, 16 * it + r16 + lead) * out_scale;
 
-    TD ra, rb;
-    TC rc;
-    auto fetch = [&](int at, int n) {
-        const int step = p.back ? -1 : 1;
-        const int64_t first = p.back ? len - 1 - at : at;
-        if (!STATES) ra.load(pa, p.a.st, first, step, n, 0, p.a.d);
-        rb.load(pb, p.b.st, first, step, n, 0, db);
-        rc.load(pc, p.c.st, first, step, n, c0, dc);
-    };
     // A product with a later tick's 0 is NaN where that tick's c is not finite: such a chunk is fetched again, as chunks of one
     // tick, up to `careful`.
     int weighed = 0, careful = begin;
-    if (begin < end) fetch(begin, min(end - begin, kTicks));
     for (int at = begin, turn = 0; at < end;) {
         const int n = at < careful ? 1 : min(end - at, kTicks);
+        int l = lane;
+        asm volatile("" : "+v"(l));   // addresses are made again for every chunk rather than kept, which would take more registers than there are
         __syncthreads();   // the last chunk's tiles have been read
-        if (!STATES) ra.store(lds_a);
-        rb.store(lds_b);
-        rc.store(lds_c);
+        if (!STATES) ra.store(lds_a, n);
+        rb.store(lds_b, n);
+        rc.store(lds_c, n);
         if (n != weighed) {
             if (threadIdx.x < kTicks) {
                 const int j = threadIdx.x;
-                weight[j] = j < n ? power(rate, n - p.lead - j) * p.in_scale : 0.0f;
+                weight[j] = j < n ? power(rate, n - lead - j) * in_scale : 0.0f;
             }
             weighed = n;
         }
@@ -261,7 +362,7 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 ? 4 : 2) k_attention(AttArg
                 f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < KD; ++k)
-                    s = M::run(rows_of<C, kRow>(lds_b, 16 * jt, k * kStep, lane), rows_of<C, kRow>(lds_a, 16 * it, k * kStep, lane), s);
+                    s = M::run(RD::rows(lds_b, 16 * jt, k * kStep, l), RD::rows(lds_a, 16 * it, k * kStep, l), s);
                 typedef C four __attribute__((ext_vector_type(4)));
                 four o;
                 const float far = it == jt ? 1.0f : power(rate, 16 * (it - jt - 1));
@@ -270,52 +371,47 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 ? 4 : 2) k_attention(AttArg
                     const float f = it == jt ? (4 * kq + r <= r16 ? s[r] * on[r] : 0.0f) : s[r] * below[r] * far;
                     o[r] = static_cast<C>(f);
                 }
-                *reinterpret_cast<four *>(lds_p + (16 * it + r16) * kRowP + (16 * jt + 4 * kq) * kSize) = o;
+                *reinterpret_cast<four *>(lds_p + RP::at(16 * it + r16, 16 * jt + 4 * kq)) = o;
             }
             __syncthreads();
         }
         if (!active) continue;
         frag fc[KT];
 #pragma unroll
-        for (int s = 0; s < KT; ++s) fc[s] = columns_of<C, kRowC, 4>(lds_c, wave * 16, s * kStep, lane);
-        if (!STATES && p.out) {
+        for (int s = 0; s < KT; ++s) fc[s] = RC::template columns<4>(lds_c, wave * 16, s * kStep, l);
+        if (!STATES && out) {
             // rows c's channels, columns i
             f32x4 o[TI] = {};
 #pragma unroll
             for (int k = 0; k < KD; ++k) {
                 frag fx;
+                if constexpr (kPer == 8) fx = __builtin_convertvector(__builtin_shufflevector(x[2 * k], x[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), frag);
+                else fx = x[k];
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) fx[e] = static_cast<C>(x[k * (kPer / 4) + e / 4][e % 4]);
-#pragma unroll
-                for (int it = 0; it < TI; ++it) o[it] = M::run(fx, rows_of<C, kRow>(lds_a, 16 * it, k * kStep, lane), o[it]);
+                for (int it = 0; it < TI; ++it) o[it] = M::run(fx, RD::rows(lds_a, 16 * it, k * kStep, l), o[it]);
             }
 #pragma unroll
-            for (int it = 0; it < TI; ++it) o[it] *= power(rate, 16 * it + r16 + p.lead);
+            for (int it = 0; it < TI; ++it) o[it] *= across[it];
 #pragma unroll
             for (int s = 0; s < KT; ++s)
 #pragma unroll
                 for (int it = 0; it < TI; ++it)
-                    if (s * kStep <= 16 * it + 15) o[it] = M::run(fc[s], rows_of<C, kRowP>(lds_p, 16 * it, s * kStep, lane), o[it]);
+                    if (s * kStep <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p, 16 * it, s * kStep, l), o[it]);
+            const int64_t apart = back ? -out_st : out_st;
+            const int64_t to = (back ? len - 1 - here : here) * out_st + out_lane + r16 * apart;
+            if (n == kTicks && (WHOLE || (dc - wc >= 16 && !wide))) {
+                T *q = static_cast<T *>(out) + to;
 #pragma unroll
-            for (int it = 0; it < TI; ++it) {
-                const int i = 16 * it + r16, ch = wc + 4 * kq, have = dc - ch;
-                if (i >= n || have <= 0) continue;
-                const int64_t tick = p.back ? len - 1 - here - i : here + i;
-                const f32x4 v = o[it] * p.out_scale;
-                const int64_t to = tick * out_st + out_at + ch;
-                if (p.wide) {
-                    float *q = static_cast<float *>(p.out) + to;
+                for (int it = 0; it < TI; ++it) *reinterpret_cast<Vec<T, 4> *>(q + 16 * it * apart) = __builtin_convertvector(o[it], Vec<T, 4>);
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < have) q[e] = v[e];
-                } else {
-                    T *q = static_cast<T *>(p.out) + to;
-                    if (have >= 4) {
-                        *reinterpret_cast<Vec<T, 4> *>(q) = __builtin_convertvector(v, Vec<T, 4>);
-                    } else {
+                for (int it = 0; it < TI; ++it) {
+                    if (16 * it + r16 >= n) continue;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < have) q[e] = from_f32<T>(v[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        if (!WHOLE && e >= have) continue;
+                        if (wide) static_cast<float *>(out)[to + 16 * it * apart + e] = o[it][e];
+                        else static_cast<T *>(out)[to + 16 * it * apart + e] = from_f32<T>(o[it][e]);
                     }
                 }
             }
@@ -329,38 +425,39 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 ? 4 : 2) k_attention(AttArg
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
             frag part[kParts];
+            typedef float many __attribute__((ext_vector_type(kPer)));
+            many v = __builtin_convertvector(fc[s], many) * *reinterpret_cast<const many *>(weight + s * kStep + kq * kPer);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                float v = static_cast<float>(fc[s][e]) * weight[s * kStep + kq * kPer + e];
-#pragma unroll
-                for (int q = 0; q < kParts; ++q) {
-                    part[q][e] = static_cast<C>(v);
-                    v -= static_cast<float>(part[q][e]);
-                }
+            for (int q = 0; q < kParts; ++q) {
+                part[q] = __builtin_convertvector(v, frag);
+                if (q + 1 < kParts) v -= __builtin_convertvector(part[q], many);
             }
 #pragma unroll
             for (int i = 0; i < XT; ++i) {
-                const frag fb = columns_of<C, kRow, GAP>(lds_b, kPer == 8 ? 32 * (i / 2) + 4 * (i % 2) : 16 * i, s * kStep, lane);
+                const frag fb = RD::template columns<GAP>(lds_b, kPer == 8 ? 32 * (i / 2) + 4 * (i % 2) : 16 * i, s * kStep, l);
 #pragma unroll
                 for (int q = 0; q < kParts; ++q) x[i] = M::run(fb, part[q], x[i]);
             }
         }
     }
     // Ticks behind the length are 0.
-    if (!STATES && p.out) {
-        const int t0 = max(len, seg * args.seg_ticks), t1 = min(args.T, (seg + 1) * args.seg_ticks), w = min(W, dc - c0);
-        for (int u = threadIdx.x; u < (t1 - t0) * w; u += NT) {
-            const int64_t to = (t0 + u / w) * out_st + out_at + c0 + u % w;
-            if (p.wide) static_cast<float *>(p.out)[to] = 0.0f;
-            else static_cast<T *>(p.out)[to] = T(0.0f);
+    if (!STATES && out) {
+        const int t0 = max(len, seg_first), w = min(W, dc - c0);
+        for (int u = threadIdx.x; u < (seg_end - t0) * w; u += NT) {
+            const int64_t to = (t0 + u / w) * out_st + static_cast<int64_t>(bh) * dc + c0 + u % w;
+            if (wide) static_cast<float *>(out)[to] = 0.0f;
+            else static_cast<T *>(out)[to] = T(0.0f);
         }
     }
-    if (p.x_out && active)
+    if (pass.x_out && active && wc + r16 < dc) {
+        const int64_t x_b = pass.x_b;
+        float *to = pass.x_out + seg * pass.x_seg + bh * pass.x_bh + (wc + r16) * pass.x_c;
 #pragma unroll
         for (int i = 0; i < XT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (row(i) + r < db && wc + r16 < dc) *const_cast<float *>(at_state(p.x_out, i, r)) = x[i][r];
+                if (row(i) + r < db) to[(row(i) + r) * x_b] = x[i][r];
+    }
 #endif
 }
 
@@ -402,29 +499,38 @@ __global__ void __launch_bounds__(kBlock) k_attention_share(const float *in, int
     }
 }
 
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, bool WHOLE>
 void run_pass(AttArgs a, bool states, hipStream_t s) {
     int widest = 0;
     for (int i = 0; i < a.passes; ++i) widest = std::max(widest, a.pass[i].c.d);
     a.tiles = ceil_div(widest, 16 * NW);
     const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
     const dim3 grid(static_cast<unsigned>(groups * a.tiles * a.passes)), block(NW * kWave);
-    if (states) hipLaunchKernelGGL((k_attention<T, D, NW, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_attention<T, D, NW, false>), grid, block, 0, s, a);
+    if (states) hipLaunchKernelGGL((k_attention<T, D, NW, true, WHOLE>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_attention<T, D, NW, false, WHOLE>), grid, block, 0, s, a);
 }
 
 template <typename T>
 void run_passes(const AttArgs &a, bool states, hipStream_t s) {
     int da = 0, dc = 0;
-    for (int i = 0; i < a.passes; ++i) da = std::max(da, a.pass[i].b.d), dc = std::max(dc, a.pass[i].c.d);
-    if (dc <= 64) {
-        if (da <= 32) run_pass<T, 32, 4>(a, states, s);
-        else if (da <= 64) run_pass<T, 64, 4>(a, states, s);
-        else run_pass<T, 128, 4>(a, states, s);
+    bool whole = true;
+    for (int i = 0; i < a.passes; ++i) {
+        const AttPass &p = a.pass[i];
+        da = std::max(da, p.b.d), dc = std::max(dc, p.c.d);
+        whole = whole && p.b.d == p.c.d && p.c.d == a.pass[0].c.d && !p.wide;
+    }
+    if (whole && dc == 64) {
+        run_pass<T, 64, 4, true>(a, states, s);
+    } else if (whole && dc == 128) {
+        run_pass<T, 128, 8, true>(a, states, s);
+    } else if (dc <= 64) {
+        if (da <= 32) run_pass<T, 32, 4, false>(a, states, s);
+        else if (da <= 64) run_pass<T, 64, 4, false>(a, states, s);
+        else run_pass<T, 128, 4, false>(a, states, s);
     } else {
-        if (da <= 32) run_pass<T, 32, 8>(a, states, s);
-        else if (da <= 64) run_pass<T, 64, 8>(a, states, s);
-        else run_pass<T, 128, 8>(a, states, s);
+        if (da <= 32) run_pass<T, 32, 8, false>(a, states, s);
+        else if (da <= 64) run_pass<T, 64, 8, false>(a, states, s);
+        else run_pass<T, 128, 8, false>(a, states, s);
     }
 }
 
@@ -506,6 +612,8 @@ int check_attention(const glif_attention *a, bool step) {
     if (!known_dtype(a->dtype)) return fail(GLIF_EINVAL, "attention: unknown type");
     if (a->n_ticks < 0 || a->n_ticks > (1 << 20) || a->n_batch < 0 || a->n_batch > 65535 || a->n_heads < 0 || a->n_heads > 4096)
         return fail(GLIF_EINVAL, "attention: at most 2^20 ticks, a batch of 65535 and 4096 heads");
+    const int64_t most = std::max({a->q_st, a->k_st, a->v_st}), least = std::min({a->q_st, a->k_st, a->v_st});
+    if (!step && (most >= (1 << 24) || least < 0)) return fail(GLIF_EINVAL, "attention: strides of ticks must be in [0, 2^24)");
     if (a->n_groups < 1 || a->n_heads % a->n_groups) return fail(GLIF_EINVAL, "attention: n_groups must divide n_heads");
     if (a->d_key < 1 || a->d_key > 128 || a->d_value < 1 || a->d_value > 128)
         return fail(GLIF_EINVAL, "attention: keys and values have 1 to 128 channels");
@@ -635,6 +743,7 @@ int glif_attention_bwd(const glif_attention *s, const glif_attention_grad *g, vo
     AttArgs a = backward_args(s);
     if (static_cast<int64_t>(a.B) * a.H == 0) return GLIF_OK;
     if (a.T && !g->dy) return fail(GLIF_EINVAL, "NULL argument");
+    if (g->dy_st < 0 || g->dy_st >= (1 << 24)) return fail(GLIF_EINVAL, "attention: strides of ticks must be in [0, 2^24)");
     Carver c(ws, ws_bytes);
     AttBack w{};
     carve(c, w, a, s);

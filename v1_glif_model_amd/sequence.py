@@ -605,13 +605,21 @@ def _tick(t):
 
 # ------------------------------------------------------------------- linear attention ----
 def _heads(t):
-    """t [..., heads, channels] with the channels contiguous."""
-    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    """t [..., heads, channels] with the channels contiguous, and ticks less than 2^24 elements apart."""
+    if t.is_contiguous() or ((t.shape[-1] == 1 or t.stride(-1) == 1) and (t.dim() < 4 or t.shape[0] == 1 or t.stride(0) < 1 << 24)):
+        return t
+    return t.contiguous()
+
+
+def _head_strides(t):
+    """The strides of ticks (0 where there is but one: it may be anything then), batch entries and heads."""
+    st, sb, sh, _ = t.stride()
+    return (st if t.shape[0] > 1 else 0), sb, sh
 
 
 def _attention_struct(q, k, v, log_decay, state, lengths, scale, ticks):
     """glif_attention of tensors with contiguous channels (held by the caller)."""
-    strides = [n for t in (q, k, v) for n in (t.stride()[:3] if ticks else (0, *t.stride()[:2]))]
+    strides = [n for t in (q, k, v) for n in (_head_strides(t) if ticks else (0, *t.stride()[:2]))]
     return _lib.Attention(_p(q), _p(k), _p(v), _p(log_decay), _p(state), _p(lengths), *strides, scale, DTYPES[q.dtype],
                           q.shape[0] if ticks else 1, q.shape[-3], q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1])
 
@@ -645,7 +653,7 @@ class _Attention(torch.autograd.Function):
         wants = ctx.needs_input_grad
         dq, dk, dv, dstate = (torch.empty(t.shape, dtype=t.dtype, device=dev) if w else None
                               for t, w in ((q, wants[0]), (k, wants[1]), (v, wants[2]), (state, wants[4])))
-        g = _lib.AttentionGrad(_p(dy), *dy.stride()[:3], _p(dlast), _p(dq), _p(dk), _p(dv), _p(dstate))
+        g = _lib.AttentionGrad(_p(dy), *_head_strides(dy), _p(dlast), _p(dq), _p(dk), _p(dv), _p(dstate))
         L = lib()
         ws = _workspace(L.glif_attention_bwd_workspace(byref(s)), dev)
         with _on(dev):
