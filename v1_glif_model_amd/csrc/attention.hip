@@ -225,6 +225,15 @@ struct Tile {
     }
 };
 
+
+// Two bfloat16 in 32 bits.
+__device__ __forceinline__ float low_half(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t two_halves(float lo, float hi) {   // to nearest even, one instruction (from conversions of both it made two)
+    uint32_t w;
+    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w) : "v"(lo), "v"(hi));
+    return w;
+}
 #endif
 
 // A block takes one entry and head, 16 of c's channels a wave and one segment of the ticks, chunk by chunk; each wave keeps the
@@ -251,6 +260,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     __shared__ __attribute__((aligned(16))) char lds_c[TC::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * RP::kBytes];
     __shared__ __attribute__((aligned(32))) float weight[kTicks];   // of tick j in the state after the chunk
+    __shared__ float apart[STATES ? 1 : kTicks + 16], across[STATES ? 1 : kTicks];   // decays of scores by distance, backwards; of the state by tick
     __shared__ int odd[2];             // whether c is not finite somewhere in this chunk, and in the next
 
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
@@ -306,21 +316,15 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
                 if (row(i) + r >= db || wc + r16 >= dc) x[i][r] = 0.0f;
     }
 
-    // decays within a 16 x 16 tile of scores (tick i in the lane, ticks j = 4 kq + r) on the diagonal and below it
-    float on[4], below[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int n = r16 - 4 * kq - r;
-        on[r] = n < 0 ? 0.0f : power(rate, n) * in_scale * out_scale;
-        below[r] = power(rate, 16 + n) * in_scale * out_scale;
-    }
     if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
         for (int u = threadIdx.x; u < kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
     }
     if (threadIdx.x < 2) odd[threadIdx.x] = 0;
-    float across[TI];   // decays of the state in tick 16 it + r16
-#pragma unroll
-    for (int it = 0; it < TI; ++it) across[it] = power(rate, 16 * it + r16 + lead) * out_scale;
+    if (!STATES && threadIdx.x < kTicks) {
+        const int i = threadIdx.x;
+        apart[kTicks - 1 - i] = power(rate, i) * in_scale * out_scale;
+        across[i] = power(rate, i + lead) * out_scale;
+    }
 
     // A product with a later tick's 0 is NaN where that tick's c is not finite: such a chunk is fetched again, as chunks of one
     // tick, up to `careful`.
@@ -357,22 +361,34 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
         if (at < end) fetch(at, at < careful ? 1 : min(end - at, kTicks));
         if (!STATES) {
             // scores: rows j, columns i
-            for (int u = wave; u < TI * (TI + 1) / 2; u += NW) {
-                const int it = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, jt = u - it * (it + 1) / 2;
-                f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+            constexpr int kTiles = TI * (TI + 1) / 2, kMost = (kTiles + NW - 1) / NW;
+            auto scores = [&](auto count) {   // of the wave's tiles wave, wave + NW, ..: their products are taken together
+                constexpr int N = decltype(count)::value;
+                int it[N], jt[N];
+                f32x4 s[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int u = wave + i * NW;
+                    it[i] = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, jt[i] = u - it[i] * (it[i] + 1) / 2;
+                    s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
 #pragma unroll
                 for (int k = 0; k < KD; ++k)
-                    s = M::run(RD::rows(lds_b, 16 * jt, k * kStep, l), RD::rows(lds_a, 16 * it, k * kStep, l), s);
-                typedef C four __attribute__((ext_vector_type(4)));
-                four o;
-                const float far = it == jt ? 1.0f : power(rate, 16 * (it - jt - 1));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float f = it == jt ? (4 * kq + r <= r16 ? s[r] * on[r] : 0.0f) : s[r] * below[r] * far;
-                    o[r] = static_cast<C>(f);
+                    for (int i = 0; i < N; ++i)
+                        s[i] = M::run(RD::rows(lds_b, 16 * jt[i], k * kStep, l), RD::rows(lds_a, 16 * it[i], k * kStep, l), s[i]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float *by = apart + kTicks - 1 - 16 * (it[i] - jt[i]) - r16 + 4 * kq;   // (past its end in scores that are masked)
+                    f32x4 o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = it[i] > jt[i] || 4 * kq + r <= r16 ? s[i][r] * by[r] : 0.0f;
+                    typedef C four __attribute__((ext_vector_type(4)));
+                    *reinterpret_cast<four *>(lds_p + RP::at(16 * it[i] + r16, 16 * jt[i] + 4 * kq)) = __builtin_convertvector(o, four);
                 }
-                *reinterpret_cast<four *>(lds_p + RP::at(16 * it + r16, 16 * jt + 4 * kq)) = o;
-            }
+            };
+            if (wave < kTiles - (kMost - 1) * NW) scores(std::integral_constant<int, kMost>{});
+            else if constexpr (kMost > 1) scores(std::integral_constant<int, kMost - 1>{});
             __syncthreads();
         }
         if (!active) continue;
@@ -391,18 +407,18 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
                 for (int it = 0; it < TI; ++it) o[it] = M::run(fx, RD::rows(lds_a, 16 * it, k * kStep, l), o[it]);
             }
 #pragma unroll
-            for (int it = 0; it < TI; ++it) o[it] *= across[it];
+            for (int it = 0; it < TI; ++it) o[it] *= across[16 * it + (l & 15)];
 #pragma unroll
             for (int s = 0; s < KT; ++s)
 #pragma unroll
                 for (int it = 0; it < TI; ++it)
                     if (s * kStep <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p, 16 * it, s * kStep, l), o[it]);
-            const int64_t apart = back ? -out_st : out_st;
-            const int64_t to = (back ? len - 1 - here : here) * out_st + out_lane + r16 * apart;
+            const int64_t by_tick = back ? -out_st : out_st;
+            const int64_t to = (back ? len - 1 - here : here) * out_st + out_lane + r16 * by_tick;
             if (n == kTicks && (WHOLE || (dc - wc >= 16 && !wide))) {
                 T *q = static_cast<T *>(out) + to;
 #pragma unroll
-                for (int it = 0; it < TI; ++it) *reinterpret_cast<Vec<T, 4> *>(q + 16 * it * apart) = __builtin_convertvector(o[it], Vec<T, 4>);
+                for (int it = 0; it < TI; ++it) *reinterpret_cast<Vec<T, 4> *>(q + 16 * it * by_tick) = __builtin_convertvector(o[it], Vec<T, 4>);
             } else {
 #pragma unroll
                 for (int it = 0; it < TI; ++it) {
@@ -410,8 +426,8 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (!WHOLE && e >= have) continue;
-                        if (wide) static_cast<float *>(out)[to + 16 * it * apart + e] = o[it][e];
-                        else static_cast<T *>(out)[to + 16 * it * apart + e] = from_f32<T>(o[it][e]);
+                        if (wide) static_cast<float *>(out)[to + 16 * it * by_tick + e] = o[it][e];
+                        else static_cast<T *>(out)[to + 16 * it * by_tick + e] = from_f32<T>(o[it][e]);
                     }
                 }
             }
@@ -426,11 +442,23 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
         for (int s = 0; s < KT; ++s) {
             frag part[kParts];
             typedef float many __attribute__((ext_vector_type(kPer)));
-            many v = __builtin_convertvector(fc[s], many) * *reinterpret_cast<const many *>(weight + s * kStep + kq * kPer);
+            const many w = *reinterpret_cast<const many *>(weight + s * kStep + kq * kPer);
+            if constexpr (kSize == 2) {
+                const u32x4 two = __builtin_bit_cast(u32x4, fc[s]);
+                u32x4 got[kParts];
 #pragma unroll
-            for (int q = 0; q < kParts; ++q) {
-                part[q] = __builtin_convertvector(v, frag);
-                if (q + 1 < kParts) v -= __builtin_convertvector(part[q], many);
+                for (int e = 0; e < 4; ++e) {
+                    float lo = low_half(two[e]) * w[2 * e], hi = high_half(two[e]) * w[2 * e + 1];
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) {
+                        got[q][e] = two_halves(lo, hi);
+                        lo -= low_half(got[q][e]), hi -= high_half(got[q][e]);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) part[q] = __builtin_bit_cast(frag, got[q]);
+            } else {
+                part[0] = fc[s] * w;
             }
 #pragma unroll
             for (int i = 0; i < XT; ++i) {
@@ -477,12 +505,19 @@ __global__ void __launch_bounds__(kBlock) k_attention_join(JoinArgs a) {
     const int bh = static_cast<int>(i / a.n), len = live_ticks(a.lengths, bh / a.H, a.T);
     const float rate = a.log_decay[bh % a.H] * 1.4426950408889634f;
     float x = a.x ? a.x[i] : 0.0f;
-    for (int s = 0; s < a.segments; ++s) {
-        const int ticks = min(max(len - s * a.seg_ticks, 0), a.seg_ticks);
-        float *p = a.states + s * a.bh * a.n + i;
-        const float more = *p;
-        *p = x;
-        if (ticks) x = x * power(rate, ticks) + more;
+    const int64_t apart = a.bh * a.n;
+    constexpr int kAhead = 8;   // loads under way
+    for (int s0 = 0; s0 < a.segments; s0 += kAhead) {
+        float more[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) more[k] = a.states[min(s0 + k, a.segments - 1) * apart + i];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int s = s0 + k, ticks = min(max(len - s * a.seg_ticks, 0), a.seg_ticks);
+            if (s >= a.segments) break;
+            a.states[s * apart + i] = x;
+            if (ticks) x = x * power(rate, ticks) + more[k];
+        }
     }
     if (a.x_out) a.x_out[i] = x;
 }
@@ -625,11 +660,13 @@ int check_attention(const glif_attention *a, bool step) {
 }
 
 // Ticks in segments where there are too few blocks for the chip: a first launch gives the state that each segment adds,
-// a second joins them, and then all segments go at once.  The first reads two of three sequences again.
-void cut(AttArgs &a, int64_t blocks, int ticks) {
+// a second joins them, and then all segments go at once.  The first reads two of three sequences again.  As many segments
+// as blocks are there at once, one a compute unit where heads have more than 64 channels, three where not (8000 ticks of 16 heads
+// of 128 in 25 segments, two rounds of blocks, 89 us, in 16 SEG_US), and none of fewer than four chunks.
+void cut(AttArgs &a, int64_t blocks, int ticks, const glif_attention *s) {
     a.segments = 1, a.seg_ticks = std::max((a.T + ticks - 1) / ticks, 1) * ticks;
-    if (blocks == 0 || blocks >= 256) return;
-    const int64_t chunks = (a.T + ticks - 1) / ticks, want = std::min<int64_t>((512 + blocks - 1) / blocks, chunks / 4);
+    const int64_t slots = std::max(s->d_key, s->d_value) > 64 ? 256 : 768;
+    const int64_t chunks = (a.T + ticks - 1) / ticks, want = blocks ? std::min<int64_t>(slots / blocks, chunks / 4) : 0;
     if (want < 2) return;
     a.seg_ticks = static_cast<int>((chunks + want - 1) / want) * ticks;
     a.segments = (a.T + a.seg_ticks - 1) / a.seg_ticks;
@@ -646,13 +683,13 @@ AttArgs common(const glif_attention *s) {
 AttArgs forward_args(const glif_attention *s) {
     AttArgs a = common(s);
     const int64_t tiles = s->d_value <= 64 ? 1 : (s->d_value + 127) / 128;
-    cut(a, static_cast<int64_t>(a.B) * a.H * tiles, chunk_ticks(s->dtype));
+    cut(a, static_cast<int64_t>(a.B) * a.H * tiles, chunk_ticks(s->dtype), s);
     return a;
 }
 
 AttArgs backward_args(const glif_attention *s) {
     AttArgs a = common(s);
-    cut(a, static_cast<int64_t>(a.B) * a.H * 3, chunk_ticks(s->dtype));
+    cut(a, static_cast<int64_t>(a.B) * a.H * 3, chunk_ticks(s->dtype), s);
     return a;
 }
 
