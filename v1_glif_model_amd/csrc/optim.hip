@@ -50,17 +50,29 @@ __global__ void __launch_bounds__(kBlock)
 // its mean is the value: moments that move by less than a code's step each time still move.  What is not 0 of v does not
 // become 0, as the step divides by its root.  The random numbers of element i of all variables' blocks are the two halves of word
 // (t - 1) P + i of the Philox stream `seed`, P the elements of all blocks.
+//
+// Bound by memory: 36M float32 elements of 20 tensors, 997 MB, 196 us (5.1 TB/s), with moments of 8 bits, 572 MB, 133 us (the
+// random numbers, roots and codes are some 100 operations an element); results past the caches gained nothing.
 constexpr int kUnit = 256;          // elements that a wave takes at once, and that share a scale
 constexpr int kUnitsPerBlock = 16;  // that a block takes at once
 constexpr int kMostTensors = 64;    // of a launch
+// Four blocks a compute unit, which go through the units in turn: each ends with an addition to one word, which come one after
+// the other (36M float32 elements 197 us; by 2048 blocks 207, by one for every 16 units 828).
+constexpr unsigned kMostBlocks = 1024;
+
+// One of a launch's tensors.  Its words are of 32 bits and more: arrays of bytes beside those of pointers, under one index, were
+// read with an index in the scalar loads' base whose last two bits those do not add (the loads fell between two pointers).
+struct AdamwTensor {
+    void *var;
+    const void *grad;
+    int64_t n;
+    int64_t home;             // the first unit of its state
+    uint32_t before, after;   // units of the launch's tensors before it, and with it
+    int32_t var_dt, grad_dt;
+};
 
 struct AdamwArgs {
-    void *var[kMostTensors];
-    const void *grad[kMostTensors];
-    int64_t n[kMostTensors];
-    int64_t home[kMostTensors];          // the first unit of its state
-    uint32_t before[kMostTensors + 1];   // units of the tensors before it in this launch
-    uint8_t var_dt[kMostTensors], grad_dt[kMostTensors];
+    AdamwTensor of[kMostTensors];
     int32_t tensors;
     void *first, *second;
     float *first_scale, *second_scale;   // 8 bits: one a unit
@@ -148,58 +160,120 @@ __device__ __forceinline__ uint32_t encode_4(f32x4 x, float most, const uint32_t
     return codes;
 }
 
+// What a lane holds of a unit: four neighbours of everything.
+template <int BITS>
+struct Quad {
+    f32x4 p, g, m, v;
+    uint32_t mc, vc;
+    float ms, vs;
+    int64_t at;   // of the moments
+
+    __device__ __forceinline__ void moments(const AdamwArgs &a, int64_t home, int lane) {
+        at = home * kUnit + lane * 4;
+        if (BITS == 8) {
+            mc = *reinterpret_cast<const uint32_t *>(static_cast<const int8_t *>(a.first) + at), ms = a.first_scale[home];
+            vc = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.second) + at), vs = a.second_scale[home];
+        } else {
+            m = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.first) + at);
+            v = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.second) + at);
+        }
+    }
+    __device__ __forceinline__ void step(const AdamwArgs &a, float size, float root) {
+        if (BITS == 8) m = decode_4<false>(mc, ms), v = decode_4<true>(vc, vs);
+        m = m * a.beta_1 + g * a.one_m_b1;
+        v = v * a.beta_2 + (g * g) * a.one_m_b2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            p[e] = p[e] * a.keep - size * (m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * root + a.eps));
+    }
+    __device__ __forceinline__ void put(const AdamwArgs &a, int64_t home, int lane, int64_t t) const {
+        if (BITS == 8) {
+            uint32_t word[4];
+            philox_block(a.seed, (static_cast<uint64_t>(t - 1) * static_cast<uint64_t>(a.total) + static_cast<uint64_t>(at)) >> 2, word);
+            const float mm = unit_most(m), vm = unit_most(v);
+            *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(a.first) + at) = encode_4<false>(m, mm, word);
+            *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a.second) + at) = encode_4<true>(v, vm, word);
+            if (lane == 0) a.first_scale[home] = mm, a.second_scale[home] = vm;
+        } else {
+            *reinterpret_cast<f32x4 *>(static_cast<float *>(a.first) + at) = m;
+            *reinterpret_cast<f32x4 *>(static_cast<float *>(a.second) + at) = v;
+        }
+    }
+};
+
+// A block's units all within one tensor whose variable and gradient are of type T: each wave's, N at a time.
+template <int BITS, typename T, int N>
+__device__ __forceinline__ void adamw_whole(const AdamwArgs &a, int i, int64_t first, float size, float root, int64_t t, int wave, int lane) {
+    constexpr int kMine = kUnitsPerBlock / (kBlock / kWave);
+    typedef Vec<T, 4> vec;
+    T *p = static_cast<T *>(a.of[i].var) + lane * 4;
+    const T *g = static_cast<const T *>(a.of[i].grad) + lane * 4;
+    const int64_t home = a.of[i].home;
+#pragma unroll 1
+    for (int u = 0; u < kMine; u += N) {
+        Quad<BITS> q[N];
+        vec pv[N], gv[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int64_t unit = first + wave * kMine + u + k;
+            gv[k] = *reinterpret_cast<const vec *>(g + unit * kUnit);
+            pv[k] = *reinterpret_cast<const vec *>(p + unit * kUnit);
+            q[k].moments(a, home + unit, lane);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int64_t unit = first + wave * kMine + u + k;
+            q[k].p = __builtin_convertvector(pv[k], f32x4), q[k].g = __builtin_convertvector(gv[k], f32x4);
+            q[k].step(a, size, root);
+            const vec o = __builtin_convertvector(q[k].p, vec);
+            *reinterpret_cast<vec *>(p + unit * kUnit) = o;
+            q[k].put(a, home + unit, lane, t);
+        }
+    }
+}
+
 template <int BITS>
 __global__ void __launch_bounds__(kBlock) k_adamw(AdamwArgs a) {
+    constexpr int kAtOnce = 2;   // units a wave has under way (four: no faster)
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t t = *static_cast<volatile int64_t *>(a.iterations) + 1;
     const double td = static_cast<double>(t);
     // 1 - beta^t without the cancellation of a beta near 1
-    const float step = static_cast<float>(static_cast<double>(a.lr) / -expm1(td * a.log_beta_1));
+    const float size = static_cast<float>(static_cast<double>(a.lr) / -expm1(td * a.log_beta_1));
     const float root = static_cast<float>(1.0 / sqrt(-expm1(td * a.log_beta_2)));
-    const uint32_t units = a.before[a.tensors];
+    const uint32_t units = a.of[a.tensors - 1].after;
     for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * kUnitsPerBlock; base < units; base += static_cast<uint64_t>(gridDim.x) * kUnitsPerBlock) {
         int i = 0;   // the tensor that holds unit `base`
 #pragma unroll
         for (int s = kMostTensors / 2; s > 0; s >>= 1)
-            if (i + s < a.tensors && a.before[i + s] <= base) i += s;
+            if (i + s < a.tensors && a.of[i + s].before <= base) i += s;
+        const int64_t first = static_cast<int64_t>(base - a.of[i].before);
+        if ((first + kUnitsPerBlock) * kUnit <= a.of[i].n && a.of[i].var_dt == a.of[i].grad_dt) {
+            const int32_t dt = a.of[i].var_dt;
+            if (dt == GLIF_F32) adamw_whole<BITS, f32, kAtOnce>(a, i, first, size, root, t, wave, lane);
+            else if (dt == GLIF_BF16) adamw_whole<BITS, bf16, kAtOnce>(a, i, first, size, root, t, wave, lane);
+            else adamw_whole<BITS, f16, kAtOnce>(a, i, first, size, root, t, wave, lane);
+            continue;
+        }
         for (uint64_t unit = base + wave; unit < min(base + kUnitsPerBlock, static_cast<uint64_t>(units)); unit += kBlock / kWave) {
-            while (a.before[i + 1] <= unit) ++i;
-            const int64_t in = static_cast<int64_t>(unit - a.before[i]), at = in * kUnit + lane * 4, home = a.home[i] + in;
-            const int have = static_cast<int>(max(static_cast<int64_t>(0), min(a.n[i] - at, static_cast<int64_t>(4))));
-            const f32x4 g = load_4(a.grad[i], a.grad_dt[i], at, have);
-            f32x4 p = load_4(a.var[i], a.var_dt[i], at, have), m, v;
-            const int64_t state = home * kUnit + lane * 4;
-            if (BITS == 8) {
-                m = decode_4<false>(*reinterpret_cast<const uint32_t *>(static_cast<const int8_t *>(a.first) + state), a.first_scale[home]);
-                v = decode_4<true>(*reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.second) + state), a.second_scale[home]);
-            } else {
-                m = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.first) + state);
-                v = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.second) + state);
-            }
-            m = m * a.beta_1 + g * a.one_m_b1;
-            v = v * a.beta_2 + (g * g) * a.one_m_b2;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                p[e] = p[e] * a.keep - step * (m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * root + a.eps));
-            store_4(a.var[i], a.var_dt[i], at, have, p);
-            if (BITS == 8) {
-                uint32_t word[4];
-                philox_block(a.seed, (static_cast<uint64_t>(t - 1) * static_cast<uint64_t>(a.total) + static_cast<uint64_t>(state)) >> 2, word);
-                const float mm = unit_most(m), vm = unit_most(v);
-                *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(a.first) + state) = encode_4<false>(m, mm, word);
-                *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a.second) + state) = encode_4<true>(v, vm, word);
-                if (lane == 0) a.first_scale[home] = mm, a.second_scale[home] = vm;
-            } else {
-                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.first) + state) = m;
-                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.second) + state) = v;
-            }
+            while (a.of[i].after <= unit) ++i;
+            const AdamwTensor &of = a.of[i];
+            const int64_t in = static_cast<int64_t>(unit - of.before), at = in * kUnit + lane * 4, home = of.home + in;
+            const int have = static_cast<int>(max(static_cast<int64_t>(0), min(of.n - at, static_cast<int64_t>(4))));
+            Quad<BITS> q;
+            q.g = load_4(of.grad, of.grad_dt, at, have);
+            q.p = load_4(of.var, of.var_dt, at, have);
+            q.moments(a, home, lane);
+            q.step(a, size, root);
+            store_4(of.var, of.var_dt, at, have, q.p);
+            q.put(a, home, lane, t);
         }
     }
     if (!a.last) return;
-    // The block that ends last counts the step: everybody has read the count by then.
+    // The block that ends last counts the step: everybody has used the count by then.  Nothing else is passed on, so no block
+    // waits for its results to be seen by others (with a fence each block's end cost 0.1 us, one after the other).
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();
         unsigned long long *ended = reinterpret_cast<unsigned long long *>(a.iterations + 1);
         if (atomicAdd(ended, 1ull) == gridDim.x - 1) {
             *ended = 0;
@@ -272,16 +346,14 @@ extern "C" int glif_adamw(int32_t n_vars, void *const *vars, const int32_t *var_
     for (int32_t i = 0; i < n_vars; ++i) {
         const int64_t units = (sizes[i] + kUnit - 1) / kUnit;
         if (grads[i] && units) {
-            const int k = a.tensors++;
-            a.var[k] = vars[i], a.grad[k] = grads[i], a.n[k] = sizes[i], a.home[k] = home;
-            a.var_dt[k] = static_cast<uint8_t>(var_dtypes[i]), a.grad_dt[k] = static_cast<uint8_t>(grad_dtypes[i]);
-            a.before[k + 1] = a.before[k] + static_cast<uint32_t>(units);
+            const uint32_t before = a.tensors ? a.of[a.tensors - 1].after : 0u, after = before + static_cast<uint32_t>(units);
+            a.of[a.tensors++] = AdamwTensor{vars[i], grads[i], sizes[i], home, before, after, var_dtypes[i], grad_dtypes[i]};
             --given;
             // units of a launch are counted in 32 bits: 2^28 of the largest size allowed fit eight times
-            const bool full = a.tensors == kMostTensors || a.before[k + 1] >= 7u << 28;
+            const bool full = a.tensors == kMostTensors || after >= 7u << 28;
             a.last = given == 0;
             if (full || a.last) {
-                const unsigned blocks = std::min<unsigned>((a.before[k + 1] + kUnitsPerBlock - 1) / kUnitsPerBlock, 2048u);
+                const unsigned blocks = std::min<unsigned>((after + kUnitsPerBlock - 1) / kUnitsPerBlock, kMostBlocks);
                 if (state_bits == 8) hipLaunchKernelGGL(k_adamw<8>, dim3(blocks), dim3(kBlock), 0, s, a);
                 else hipLaunchKernelGGL(k_adamw<32>, dim3(blocks), dim3(kBlock), 0, s, a);
                 a.tensors = 0;

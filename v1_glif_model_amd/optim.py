@@ -148,6 +148,7 @@ class AdamW:
         for p in self.variables:
             self._homes.append(self._homes[-1] + -(-p.numel() // self.BLOCK) * self.BLOCK)
         n = self._homes[-1]
+        self._strides = [torch.empty(s, device="meta").stride() for s in self._shapes]
 
         def zeros(n, dtype):
             return torch.zeros(n, dtype=dtype, device=dev)
@@ -158,6 +159,7 @@ class AdamW:
         else:
             self._first, self._second = zeros(n, torch.int8), zeros(n, torch.uint8)
             self._scales = zeros(n // self.BLOCK, torch.float32), zeros(n // self.BLOCK, torch.float32)
+        self._own = [[self._views(flat, i) for i in range(len(self.variables))] for flat in (self._first, self._second)]
         self._count = zeros(2, torch.int64)      # steps done; the kernel's own
         count = len(self.variables)
         self._sizes = (ctypes.c_int64 * count)(*(p.numel() for p in self.variables))
@@ -183,50 +185,53 @@ class AdamW:
         gradients = list(gradients)
         if len(gradients) != len(self.variables):
             raise ValueError(f"there are {len(self.variables)} variables and {len(gradients)} gradients")
-        held, changed = [], []
+        held, kinds, changed, index = [], [], [], self.device.index
         for g, p, dtype, shape in zip(gradients, self.variables, self._types, self._shapes):
-            if p.dtype is not dtype or p.shape != shape or p.device != self.device or not p.is_contiguous():
+            if p.dtype is not dtype or p.shape != shape or p.get_device() != index or not p.is_contiguous():
                 raise ValueError("a variable is not laid out as it was when the optimizer was made")
-            if g is not None:
-                if not isinstance(g, torch.Tensor) or g.device != self.device or g.shape != shape or (
-                        g.dtype is not dtype and g.dtype is not torch.float32):
-                    raise ValueError(f"a gradient must be a tensor of its variable's shape {tuple(shape)} and device, float32 or of its type")
-                g = g if g.is_contiguous() else g.contiguous()
-                changed.append(p)
+            if g is None:
+                held.append(None)
+                kinds.append(0)
+                continue
+            if not isinstance(g, torch.Tensor) or g.get_device() != index or g.shape != shape or (
+                    g.dtype is not dtype and g.dtype is not torch.float32):
+                raise ValueError(f"a gradient must be a tensor of its variable's shape {tuple(shape)} and device, float32 or of its type")
+            if not g.is_contiguous():
+                g = g.contiguous()
             held.append(g)
+            kinds.append(DTYPES[g.dtype])
+            changed.append(p)
         if not changed:
             return
         first_scale, second_scale = self._scales or (None, None)
         with _on(self.device):
             check(lib().glif_adamw(len(held), self._pointers(*(p.data_ptr() for p in self.variables)), self._codes,
-                                   self._pointers(*(_p(g) for g in held)),
-                                   self._ints(*(0 if g is None else DTYPES[g.dtype] for g in held)), self._sizes, self.state_bits,
+                                   self._pointers(*(_p(g) for g in held)), self._ints(*kinds), self._sizes, self.state_bits,
                                    _p(self._first), _p(self._second), _p(first_scale), _p(second_scale), _p(self._count),
                                    float(self.learning_rate), self.beta_1, self.beta_2, self.epsilon, self.weight_decay, self.seed,
                                    stream_ptr(self.device)))
         torch.autograd.graph.increment_version(changed)
 
     def _views(self, flat, i):
-        return flat[self._homes[i]:self._homes[i] + self._sizes[i]].view(self._shapes[i])
+        return flat.as_strided(self._shapes[i], self._strides[i], self._homes[i])
 
     def moments(self):
         """The first and the second moments as float32 values, a list of each: the state itself where it is held in 32 bits,
         what the codes stand for where in 8."""
-        first, second = self._first, self._second
-        if self.state_bits == 8:
-            values = torch.empty((2, first.numel()), dtype=torch.float32, device=self.device)
-            with _on(self.device):
-                check(lib().glif_adamw_values(_p(first), _p(self._scales[0]), _p(second), _p(self._scales[1]), first.numel(),
-                                              _p(values[0]), _p(values[1]), stream_ptr(self.device)))
-            first, second = values
-        count = range(len(self.variables))
-        return [self._views(first, i) for i in count], [self._views(second, i) for i in count]
+        if self.state_bits == 32:
+            return list(self._own[0]), list(self._own[1])
+        first, second = (torch.empty(self._first.numel(), dtype=torch.float32, device=self.device) for _ in range(2))
+        with _on(self.device):
+            check(lib().glif_adamw_values(_p(self._first), _p(self._scales[0]), _p(self._second), _p(self._scales[1]), first.numel(),
+                                          _p(first), _p(second), stream_ptr(self.device)))
+        homes = list(zip(self._shapes, self._strides, self._homes))
+        return [first.as_strided(*h) for h in homes], [second.as_strided(*h) for h in homes]
 
     def _scale_views(self, k, i):
         return self._scales[k][self._homes[i] // self.BLOCK:self._homes[i + 1] // self.BLOCK]
 
     def _state(self, k, i):
-        codes = self._views((self._first, self._second)[k], i)
+        codes = self._own[k][i]
         return codes if self.state_bits == 32 else (codes, self._scale_views(k, i))
 
     def state_dict(self):
