@@ -78,7 +78,7 @@ def test_shapes(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", [(700, 2, 2, 1, 20, 36), (1030, 1, 3, 3, 64, 70)])
+@pytest.mark.parametrize("shape", [(700, 2, 2, 1, 20, 36), (1030, 1, 3, 3, 64, 70), (1030, 1, 2, 2, 64, 64), (600, 2, 2, 2, 128, 128)])
 def test_time_in_segments(shape, dtype):
     """Few heads and many ticks: segments of the time go at once."""
     T, B = shape[:2]
@@ -87,12 +87,13 @@ def test_time_in_segments(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_lengths(dtype):
+@pytest.mark.parametrize("G,K,V", [(1, 20, 24), (3, 64, 64)])
+def test_lengths(G, K, V, dtype):
     """Ticks behind a length may hold anything; lengths of nothing and beyond the end."""
     T, B = 70, 6
-    q, k, v, decay, scale, state = make(T, B, 3, 1, 20, 24, dtype)
+    q, k, v, decay, scale, state = make(T, B, 3, G, K, V, dtype)
     lengths = torch.tensor([0, 1, 64, 65, 70, 99], dtype=torch.int32, device=DEV)
-    dy = rnd(5, T, B, 3, 24, dtype=dtype)
+    dy = rnd(5, T, B, 3, V, dtype=dtype)
     case(q, k, v, decay, 0.3, state, lengths, dy)
     from v1_glif_model_amd import sequence as seq
 
@@ -112,10 +113,11 @@ def test_lengths(dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("where", ["q", "k", "v"])
-def test_what_is_not_finite_does_not_go_back_in_time(where, dtype):
+@pytest.mark.parametrize("K,V", [(40, 48), (64, 64), (128, 128)])
+def test_what_is_not_finite_does_not_go_back_in_time(K, V, where, dtype):
     from v1_glif_model_amd import sequence as seq
     T = 90
-    x = dict(zip("qkv", make(T, 1, 2, 2, 40, 48, dtype)[:3]))
+    x = dict(zip("qkv", make(T, 1, 2, 2, K, V, dtype)[:3]))
     decay = torch.tensor([-0.1, -1.0], device=DEV)
     clean, last = seq.linear_attention(*x.values(), decay)
     for tick, bad in ((0, float("nan")), (20, float("inf")), (63, float("nan")), (64, float("-inf")), (89, float("nan"))):
@@ -127,15 +129,15 @@ def test_what_is_not_finite_does_not_go_back_in_time(where, dtype):
         assert torch.equal(out[:, :, 0], clean[:, :, 0]) and torch.equal(end[:, 0], last[:, 0])
         assert not out[tick, 0, 1].isfinite().all() and (where == "q" or not end[0, 1].isfinite().all())
         if where == "v":     # only its own channel
-            rest = [c for c in range(48) if c != 3]
+            rest = [c for c in range(V) if c != 3]
             assert out[:, :, 1][..., rest].isfinite().all() and end[0, 1][:, rest].isfinite().all()
         if where == "k":
-            assert end[0, 1][[c for c in range(40) if c != 3]].isfinite().all()
+            assert end[0, 1][[c for c in range(K) if c != 3]].isfinite().all()
     # two of them in one chunk: what lies between sees only the first
     y = {n: t.clone() for n, t in x.items()}
     y["v"][10, 0, 1, 3], y["k"][30, 0, 1, 5] = float("nan"), float("nan")
     out, _ = seq.linear_attention(*y.values(), decay)
-    assert out[:30, 0, 1][:, [c for c in range(48) if c != 3]].isfinite().all() and out[30:, 0, 1].isnan().all()
+    assert out[:30, 0, 1][:, [c for c in range(V) if c != 3]].isfinite().all() and out[30:, 0, 1].isnan().all()
     assert out[:10].isfinite().all() and out[10:, 0, 1, 3].isnan().all()
 
 
@@ -155,6 +157,20 @@ def test_strides(dtype):
     q, k, v = rnd(4, B, H, K, T, dtype=dtype).permute(3, 0, 1, 2), rnd(5, B, T, 1, K, dtype=dtype).transpose(0, 1), rnd(6, B, T, 1, V, dtype=dtype).transpose(0, 1)
     case(q, k.expand(T, B, H, K), v.expand(T, B, H, V), rates(2 * H)[::2], 2.0)
     case(q, k, v, rates(H), -0.5)
+
+
+def test_heads_of_64_off_16_bytes():
+    """They go by way of registers, the others straight into LDS."""
+    from v1_glif_model_amd import sequence as seq
+    T, B, H = 70, 2, 2
+    wide = [rnd(i, T, B, H, 65, dtype=BF16) for i in range(3)]
+    case(*(t[..., 1:] for t in wide), rates(H))
+    flat = [rnd(i, T * B * H * 64 + 1, dtype=BF16) for i in range(3)]
+    off = [t[1:].view(T, B, H, 64) for t in flat]
+    case(*off, rates(H))
+    y, last = seq.linear_attention(*off, rates(H))
+    z, end = seq.linear_attention(*(t.clone() for t in off), rates(H))
+    assert torch.equal(y, z) and torch.equal(last, end)
 
 
 def test_gradients_against_differences():

@@ -186,9 +186,12 @@ struct Tile {
             const int to_row = mine + i * kRows;
             if (kN * kRows > F::kTicks && to_row >= F::kTicks) break;
             u64x2 w = __builtin_bit_cast(u64x2, r[i]);
-            if (bits >= 128 || to_row >= n) w = u64x2{0, 0};
-            else if (bits >= 64) w = u64x2{w[1] >> (bits - 64), 0};
-            else if (bits > 0) w = u64x2{w[0] >> bits | w[1] << (64 - bits), w[1] >> bits};
+            if (bits >= 128 || to_row >= n) {
+                w = u64x2{0, 0};
+            } else if constexpr (!WHOLE) {
+                if (bits >= 64) w = u64x2{w[1] >> (bits - 64), 0};
+                else if (bits > 0) w = u64x2{w[0] >> bits | w[1] << (64 - bits), w[1] >> bits};
+            }
             const vec v = __builtin_bit_cast(vec, w);
 #pragma unroll
             for (int s = 0; s < kV / kE; ++s) {
@@ -229,6 +232,10 @@ struct Tile {
 // Two bfloat16 in 32 bits.
 __device__ __forceinline__ float low_half(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t larger_halves(uint32_t a, uint32_t b) {
+    typedef uint16_t pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b)));
+}
 __device__ __forceinline__ uint32_t two_halves(float lo, float hi) {   // to nearest even, one instruction (from conversions of both it made two)
     uint32_t w;
     asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w) : "v"(lo), "v"(hi));
@@ -489,6 +496,250 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
 #endif
 }
 
+// The same for bfloat16 heads of D = 16 NW channels in all three sequences, on 16 bytes, of which the tiles go to LDS without
+// registers, a chunk ahead: two of each, and two barriers a chunk.
+template <int D, int NW, bool STATES>
+__global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args) {
+#ifdef __HIP_DEVICE_COMPILE__
+    using M = Mma<bf16>;
+    typedef M::frag frag;
+    using R = Rows<bf16, D>;
+    using RP = Rows<bf16, 64>;
+    constexpr int kTicks = 64, TI = 4, KT = 2, KD = D / 32, XT = D / 16, NT = NW * kWave, kTile = kTicks * R::kBytes;
+    constexpr int kLoad = 16 * kWave, kN = kTile / kLoad / NW, kAcross = R::kBytes / 16;   // bytes of a wave's load, a wave's loads, lanes of a row
+    static_assert(D == 16 * NW && kN * kLoad * NW == kTile, "the tiles divide among the waves");
+    __shared__ __attribute__((aligned(1024))) char lds_a[STATES ? 16 : 2 * kTile];
+    __shared__ __attribute__((aligned(1024))) char lds_b[2 * kTile];
+    __shared__ __attribute__((aligned(1024))) char lds_c[2 * kTile];
+    __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * RP::kBytes];
+    __shared__ __attribute__((aligned(32))) float weight[kTicks];
+    __shared__ float apart[STATES ? 1 : kTicks + 16], across[STATES ? 1 : kTicks];
+
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
+    const int passes = args.passes, slot = static_cast<int>(blockIdx.x >> 3);
+    const int64_t group = static_cast<int64_t>(slot / passes) * 8 + (blockIdx.x & 7);
+    if (group >= static_cast<int64_t>(args.B) * args.H * args.segments) return;
+    const AttPass &pass = args.pass[slot % passes];
+    const int seg = static_cast<int>(group % args.segments);
+    const int bh = static_cast<int>(group / args.segments), b = bh / args.H, h = bh % args.H;
+    const int len = live_ticks(args.lengths, b, args.T), seg_first = seg * args.seg_ticks, seg_end = min(args.T, seg_first + args.seg_ticks);
+    const int begin = min(seg_first, len), end = min(seg_end, len);
+    const float rate = args.log_decay[h] * 1.4426950408889634f;
+    const int wc = wave * 16, lead = pass.lead;
+    const bool back = pass.back;
+    const float in_scale = pass.in_scale, out_scale = pass.out_scale;
+    const int64_t out_st = static_cast<int64_t>(args.B) * args.H * D;
+    bf16 *const out = static_cast<bf16 *>(pass.out);
+    const int64_t out_lane = static_cast<int64_t>(bh) * D + wc + 4 * kq;
+
+    const bf16 *const pa = static_cast<const bf16 *>(pass.a.p) + b * pass.a.sb + h / pass.a.share * pass.a.sh;
+    const bf16 *const pb = static_cast<const bf16 *>(pass.b.p) + b * pass.b.sb + h / pass.b.share * pass.b.sh;
+    const bf16 *const pc = static_cast<const bf16 *>(pass.c.p) + b * pass.c.sb + h / pass.c.share * pass.c.sh;
+    const int64_t a_st = pass.a.st, b_st = pass.b.st, c_st = pass.c.st;
+    // n ticks from `at` on to a tile: what lands at a lane's place is the piece that belongs there by the rows' permutation;
+    // rows past the n repeat the last
+    auto bring = [&](const bf16 *p, int64_t st, int at, int n, char *to) {
+        typedef __attribute__((address_space(3))) void *lptr;
+        const bf16 *low = p + (back ? len - at - n : at) * st;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16 *>(low), 0, -1, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int inst = wave * kN + i, row = inst * (kWave / kAcross) + lane / kAcross, piece = lane % kAcross ^ R::key(row), have = min(row, n - 1);
+            const uint32_t off = static_cast<uint32_t>(back ? n - 1 - have : have) * static_cast<uint32_t>(st * 2) + static_cast<uint32_t>(piece * 16);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr)(to + inst * kLoad), 16, off, 0, 0, 0);
+        }
+    };
+    auto fetch = [&](int at, int n, int buf) {
+        if (!STATES) bring(pa, a_st, at, n, lds_a + buf * kTile);
+        bring(pb, b_st, at, n, lds_b + buf * kTile);
+        bring(pc, c_st, at, n, lds_c + buf * kTile);
+    };
+    if (begin < end) fetch(begin, min(end - begin, kTicks), 0);
+
+    // state: x[i][r] is of b's channel row(i) + r and c's channel wc + r16
+    auto row = [&](int i) { return 32 * (i / 2) + 8 * kq + 4 * (i % 2); };
+    f32x4 x[XT] = {};
+    if (!STATES && pass.x) {
+        const int64_t x_b = pass.x_b;
+        const float *from = pass.x + seg * pass.x_seg + bh * pass.x_bh + (wc + r16) * pass.x_c;
+        if (x_b == 1) {
+#pragma unroll
+            for (int i = 0; i < XT; ++i) x[i] = *reinterpret_cast<const Vec<f32, 4> *>(from + row(i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < XT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[i][r] = from[(row(i) + r) * x_b];
+        }
+    }
+    if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
+        for (int u = threadIdx.x; u < kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
+        if (threadIdx.x < kTicks) {
+            const int i = threadIdx.x;
+            apart[kTicks - 1 - i] = power(rate, i) * in_scale * out_scale;
+            across[i] = power(rate, i + lead) * out_scale;
+        }
+    }
+
+    // What has to be there before a chunk is gone through: its tiles, without what is behind its n ticks, its weights and
+    // scores.
+    auto ready = [&](int n, int buf) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (n < kTicks) {
+            for (int u = threadIdx.x; u < (kTicks - n) * R::kBytes / 4; u += NT) {
+                const int at = buf * kTile + n * R::kBytes + u * 4;
+                if (!STATES) *reinterpret_cast<uint32_t *>(lds_a + at) = 0u;
+                *reinterpret_cast<uint32_t *>(lds_b + at) = 0u;
+                *reinterpret_cast<uint32_t *>(lds_c + at) = 0u;
+            }
+            __syncthreads();
+        }
+        if (threadIdx.x < kTicks) {
+            const int j = threadIdx.x;
+            weight[j] = j < n ? power(rate, n - lead - j) * in_scale : 0.0f;
+        }
+        if (!STATES) {
+            const char *ta = lds_a + buf * kTile, *tb = lds_b + buf * kTile;
+            constexpr int kTiles = TI * (TI + 1) / 2, kMost = (kTiles + NW - 1) / NW;
+            auto scores = [&](auto count) {   // of the wave's tiles wave, wave + NW, ..: their products are taken together
+                constexpr int N = decltype(count)::value;
+                int it[N], jt[N];
+                f32x4 s[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int u = wave + i * NW;
+                    it[i] = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, jt[i] = u - it[i] * (it[i] + 1) / 2;
+                    s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+#pragma unroll
+                for (int k = 0; k < KD; ++k)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) s[i] = M::run(R::rows(tb, 16 * jt[i], k * 32, lane), R::rows(ta, 16 * it[i], k * 32, lane), s[i]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float *by = apart + kTicks - 1 - 16 * (it[i] - jt[i]) - r16 + 4 * kq;   // (past its end in scores that are masked)
+                    f32x4 o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = it[i] > jt[i] || 4 * kq + r <= r16 ? s[i][r] * by[r] : 0.0f;
+                    typedef bf16 four __attribute__((ext_vector_type(4)));
+                    *reinterpret_cast<four *>(lds_p + RP::at(16 * it[i] + r16, 16 * jt[i] + 4 * kq)) = __builtin_convertvector(o, four);
+                }
+            };
+            if (wave < kTiles - (kMost - 1) * NW) scores(std::integral_constant<int, kMost>{});
+            else if constexpr (kMost > 1) scores(std::integral_constant<int, kMost - 1>{});
+        }
+        __syncthreads();
+    };
+
+    if (begin < end) ready(min(end - begin, kTicks), 0);
+    for (int at = begin, buf = 0; at < end; buf ^= 1) {
+        const int n = min(end - at, kTicks), here = at;
+        at += n;
+        if (at < end) fetch(at, min(end - at, kTicks), buf ^ 1);
+        const char *ta = lds_a + (STATES ? 0 : buf * kTile), *tb = lds_b + buf * kTile, *tc = lds_c + buf * kTile;
+        frag fc[KT];
+        uint32_t most = 0;
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+            fc[s] = R::template columns<4>(tc, wc, s * 32, lane);
+            const u32x4 w = __builtin_bit_cast(u32x4, fc[s]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = larger_halves(most, w[e] & 0x7fff7fffu);
+        }
+        const bool odd = (most & 0xffffu) >= 0x7f80u || most >> 16 >= 0x7f80u;
+        if (!STATES && __builtin_amdgcn_ballot_w64(odd)) {
+            // A product with a later tick's 0 is NaN where that tick's c is not finite: the wave goes tick by tick.
+            const float before = power(rate, lead), after = power(rate, 1 - lead);
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                const float c = static_cast<float>(*reinterpret_cast<const bf16 *>(tc + R::at(i, wc + r16))) * in_scale;
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KD; ++k) {
+                    const frag fb = *reinterpret_cast<const frag *>(tb + R::at(i, 32 * k + 8 * kq)), fa = *reinterpret_cast<const frag *>(ta + R::at(i, 32 * k + 8 * kq));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float z = x[2 * k + e / 4][e % 4] * before + static_cast<float>(fb[e]) * c;
+                        sum += static_cast<float>(fa[e]) * z;
+                        x[2 * k + e / 4][e % 4] = z * after;
+                    }
+                }
+                sum += __shfl_xor(sum, 16, kWave);
+                sum += __shfl_xor(sum, 32, kWave);
+                if (kq == 0 && out) out[(back ? len - 1 - here - i : here + i) * out_st + static_cast<int64_t>(bh) * D + wc + r16] = static_cast<bf16>(sum * out_scale);
+            }
+        } else {
+            if (!STATES && out) {
+                // rows c's channels, columns i
+                f32x4 o[TI] = {};
+#pragma unroll
+                for (int k = 0; k < KD; ++k) {
+                    const frag fx = __builtin_convertvector(__builtin_shufflevector(x[2 * k], x[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), frag);
+#pragma unroll
+                    for (int it = 0; it < TI; ++it) o[it] = M::run(fx, R::rows(ta, 16 * it, k * 32, lane), o[it]);
+                }
+#pragma unroll
+                for (int it = 0; it < TI; ++it) o[it] *= across[16 * it + r16];
+#pragma unroll
+                for (int s = 0; s < KT; ++s)
+#pragma unroll
+                    for (int it = 0; it < TI; ++it)
+                        if (s * 32 <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p, 16 * it, s * 32, lane), o[it]);
+                const int64_t by_tick = back ? -out_st : out_st;
+                bf16 *to = out + (back ? len - 1 - here : here) * out_st + out_lane + r16 * by_tick;
+#pragma unroll
+                for (int it = 0; it < TI; ++it)
+                    if (16 * it + r16 < n) *reinterpret_cast<Vec<bf16, 4> *>(to + 16 * it * by_tick) = __builtin_convertvector(o[it], Vec<bf16, 4>);
+            }
+            const float f = power(rate, n);
+#pragma unroll
+            for (int i = 0; i < XT; ++i) x[i] *= f;
+            // The state is float32, but what a matrix instruction multiplies is not: a weighted value is three bfloat16 ones, 24
+            // bits together.
+#pragma unroll
+            for (int s = 0; s < KT; ++s) {
+                typedef float many __attribute__((ext_vector_type(8)));
+                const many w = *reinterpret_cast<const many *>(weight + s * 32 + kq * 8);
+                const u32x4 two = __builtin_bit_cast(u32x4, fc[s]);
+                u32x4 part[3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float lo = low_half(two[e]) * w[2 * e], hi = high_half(two[e]) * w[2 * e + 1];
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        part[q][e] = two_halves(lo, hi);
+                        lo -= low_half(part[q][e]), hi -= high_half(part[q][e]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < XT; ++i) {
+                    const frag fb = R::template columns<8>(tb, 32 * (i / 2) + 4 * (i % 2), s * 32, lane);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) x[i] = M::run(fb, __builtin_bit_cast(frag, part[q]), x[i]);
+                }
+            }
+        }
+        if (at < end) ready(min(end - at, kTicks), buf ^ 1);
+    }
+    // Ticks behind the length are 0.
+    if (!STATES && out) {
+        const int t0 = max(len, seg_first);
+        typedef bf16 many __attribute__((ext_vector_type(8)));
+        for (int u = threadIdx.x; u < (seg_end - t0) * (D / 8); u += NT)
+            *reinterpret_cast<many *>(out + (t0 + u / (D / 8)) * out_st + static_cast<int64_t>(bh) * D + u % (D / 8) * 8) = many{};
+    }
+    if (pass.x_out) {
+        const int64_t x_b = pass.x_b;
+        float *to = pass.x_out + seg * pass.x_seg + bh * pass.x_bh + (wc + r16) * pass.x_c;
+#pragma unroll
+        for (int i = 0; i < XT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[(row(i) + r) * x_b] = x[i][r];
+    }
+#endif
+}
+
 struct JoinArgs {
     float *states;          // [segments][B H][n]: what each segment adds; becomes the state before each
     const float *x;         // [B H][n] before the first, or NULL
@@ -545,16 +796,32 @@ void run_pass(AttArgs a, bool states, hipStream_t s) {
     else hipLaunchKernelGGL((k_attention<T, D, NW, false, WHOLE>), grid, block, 0, s, a);
 }
 
+template <int D, int NW>
+void run_direct(const AttArgs &a, bool states, hipStream_t s) {
+    const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
+    const dim3 grid(static_cast<unsigned>(groups * a.passes)), block(NW * kWave);
+    if (states) hipLaunchKernelGGL((k_attention_direct<D, NW, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_attention_direct<D, NW, false>), grid, block, 0, s, a);
+}
+
+// Whether all of a sequence's heads begin on 16 bytes.
+bool on_16(const AttSeq &q) { return reinterpret_cast<uintptr_t>(q.p) % 16 == 0 && (q.st | q.sb | q.sh) % 8 == 0; }
+
 template <typename T>
 void run_passes(const AttArgs &a, bool states, hipStream_t s) {
     int da = 0, dc = 0;
-    bool whole = true;
+    bool whole = true, direct = std::is_same_v<T, bf16>;
     for (int i = 0; i < a.passes; ++i) {
         const AttPass &p = a.pass[i];
         da = std::max(da, p.b.d), dc = std::max(dc, p.c.d);
         whole = whole && p.b.d == p.c.d && p.c.d == a.pass[0].c.d && !p.wide;
+        direct = direct && on_16(p.a) && on_16(p.b) && on_16(p.c) && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
     }
-    if (whole && dc == 64) {
+    if (direct && whole && dc == 64) {
+        run_direct<64, 4>(a, states, s);
+    } else if (direct && whole && dc == 128) {
+        run_direct<128, 8>(a, states, s);
+    } else if (whole && dc == 64) {
         run_pass<T, 64, 4, true>(a, states, s);
     } else if (whole && dc == 128) {
         run_pass<T, 128, 8, true>(a, states, s);
