@@ -617,21 +617,21 @@ def _head_strides(t):
     return (st if t.shape[0] > 1 else 0), sb, sh
 
 
-def _attention_struct(q, k, v, log_decay, state, lengths, scale, ticks):
-    """glif_attention of tensors with contiguous channels (held by the caller)."""
-    strides = [n for t in (q, k, v) for n in (_head_strides(t) if ticks else (0, *t.stride()[:2]))]
-    return _lib.Attention(_p(q), _p(k), _p(v), _p(log_decay), _p(state), _p(lengths), *strides, scale, DTYPES[q.dtype],
-                          q.shape[0] if ticks else 1, q.shape[-3], q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1])
+def _attention_struct(q, k, v, log_decay, state, lengths, scale, dims):
+    """glif_attention of tensors with contiguous channels (held by the caller) and ``dims`` ticks, entries, heads, groups and
+    channels."""
+    return _lib.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _p(state), _p(lengths), *_head_strides(q),
+                          *_head_strides(k), *_head_strides(v), scale, DTYPES[q.dtype], *dims)
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, lengths, scale):
         ctx.set_materialize_grads(False)
-        (T, B, H, K), V, dev = q.shape, v.shape[-1], q.device
-        held = [_heads(q), _heads(k), _heads(v), _dense(log_decay), _dense(state), lengths]
-        s = _attention_struct(*held, scale, True)
-        y = torch.empty((T, B, H, V), dtype=q.dtype, device=dev)
+        (T, B, H, K), (G, V), dev = q.shape, v.shape[2:], q.device
+        held = (_heads(q), _heads(k), _heads(v), _dense(log_decay), _dense(state), lengths)
+        s = _attention_struct(*held, scale, (T, B, H, G, K, V))
+        y = q.new_empty((T, B, H, V))
         last = torch.empty((B, H, K, V), dtype=torch.float32, device=dev)
         L = lib()
         ws = _workspace(L.glif_attention_fwd_workspace(byref(s)), dev)
@@ -645,14 +645,17 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dy, dlast):
         _first_only("linear_attention")
         q, k, v, log_decay, state, lengths = ctx.saved_tensors
-        (T, B, H, K), V, dev = q.shape, v.shape[-1], q.device
-        held = [_heads(q), _heads(k), _heads(v), _dense(log_decay), _dense(state), lengths]
-        s = _attention_struct(*held, ctx.scale, True)
+        (T, B, H, K), (G, V), dev = q.shape, v.shape[2:], q.device
+        held = (_heads(q), _heads(k), _heads(v), _dense(log_decay), _dense(state), lengths)
+        s = _attention_struct(*held, ctx.scale, (T, B, H, G, K, V))
         dy = _heads(dy) if dy is not None else torch.zeros((T, B, H, V), dtype=q.dtype, device=dev)
         dlast = _dense(dlast)
-        wants = ctx.needs_input_grad
-        dq, dk, dv, dstate = (torch.empty(t.shape, dtype=t.dtype, device=dev) if w else None
-                              for t, w in ((q, wants[0]), (k, wants[1]), (v, wants[2]), (state, wants[4])))
+        wq, wk, wv, _, ws_, _, _ = ctx.needs_input_grad
+        dense = torch.contiguous_format
+        dq = torch.empty_like(q, memory_format=dense) if wq else None
+        dk = torch.empty_like(k, memory_format=dense) if wk else None
+        dv = torch.empty_like(v, memory_format=dense) if wv else None
+        dstate = torch.empty_like(state, memory_format=dense) if ws_ else None
         g = _lib.AttentionGrad(_p(dy), *_head_strides(dy), _p(dlast), _p(dq), _p(dk), _p(dv), _p(dstate))
         L = lib()
         ws = _workspace(L.glif_attention_bwd_workspace(byref(s)), dev)
@@ -710,9 +713,12 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None) -> torch.Tensor
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is written in place")
     _refuse_grad("linear_attention_step", q, state, k, v, log_decay)
-    held = [_heads(q), _heads(k), _heads(v), _dense(log_decay), None, None]
-    s = _attention_struct(*held, scale, False)
-    y = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
+    q, k, v, log_decay = _heads(q), _heads(k), _heads(v), _dense(log_decay)
+    (B, H, K), (G, V) = q.shape, v.shape[1:]
+    (q_sb, q_sh, _), (k_sb, k_sh, _), (v_sb, v_sh, _) = q.stride(), k.stride(), v.stride()
+    s = _lib.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), None, None, 0, q_sb, q_sh, 0, k_sb, k_sh, 0,
+                       v_sb, v_sh, scale, DTYPES[q.dtype], 1, B, H, G, K, V)
+    y = q.new_empty((B, H, V))
     with _on(q.device):
         check(lib().glif_attention_step(byref(s), _p(y), _p(state), _stream(q.device)))
     torch.autograd.graph.increment_version(state)
