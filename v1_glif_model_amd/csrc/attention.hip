@@ -508,11 +508,11 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
     constexpr int kTicks = 64, TI = 4, KT = 2, KD = D / 32, XT = D / 16, NT = NW * kWave, kTile = kTicks * R::kBytes;
     constexpr int kLoad = 16 * kWave, kN = kTile / kLoad / NW, kAcross = R::kBytes / 16;   // bytes of a wave's load, a wave's loads, lanes of a row
     static_assert(D == 16 * NW && kN * kLoad * NW == kTile, "the tiles divide among the waves");
-    __shared__ __attribute__((aligned(1024))) char lds_a[STATES ? 16 : 2 * kTile];
-    __shared__ __attribute__((aligned(1024))) char lds_b[2 * kTile];
-    __shared__ __attribute__((aligned(1024))) char lds_c[2 * kTile];
+    // two of each, by names of their own: reads of the one must not wait for loads to the other
+    __shared__ __attribute__((aligned(1024))) char a0[STATES ? 16 : kTile], a1[STATES ? 16 : kTile];
+    __shared__ __attribute__((aligned(1024))) char b0[kTile], b1[kTile], c0[kTile], c1[kTile];
     __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * RP::kBytes];
-    __shared__ __attribute__((aligned(32))) float weight[kTicks];
+    __shared__ f32x4 weight[kTicks / 4];
     __shared__ float apart[STATES ? 1 : kTicks + 16], across[STATES ? 1 : kTicks];
 
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
@@ -549,12 +549,12 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr)(to + inst * kLoad), 16, off, 0, 0, 0);
         }
     };
-    auto fetch = [&](int at, int n, int buf) {
-        if (!STATES) bring(pa, a_st, at, n, lds_a + buf * kTile);
-        bring(pb, b_st, at, n, lds_b + buf * kTile);
-        bring(pc, c_st, at, n, lds_c + buf * kTile);
+    auto fetch = [&](int at, int n, char *ta, char *tb, char *tc) {
+        if (!STATES) bring(pa, a_st, at, n, ta);
+        bring(pb, b_st, at, n, tb);
+        bring(pc, c_st, at, n, tc);
     };
-    if (begin < end) fetch(begin, min(end - begin, kTicks), 0);
+    if (begin < end) fetch(begin, min(end - begin, kTicks), a0, b0, c0);
 
     // state: x[i][r] is of b's channel row(i) + r and c's channel wc + r16
     auto row = [&](int i) { return 32 * (i / 2) + 8 * kq + 4 * (i % 2); };
@@ -583,24 +583,23 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
 
     // What has to be there before a chunk is gone through: its tiles, without what is behind its n ticks, its weights and
     // scores.
-    auto ready = [&](int n, int buf) {
+    auto ready = [&](int n, char *ta, char *tb, char *tc) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (n < kTicks) {
             for (int u = threadIdx.x; u < (kTicks - n) * R::kBytes / 4; u += NT) {
-                const int at = buf * kTile + n * R::kBytes + u * 4;
-                if (!STATES) *reinterpret_cast<uint32_t *>(lds_a + at) = 0u;
-                *reinterpret_cast<uint32_t *>(lds_b + at) = 0u;
-                *reinterpret_cast<uint32_t *>(lds_c + at) = 0u;
+                const int at = n * R::kBytes + u * 4;
+                if (!STATES) *reinterpret_cast<uint32_t *>(ta + at) = 0u;
+                *reinterpret_cast<uint32_t *>(tb + at) = 0u;
+                *reinterpret_cast<uint32_t *>(tc + at) = 0u;
             }
             __syncthreads();
         }
         if (threadIdx.x < kTicks) {
             const int j = threadIdx.x;
-            weight[j] = j < n ? power(rate, n - lead - j) * in_scale : 0.0f;
+            weight[j / 4][j % 4] = j < n ? power(rate, n - lead - j) * in_scale : 0.0f;
         }
         if (!STATES) {
-            const char *ta = lds_a + buf * kTile, *tb = lds_b + buf * kTile;
             constexpr int kTiles = TI * (TI + 1) / 2, kMost = (kTiles + NW - 1) / NW;
             auto scores = [&](auto count) {   // of the wave's tiles wave, wave + NW, ..: their products are taken together
                 constexpr int N = decltype(count)::value;
@@ -632,12 +631,11 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
         __syncthreads();
     };
 
-    if (begin < end) ready(min(end - begin, kTicks), 0);
-    for (int at = begin, buf = 0; at < end; buf ^= 1) {
+    int at = begin;
+    auto chunk = [&](const char *ta, const char *tb, const char *tc, char *na, char *nb, char *nc) {   // and the next one's tiles
         const int n = min(end - at, kTicks), here = at;
         at += n;
-        if (at < end) fetch(at, min(end - at, kTicks), buf ^ 1);
-        const char *ta = lds_a + (STATES ? 0 : buf * kTile), *tb = lds_b + buf * kTile, *tc = lds_c + buf * kTile;
+        if (at < end) fetch(at, min(end - at, kTicks), na, nb, nc);
         frag fc[KT];
         uint32_t most = 0;
 #pragma unroll
@@ -699,13 +697,12 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
             // bits together.
 #pragma unroll
             for (int s = 0; s < KT; ++s) {
-                typedef float many __attribute__((ext_vector_type(8)));
-                const many w = *reinterpret_cast<const many *>(weight + s * 32 + kq * 8);
+                const f32x4 w4[2] = {weight[s * 8 + kq * 2], weight[s * 8 + kq * 2 + 1]};
                 const u32x4 two = __builtin_bit_cast(u32x4, fc[s]);
                 u32x4 part[3];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float lo = low_half(two[e]) * w[2 * e], hi = high_half(two[e]) * w[2 * e + 1];
+                    float lo = low_half(two[e]) * w4[e / 2][e % 2 * 2], hi = high_half(two[e]) * w4[e / 2][e % 2 * 2 + 1];
 #pragma unroll
                     for (int q = 0; q < 3; ++q) {
                         part[q][e] = two_halves(lo, hi);
@@ -720,7 +717,12 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
                 }
             }
         }
-        if (at < end) ready(min(end - at, kTicks), buf ^ 1);
+        if (at < end) ready(min(end - at, kTicks), na, nb, nc);
+    };
+    if (begin < end) ready(min(end - begin, kTicks), a0, b0, c0);
+    while (at < end) {
+        chunk(a0, b0, c0, a1, b1, c1);
+        if (at < end) chunk(a1, b1, c1, a0, b0, c0);
     }
     // Ticks behind the length are 0.
     if (!STATES && out) {
