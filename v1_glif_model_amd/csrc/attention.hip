@@ -498,14 +498,14 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
 
 // The same for bfloat16 heads of D = 16 NW channels in all three sequences, on 16 bytes, of which the tiles go to LDS without
 // registers, a chunk ahead: two of each, and two barriers a chunk.
-template <int D, int NW, bool STATES>
-__global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args) {
+template <int D, int NW, int TICKS, bool STATES>
+__global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_attention_direct(AttArgs args) {
 #ifdef __HIP_DEVICE_COMPILE__
     using M = Mma<bf16>;
     typedef M::frag frag;
     using R = Rows<bf16, D>;
-    using RP = Rows<bf16, 64>;
-    constexpr int kTicks = 64, TI = 4, KT = 2, KD = D / 32, XT = D / 16, NT = NW * kWave, kTile = kTicks * R::kBytes;
+    using RP = Rows<bf16, TICKS>;
+    constexpr int kTicks = TICKS, TI = TICKS / 16, KT = TICKS / 32, KD = D / 32, XT = D / 16, NT = NW * kWave, kTile = kTicks * R::kBytes;
     constexpr int kLoad = 16 * kWave, kN = kTile / kLoad / NW, kAcross = R::kBytes / 16;   // bytes of a wave's load, a wave's loads, lanes of a row
     static_assert(D == 16 * NW && kN * kLoad * NW == kTile, "the tiles divide among the waves");
     // two of each, by names of their own: reads of the one must not wait for loads to the other
@@ -584,10 +584,13 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
     // What has to be there before a chunk is gone through: its tiles, without what is behind its n ticks, its weights and
     // scores.
     auto ready = [&](int n, char *ta, char *tb, char *tc) {
+        int l = lane, tid = threadIdx.x;
+        if (TICKS == 32) asm volatile("" : "+v"(l), "+v"(tid));   // addresses are made again for every chunk: kept, they take more registers than two blocks have
+        const int r16 = l % 16, kq = l / 16;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (n < kTicks) {
-            for (int u = threadIdx.x; u < (kTicks - n) * R::kBytes / 4; u += NT) {
+            for (int u = tid; u < (kTicks - n) * R::kBytes / 4; u += NT) {
                 const int at = n * R::kBytes + u * 4;
                 if (!STATES) *reinterpret_cast<uint32_t *>(ta + at) = 0u;
                 *reinterpret_cast<uint32_t *>(tb + at) = 0u;
@@ -595,8 +598,8 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
             }
             __syncthreads();
         }
-        if (threadIdx.x < kTicks) {
-            const int j = threadIdx.x;
+        if (tid < kTicks) {
+            const int j = tid;
             weight[j / 4][j % 4] = j < n ? power(rate, n - lead - j) * in_scale : 0.0f;
         }
         if (!STATES) {
@@ -614,7 +617,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
 #pragma unroll
                 for (int k = 0; k < KD; ++k)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) s[i] = M::run(R::rows(tb, 16 * jt[i], k * 32, lane), R::rows(ta, 16 * it[i], k * 32, lane), s[i]);
+                    for (int i = 0; i < N; ++i) s[i] = M::run(R::rows(tb, 16 * jt[i], k * 32, l), R::rows(ta, 16 * it[i], k * 32, l), s[i]);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float *by = apart + kTicks - 1 - 16 * (it[i] - jt[i]) - r16 + 4 * kq;   // (past its end in scores that are masked)
@@ -634,13 +637,16 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
     int at = begin;
     auto chunk = [&](const char *ta, const char *tb, const char *tc, char *na, char *nb, char *nc) {   // and the next one's tiles
         const int n = min(end - at, kTicks), here = at;
+        int l = lane;
+        if (TICKS == 32) asm volatile("" : "+v"(l));
+        const int r16 = l % 16, kq = l / 16;
         at += n;
         if (at < end) fetch(at, min(end - at, kTicks), na, nb, nc);
         frag fc[KT];
         uint32_t most = 0;
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
-            fc[s] = R::template columns<4>(tc, wc, s * 32, lane);
+            fc[s] = R::template columns<4>(tc, wc, s * 32, l);
             const u32x4 w = __builtin_bit_cast(u32x4, fc[s]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) most = larger_halves(most, w[e] & 0x7fff7fffu);
@@ -675,7 +681,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
                 for (int k = 0; k < KD; ++k) {
                     const frag fx = __builtin_convertvector(__builtin_shufflevector(x[2 * k], x[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), frag);
 #pragma unroll
-                    for (int it = 0; it < TI; ++it) o[it] = M::run(fx, R::rows(ta, 16 * it, k * 32, lane), o[it]);
+                    for (int it = 0; it < TI; ++it) o[it] = M::run(fx, R::rows(ta, 16 * it, k * 32, l), o[it]);
                 }
 #pragma unroll
                 for (int it = 0; it < TI; ++it) o[it] *= across[16 * it + r16];
@@ -683,7 +689,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
                 for (int s = 0; s < KT; ++s)
 #pragma unroll
                     for (int it = 0; it < TI; ++it)
-                        if (s * 32 <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p, 16 * it, s * 32, lane), o[it]);
+                        if (s * 32 <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p, 16 * it, s * 32, l), o[it]);
                 const int64_t by_tick = back ? -out_st : out_st;
                 bf16 *to = out + (back ? len - 1 - here : here) * out_st + out_lane + r16 * by_tick;
 #pragma unroll
@@ -711,7 +717,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention_direct(AttArgs args)
                 }
 #pragma unroll
                 for (int i = 0; i < XT; ++i) {
-                    const frag fb = R::template columns<8>(tb, 32 * (i / 2) + 4 * (i % 2), s * 32, lane);
+                    const frag fb = R::template columns<8>(tb, 32 * (i / 2) + 4 * (i % 2), s * 32, l);
 #pragma unroll
                     for (int q = 0; q < 3; ++q) x[i] = M::run(fb, __builtin_bit_cast(frag, part[q]), x[i]);
                 }
@@ -798,12 +804,21 @@ void run_pass(AttArgs a, bool states, hipStream_t s) {
     else hipLaunchKernelGGL((k_attention<T, D, NW, false, WHOLE>), grid, block, 0, s, a);
 }
 
+// Chunks of 64 ticks are the faster for blocks that are alone on their compute unit, of 32 leave room for others (500 x 32 ticks
+// of 8 heads of 128, 256 blocks forward, 37 us and 43, 768 backward, trials of any length, 82 and 69; of 16 heads of 64, 512 and
+// 1536 blocks, 32 and 37, 84 and 75).
 template <int D, int NW>
 void run_direct(const AttArgs &a, bool states, hipStream_t s) {
     const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
     const dim3 grid(static_cast<unsigned>(groups * a.passes)), block(NW * kWave);
-    if (states) hipLaunchKernelGGL((k_attention_direct<D, NW, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_attention_direct<D, NW, false>), grid, block, 0, s, a);
+    const bool few = groups * a.passes <= (NW == 8 ? 256 : 512);
+    if (states) {
+        if (few) hipLaunchKernelGGL((k_attention_direct<D, NW, 64, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_attention_direct<D, NW, 32, true>), grid, block, 0, s, a);
+    } else {
+        if (few) hipLaunchKernelGGL((k_attention_direct<D, NW, 64, false>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_attention_direct<D, NW, 32, false>), grid, block, 0, s, a);
+    }
 }
 
 // Whether all of a sequence's heads begin on 16 bytes.
@@ -929,14 +944,15 @@ int check_attention(const glif_attention *a, bool step) {
 }
 
 // Ticks in segments where there are too few blocks for the chip: a first launch gives the state that each segment adds,
-// a second joins them, and then all segments go at once.  The first reads two of three sequences again.  As many segments
-// as blocks are there at once, one a compute unit where heads have more than 64 channels, three where not (8000 ticks of 16 heads
-// of 128 in 25 segments, two rounds of blocks, 89 us, in 16 SEG_US), and none of fewer than four chunks.
+// a second joins them, and then all segments go at once.  The first reads two of three sequences again and takes more than
+// half as long, so that two segments gain nothing (500 x 16 ticks of 8 heads of 128 in two 52 us, in one 37).  As many segments as
+// blocks are there at once, one a compute unit where heads have more than 64 channels, three where not (8000 ticks of 16 heads of
+// 128 in 25 segments, two rounds of blocks, 89 us, in 16 76), and none of fewer than four chunks.
 void cut(AttArgs &a, int64_t blocks, int ticks, const glif_attention *s) {
     a.segments = 1, a.seg_ticks = std::max((a.T + ticks - 1) / ticks, 1) * ticks;
     const int64_t slots = std::max(s->d_key, s->d_value) > 64 ? 256 : 768;
     const int64_t chunks = (a.T + ticks - 1) / ticks, want = blocks ? std::min<int64_t>(slots / blocks, chunks / 4) : 0;
-    if (want < 2) return;
+    if (want < 3) return;
     a.seg_ticks = static_cast<int>((chunks + want - 1) / want) * ticks;
     a.segments = (a.T + a.seg_ticks - 1) / a.seg_ticks;
 }
