@@ -7,7 +7,8 @@ Python mirror of the reference interface:
   ops.make_pre_ind_table, ops.calculate_synaptic_currents   (models.py:103-373)
   models.V1Column                                          (models.py:450-1135)
 Sequence operators and the readout that is trained with the column and runs beside it:
-  sequence.layer_norm, dropout, linear, short_conv, state_space_scan; readout.SequenceReadout
+  sequence.layer_norm, dropout, linear, gated_linear, short_conv, state_space_scan, linear_attention;
+  readout.SequenceReadout; optim.AdamW
 Synthetic networks of the benchmark configurations: synthetic.make_network.
 """
 __version__ = "0.1.0"

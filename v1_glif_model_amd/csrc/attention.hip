@@ -9,6 +9,11 @@
 //   dk = F(v, dy, scale q; dS^T)                 lead 0, time backwards: the gradient of the last state comes undecayed to the
 //   dv = F(k, scale q, dy; dS)                   last tick, and what is left behind the first is dS0
 // No power is of a negative exponent, so no decay, 0 among them, can overflow.
+//
+// Bound by latency within a chunk: 500 x 32 ticks of 8 heads of 128, bfloat16, trials of any length, 38 us forward (a block
+// of eight waves alone on its compute unit; 8.0k cycles a chunk of 64 ticks, of which the matrix instructions are 2.5k), 69 us for
+// the backward's three passes; of 32 heads, all ticks, 148 us (3.5 TB/s) and 363 (4.3 TB/s, 9 sequences read and 3 written).
+// In float32 (its products at 1/16 of the rate) 290 x 18 ticks of 4 heads of 128 and 64 50 us.
 #include <type_traits>
 
 #include "mma.h"
@@ -861,7 +866,8 @@ void run_share(const float *in, int64_t rows, int groups, int share, int d, void
                        in, rows, groups, share, d, static_cast<T *>(out));
 }
 
-// One tick: a block takes 32 of v's channels of an entry and head, 8 lanes by 32 lots of k's channels.
+// One tick, bound by the state's way to the registers and back (32 entries of 8 heads of 64 x 64, 8.4 MB, 4.6 us of which a launch
+// is 4): a block takes 32 of v's channels of an entry and head, 8 lanes by 32 lots of k's channels.
 struct StepArgs {
     const void *q, *k, *v;
     int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;

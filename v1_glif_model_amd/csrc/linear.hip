@@ -7,6 +7,12 @@
 // of 2500); short ones and ones of few tiles by the fill and drain of their blocks and by the way of their operands from memory
 // (2500 x 66000 x 512 bfloat16, each in a loop of its own: forward 222 us, dx 259, dW 178; after each other in a training step
 // 227, 303 and 202); single ticks by the stream of the weights.
+//
+// The gated projection is the same product of rows taken in turns, with both arguments of a result in one lane: y = act(g) u.
+// 16000 x 1024 x 4096 bfloat16 forward 390 us: a tile of 256 x 256 is 30 us of products and 16 of results, 320 KB of them, since
+// both arguments are kept in float32 (evaluation, which keeps neither, 320; two products and the activation by themselves 387);
+// backward 168 us for the gradients at the arguments (5.5 TB/s), 230 for dx and 237 for dW.  2500 x 512 x 1365 float16 forward 18
+// us, 5 x 1024 x 4096 bfloat16 8.7.
 #include "mma.h"
 
 namespace glif {
@@ -200,7 +206,8 @@ struct FinishGated {
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) u[e] *= act_of(g[e], a.act);
-        Finish<T>::write(static_cast<T *>(a.c) + m * a.ldc + n, u, have, a.past);
+        // not past the caches: a wave's rows are half a cache line (16000 x 1024 x 4096 with gradients 984 us, so 957)
+        Finish<T>::write(static_cast<T *>(a.c) + m * a.ldc + n, u, have, 0);
     }
 };
 
