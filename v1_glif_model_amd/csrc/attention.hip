@@ -40,7 +40,7 @@ struct AttPass {
 
 struct AttArgs {
     AttPass pass[3];
-    int32_t passes, tiles;         // tiles of c's channels
+    int32_t passes;
     const float *log_decay;
     const int32_t *lengths;
     int32_t T, B, H, segments, seg_ticks;
@@ -233,7 +233,6 @@ struct Tile {
     }
 };
 
-
 // Two bfloat16 in 32 bits.
 __device__ __forceinline__ float low_half(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
@@ -248,7 +247,7 @@ __device__ __forceinline__ uint32_t two_halves(float lo, float hi) {   // to nea
 }
 #endif
 
-// A block takes one entry and head, 16 of c's channels a wave and one segment of the ticks, chunk by chunk; each wave keeps the
+// A block takes one pass of one entry and head, 16 of c's channels a wave, and one segment of the ticks, chunk by chunk; each wave keeps the
 // state of its channels in registers, as a matrix product's result and the next one's operand (which of b's channels a row of it
 // is, is chosen so that a lane's values are kPer neighbours).  STATES: no outputs, only the state that the segment adds to
 // nothing.
@@ -277,32 +276,30 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
 
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
     // The blocks that read the same sequences are on one XCD (block id mod 8), after each other.
-    const int kin = args.tiles * args.passes, slot = static_cast<int>(blockIdx.x >> 3);
-    const int64_t group = static_cast<int64_t>(slot / kin) * 8 + (blockIdx.x & 7);
+    const int passes = args.passes, slot = static_cast<int>(blockIdx.x >> 3);
+    const int64_t group = static_cast<int64_t>(slot / passes) * 8 + (blockIdx.x & 7);
     if (group >= static_cast<int64_t>(args.B) * args.H * args.segments) return;
-    const AttPass &pass = args.pass[slot % kin / args.tiles];
-    const int tile = slot % args.tiles, seg = static_cast<int>(group % args.segments);
+    const AttPass &pass = args.pass[slot % passes];
+    const int seg = static_cast<int>(group % args.segments);
     const int bh = static_cast<int>(group / args.segments), b = bh / args.H, h = bh % args.H;
-    const int c0 = WHOLE ? 0 : tile * W, dc = WHOLE ? W : pass.c.d, db = WHOLE ? D : pass.b.d;
-    if (c0 >= dc) return;
-    const int T_ = args.T, len = live_ticks(args.lengths, b, T_), seg_first = seg * args.seg_ticks, seg_end = min(T_, seg_first + args.seg_ticks);
+    const int dc = WHOLE ? W : pass.c.d, db = WHOLE ? D : pass.b.d;
+    const int len = live_ticks(args.lengths, b, args.T), seg_first = seg * args.seg_ticks, seg_end = min(args.T, seg_first + args.seg_ticks);
     const int begin = min(seg_first, len), end = min(seg_end, len);
     const float rate = args.log_decay[h] * 1.4426950408889634f;
-    const int wc = c0 + wave * 16;       // the wave's first channel
+    const int wc = wave * 16;            // the wave's first channel
     const bool active = wc < dc, back = pass.back, wide = !WHOLE && pass.wide;
     const int lead = pass.lead;
     const float in_scale = pass.in_scale, out_scale = pass.out_scale;
     const int64_t out_st = static_cast<int64_t>(args.B) * args.H * dc;
-    // out: the lane's four channels of tick r16, in ticks from the segment's first
     void *const out = pass.out;
-    const int64_t out_lane = static_cast<int64_t>(bh) * dc + wc + 4 * kq;
-    const int have = dc - wc - 4 * kq;
+    const int64_t out_lane = static_cast<int64_t>(bh) * dc + wc + 4 * kq;   // of the four channels that the lane writes
+    const int have = dc - wc - 4 * kq;                                      // those that are there
 
     TD ra, rb;
     TC rc;
     if (!STATES) ra.init(lds_a, static_cast<const T *>(pass.a.p) + b * pass.a.sb + h / pass.a.share * pass.a.sh, pass.a.st, back, db);
     rb.init(lds_b, static_cast<const T *>(pass.b.p) + b * pass.b.sb + h / pass.b.share * pass.b.sh, pass.b.st, back, db);
-    rc.init(lds_c, static_cast<const T *>(pass.c.p) + b * pass.c.sb + h / pass.c.share * pass.c.sh + c0, pass.c.st, back, min(dc - c0, W));
+    rc.init(lds_c, static_cast<const T *>(pass.c.p) + b * pass.c.sb + h / pass.c.share * pass.c.sh, pass.c.st, back, dc);
     auto fetch = [&](int at, int n) {
         const int64_t first = back ? len - 1 - at : at;
         if (!STATES) ra.load(first, n);
@@ -482,9 +479,9 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     }
     // Ticks behind the length are 0.
     if (!STATES && out) {
-        const int t0 = max(len, seg_first), w = min(W, dc - c0);
-        for (int u = threadIdx.x; u < (seg_end - t0) * w; u += NT) {
-            const int64_t to = (t0 + u / w) * out_st + static_cast<int64_t>(bh) * dc + c0 + u % w;
+        const int t0 = max(len, seg_first);
+        for (int u = threadIdx.x; u < (seg_end - t0) * dc; u += NT) {
+            const int64_t to = (t0 + u / dc) * out_st + static_cast<int64_t>(bh) * dc + u % dc;
             if (wide) static_cast<float *>(out)[to] = 0.0f;
             else static_cast<T *>(out)[to] = T(0.0f);
         }
@@ -799,12 +796,9 @@ __global__ void __launch_bounds__(kBlock) k_attention_share(const float *in, int
 }
 
 template <typename T, int D, int NW, bool WHOLE>
-void run_pass(AttArgs a, bool states, hipStream_t s) {
-    int widest = 0;
-    for (int i = 0; i < a.passes; ++i) widest = std::max(widest, a.pass[i].c.d);
-    a.tiles = ceil_div(widest, 16 * NW);
+void run_pass(const AttArgs &a, bool states, hipStream_t s) {
     const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
-    const dim3 grid(static_cast<unsigned>(groups * a.tiles * a.passes)), block(NW * kWave);
+    const dim3 grid(static_cast<unsigned>(groups * a.passes)), block(NW * kWave);
     if (states) hipLaunchKernelGGL((k_attention<T, D, NW, true, WHOLE>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((k_attention<T, D, NW, false, WHOLE>), grid, block, 0, s, a);
 }
@@ -973,8 +967,7 @@ AttArgs common(const glif_attention *s) {
 
 AttArgs forward_args(const glif_attention *s) {
     AttArgs a = common(s);
-    const int64_t tiles = s->d_value <= 64 ? 1 : (s->d_value + 127) / 128;
-    cut(a, static_cast<int64_t>(a.B) * a.H * tiles, chunk_ticks(s->dtype), s);
+    cut(a, static_cast<int64_t>(a.B) * a.H, chunk_ticks(s->dtype), s);
     return a;
 }
 
