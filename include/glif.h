@@ -304,7 +304,7 @@ int glif_rate_dist_loss(const int32_t *count, int32_t count_rows, int32_t n_neur
  *   - Gradient outputs may be NULL where they are not wanted.
  *   - Sizes beyond these are refused (GLIF_EINVAL): layer norm 2^31 - 1 rows and columns; linear M and N of 2^21, K of 2^24 - 1;
  *     sequences of 2^20 ticks, batches of 65535; the scan's 2^24 channels, 2^24 - 1 groups and 64 states; the attention's 4096
- *     heads, 2^20 heads of a batch, 128 channels of a head and 2^24 - 1 elements from tick to tick. */
+ *     heads, 2^20 heads of a batch, 128 channels of a head and 2^24 - 1 elements from tick to tick, in y too. */
 typedef enum { GLIF_F32 = 0, GLIF_BF16 = 1, GLIF_F16 = 2 } glif_dtype;
 typedef enum { GLIF_ACT_NONE = 0, GLIF_ACT_RELU = 1, GLIF_ACT_GELU = 2, GLIF_ACT_SILU = 3 } glif_activation;
 

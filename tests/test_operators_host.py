@@ -54,6 +54,16 @@ def test_attention_refuses(kw):
     refused(L.glif_attention_step(attention(**kw), 1 << 22, 1 << 23, None))
 
 
+def test_attention_refuses_results_whose_gradient_it_would_refuse():
+    """Narrow queries and shared values, wide results: 2^24 elements from tick to tick in y, fewer in q, k and v."""
+    L, wide = _lib.lib(), dict(n_batch=2 ** 13, n_heads=16, n_groups=1, d_key=8, d_value=128, q_st=2 ** 20, k_st=2 ** 16, v_st=2 ** 20)
+    refused(L.glif_attention_fwd(attention(**wide), 1 << 22, None, None, 0, None), "2^24")
+    assert L.glif_attention_fwd_workspace(attention(**wide)) == 0
+    refused(L.glif_attention_bwd(attention(**wide), C.byref(_lib.AttentionGrad(dy=1 << 21)), None, 0, None), "2^24")
+    for fits in (dict(wide, n_ticks=1), dict(wide, n_batch=2 ** 13 - 1)):   # without an output's address they get as far as that
+        refused(L.glif_attention_fwd(attention(**fits), None, None, None, 0, None), "NULL")
+
+
 def test_attention_refuses_missing_outputs_and_workspaces():
     L, g = _lib.lib(), _lib.AttentionGrad(dq=1 << 21)
     refused(L.glif_attention_fwd(attention(), None, None, None, 0, None), "NULL")

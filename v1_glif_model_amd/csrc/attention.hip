@@ -933,6 +933,8 @@ int check_attention(const glif_attention *a, bool step) {
         return fail(GLIF_EINVAL, "attention: at most 2^20 ticks, a batch of 65535 and 4096 heads");
     const int64_t most = std::max({a->q_st, a->k_st, a->v_st}), least = std::min({a->q_st, a->k_st, a->v_st});
     if (!step && (most >= (1 << 24) || least < 0)) return fail(GLIF_EINVAL, "attention: strides of ticks must be in [0, 2^24)");
+    if (!step && a->n_ticks > 1 && static_cast<int64_t>(a->n_batch) * a->n_heads * std::max(a->d_value, 0) >= (1 << 24))
+        return fail(GLIF_EINVAL, "attention: a tick of y must have fewer than 2^24 elements");
     if (a->n_groups < 1 || a->n_heads % a->n_groups) return fail(GLIF_EINVAL, "attention: n_groups must divide n_heads");
     if (a->d_key < 1 || a->d_key > 128 || a->d_value < 1 || a->d_value > 128)
         return fail(GLIF_EINVAL, "attention: keys and values have 1 to 128 channels");

@@ -689,7 +689,7 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     q [T, B, H, K], k [T, B, G, K], v [T, B, G, V] (K and V at most 128; H / G heads share a k and a v); log_decay [H]
     float32, at most 0, -inf for a head that sees only its own tick, a constant without a gradient; ``scale`` K^-0.5 if None;
     initial_state [B, H, K, V] float32 or None.  Returns y [T, B, H, V] and the state [B, H, K, V] after each batch entry's
-    last tick.
+    last tick.  At most 4096 heads, B H 2^20, and B H V and B H K below 2^24 where there is more than one tick.
 
     Ticks are taken in chunks, as matrix products.  Those of bfloat16 sequences multiply scores and states rounded to bfloat16
     (their sums, and the states themselves, are float32); those of float16 ones are float32, as states and scores go beyond
