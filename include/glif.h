@@ -446,6 +446,7 @@ int glif_exp_adam(float *w, float *m, float *v, float *vhat, const float *g, con
  *   state_bits 8: first int8, second uint8, with a float32 scale for every 256 elements: m = s (c / 127) |c / 127|,
  *     v = s (c / 255)^4, rounded to the code below or above by the halves of word (t - 1) home(n_vars) + home(i) + k of the
  *     Philox stream seed, so that the mean is kept; v > 0 does not become 0.
+ * epsilon is at least 1e-12: squares below float32's normal numbers are 0 to v.
  * device: first and second on 16 bytes; iterations [2] int64, the steps done and 0, counted on by the call (by none without
  * a gradient), so that a captured call goes on.
  * glif_adamw_values: the values of n (a multiple of 256) codes. */

@@ -258,3 +258,23 @@ def test_refusals():
                    dict(first=AdamW(opt.variables, state_bits=8).state_dict()["first"])):
         with pytest.raises(ValueError):
             opt.load_state_dict({**state, **change})
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 9e-13, float("inf"), float("nan")])
+def test_refuses_an_epsilon_below_what_squares_leave(eps):
+    from v1_glif_model_amd.optim import AdamW
+    with pytest.raises(ValueError, match="epsilon"):
+        AdamW([rnd(0, (4,))], epsilon=eps)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_smallest_epsilon_and_gradients_whose_squares_vanish(bits):
+    """Gradients of 1e-30 to 1e-18 and 0, of which the update is m size / epsilon to what is left of sqrt(v): the second moment of
+    the largest, 1e-36 (1 - b2) = 1e-38, has a root of 1e-19 and, made up for (1 - b2 = 0.01), 1e-18; that is 1e-6 of epsilon."""
+    from v1_glif_model_amd.optim import AdamW
+    p = torch.zeros(1024, device=DEV)
+    g = torch.cat([torch.zeros(256), torch.logspace(-30, -18, 256), torch.full((256,), 1e-20), -torch.logspace(-25, -19, 256)]).to(DEV)
+    AdamW([p], LR, B1, B2, 1e-12, 0.0, state_bits=bits).apply_gradients([g])
+    assert not p[:256].any()
+    # the first step takes its gradient itself for m / (1 - b1), before a moment is ever a code
+    near(p, -LR * host(g) / 1e-12, (1e-6 + 24 * U) * LR * np.abs(host(g)) / 1e-12, bits)

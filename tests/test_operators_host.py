@@ -27,6 +27,13 @@ def test_adamw_refuses(kw):
     refused(adamw(**kw), "NULL" if None in kw.values() else "adamw")
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 9e-13, float("inf"), float("nan")])
+def test_adamw_refuses_an_epsilon_that_the_squares_of_float32_do_not_reach(eps):
+    """A gradient of 1e-20 has a square of 0 there: without the epsilon its step would be one of 1e-20 / 0."""
+    refused(adamw(eps=eps), "epsilon")
+    assert adamw(eps=1e-12, grad=None) == 0
+
+
 def test_adamw_without_work():
     """No variables, no gradient, no elements: nothing to do, and no GPU needed."""
     assert adamw(n=0) == 0 and adamw(grad=None) == 0 and adamw(size=0) == 0

@@ -315,7 +315,10 @@ extern "C" int glif_adamw(int32_t n_vars, void *const *vars, const int32_t *var_
                           double beta_2, double epsilon, double weight_decay, uint64_t seed, void *stream) {
     if (n_vars < 0 || (state_bits != 8 && state_bits != 32)) return fail(GLIF_EINVAL, "adamw: n_vars must be >= 0 and state_bits 8 or 32");
     if (!(beta_1 >= 0.0 && beta_1 < 1.0 && beta_2 >= 0.0 && beta_2 < 1.0)) return fail(GLIF_EINVAL, "adamw: the betas must be in [0, 1)");
-    if (!(epsilon >= 0.0 && weight_decay >= 0.0)) return fail(GLIF_EINVAL, "adamw: epsilon and weight_decay must be >= 0");
+    // What v keeps of gradients below some 1e-19 is 0 (their squares are below float32's normal numbers): beside an epsilon of 1e-12
+    // their roots are nothing.
+    if (!(epsilon >= 1e-12 && std::isfinite(epsilon) && weight_decay >= 0.0))
+        return fail(GLIF_EINVAL, "adamw: epsilon must be finite and at least 1e-12, weight_decay >= 0");
     if (n_vars == 0) return GLIF_OK;
     if (!vars || !var_dtypes || !grads || !grad_dtypes || !sizes) return fail(GLIF_EINVAL, "NULL argument");
     int64_t total = 0, given = 0;

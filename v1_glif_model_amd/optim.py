@@ -110,7 +110,8 @@ class AdamW:
     ``variables``: contiguous float32, bfloat16 or float16 tensors of one GPU, updated in place (16-bit ones rounded to nearest).
     ``state_bits``: 32, or 8 for moments of a byte each with a float32 scale for every 256: m as ``s (c / 127) |c / 127|`` and v
     as ``s (c / 255)^4``, rounded up or down by words of the Philox stream ``seed`` so that their mean is kept.  A gradient that is
-    not finite makes its variable's moments so, in 8 bits those of all 256.
+    not finite makes its variable's moments so, in 8 bits those of all 256.  The square of one below some 1e-19 is 0 to v, so
+    ``epsilon`` is at least 1e-12.
 
     The count of steps lies on the device: a captured step that is replayed goes on counting.  It keeps the ``learning_rate``
     that it was captured with; eager steps read the attribute each time."""
@@ -128,9 +129,9 @@ class AdamW:
         for what, b in (("beta_1", beta_1), ("beta_2", beta_2)):
             if not 0.0 <= b < 1.0:
                 raise ValueError(f"{what} must be in [0, 1), got {b}")
-        for what, b in (("epsilon", epsilon), ("weight_decay", weight_decay)):
-            if not 0.0 <= b < math.inf:
-                raise ValueError(f"{what} must be >= 0 and finite, got {b}")
+        for what, b, least in (("epsilon", epsilon, 1e-12), ("weight_decay", weight_decay, 0.0)):
+            if not least <= b < math.inf:
+                raise ValueError(f"{what} must be >= {least:g} and finite, got {b}")
         dev = getattr(self.variables[0], "device", None)
         for p in self.variables:
             self._check(p)
