@@ -278,3 +278,15 @@ def test_smallest_epsilon_and_gradients_whose_squares_vanish(bits):
     assert not p[:256].any()
     # the first step takes its gradient itself for m / (1 - b1), before a moment is ever a code
     near(p, -LR * host(g) / 1e-12, (1e-6 + 24 * U) * LR * np.abs(host(g)) / 1e-12, bits)
+
+
+def test_refuses_sparse_gradients_and_variables():
+    from v1_glif_model_amd.optim import AdamW
+    p = rnd(0, (6, 4))
+    before, opt = p.clone(), AdamW([p])
+    for g in (p.to_sparse(), p.to_sparse_csr()):
+        with pytest.raises(ValueError, match="gradient"):
+            opt.apply_gradients([g])
+        with pytest.raises(ValueError, match="variables"):
+            AdamW([g])
+    assert torch.equal(p, before) and opt.iterations == 0

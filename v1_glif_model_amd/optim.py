@@ -170,7 +170,8 @@ class AdamW:
 
     @staticmethod
     def _check(p):
-        if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in DTYPES or not p.is_contiguous():
+        if (not isinstance(p, torch.Tensor) or p.layout is not torch.strided or not p.is_cuda or p.dtype not in DTYPES
+                or not p.is_contiguous()):
             raise ValueError("variables must be contiguous float32, bfloat16 or float16 tensors on the GPU")
 
     @property
@@ -194,9 +195,9 @@ class AdamW:
                 held.append(None)
                 kinds.append(0)
                 continue
-            if not isinstance(g, torch.Tensor) or g.get_device() != index or g.shape != shape or (
+            if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.get_device() != index or g.shape != shape or (
                     g.dtype is not dtype and g.dtype is not torch.float32):
-                raise ValueError(f"a gradient must be a tensor of its variable's shape {tuple(shape)} and device, float32 or of its type")
+                raise ValueError(f"a gradient must be a dense tensor of its variable's shape {tuple(shape)} and device, float32 or of its type")
             if not g.is_contiguous():
                 g = g.contiguous()
             held.append(g)
