@@ -32,7 +32,7 @@ def rounded(dtype):
     return 2.0 ** -8 if dtype is BF16 else 0.0
 
 
-def case(q, k, v, decay, scale=None, state=None, lengths=None, dy=None, dlast=None):
+def case(q, k, v, decay, scale=None, state=None, lengths=None, dy=None, dlast=None, more=None):
     """Forward and all gradients against 64 bits."""
     from v1_glif_model_amd import sequence as seq
     leaves = [None if t is None else t.detach().requires_grad_(True) for t in (q, k, v, state)]
@@ -47,7 +47,7 @@ def case(q, k, v, decay, scale=None, state=None, lengths=None, dy=None, dlast=No
     y6, last6 = ref.linear_attention(*l6[:3], f64(decay, False), s, l6[3], ends)
     ab = [None if t is None else t.detach().abs().requires_grad_(True) for t in l6]
     ya, lasta = ref.linear_attention(*ab[:3], f64(decay, False), abs(s), ab[3], ends)
-    more = rounded(q.dtype)
+    more = rounded(q.dtype) if more is None else more
     near(y, y6, ya.detach(), "y", more * ya.detach())
     near(last, last6, lasta.detach(), "last")
     dy = rnd(91, *y.shape, dtype=q.dtype) if dy is None else dy
@@ -139,6 +139,33 @@ def test_what_is_not_finite_does_not_go_back_in_time(K, V, where, dtype):
     out, _ = seq.linear_attention(*y.values(), decay)
     assert out[:30, 0, 1][:, [c for c in range(V) if c != 3]].isfinite().all() and out[30:, 0, 1].isnan().all()
     assert out[:10].isfinite().all() and out[10:, 0, 1, 3].isnan().all()
+
+
+@pytest.mark.parametrize("B,K,V", [(2, 40, 48), (1, 64, 64), (600, 64, 64), (1, 128, 128), (300, 128, 128)])
+def test_scores_of_bfloat16_keep_16_bits(B, K, V):
+    """32 ticks are one chunk, and without a state before it and a gradient of that behind it there are only scores, which are two
+    bfloat16 values: what the first leaves is 2^-8 of it, what the second leaves 2^-8 of that."""
+    case(*make(32, B, 3, 3, K, V, BF16, state=False), dlast=torch.zeros(B, 3, K, V, device=DEV), more=2.0 ** -16)
+
+
+@pytest.mark.parametrize("K,V", [(40, 48), (64, 64), (128, 128)])
+def test_an_infinite_state_stays_one(K, V):
+    """Positive queries and keys: a column of the state that is infinite gives infinite answers, of its sign, in the scores of the
+    same chunk as in those of later ones; the others are as they were."""
+    from v1_glif_model_amd import sequence as seq
+    q, k, v = (rnd(i, 150, 1, 1, d, dtype=BF16).abs() + 0.1 for i, d in ((1, K), (2, K), (3, V)))
+    decay, state = torch.tensor([-0.1], device=DEV), rnd(4, 1, 1, K, V)
+    clean, _ = seq.linear_attention(q, k, v, decay, None, state)
+    spoilt = state.clone()
+    spoilt[0, 0, :, 2], spoilt[0, 0, 5, 7] = float("-inf"), float("inf")
+    out, end = seq.linear_attention(q, k, v, decay, None, spoilt)
+    rest = [c for c in range(V) if c not in (2, 7)]
+    assert (out[..., 2] == float("-inf")).all() and (out[..., 7] == float("inf")).all() and (end[0, 0, :, 2] == float("-inf")).all()
+    assert torch.equal(out[..., rest], clean[..., rest])
+    k[70, 0, 0, 5] = float("inf")     # an infinite key: its row of the state is not finite (infinite or NaN), and nothing before it
+    out, end = seq.linear_attention(q, k, v, decay, None, state)
+    assert torch.equal(out[:70], clean[:70]) and not out[70:].isfinite().any() and not end[0, 0, 5].isfinite().any()
+    assert end[0, 0][[c for c in range(K) if c != 5]].isfinite().all()
 
 
 def test_large_states_of_float16():

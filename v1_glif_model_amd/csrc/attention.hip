@@ -245,6 +245,19 @@ __device__ __forceinline__ uint32_t two_halves(float lo, float hi) {   // to nea
     asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w) : "v"(lo), "v"(hi));
     return w;
 }
+// Scores that are multiplied as bfloat16: four as two values each, 16 bits together, which leaves the outputs of a chunk's own ticks
+// at their last rounding (500 x 32 ticks of 8 heads of 128 forward 40.6 us, backward 71.5, with one value 38.2 and 70.5).  Of states,
+// which are converted anew in every chunk, a second value costs more than it is worth (43.4 and 85.8): they are rounded to one.
+// What is left of an infinity, NaN by the difference, is made finite (what is left of a finite value is within it).
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void two_parts(f32x4 v, u32x2 &first, u32x2 &rest) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const float lo = v[2 * e], hi = v[2 * e + 1];
+        first[e] = two_halves(lo, hi);
+        rest[e] = two_halves(fmaxf(lo - low_half(first[e]), -1e36f), fmaxf(hi - high_half(first[e]), -1e36f));
+    }
+}
 #endif
 
 // A block takes one pass of one entry and head, 16 of c's channels a wave, and one segment of the ticks, chunk by chunk; each wave keeps the
@@ -261,6 +274,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     typedef typename M::frag frag;
     constexpr int kTicks = F::kTicks, kStep = F::kStep, kPer = F::kPer, TI = kTicks / 16, KT = kTicks / kStep, KD = D / kStep;
     constexpr int NT = NW * kWave, W = NW * 16, XT = D / 16, GAP = kPer == 8 ? 8 : 4, kSize = static_cast<int>(sizeof(C));
+    constexpr int kHalves = kSize == 2 ? 2 : 1;   // parts of a score
     using TD = Tile<T, D, NT, WHOLE>;
     using TC = Tile<T, W, NT, WHOLE>;
     using RD = Rows<C, D>;
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     __shared__ __attribute__((aligned(16))) char lds_a[STATES ? 16 : TD::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_b[TD::kBytes];
     __shared__ __attribute__((aligned(16))) char lds_c[TC::kBytes];
-    __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * RP::kBytes];
+    __shared__ __attribute__((aligned(16))) char lds_p[kHalves][STATES ? 16 : kTicks * RP::kBytes];
     __shared__ __attribute__((aligned(32))) float weight[kTicks];   // of tick j in the state after the chunk
     __shared__ float apart[STATES ? 1 : kTicks + 16], across[STATES ? 1 : kTicks];   // decays of scores by distance, backwards; of the state by tick
     __shared__ int odd[2];             // whether c is not finite somewhere in this chunk, and in the next
@@ -326,7 +340,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     }
 
     if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
-        for (int u = threadIdx.x; u < kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
+        for (int u = threadIdx.x; u < kHalves * kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
     }
     if (threadIdx.x < 2) odd[threadIdx.x] = 0;
     if (!STATES && threadIdx.x < kTicks) {
@@ -392,8 +406,14 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
                     f32x4 o;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[r] = it[i] > jt[i] || 4 * kq + r <= r16 ? s[i][r] * by[r] : 0.0f;
-                    typedef C four __attribute__((ext_vector_type(4)));
-                    *reinterpret_cast<four *>(lds_p + RP::at(16 * it[i] + r16, 16 * jt[i] + 4 * kq)) = __builtin_convertvector(o, four);
+                    const int to = RP::at(16 * it[i] + r16, 16 * jt[i] + 4 * kq);
+                    if constexpr (kHalves == 2) {
+                        u32x2 first, rest;
+                        two_parts(o, first, rest);
+                        *reinterpret_cast<u32x2 *>(lds_p[0] + to) = first, *reinterpret_cast<u32x2 *>(lds_p[1] + to) = rest;
+                    } else {
+                        *reinterpret_cast<f32x4 *>(lds_p[0] + to) = o;
+                    }
                 }
             };
             if (wave < kTiles - (kMost - 1) * NW) scores(std::integral_constant<int, kMost>{});
@@ -421,7 +441,9 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
             for (int s = 0; s < KT; ++s)
 #pragma unroll
                 for (int it = 0; it < TI; ++it)
-                    if (s * kStep <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p, 16 * it, s * kStep, l), o[it]);
+#pragma unroll
+                    for (int q = 0; q < kHalves; ++q)
+                        if (s * kStep <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p[q], 16 * it, s * kStep, l), o[it]);
             const int64_t by_tick = back ? -out_st : out_st;
             const int64_t to = (back ? len - 1 - here : here) * out_st + out_lane + r16 * by_tick;
             if (n == kTicks && (WHOLE || (dc - wc >= 16 && !wide))) {
@@ -513,7 +535,7 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
     // two of each, by names of their own: reads of the one must not wait for loads to the other
     __shared__ __attribute__((aligned(1024))) char a0[STATES ? 16 : kTile], a1[STATES ? 16 : kTile];
     __shared__ __attribute__((aligned(1024))) char b0[kTile], b1[kTile], c0[kTile], c1[kTile];
-    __shared__ __attribute__((aligned(16))) char lds_p[STATES ? 16 : kTicks * RP::kBytes];
+    __shared__ __attribute__((aligned(16))) char lds_p[2][STATES ? 16 : kTicks * RP::kBytes];   // the scores' two parts
     __shared__ f32x4 weight[kTicks / 4];
     __shared__ float apart[STATES ? 1 : kTicks + 16], across[STATES ? 1 : kTicks];
 
@@ -575,7 +597,7 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
         }
     }
     if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
-        for (int u = threadIdx.x; u < kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
+        for (int u = threadIdx.x; u < 2 * kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
         if (threadIdx.x < kTicks) {
             const int i = threadIdx.x;
             apart[kTicks - 1 - i] = power(rate, i) * in_scale * out_scale;
@@ -626,8 +648,10 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
                     f32x4 o;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[r] = it[i] > jt[i] || 4 * kq + r <= r16 ? s[i][r] * by[r] : 0.0f;
-                    typedef bf16 four __attribute__((ext_vector_type(4)));
-                    *reinterpret_cast<four *>(lds_p + RP::at(16 * it[i] + r16, 16 * jt[i] + 4 * kq)) = __builtin_convertvector(o, four);
+                    u32x2 first, rest;
+                    two_parts(o, first, rest);
+                    const int to = RP::at(16 * it[i] + r16, 16 * jt[i] + 4 * kq);
+                    *reinterpret_cast<u32x2 *>(lds_p[0] + to) = first, *reinterpret_cast<u32x2 *>(lds_p[1] + to) = rest;
                 }
             };
             if (wave < kTiles - (kMost - 1) * NW) scores(std::integral_constant<int, kMost>{});
@@ -691,7 +715,9 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
                 for (int s = 0; s < KT; ++s)
 #pragma unroll
                     for (int it = 0; it < TI; ++it)
-                        if (s * 32 <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p, 16 * it, s * 32, l), o[it]);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            if (s * 32 <= 16 * it + 15) o[it] = M::run(fc[s], RP::rows(lds_p[q], 16 * it, s * 32, l), o[it]);
                 const int64_t by_tick = back ? -out_st : out_st;
                 bf16 *to = out + (back ? len - 1 - here : here) * out_st + out_lane + r16 * by_tick;
 #pragma unroll
