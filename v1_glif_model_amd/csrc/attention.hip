@@ -10,9 +10,9 @@
 //   dv = F(k, scale q, dy; dS)                   last tick, and what is left behind the first is dS0
 // No power is of a negative exponent, so no decay, 0 among them, can overflow.
 //
-// Bound by latency within a chunk: 500 x 32 ticks of 8 heads of 128, bfloat16, trials of any length, 38 us forward (a block
-// of eight waves alone on its compute unit; 8.0k cycles a chunk of 64 ticks, of which the matrix instructions are 2.5k), 69 us for
-// the backward's three passes; of 32 heads, all ticks, 148 us (3.5 TB/s) and 363 (4.3 TB/s, 9 sequences read and 3 written).
+// Bound by latency within a chunk: 500 x 32 ticks of 8 heads of 128, bfloat16, trials of any length, 41 us forward (a block
+// of eight waves alone on its compute unit; 8.6k cycles a chunk of 64 ticks, of which the matrix instructions are 2.7k), 71 us for
+// the backward's three passes; of 32 heads, all ticks, 148 us (3.5 TB/s) and 370 (4.3 TB/s, 9 sequences read and 3 written).
 // In float32 (its products at 1/16 of the rate) 290 x 18 ticks of 4 heads of 128 and 64 50 us.
 #include <type_traits>
 
@@ -830,8 +830,8 @@ void run_pass(const AttArgs &a, bool states, hipStream_t s) {
 }
 
 // Chunks of 64 ticks are the faster for blocks that are alone on their compute unit, of 32 leave room for others (500 x 32 ticks
-// of 8 heads of 128, 256 blocks forward, 37 us and 43, 768 backward, trials of any length, 82 and 69; of 16 heads of 64, 512 and
-// 1536 blocks, 32 and 37, 84 and 75).
+// of 8 heads of 128, 256 blocks forward, 41 us and 46, 768 backward, trials of any length, 88 and 71; of 16 heads of 64, 512 and
+// 1536 blocks, 36 and 38, 95 and 78).
 template <int D, int NW>
 void run_direct(const AttArgs &a, bool states, hipStream_t s) {
     const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
@@ -973,9 +973,9 @@ int check_attention(const glif_attention *a, bool step) {
 
 // Ticks in segments where there are too few blocks for the chip: a first launch gives the state that each segment adds,
 // a second joins them, and then all segments go at once.  The first reads two of three sequences again and takes more than
-// half as long, so that two segments gain nothing (500 x 16 ticks of 8 heads of 128 in two 52 us, in one 37).  As many segments as
-// blocks are there at once, one a compute unit where heads have more than 64 channels, three where not (8000 ticks of 16 heads of
-// 128 in 25 segments, two rounds of blocks, 89 us, in 16 76), and none of fewer than four chunks.
+// half as long, so that two segments gain nothing (500 x 16 ticks of 8 heads of 128 in two 52 us, in one 37, by scores of one value).
+// As many segments as blocks are there at once, one a compute unit where heads have more than 64 channels, three where not (8000 ticks
+// of 16 heads of 128 in 25 segments, two rounds of blocks, 89 us, in 16 76, likewise), and none of fewer than four chunks.
 void cut(AttArgs &a, int64_t blocks, int ticks, const glif_attention *s) {
     a.segments = 1, a.seg_ticks = std::max((a.T + ticks - 1) / ticks, 1) * ticks;
     const int64_t slots = std::max(s->d_key, s->d_value) > 64 ? 256 : 768;
