@@ -398,7 +398,8 @@ int glif_scan_step(const glif_scan *s, void *y, float *state, void *stream);
 
 /* Linear attention with a decay for each head; k and v are shared by the n_heads / n_groups heads of a group:
  *   S[t] = exp(log_decay[h]) S[t - 1] + k[t] v[t]^T,   y[t] = scale q[t] S[t]
- * S [d_key][d_value] float32, both at most 128.  exp(-infinity) is 0: nothing is remembered.  log_decay has no gradient. */
+ * S [d_key][d_value] float32, both at most 128.  exp(-infinity) is 0: nothing is remembered.  log_decay has no gradient.
+ * bfloat16 sequences: scores and states are multiplied as two bfloat16 values each, but for the step's, which are float32. */
 typedef struct {
     const void *q, *k, *v;           /* [T][B][n_heads][d_key], [T][B][n_groups][d_key], .. [d_value], channels contiguous */
     const float *log_decay;          /* [n_heads] */

@@ -245,9 +245,9 @@ __device__ __forceinline__ uint32_t two_halves(float lo, float hi) {   // to nea
     asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w) : "v"(lo), "v"(hi));
     return w;
 }
-// Scores that are multiplied as bfloat16: four as two values each, 16 bits together, which leaves the outputs of a chunk's own ticks
-// at their last rounding (500 x 32 ticks of 8 heads of 128 forward 40.6 us, backward 71.5, with one value 38.2 and 70.5).  Of states,
-// which are converted anew in every chunk, a second value costs more than it is worth (43.4 and 85.8): they are rounded to one.
+// Scores and states that are multiplied as bfloat16: four as two values each, 16 bits together, which leaves outputs at their last
+// rounding (500 x 32 ticks of 8 heads of 128 forward 44.6 us, backward 85.4; states as one value,
+// 40.2 and 70.4, put as much error again into outputs that come from before their chunk, and far more where their terms cancel).
 // What is left of an infinity, NaN by the difference, is made finite (what is left of a finite value is within it).
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void two_parts(f32x4 v, u32x2 &first, u32x2 &rest) {
@@ -257,6 +257,14 @@ __device__ __forceinline__ void two_parts(f32x4 v, u32x2 &first, u32x2 &rest) {
         first[e] = two_halves(lo, hi);
         rest[e] = two_halves(fmaxf(lo - low_half(first[e]), -1e36f), fmaxf(hi - high_half(first[e]), -1e36f));
     }
+}
+// Likewise eight of a state, as two operands.
+__device__ __forceinline__ void two_parts(f32x4 v, f32x4 w, Mma<bf16>::frag (&parts)[2]) {
+    u32x2 first[2], rest[2];
+    two_parts(v, first[0], rest[0]);
+    two_parts(w, first[1], rest[1]);
+    parts[0] = __builtin_bit_cast(Mma<bf16>::frag, __builtin_shufflevector(first[0], first[1], 0, 1, 2, 3));
+    parts[1] = __builtin_bit_cast(Mma<bf16>::frag, __builtin_shufflevector(rest[0], rest[1], 0, 1, 2, 3));
 }
 #endif
 
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     typedef typename M::frag frag;
     constexpr int kTicks = F::kTicks, kStep = F::kStep, kPer = F::kPer, TI = kTicks / 16, KT = kTicks / kStep, KD = D / kStep;
     constexpr int NT = NW * kWave, W = NW * 16, XT = D / 16, GAP = kPer == 8 ? 8 : 4, kSize = static_cast<int>(sizeof(C));
-    constexpr int kHalves = kSize == 2 ? 2 : 1;   // parts of a score
+    constexpr int kHalves = kSize == 2 ? 2 : 1;   // parts of a score, and of a state
     using TD = Tile<T, D, NT, WHOLE>;
     using TC = Tile<T, W, NT, WHOLE>;
     using RD = Rows<C, D>;
@@ -429,11 +437,15 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
             f32x4 o[TI] = {};
 #pragma unroll
             for (int k = 0; k < KD; ++k) {
-                frag fx;
-                if constexpr (kPer == 8) fx = __builtin_convertvector(__builtin_shufflevector(x[2 * k], x[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), frag);
-                else fx = x[k];
+                frag fx[kHalves];
+                if constexpr (kHalves == 2) two_parts(x[2 * k], x[2 * k + 1], fx);
+                else fx[0] = x[k];
 #pragma unroll
-                for (int it = 0; it < TI; ++it) o[it] = M::run(fx, RD::rows(lds_a, 16 * it, k * kStep, l), o[it]);
+                for (int it = 0; it < TI; ++it) {
+                    const frag fa = RD::rows(lds_a, 16 * it, k * kStep, l);
+#pragma unroll
+                    for (int q = 0; q < kHalves; ++q) o[it] = M::run(fx[q], fa, o[it]);
+                }
             }
 #pragma unroll
             for (int it = 0; it < TI; ++it) o[it] *= across[16 * it + (l & 15)];
@@ -705,9 +717,14 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
                 f32x4 o[TI] = {};
 #pragma unroll
                 for (int k = 0; k < KD; ++k) {
-                    const frag fx = __builtin_convertvector(__builtin_shufflevector(x[2 * k], x[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), frag);
+                    frag fx[2];
+                    two_parts(x[2 * k], x[2 * k + 1], fx);
 #pragma unroll
-                    for (int it = 0; it < TI; ++it) o[it] = M::run(fx, R::rows(ta, 16 * it, k * 32, l), o[it]);
+                    for (int it = 0; it < TI; ++it) {
+                        const frag fa = R::rows(ta, 16 * it, k * 32, l);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) o[it] = M::run(fx[q], fa, o[it]);
+                    }
                 }
 #pragma unroll
                 for (int it = 0; it < TI; ++it) o[it] *= across[16 * it + r16];

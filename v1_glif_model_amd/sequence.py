@@ -691,9 +691,10 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     initial_state [B, H, K, V] float32 or None.  Returns y [T, B, H, V] and the state [B, H, K, V] after each batch entry's
     last tick.  At most 4096 heads, B H 2^20, and B H V and B H K below 2^24 where there is more than one tick.
 
-    Ticks are taken in chunks, as matrix products.  Those of bfloat16 sequences multiply scores as two bfloat16 values, 16 bits
-    together, and states rounded to one (their sums, and the states themselves, are float32); those of float16 ones are float32,
-    as states and scores go beyond float16's range.  An infinite key may make its row of the state NaN where it would be infinite."""
+    Ticks are taken in chunks, as matrix products.  Those of bfloat16 sequences multiply scores and states as two bfloat16
+    values each, 16 bits together (their sums, and the states themselves, are float32); those of float16 ones are float32, as
+    states and scores go beyond float16's range.  What an infinite key makes infinite of the state, or an infinite query of its
+    tick's answer, may be NaN instead; likewise in the gradients."""
     if torch.is_tensor(q) and q.dim() != 4:
         raise ValueError(f"q must be [T, B, H, K], got shape {tuple(q.shape)}")
     scale = _attention_args(q, k, v, log_decay, scale)
