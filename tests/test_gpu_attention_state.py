@@ -5,8 +5,8 @@ are within 2^-16 of the sum of their absolute terms, and what near() allows for 
 import pytest
 import torch
 
-from tests.test_gpu_attention import BF16, DEV, F32, SHAPES, case, make, rnd
-from tests.seq_ref import f64, near
+from tests.test_gpu_attention import BF16, DEV, DTYPES, F32, SHAPES, case, make, rnd
+from tests.seq_ref import UNIT, f64, near
 
 pytestmark = pytest.mark.gpu
 TWO_VALUES = 2.0 ** -16
@@ -79,3 +79,60 @@ def test_a_prompt_answers_as_its_ticks_do(K, V):
     terms, size = f64(terms, False), f64(size, False)
     near(y, f64(steps, False), terms, "y", 2.0 ** -8 * f64(steps, False).abs() + (1e-5 + TWO_VALUES) * terms)
     near(last, f64(st, False), size, "state", 1e-5 * size)
+
+
+def positive(T, K, V, dtype):
+    """Queries and keys above 0: an infinity anywhere makes infinities of its own sign, never their difference."""
+    q, k = (rnd(i, T, 1, 2, K, dtype=dtype).abs() + 0.1 for i in (1, 2))
+    return q, k, rnd(3, T, 1, 2, V, dtype=dtype), torch.tensor([-0.1, -2.0], device=DEV)
+
+
+WIDTHS = [(16, 128), (40, 48), (64, 64), (128, 24), (128, 128)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [150, 1100])
+@pytest.mark.parametrize("K,V", WIDTHS)
+def test_an_infinite_value_makes_its_channel_infinite(K, V, T, dtype):
+    """From its tick on, in the state too, however much is forgotten since, whether segments of the time go at once (the 1100 ticks)
+    or not; the other channels stay as they were.  Likewise back in time from an infinite gradient of an answer."""
+    from v1_glif_model_amd import sequence as seq
+    q, k, v, decay = positive(T, K, V, dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)] + [torch.zeros(1, 2, K, V, device=DEV, requires_grad=True)]
+    dy = rnd(5, T, 1, 2, V, dtype=dtype)
+    y, last = seq.linear_attention(*leaves[:3], decay, None, leaves[3])
+    dv, dstate = torch.autograd.grad(y, leaves[2:], dy)
+    wide = [t.detach().float().abs().requires_grad_(True) for t in leaves]     # the sums of the absolute terms
+    sums = seq.linear_attention(*wide[:3], decay, None, wide[3])
+    sums += torch.autograd.grad(sums[0], wide[2:], dy.float().abs())
+    rest = [c for c in range(V) if c not in (3, 7)]
+    for at in (0, 17, 70, 149):
+        spoilt, bad = v.clone(), dy.clone()
+        spoilt[at, :, :, 3], spoilt[at, :, :, 7] = float("inf"), float("-inf")
+        bad[at, :, :, 3], bad[at, :, :, 7] = float("inf"), float("-inf")
+        out, end = seq.linear_attention(q, k, spoilt, decay)
+        assert (out[at:, ..., 3] == float("inf")).all() and (out[at:, ..., 7] == float("-inf")).all()
+        assert (end[..., 3] == float("inf")).all() and (end[..., 7] == float("-inf")).all()
+        y1, last1 = seq.linear_attention(*leaves[:3], decay, None, leaves[3])
+        gv, gstate = torch.autograd.grad((y1, last1), leaves[2:], (bad, torch.zeros_like(last)))
+        assert (gv[:at + 1, ..., 3] == float("inf")).all() and (gv[:at + 1, ..., 7] == float("-inf")).all()
+        assert (gstate[..., 3] == float("inf")).all() and (gstate[..., 7] == float("-inf")).all()
+        for a, b, size in zip((out, end, gv, gstate), (y, last, dv, dstate), sums):     # each within its bound of the same sums
+            b, size = f64(b[..., rest], False), f64(size[..., rest], False)
+            near(a[..., rest], b, size, at, UNIT[a.dtype] * b.abs() + (1e-5 + (2 * TWO_VALUES if a.dtype is BF16 else 0.0)) * size)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [150, 1100])
+@pytest.mark.parametrize("K,V", WIDTHS)
+def test_an_infinite_state_stays_one_however_much_is_forgotten(K, V, T, dtype):
+    from v1_glif_model_amd import sequence as seq
+    q, k, v, decay = positive(T, K, V, dtype)
+    state = rnd(4, 1, 2, K, V)
+    y, last = seq.linear_attention(q, k, v, decay, None, state)
+    state[..., 2], state[:, :, 5, 7] = float("-inf"), float("inf")
+    out, end = seq.linear_attention(q, k, v, decay, None, state)
+    assert (out[..., 2] == float("-inf")).all() and (out[..., 7] == float("inf")).all()
+    assert (end[..., 2] == float("-inf")).all() and (end[:, :, 5, 7] == float("inf")).all()
+    rest = [c for c in range(V) if c not in (2, 7)]
+    assert torch.equal(out[..., rest], y[..., rest]) and torch.equal(end[..., rest], last[..., rest])

@@ -46,8 +46,13 @@ struct AttArgs {
     int32_t T, B, H, segments, seg_ticks;
 };
 
-// lam^n for n >= 0: 1 for n = 0 whatever the decay is
-__device__ __forceinline__ float power(float rate, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(rate * static_cast<float>(n)); }
+// lam = exp(log_decay) to whole powers n >= 0: 1 for n = 0 whatever the decay is.  What is below the normal numbers is the least of
+// them, as long as lam itself is not: 1e-38 of a state is nothing, and an infinite one stays infinite, as it does tick by tick.
+struct Decay {
+    float rate, least;   // logarithms to base 2
+    __device__ __forceinline__ explicit Decay(float log_decay) : rate(log_decay * 1.4426950408889634f), least(rate >= -126.0f ? -126.0f : rate) {}
+    __device__ __forceinline__ float power(int n) const { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(fmaxf(rate * static_cast<float>(n), least)); }
+};
 
 __device__ __forceinline__ int live_ticks(const int32_t *lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }
 
@@ -207,30 +212,6 @@ struct Tile {
             }
         }
     }
-    __device__ __forceinline__ bool finite() const {
-        if constexpr (kSize == 2) {
-            typedef uint16_t pair __attribute__((ext_vector_type(2)));
-            pair most = {0, 0};
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                const u32x4 w = __builtin_bit_cast(u32x4, r[i]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(pair, w[e] & 0x7fff7fffu));
-            }
-            const uint16_t inf = std::is_same_v<T, bf16> ? 0x7f80 : 0x7c00;
-            return (most[0] > most[1] ? most[0] : most[1]) < inf;
-        } else {
-            uint32_t most = 0;
-#pragma unroll
-            for (int i = 0; i < kN; ++i)
-#pragma unroll
-                for (int e = 0; e < kV; ++e) {
-                    const uint32_t w = __builtin_bit_cast(uint32_t, static_cast<float>(r[i][e])) & 0x7fffffffu;
-                    most = most > w ? most : w;
-                }
-            return most < 0x7f800000u;
-        }
-    }
 };
 
 // Two bfloat16 in 32 bits.
@@ -266,6 +247,91 @@ __device__ __forceinline__ void two_parts(f32x4 v, f32x4 w, Mma<bf16>::frag (&pa
     parts[0] = __builtin_bit_cast(Mma<bf16>::frag, __builtin_shufflevector(first[0], first[1], 0, 1, 2, 3));
     parts[1] = __builtin_bit_cast(Mma<bf16>::frag, __builtin_shufflevector(rest[0], rest[1], 0, 1, 2, 3));
 }
+
+// The state's first row (b's channel) of the four that a lane holds in x[i].
+template <int PER>
+__device__ __forceinline__ int state_row(int i, int kq) { return PER == 8 ? 32 * (i / 2) + 8 * kq + 4 * (i % 2) : 16 * i + 4 * kq; }
+
+// Whether some value of the wave's operands is not finite.
+template <int N>
+__device__ __forceinline__ bool any_odd(const Mma<bf16>::frag (&f)[N]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+        const u32x4 w = __builtin_bit_cast(u32x4, f[s]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = larger_halves(most, w[e] & 0x7fff7fffu);
+    }
+    return __builtin_amdgcn_ballot_w64((most & 0xffffu) >= 0x7f80u || most >> 16 >= 0x7f80u) != 0;
+}
+template <int N>
+__device__ __forceinline__ bool any_odd(const f32x4 (&f)[N]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(f[s][e]) & 0x7fffffffu);   // (a bit cast of an element takes the first)
+    return __builtin_amdgcn_ballot_w64(most >= 0x7f800000u) != 0;
+}
+
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+    return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+}
+// A chunk's values times their weights, which the float32 state adds up: what a matrix instruction multiplies is not float32, so they
+// are three bfloat16 values, 24 bits together.  odd: of one that is not finite the first is all (the difference would be NaN).
+template <typename W>
+__device__ __forceinline__ void three_parts(Mma<bf16>::frag c, W weight, bool odd, Mma<bf16>::frag (&parts)[3]) {
+    const u32x4 two = __builtin_bit_cast(u32x4, c);
+    u32x4 got[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float lo = low_half(two[e]) * weight(2 * e), hi = high_half(two[e]) * weight(2 * e + 1);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            got[q][e] = two_halves(lo, hi);
+            lo -= low_half(got[q][e]), hi -= high_half(got[q][e]);
+        }
+    }
+    if (odd)
+#pragma unroll
+        for (int q = 1; q < 3; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) got[q][e] = finite_halves(got[q][e]);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) parts[q] = __builtin_bit_cast(Mma<bf16>::frag, got[q]);
+}
+
+// Answers to a chunk whose c is not finite in a wave's channels: tick by tick, as the definition has it, since a later tick's c
+// would be multiplied by an earlier one's 0, and an infinite one, in scores of several values and with b's zeros from channel d on, by
+// numbers of both signs and 0.  put(i, sum) takes tick i's answers, before their scale, of the lanes with kq = 0.
+template <typename C, typename RD, typename RC, int PER, bool WHOLE, int XT, typename Put>
+__device__ __forceinline__ void by_ticks(const char *ta, const char *tb, const char *tc, int n, int d, int wc, int lane, Decay decay,
+                                         int lead, float in_scale, f32x4 (&x)[XT], Put put) {
+    typedef C four __attribute__((ext_vector_type(4)));
+    const float before = decay.power(lead), after = decay.power(1 - lead);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        asm volatile("" : "+v"(lane));   // this way is rare: its addresses and rows take no registers of the other
+        const int r16 = lane % 16, kq = lane / 16;
+        const float c = static_cast<float>(*reinterpret_cast<const C *>(tc + RC::at(i, wc + r16))) * in_scale;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < XT; ++k) {
+            const int row = state_row<PER>(k, kq), at = RD::at(i, row);
+            const four fb = *reinterpret_cast<const four *>(tb + at), fa = *reinterpret_cast<const four *>(ta + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float z = WHOLE || row + e < d ? x[k][e] * before + static_cast<float>(fb[e]) * c : 0.0f;
+                sum += static_cast<float>(fa[e]) * z;
+                x[k][e] = z * after;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        sum += __shfl_xor(sum, 16, kWave);
+        sum += __shfl_xor(sum, 32, kWave);
+        if (kq == 0) put(i, sum);
+    }
+}
 #endif
 
 // A block takes one pass of one entry and head, 16 of c's channels a wave, and one segment of the ticks, chunk by chunk; each wave keeps the
@@ -273,8 +339,10 @@ __device__ __forceinline__ void two_parts(f32x4 v, f32x4 w, Mma<bf16>::frag (&pa
 // is, is chosen so that a lane's values are kPer neighbours).  STATES: no outputs, only the state that the segment adds to
 // nothing.
 // WHOLE: all heads have D channels in b and 16 NW in c, and outputs are of type T.
+// Two blocks of float16 heads of 128 share a unit by 128 registers a wave (16 to 48 bytes spilled by the way of single ticks; 500 x 32
+// ticks of 8 heads with gradients 377 us, one block 398; float32 ones lose by it, 450 against 415).
 template <typename T, int D, int NW, bool STATES, bool WHOLE>
-__global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
+__global__ void __launch_bounds__(NW *kWave, D == 32 || (std::is_same_v<T, f16> && NW == 8) ? 4 : 2) k_attention(AttArgs args) {
 #ifdef __HIP_DEVICE_COMPILE__
     using F = Form<T>;
     using C = typename F::C;
@@ -294,7 +362,6 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     __shared__ __attribute__((aligned(16))) char lds_p[kHalves][STATES ? 16 : kTicks * RP::kBytes];
     __shared__ __attribute__((aligned(32))) float weight[kTicks];   // of tick j in the state after the chunk
     __shared__ float apart[STATES ? 1 : kTicks + 16], across[STATES ? 1 : kTicks];   // decays of scores by distance, backwards; of the state by tick
-    __shared__ int odd[2];             // whether c is not finite somewhere in this chunk, and in the next
 
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), r16 = lane % 16, kq = lane / 16;
     // The blocks that read the same sequences are on one XCD (block id mod 8), after each other.
@@ -307,7 +374,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     const int dc = WHOLE ? W : pass.c.d, db = WHOLE ? D : pass.b.d;
     const int len = live_ticks(args.lengths, b, args.T), seg_first = seg * args.seg_ticks, seg_end = min(args.T, seg_first + args.seg_ticks);
     const int begin = min(seg_first, len), end = min(seg_end, len);
-    const float rate = args.log_decay[h] * 1.4426950408889634f;
+    const Decay decay(args.log_decay[h]);
     const int wc = wave * 16;            // the wave's first channel
     const bool active = wc < dc, back = pass.back, wide = !WHOLE && pass.wide;
     const int lead = pass.lead;
@@ -331,7 +398,7 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     if (begin < end) fetch(begin, min(end - begin, kTicks));
 
     // state: x[i][r] is of b's channel row(i) + r and c's channel wc + r16
-    auto row = [&](int i) { return kPer == 8 ? 32 * (i / 2) + 8 * kq + 4 * (i % 2) : 16 * i + 4 * kq; };
+    auto row = [&](int i) { return state_row<kPer>(i, kq); };
     f32x4 x[XT] = {};
     if (!STATES && pass.x && active) {
         const int64_t x_b = pass.x_b;
@@ -350,18 +417,15 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
     if (!STATES) {   // scores above the diagonal tiles are 0, and stay so
         for (int u = threadIdx.x; u < kHalves * kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
     }
-    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
     if (!STATES && threadIdx.x < kTicks) {
         const int i = threadIdx.x;
-        apart[kTicks - 1 - i] = power(rate, i) * in_scale * out_scale;
-        across[i] = power(rate, i + lead) * out_scale;
+        apart[kTicks - 1 - i] = decay.power(i) * in_scale * out_scale;
+        across[i] = decay.power(i + lead) * out_scale;
     }
 
-    // A product with a later tick's 0 is NaN where that tick's c is not finite: such a chunk is fetched again, as chunks of one
-    // tick, up to `careful`.
-    int weighed = 0, careful = begin;
-    for (int at = begin, turn = 0; at < end;) {
-        const int n = at < careful ? 1 : min(end - at, kTicks);
+    int weighed = 0;
+    for (int at = begin; at < end;) {
+        const int n = min(end - at, kTicks);
         int l = lane;
         asm volatile("" : "+v"(l));   // addresses are made again for every chunk rather than kept, which would take more registers than there are
         __syncthreads();   // the last chunk's tiles have been read
@@ -371,25 +435,14 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
         if (n != weighed) {
             if (threadIdx.x < kTicks) {
                 const int j = threadIdx.x;
-                weight[j] = j < n ? power(rate, n - lead - j) * in_scale : 0.0f;
+                weight[j] = j < n ? decay.power(n - lead - j) * in_scale : 0.0f;
             }
             weighed = n;
         }
-        if (!STATES && n > 1 && !rc.finite()) odd[turn] = 1;
-        if (threadIdx.x == 0) odd[turn ^ 1] = 0;
         __syncthreads();
-        if (!STATES) {
-            const bool again = odd[turn] != 0;
-            turn ^= 1;
-            if (again) {
-                careful = at + n;
-                fetch(at, 1);
-                continue;
-            }
-        }
         const int here = at;
         at += n;
-        if (at < end) fetch(at, at < careful ? 1 : min(end - at, kTicks));
+        if (at < end) fetch(at, min(end - at, kTicks));
         if (!STATES) {
             // scores: rows j, columns i
             constexpr int kTiles = TI * (TI + 1) / 2, kMost = (kTiles + NW - 1) / NW;
@@ -432,6 +485,16 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
         frag fc[KT];
 #pragma unroll
         for (int s = 0; s < KT; ++s) fc[s] = RC::template columns<4>(lds_c, wave * 16, s * kStep, l);
+        const bool odd = (!STATES || kSize == 2) && any_odd(fc);
+        if (!STATES && odd) {
+            by_ticks<C, RD, RC, kPer, WHOLE>(lds_a, lds_b, lds_c, n, db, wc, l, decay, lead, in_scale, x, [&](int i, float sum) {
+                if (!out || wc + r16 >= dc) return;
+                const int64_t to = (back ? len - 1 - here - i : here + i) * out_st + static_cast<int64_t>(bh) * dc + wc + r16;
+                if (wide) static_cast<float *>(out)[to] = sum * out_scale;
+                else static_cast<T *>(out)[to] = from_f32<T>(sum * out_scale);
+            });
+            continue;
+        }
         if (!STATES && out) {
             // rows c's channels, columns i
             f32x4 o[TI] = {};
@@ -475,34 +538,17 @@ __global__ void __launch_bounds__(NW *kWave, 2) k_attention(AttArgs args) {
                 }
             }
         }
-        const float f = power(rate, n);
+        const float f = decay.power(n);
 #pragma unroll
         for (int i = 0; i < XT; ++i) x[i] *= f;
-        // The state is float32, but what a matrix instruction multiplies is not: a weighted value is three bfloat16 ones, 24
-        // bits together.
         constexpr int kParts = kSize == 2 ? 3 : 1;
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
             frag part[kParts];
             typedef float many __attribute__((ext_vector_type(kPer)));
             const many w = *reinterpret_cast<const many *>(weight + s * kStep + kq * kPer);
-            if constexpr (kSize == 2) {
-                const u32x4 two = __builtin_bit_cast(u32x4, fc[s]);
-                u32x4 got[kParts];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float lo = low_half(two[e]) * w[2 * e], hi = high_half(two[e]) * w[2 * e + 1];
-#pragma unroll
-                    for (int q = 0; q < kParts; ++q) {
-                        got[q][e] = two_halves(lo, hi);
-                        lo -= low_half(got[q][e]), hi -= high_half(got[q][e]);
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < kParts; ++q) part[q] = __builtin_bit_cast(frag, got[q]);
-            } else {
-                part[0] = fc[s] * w;
-            }
+            if constexpr (kSize == 2) three_parts(fc[s], [&](int e) { return w[e]; }, STATES && odd, part);
+            else part[0] = fc[s] * w;
 #pragma unroll
             for (int i = 0; i < XT; ++i) {
                 const frag fb = RD::template columns<GAP>(lds_b, kPer == 8 ? 32 * (i / 2) + 4 * (i % 2) : 16 * i, s * kStep, l);
@@ -560,7 +606,7 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
     const int bh = static_cast<int>(group / args.segments), b = bh / args.H, h = bh % args.H;
     const int len = live_ticks(args.lengths, b, args.T), seg_first = seg * args.seg_ticks, seg_end = min(args.T, seg_first + args.seg_ticks);
     const int begin = min(seg_first, len), end = min(seg_end, len);
-    const float rate = args.log_decay[h] * 1.4426950408889634f;
+    const Decay decay(args.log_decay[h]);
     const int wc = wave * 16, lead = pass.lead;
     const bool back = pass.back;
     const float in_scale = pass.in_scale, out_scale = pass.out_scale;
@@ -593,7 +639,7 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
     if (begin < end) fetch(begin, min(end - begin, kTicks), a0, b0, c0);
 
     // state: x[i][r] is of b's channel row(i) + r and c's channel wc + r16
-    auto row = [&](int i) { return 32 * (i / 2) + 8 * kq + 4 * (i % 2); };
+    auto row = [&](int i) { return state_row<8>(i, kq); };
     f32x4 x[XT] = {};
     if (!STATES && pass.x) {
         const int64_t x_b = pass.x_b;
@@ -612,8 +658,8 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
         for (int u = threadIdx.x; u < 2 * kTicks * RP::kBytes / 4; u += NT) reinterpret_cast<uint32_t *>(lds_p)[u] = 0u;
         if (threadIdx.x < kTicks) {
             const int i = threadIdx.x;
-            apart[kTicks - 1 - i] = power(rate, i) * in_scale * out_scale;
-            across[i] = power(rate, i + lead) * out_scale;
+            apart[kTicks - 1 - i] = decay.power(i) * in_scale * out_scale;
+            across[i] = decay.power(i + lead) * out_scale;
         }
     }
 
@@ -636,7 +682,7 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
         }
         if (tid < kTicks) {
             const int j = tid;
-            weight[j / 4][j % 4] = j < n ? power(rate, n - lead - j) * in_scale : 0.0f;
+            weight[j / 4][j % 4] = j < n ? decay.power(n - lead - j) * in_scale : 0.0f;
         }
         if (!STATES) {
             constexpr int kTiles = TI * (TI + 1) / 2, kMost = (kTiles + NW - 1) / NW;
@@ -681,36 +727,13 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
         at += n;
         if (at < end) fetch(at, min(end - at, kTicks), na, nb, nc);
         frag fc[KT];
-        uint32_t most = 0;
 #pragma unroll
-        for (int s = 0; s < KT; ++s) {
-            fc[s] = R::template columns<4>(tc, wc, s * 32, l);
-            const u32x4 w = __builtin_bit_cast(u32x4, fc[s]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) most = larger_halves(most, w[e] & 0x7fff7fffu);
-        }
-        const bool odd = (most & 0xffffu) >= 0x7f80u || most >> 16 >= 0x7f80u;
-        if (!STATES && __builtin_amdgcn_ballot_w64(odd)) {
-            // A product with a later tick's 0 is NaN where that tick's c is not finite: the wave goes tick by tick.
-            const float before = power(rate, lead), after = power(rate, 1 - lead);
-#pragma unroll 1
-            for (int i = 0; i < n; ++i) {
-                const float c = static_cast<float>(*reinterpret_cast<const bf16 *>(tc + R::at(i, wc + r16))) * in_scale;
-                float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KD; ++k) {
-                    const frag fb = *reinterpret_cast<const frag *>(tb + R::at(i, 32 * k + 8 * kq)), fa = *reinterpret_cast<const frag *>(ta + R::at(i, 32 * k + 8 * kq));
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float z = x[2 * k + e / 4][e % 4] * before + static_cast<float>(fb[e]) * c;
-                        sum += static_cast<float>(fa[e]) * z;
-                        x[2 * k + e / 4][e % 4] = z * after;
-                    }
-                }
-                sum += __shfl_xor(sum, 16, kWave);
-                sum += __shfl_xor(sum, 32, kWave);
-                if (kq == 0 && out) out[(back ? len - 1 - here - i : here + i) * out_st + static_cast<int64_t>(bh) * D + wc + r16] = static_cast<bf16>(sum * out_scale);
-            }
+        for (int s = 0; s < KT; ++s) fc[s] = R::template columns<4>(tc, wc, s * 32, l);
+        const bool odd = any_odd(fc);
+        if (!STATES && odd) {
+            by_ticks<bf16, R, R, 8, true>(ta, tb, tc, n, D, wc, l, decay, lead, in_scale, x, [&](int i, float sum) {
+                if (out) out[(back ? len - 1 - here - i : here + i) * out_st + static_cast<int64_t>(bh) * D + wc + r16] = static_cast<bf16>(sum * out_scale);
+            });
         } else {
             if (!STATES && out) {
                 // rows c's channels, columns i
@@ -741,30 +764,19 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
                 for (int it = 0; it < TI; ++it)
                     if (16 * it + r16 < n) *reinterpret_cast<Vec<bf16, 4> *>(to + 16 * it * by_tick) = __builtin_convertvector(o[it], Vec<bf16, 4>);
             }
-            const float f = power(rate, n);
+            const float f = decay.power(n);
 #pragma unroll
             for (int i = 0; i < XT; ++i) x[i] *= f;
-            // The state is float32, but what a matrix instruction multiplies is not: a weighted value is three bfloat16 ones, 24
-            // bits together.
 #pragma unroll
             for (int s = 0; s < KT; ++s) {
                 const f32x4 w4[2] = {weight[s * 8 + kq * 2], weight[s * 8 + kq * 2 + 1]};
-                const u32x4 two = __builtin_bit_cast(u32x4, fc[s]);
-                u32x4 part[3];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float lo = low_half(two[e]) * w4[e / 2][e % 2 * 2], hi = high_half(two[e]) * w4[e / 2][e % 2 * 2 + 1];
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                        part[q][e] = two_halves(lo, hi);
-                        lo -= low_half(part[q][e]), hi -= high_half(part[q][e]);
-                    }
-                }
+                frag part[3];
+                three_parts(fc[s], [&](int e) { return w4[e / 4][e % 4]; }, STATES && odd, part);
 #pragma unroll
                 for (int i = 0; i < XT; ++i) {
                     const frag fb = R::template columns<8>(tb, 32 * (i / 2) + 4 * (i % 2), s * 32, l);
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) x[i] = M::run(fb, __builtin_bit_cast(frag, part[q]), x[i]);
+                    for (int q = 0; q < 3; ++q) x[i] = M::run(fb, part[q], x[i]);
                 }
             }
         }
@@ -807,7 +819,7 @@ __global__ void __launch_bounds__(kBlock) k_attention_join(JoinArgs a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
     if (i >= a.bh * a.n) return;
     const int bh = static_cast<int>(i / a.n), len = live_ticks(a.lengths, bh / a.H, a.T);
-    const float rate = a.log_decay[bh % a.H] * 1.4426950408889634f;
+    const Decay decay(a.log_decay[bh % a.H]);
     float x = a.x ? a.x[i] : 0.0f;
     const int64_t apart = a.bh * a.n;
     constexpr int kAhead = 8;   // loads under way
@@ -820,7 +832,7 @@ __global__ void __launch_bounds__(kBlock) k_attention_join(JoinArgs a) {
             const int s = s0 + k, ticks = min(max(len - s * a.seg_ticks, 0), a.seg_ticks);
             if (s >= a.segments) break;
             a.states[s * apart + i] = x;
-            if (ticks) x = x * power(rate, ticks) + more[k];
+            if (ticks) x = x * decay.power(ticks) + more[k];
         }
     }
     if (a.x_out) a.x_out[i] = x;
@@ -924,7 +936,7 @@ __global__ void __launch_bounds__(kBlock) k_attention_step(StepArgs a) {
     const T *q = static_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh;
     const T *k = static_cast<const T *>(a.k) + b * a.k_sb + h / a.share * a.k_sh;
     const T *v = static_cast<const T *>(a.v) + b * a.v_sb + h / a.share * a.v_sh;
-    const float lam = __builtin_amdgcn_exp2f(a.log_decay[h] * 1.4426950408889634f);
+    const float lam = Decay(a.log_decay[h]).power(1);
     float *state = a.state + static_cast<int64_t>(bh) * a.K * a.V + c;
     f32x4 vv = {0.0f, 0.0f, 0.0f, 0.0f}, sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll

@@ -693,8 +693,9 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
 
     Ticks are taken in chunks, as matrix products.  Those of bfloat16 sequences multiply scores and states as two bfloat16
     values each, 16 bits together (their sums, and the states themselves, are float32); those of float16 ones are float32, as
-    states and scores go beyond float16's range.  What an infinite key makes infinite of the state, or an infinite query of its
-    tick's answer, may be NaN instead; likewise in the gradients."""
+    states and scores go beyond float16's range.  An infinite value or state makes its channel infinite from there on, or NaN where
+    the definition does; what an infinite key makes infinite of the state, or an infinite query of its tick's answer, may be NaN
+    instead; likewise in the gradients."""
     if torch.is_tensor(q) and q.dim() != 4:
         raise ValueError(f"q must be [T, B, H, K], got shape {tuple(q.shape)}")
     scale = _attention_args(q, k, v, log_decay, scale)
