@@ -866,9 +866,13 @@ void run_direct(const AttArgs &a, bool states, hipStream_t s) {
     const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
     const dim3 grid(static_cast<unsigned>(groups * a.passes)), block(NW * kWave);
     const bool few = groups * a.passes <= (NW == 8 ? 256 : 512);
-    if (states) {
-        if (few) hipLaunchKernelGGL((k_attention_direct<D, NW, 64, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_attention_direct<D, NW, 32, true>), grid, block, 0, s, a);
+    if (states) {   // (of 128 channels at most 256 blocks: cut())
+        if constexpr (NW == 4)
+            if (!few) {
+                hipLaunchKernelGGL((k_attention_direct<D, NW, 32, true>), grid, block, 0, s, a);
+                return;
+            }
+        hipLaunchKernelGGL((k_attention_direct<D, NW, 64, true>), grid, block, 0, s, a);
     } else {
         if (few) hipLaunchKernelGGL((k_attention_direct<D, NW, 64, false>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((k_attention_direct<D, NW, 32, false>), grid, block, 0, s, a);
