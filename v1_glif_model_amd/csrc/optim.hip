@@ -79,7 +79,7 @@ struct AdamwArgs {
     int64_t *iterations;                 // steps done, and the blocks that have ended (0 between launches)
     int64_t total;                       // elements of all units
     double log_beta_1, log_beta_2;
-    float beta_1, beta_2, one_m_b1, one_m_b2, lr, eps, keep;
+    float beta_1, beta_2, one_m_b1, one_m_b2, lr, eps, decay;   // decay: lr times the weights'
     uint64_t seed;
     int32_t last;                        // this launch ends the step
 };
@@ -182,9 +182,13 @@ struct Quad {
         if (BITS == 8) m = decode_4<false>(mc, ms), v = decode_4<true>(vc, vs);
         m = m * a.beta_1 + g * a.one_m_b1;
         v = v * a.beta_2 + (g * g) * a.one_m_b2;
+        // The decay joins the update before anything is rounded to p's digits: of 1 - decay, float32 keeps nothing of a decay below 3e-8.
+        // (An infinite p stays: what is taken off it is finite.)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            p[e] = p[e] * a.keep - size * (m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * root + a.eps));
+        for (int e = 0; e < 4; ++e) {
+            const float update = size * (m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * root + a.eps));
+            p[e] -= __builtin_fmaf(a.decay, __builtin_amdgcn_fmed3f(p[e], -3.40282347e38f, 3.40282347e38f), update);
+        }
     }
     __device__ __forceinline__ void put(const AdamwArgs &a, int64_t home, int lane, int64_t t) const {
         if (BITS == 8) {
@@ -343,7 +347,7 @@ extern "C" int glif_adamw(int32_t n_vars, void *const *vars, const int32_t *var_
     a.beta_1 = static_cast<float>(beta_1), a.beta_2 = static_cast<float>(beta_2);
     a.one_m_b1 = static_cast<float>(1.0 - beta_1), a.one_m_b2 = static_cast<float>(1.0 - beta_2);
     a.lr = static_cast<float>(learning_rate), a.eps = static_cast<float>(epsilon);
-    a.keep = static_cast<float>(1.0 - learning_rate * weight_decay), a.seed = seed;
+    a.decay = static_cast<float>(learning_rate * weight_decay), a.seed = seed;
     hipStream_t s = static_cast<hipStream_t>(stream);
     int64_t home = 0;
     for (int32_t i = 0; i < n_vars; ++i) {
