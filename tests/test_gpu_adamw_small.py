@@ -35,3 +35,55 @@ def test_infinite_variables_stay(dtype):
         p = torch.tensor([float("inf"), float("-inf"), 1.0, 3e38, float("nan")], device=DEV).to(dtype)
         AdamW([p], 1e-3, weight_decay=decay).apply_gradients([torch.ones(5, device=DEV)])
         assert p[0] == float("inf") and p[1] == float("-inf") and p[2:4].isfinite().all() and p[4].isnan()
+
+
+STEPS, KEEP = 300, 0.999
+
+
+def held_state(n):
+    """Blocks whose first element has the scale, 1, and gradients that keep it there; the others' codes are 30 to 60 and their
+    gradients 0."""
+    g = np.random.default_rng(5)
+    codes = [g.integers(30, 61, n) * g.choice([-1, 1], n), g.integers(30, 61, n)]
+    for c, top in zip(codes, (127, 255)):
+        c[::256] = top
+    grad = np.zeros(n, np.float32)
+    grad[::256] = 1.0
+    return [c.astype(t) for c, t in zip(codes, (np.int8, np.uint8))], grad
+
+
+def left_of(values, at_first):
+    """The share that is left of moments in the mean of their magnitudes, without the elements that hold the scales."""
+    rest = np.arange(values.size) % 256 != 0
+    return np.abs(values[rest]).mean() / np.abs(at_first[rest]).mean() / KEEP ** STEPS
+
+
+def test_moments_that_move_by_less_than_a_code():
+    """They lose 0.1 % a step where codes are 3 to 14 % apart: 300 steps of 65,280 moments.  One rounding is off by at
+    most half the way between two codes (standard deviation), which are 2 (60 / 127) / 127 or 4 (60 / 255)^3 / 255 of the scale apart: the
+    mean of all, by sqrt(300 / 65,280) of that.  Six deviations allowed; roundings to the nearest, up and down are all
+    outside."""
+    from v1_glif_model_amd.optim import AdamW
+    n = 65536
+    codes, grad = held_state(n)
+    p = torch.zeros(n, device=DEV)
+    opt = AdamW([p], 0.0, KEEP, KEEP, state_bits=8, seed=11)
+    ones = torch.ones(n // 256, device=DEV)
+    opt.load_state_dict(dict(iterations=10, first=[(torch.from_numpy(codes[0]).to(DEV), ones)],
+                             second=[(torch.from_numpy(codes[1]).to(DEV), ones)]))
+    g = torch.from_numpy(grad).to(DEV)
+    start = [host(x[0]) for x in opt.moments()]
+    for _ in range(STEPS):
+        opt.apply_gradients([g])
+    end = [host(x[0]) for x in opt.moments()]
+    F = np.float32
+    for k, (top, step) in enumerate(((127, 2 * 60 / 127 / 127), (255, 4 * (60 / 255) ** 3 / 255))):
+        assert end[k][::256] == pytest.approx(1.0, abs=1e-4)
+        allowed = 6 * step / 2 * np.sqrt(STEPS / (n - n // 256)) / (np.abs(start[k]).reshape(-1, 256)[:, 1:].mean() * KEEP ** STEPS)
+        assert abs(left_of(end[k], start[k]) - 1.0) <= allowed, (top, left_of(end[k], start[k]), allowed)
+        for u in (0, 32768, 65535):          # up, to the nearest, down: two blocks are enough
+            code, scale = codes[k][:512], np.ones(2, F)
+            for _ in range(STEPS):
+                x = ref.decode(code, scale, top) * F(KEEP) + (grad[:512] if top == 127 else grad[:512] ** 2) * F(1 - KEEP)
+                code, scale = ref.encode(x, top, np.full(512, u))
+            assert abs(left_of(ref.decode(code, scale, top), start[k][:512]) - 1.0) > 2 * allowed, (top, u)
