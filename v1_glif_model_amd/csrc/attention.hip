@@ -10,10 +10,10 @@
 //   dv = F(k, scale q, dy; dS)                   last tick, and what is left behind the first is dS0
 // No power is of a negative exponent, so no decay, 0 among them, can overflow.
 //
-// Bound by latency within a chunk: 500 x 32 ticks of 8 heads of 128, bfloat16, trials of any length, 41 us forward (a block
-// of eight waves alone on its compute unit; 8.6k cycles a chunk of 64 ticks, of which the matrix instructions are 2.7k), 71 us for
-// the backward's three passes; of 32 heads, all ticks, 148 us (3.5 TB/s) and 370 (4.3 TB/s, 9 sequences read and 3 written).
-// In float32 (its products at 1/16 of the rate) 290 x 18 ticks of 4 heads of 128 and 64 50 us.
+// Bound by latency within a chunk: 500 x 32 ticks of 8 heads of 128, bfloat16, trials of any length, 43 us forward (a block
+// of eight waves alone on its compute unit; 10.0k cycles a chunk of 64 ticks, of which the matrix instructions are 3.2k), 85 us for
+// the backward's three passes; of 32 heads, all ticks, 194 us (2.7 TB/s) and 525 (3.0 TB/s, 9 sequences read and 3 written).
+// In float32 (its products at 1/16 of the rate) 290 x 18 ticks of 4 heads of 128 and 64 56 us.
 #include <type_traits>
 
 #include "mma.h"
@@ -50,8 +50,11 @@ struct AttArgs {
 // them, as long as lam itself is not: 1e-38 of a state is nothing, and an infinite one stays infinite, as it does tick by tick.
 struct Decay {
     float rate, least;   // logarithms to base 2
-    __device__ __forceinline__ explicit Decay(float log_decay) : rate(log_decay * 1.4426950408889634f), least(rate >= -126.0f ? -126.0f : rate) {}
-    __device__ __forceinline__ float power(int n) const { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(fmaxf(rate * static_cast<float>(n), least)); }
+    __device__ __forceinline__ explicit Decay(float log_decay)
+        : rate(log_decay * 1.4426950408889634f), least(rate >= -126.0f ? -126.0f : rate) {}
+    __device__ __forceinline__ float power(int n) const {
+        return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(fmaxf(rate * static_cast<float>(n), least));
+    }
 };
 
 __device__ __forceinline__ int live_ticks(const int32_t *lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }
@@ -227,7 +230,7 @@ __device__ __forceinline__ uint32_t two_halves(float lo, float hi) {   // to nea
     return w;
 }
 // Scores and states that are multiplied as bfloat16: four as two values each, 16 bits together, which leaves outputs at their last
-// rounding (500 x 32 ticks of 8 heads of 128 forward 44.6 us, backward 85.4; states as one value,
+// rounding (500 x 32 ticks of 8 heads of 128 forward 42.9 us, backward 84.8; states as one value,
 // 40.2 and 70.4, put as much error again into outputs that come from before their chunk, and far more where their terms cancel).
 // What is left of an infinity, NaN by the difference, is made finite (what is left of a finite value is within it).
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -732,7 +735,8 @@ __global__ void __launch_bounds__(NW *kWave, NW == 8 && TICKS == 32 ? 4 : 2) k_a
         const bool odd = any_odd(fc);
         if (!STATES && odd) {
             by_ticks<bf16, R, R, 8, true>(ta, tb, tc, n, D, wc, l, decay, lead, in_scale, x, [&](int i, float sum) {
-                if (out) out[(back ? len - 1 - here - i : here + i) * out_st + static_cast<int64_t>(bh) * D + wc + r16] = static_cast<bf16>(sum * out_scale);
+                const int64_t to = (back ? len - 1 - here - i : here + i) * out_st + static_cast<int64_t>(bh) * D + wc + r16;
+                if (out) out[to] = static_cast<bf16>(sum * out_scale);
             });
         } else {
             if (!STATES && out) {
@@ -859,8 +863,8 @@ void run_pass(const AttArgs &a, bool states, hipStream_t s) {
 }
 
 // Chunks of 64 ticks are the faster for blocks that are alone on their compute unit, of 32 leave room for others (500 x 32 ticks
-// of 8 heads of 128, 256 blocks forward, 41 us and 46, 768 backward, trials of any length, 88 and 71; of 16 heads of 64, 512 and
-// 1536 blocks, 36 and 38, 95 and 78).
+// of 8 heads of 128, trials of any length, 256 blocks forward, 43 us and 52, 768 backward, 96 and 85; of 16 heads of 64, 512 and 1536
+// blocks, 34 and 36, 74 and 57).
 template <int D, int NW>
 void run_direct(const AttArgs &a, bool states, hipStream_t s) {
     const int64_t groups = (static_cast<int64_t>(a.B) * a.H * a.segments + 7) / 8 * 8;
@@ -1006,9 +1010,10 @@ int check_attention(const glif_attention *a, bool step) {
 
 // Ticks in segments where there are too few blocks for the chip: a first launch gives the state that each segment adds,
 // a second joins them, and then all segments go at once.  The first reads two of three sequences again and takes more than
-// half as long, so that two segments gain nothing (500 x 16 ticks of 8 heads of 128 in two 52 us, in one 37, by scores of one value).
-// As many segments as blocks are there at once, one a compute unit where heads have more than 64 channels, three where not (8000 ticks
-// of 16 heads of 128 in 25 segments, two rounds of blocks, 89 us, in 16 76, likewise), and none of fewer than four chunks.
+// half as long, so that two segments lose (500 x 16 ticks of 8 heads of 128 in two 59 us, in one 43; 8000 x 16 of 24 heads of 64 615 and
+// 496), but for thousands of ticks of 128-channel heads (8000 x 12 of 8 438 and 524).  As many segments as blocks are there at once,
+// one a compute unit where heads have more than 64 channels, three where not (8000 ticks of 16 heads of 128 in 25 segments, two rounds of
+// blocks, 86 us, in 16 75), and none of fewer than four chunks.
 void cut(AttArgs &a, int64_t blocks, int ticks, const glif_attention *s) {
     a.segments = 1, a.seg_ticks = std::max((a.T + ticks - 1) / ticks, 1) * ticks;
     const int64_t slots = std::max(s->d_key, s->d_value) > 64 ? 256 : 768;

@@ -849,7 +849,8 @@ __global__ void __launch_bounds__(kBlock) k_slope(SlopeArgs a) {
 }
 
 // Of a gated product: dp's first N columns are dy u act'(g), the others dy act(g), as above rounded for the products and summed
-// by columns before.
+// by columns before (dx and dW of bfloat16 2.3e-3 from 64 bits, with operands of float32 1.7e-3; as two values they would take both
+// products twice, 16000 x 1024 x 4096 450 us more).
 template <typename T>
 __global__ void __launch_bounds__(kBlock) k_gate_slope(SlopeArgs a) {
     constexpr int V = kVecBytes16<T>;

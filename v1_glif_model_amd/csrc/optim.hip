@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kBlock)
 // become 0, as the step divides by its root.  The random numbers of element i of all variables' blocks are the two halves of word
 // (t - 1) P + i of the Philox stream `seed`, P the elements of all blocks.
 //
-// Bound by memory: 36M float32 elements of 20 tensors, 997 MB, 196 us (5.1 TB/s), with moments of 8 bits, 572 MB, 133 us (the
+// Bound by memory: 36M float32 elements of 20 tensors, 997 MB, 195 us (5.1 TB/s), with moments of 8 bits, 572 MB, 139 us (the
 // random numbers, roots and codes are some 100 operations an element); results past the caches gained nothing.
 constexpr int kUnit = 256;          // elements that a wave takes at once, and that share a scale
 constexpr int kUnitsPerBlock = 16;  // that a block takes at once
