@@ -187,3 +187,31 @@ def test_what_is_not_finite_in_chunks_of_32_ticks(B, H, K, V, bad):
         assert torch.equal(a[:, same], b[:, same])
         w, s = f64(b[:, entry], False), f64(s[:, 0], False)
         near(a[:, entry], w, s, "the entry's others", UNIT[BF16] * w.abs() + (1e-5 + 2 * more(BF16)) * s)
+
+
+@pytest.mark.parametrize("K,V", [(128, 128), (120, 128)])
+def test_sequences_of_more_than_2_to_the_31_elements(K, V):
+    """The last entry of a batch against itself alone, whose sums are by other chunks: each within its bound."""
+    from v1_glif_model_amd import sequence as seq
+    T, B, H = 9200, 64, 32
+    assert T * B * H * min(K, V) > 2 ** 31
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, v, dy = (torch.randn(T, B, H, d, generator=g, device=DEV, dtype=BF16) for d in (K, K, V, V))
+    decay, lengths = -torch.logspace(-3, 0, H, device=DEV), torch.full((B,), T, dtype=torch.int32, device=DEV)
+    lengths[-1] = T - 5
+
+    def run(q, k, v, dy, lengths):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = seq.linear_attention(*leaves, decay, None, None, lengths)
+        return (*(o.detach() for o in out), *torch.autograd.grad(out[0], leaves, dy))
+
+    got = run(q, k, v, dy, lengths)
+    got = [got[0][:, -1:].clone(), got[1][-1:].clone(), *(t[:, -1:].clone() for t in got[2:])]
+    one = [t[:, -1:].contiguous() for t in (q, k, v, dy)]
+    del q, k, v, dy
+    want, size = run(*one, lengths[-1:]), run(*(t.float().abs() for t in one), lengths[-1:])
+    for name, a, w, s in zip(("y", "last", "dq", "dk", "dv"), got, want, size):
+        assert not name == "y" or (a[-6].any() and not a[-5:].any())
+        w, s = f64(w, False), f64(s, False)
+        near(a, w, s, name, UNIT[a.dtype] * w.abs() + (1e-5 + (2 * more(BF16) if a.dtype is BF16 else 0.0)) * s)
+    torch.cuda.empty_cache()
